@@ -1,0 +1,359 @@
+// Attention over packed sequences of any length: argument checks, choice of kernel, and the
+// FP32 kernel for float operands and for bfloat16 ones that TMA cannot describe.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(scale log2(e) q_i . k_j - m_i)
+//
+// in one pass over the keys: m_i is the maximum so far, and sums and outputs so far are
+// multiplied by 2^(old m - new m) when it rises. A row that sees no key keeps a sum of zero and
+// is written as zeros.
+#include "attention_varlen.hpp"
+#include "ptx.cuh"
+#include "varlen.cuh"
+
+#include <cuda_bf16.h>
+
+#include <cmath>
+#include <cstdint>
+
+namespace cuvit::attn {
+namespace {
+
+constexpr int kSimtRows = 64;
+constexpr int kSimtKeys = 64;
+constexpr int kSimtThreads = 256;
+constexpr int kSimtPitch = kSimtKeys + 4;
+
+template <typename T>
+__device__ __forceinline__ float load_value(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+        return __bfloat162float(*p);
+    } else {
+        return *p;
+    }
+}
+
+template <int DPad>
+constexpr int simt_smem_bytes() {
+    return 4 * (2 * DPad * kSimtPitch + kSimtKeys * DPad + kSimtKeys * kSimtPitch);
+}
+
+// 64 query rows of one head per block, keys in tiles of 64; thread (ty, tx) has rows 4 ty .. + 3
+// and, of the scores, keys 4 tx .. + 3, of the output, elements 4 tx .. + 3 of every 64.
+template <typename T, int DPad>
+__global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const VarlenParams p) {
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+    extern __shared__ __align__(16) float smem[];
+    float* const qs = smem;                       // [DPad][pitch], element-major
+    float* const ks = qs + DPad * kSimtPitch;     // [DPad][pitch]
+    float* const vs = ks + DPad * kSimtPitch;     // [keys][DPad]
+    float* const ps = vs + kSimtKeys * DPad;      // [keys][pitch], key-major
+    constexpr int kChunks = DPad / 64;
+
+    const long long block = blockIdx.x / p.q_heads;
+    const int head = static_cast<int>(blockIdx.x - block * p.q_heads);
+    const Sequence s = find_block<kSimtRows>(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens,
+                                             p.kv_tokens, block);
+    if (s.index < 0) {
+        return;
+    }
+    const int rows = min(kSimtRows, s.q_end - s.q_first);
+    const int keys = s.kv_end - s.kv_begin;
+    // Query row r of this block sees keys j <= r + reach.
+    const long long reach =
+        static_cast<long long>(s.q_first - s.q_begin) + keys - (s.q_end - s.q_begin);
+    const int last_key = p.causal ? static_cast<int>(min(static_cast<long long>(keys),
+                                                         max(0LL, reach + rows)))
+                                  : keys;
+    const int d = p.head_dim;
+    const T* const q = static_cast<const T*>(p.q) + s.q_first * p.q_stride +
+                       static_cast<long long>(head) * d;
+    const T* const k = static_cast<const T*>(p.k) + s.kv_begin * p.k_stride +
+                       static_cast<long long>(head / p.group) * d;
+    const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
+                       static_cast<long long>(head / p.group) * d;
+
+    for (int i = threadIdx.x; i < kSimtRows * DPad; i += kSimtThreads) {
+        const int r = i / DPad;
+        const int e = i - r * DPad;
+        qs[e * kSimtPitch + r] = r < rows && e < d ? load_value(q + r * p.q_stride + e) : 0.0F;
+    }
+    const int tx = threadIdx.x % 16;
+    const int ty = threadIdx.x / 16;
+    float o[4][4 * kChunks] = {};
+    float maximum[4], sum[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        maximum[r] = -INFINITY;
+        sum[r] = 0.0F;
+    }
+    for (int first = 0; first < last_key; first += kSimtKeys) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < kSimtKeys * DPad; i += kSimtThreads) {
+            const int j = i / DPad;
+            const int e = i - j * DPad;
+            const bool live = first + j < last_key && e < d;
+            const long long row = first + j;
+            ks[e * kSimtPitch + j] = live ? load_value(k + row * p.k_stride + e) : 0.0F;
+            vs[j * DPad + e] = live ? load_value(v + row * p.v_stride + e) : 0.0F;
+        }
+        __syncthreads();
+        float sc[4][4] = {};
+#pragma unroll 8
+        for (int e = 0; e < d; ++e) {
+            const float4 a = *reinterpret_cast<const float4*>(qs + e * kSimtPitch + 4 * ty);
+            const float4 b = *reinterpret_cast<const float4*>(ks + e * kSimtPitch + 4 * tx);
+            const float av[4] = {a.x, a.y, a.z, a.w};
+            const float bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sc[r][j] = fmaf(av[r], bv[j], sc[r][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long long limit = p.causal ? min(static_cast<long long>(last_key),
+                                                   reach + 4 * ty + r + 1)
+                                             : static_cast<long long>(last_key);
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sc[r][j] = first + 4 * tx + j < limit ? sc[r][j] * p.scale_log2 : -INFINITY;
+                top = fmaxf(top, sc[r][j]);
+            }
+#pragma unroll
+            for (int offset = 8; offset > 0; offset /= 2) {
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
+            }
+            const float raised = fmaxf(maximum[r], top);
+            // A row without a key so far: any finite stand-in keeps 2^(-inf - m) at zero.
+            const float base = raised == -INFINITY ? 0.0F : raised;
+            const float factor = exp2f(maximum[r] - base);
+            maximum[r] = raised;
+            float part = 0.0F;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sc[r][j] = exp2f(sc[r][j] - base);
+                part += sc[r][j];
+                ps[(4 * tx + j) * kSimtPitch + 4 * ty + r] = sc[r][j];
+            }
+            sum[r] = fmaf(sum[r], factor, part);
+#pragma unroll
+            for (int c = 0; c < 4 * kChunks; ++c) {
+                o[r][c] *= factor;
+            }
+        }
+        __syncwarp(); // a row's 16 threads are in one warp
+        const int live = min(kSimtKeys, last_key - first);
+#pragma unroll 4
+        for (int j = 0; j < live; ++j) {
+            const float4 a = *reinterpret_cast<const float4*>(ps + j * kSimtPitch + 4 * ty);
+            const float av[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const float4 b =
+                    *reinterpret_cast<const float4*>(vs + j * DPad + 64 * c + 4 * tx);
+                const float bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        o[r][4 * c + x] = fmaf(av[r], bv[x], o[r][4 * c + x]);
+                    }
+                }
+            }
+        }
+    }
+    T* const out = static_cast<T*>(p.out) + s.q_first * p.out_stride +
+                   static_cast<long long>(head) * d;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int offset = 8; offset > 0; offset /= 2) {
+            sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], offset);
+        }
+        const float inverse = sum[r] == 0.0F ? 0.0F : 1.0F / sum[r];
+        const int row = 4 * ty + r;
+        if (row < rows) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int e = 64 * c + 4 * tx + x;
+                    if (e < d) {
+                        const float value = o[r][4 * c + x] * inverse;
+                        if constexpr (sizeof(T) == 2) {
+                            out[row * p.out_stride + e] = __float2bfloat16_rn(value);
+                        } else {
+                            out[row * p.out_stride + e] = value;
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int DPad>
+int launch_simt(const VarlenParams& p, cudaStream_t stream) {
+    auto* kernel = &attention_varlen_simt<T, DPad>;
+    constexpr int kBytes = simt_smem_bytes<DPad>();
+    CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
+    const long long blocks = (static_cast<long long>(p.q_tokens) / kSimtRows + p.batch) * p.q_heads;
+    if (blocks > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
+    }
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSimtThreads), kBytes,
+                     stream, p);
+    return host::after_launch("attention_varlen_simt");
+}
+
+// Checks a problem's numbers and resolves its defaults; pointers stay null.
+int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* empty) {
+    if (problem == nullptr) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "attention problem cannot be null");
+    }
+    const cuvit_attention_problem& c = *problem;
+    if (c.batch < 0 || c.q_tokens < 0 || c.kv_tokens < 0 || c.q_heads < 0 || c.kv_heads < 0) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "attention dimensions cannot be negative");
+    }
+    if (c.head_dim < 1 || c.head_dim > 128) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "attention head_dim must be from 1 to 128");
+    }
+    if (c.dtype != CUVIT_DTYPE_F32 && c.dtype != CUVIT_DTYPE_BF16) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "packed attention operands must be F32 or BF16");
+    }
+    if (!std::isfinite(c.scale) || c.scale <= 0.0F) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "the attention scale must be finite and positive");
+    }
+    constexpr int kMaxTokens = 0x7FFFFFFF - 4096; // tile ends past the last row stay in int
+    if (c.q_tokens > kMaxTokens || c.kv_tokens > kMaxTokens) {
+        return host::fail(CUVIT_LENGTH_ERROR, "too many packed attention rows");
+    }
+    *empty = c.batch == 0 || c.q_tokens == 0 || c.q_heads == 0;
+    if (*empty) {
+        return CUVIT_OK;
+    }
+    if (c.kv_heads == 0 || c.q_heads % c.kv_heads != 0) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "kv_heads must divide q_heads");
+    }
+    VarlenParams p{};
+    p.batch = c.batch;
+    p.q_tokens = c.q_tokens;
+    p.kv_tokens = c.kv_tokens;
+    p.q_heads = c.q_heads;
+    p.kv_heads = c.kv_heads;
+    p.group = c.q_heads / c.kv_heads;
+    p.head_dim = c.head_dim;
+    p.causal = c.causal ? 1 : 0;
+    p.scale_log2 = c.scale * 1.4426950408889634F;
+    const int64_t q_width = static_cast<int64_t>(c.q_heads) * c.head_dim;
+    const int64_t kv_width = static_cast<int64_t>(c.kv_heads) * c.head_dim;
+    p.q_stride = c.q_stride != 0 ? c.q_stride : q_width;
+    p.k_stride = c.k_stride != 0 ? c.k_stride : kv_width;
+    p.v_stride = c.v_stride != 0 ? c.v_stride : kv_width;
+    p.out_stride = c.out_stride != 0 ? c.out_stride : q_width;
+    if (p.q_stride < q_width || p.out_stride < q_width || p.k_stride < kv_width ||
+        p.v_stride < kv_width) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "an attention row stride is smaller than its row");
+    }
+    const int64_t q_limit = (int64_t{1} << 58) / c.q_tokens;
+    const int64_t kv_limit = (int64_t{1} << 58) / (c.kv_tokens > 0 ? c.kv_tokens : 1);
+    if (p.q_stride > q_limit || p.out_stride > q_limit || p.k_stride > kv_limit ||
+        p.v_stride > kv_limit) {
+        return host::fail(CUVIT_LENGTH_ERROR, "an attention row stride is too large");
+    }
+    *out = p;
+    return CUVIT_OK;
+}
+
+int run(const void* q, const void* k, const void* v, void* out, const int32_t* q_offsets,
+        const int32_t* kv_offsets, const cuvit_attention_problem* problem, void* workspace,
+        size_t workspace_bytes, cudaStream_t stream) {
+    VarlenParams p{};
+    bool empty = false;
+    CUVIT_TRY(resolve(problem, &p, &empty));
+    if (empty) {
+        return CUVIT_OK;
+    }
+    if (q == nullptr || out == nullptr || q_offsets == nullptr ||
+        (p.kv_tokens > 0 && (k == nullptr || v == nullptr))) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "attention operands cannot be null");
+    }
+    if (kv_offsets == nullptr) {
+        if (p.kv_tokens != p.q_tokens) {
+            return host::fail(CUVIT_INVALID_ARGUMENT,
+                              "without key offsets there are as many keys as queries");
+        }
+        kv_offsets = q_offsets;
+    }
+    const bool bf16 = problem->dtype == CUVIT_DTYPE_BF16;
+    const int element = bf16 ? 2 : 4;
+    for (const void* operand : {q, k, v, static_cast<const void*>(out)}) {
+        if (reinterpret_cast<uintptr_t>(operand) % element != 0) {
+            return host::fail(CUVIT_INVALID_ARGUMENT,
+                              "attention operands must be aligned to their type");
+        }
+    }
+    if (reinterpret_cast<uintptr_t>(q_offsets) % 4 != 0 ||
+        reinterpret_cast<uintptr_t>(kv_offsets) % 4 != 0) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "offsets must be aligned to their type");
+    }
+    const int64_t q_width = static_cast<int64_t>(p.q_heads) * p.head_dim * element;
+    const int64_t kv_width = static_cast<int64_t>(p.kv_heads) * p.head_dim * element;
+    const host::RowSpan out_span{out, p.q_tokens, q_width, p.out_stride * element};
+    if (host::rows_overlap(out_span, {q, p.q_tokens, q_width, p.q_stride * element}) ||
+        host::rows_overlap(out_span, {k, p.kv_tokens, kv_width, p.k_stride * element}) ||
+        host::rows_overlap(out_span, {v, p.kv_tokens, kv_width, p.v_stride * element})) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "the attention output overlaps an operand");
+    }
+    (void)workspace;
+    (void)workspace_bytes;
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.out = out;
+    p.q_offsets = q_offsets;
+    p.kv_offsets = kv_offsets;
+    const host::DeviceContext* context = nullptr;
+    CUVIT_TRY(host::current_context(&context));
+    CUVIT_TRY(host::check_operands({q, k, v, out, q_offsets, kv_offsets}));
+    if (bf16) {
+        return p.head_dim <= 64 ? launch_simt<__nv_bfloat16, 64>(p, stream)
+                                : launch_simt<__nv_bfloat16, 128>(p, stream);
+    }
+    return p.head_dim <= 64 ? launch_simt<float, 64>(p, stream)
+                            : launch_simt<float, 128>(p, stream);
+}
+
+} // namespace
+} // namespace cuvit::attn
+
+extern "C" {
+
+int cuvit_attention_varlen(const void* q, const void* k, const void* v, void* out,
+                           const int32_t* q_offsets, const int32_t* kv_offsets,
+                           const cuvit_attention_problem* problem, void* workspace,
+                           size_t workspace_bytes, cuvit_stream_t stream) {
+    return cuvit::host::guarded([&]() {
+        return cuvit::attn::run(q, k, v, out, q_offsets, kv_offsets, problem, workspace,
+                                workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+int cuvit_attention_varlen_workspace(const cuvit_attention_problem* problem, size_t* bytes) {
+    return cuvit::host::guarded([&]() {
+        if (bytes == nullptr) {
+            return cuvit::host::fail(CUVIT_INVALID_ARGUMENT, "workspace size cannot be null");
+        }
+        *bytes = 0;
+        cuvit::attn::VarlenParams p{};
+        bool empty = false;
+        return cuvit::attn::resolve(problem, &p, &empty);
+    });
+}
+
+} // extern "C"

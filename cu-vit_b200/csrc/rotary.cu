@@ -1,0 +1,431 @@
+// Rotary positions with several axes, and per-head norms of queries and keys with the rotation
+// in the same pass.
+//
+// For a head x of token t:  y = x / sqrt(mean(x^2) + eps) * gamma + beta        (RMS)
+//                           y = (x - mean) / sqrt(var + eps) * gamma + beta     (layer)
+//                           y = x                                               (rotation alone)
+// then each pair (y_a, y_b) of axis c turns by the angle positions[c][t] * rate, in FP32 with
+// one rounding at the store. The angle is formed in fixed point: rates are kept in units of
+// 2^-64 turn, so position * rate modulo 2^64 is the fraction of a turn without any range
+// reduction, and no position loses accuracy (FP32 angles are off by 6e-3 rad at position 1e5).
+#include "cuvit_b200.h"
+#include "ptx.cuh"
+#include "runtime.hpp"
+
+#include <cuda_bf16.h>
+
+#include <cmath>
+#include <cstdint>
+
+namespace cuvit::rotary {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxHeadDim = 256;
+constexpr int kNormNone = -1;
+
+struct Side {
+    const void* in;
+    void* out;
+    const float* gamma;
+    const float* beta;
+    long long in_stride;
+    long long out_stride;
+    int heads;
+};
+
+struct Params {
+    Side side[2]; // queries, keys
+    int tokens;
+    int head_dim;
+    int pairs; // rotated pairs per head
+    int adjacent;
+    float epsilon;
+    const int* positions;
+    long long position_stride;
+    cuvit_rotary rotary;
+};
+
+template <typename T>
+__device__ __forceinline__ float load_value(const T* p) {
+    if constexpr (sizeof(T) == 2) {
+        return __bfloat162float(*p);
+    } else {
+        return *p;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_value(T* p, float v) {
+    if constexpr (sizeof(T) == 2) {
+        *p = __float2bfloat16_rn(v);
+    } else {
+        *p = v;
+    }
+}
+
+// Elements of pair i of a head: the rotated pairs first, then what is left of the head, paired
+// the same way (those turn by nothing).
+__device__ __forceinline__ void pair_elements(int i, int pairs, int half_dim, int adjacent, int& a,
+                                              int& b) {
+    if (adjacent) {
+        a = 2 * i;
+        b = 2 * i + 1;
+    } else if (i < pairs) {
+        a = i;
+        b = i + pairs;
+    } else {
+        a = 2 * pairs + (i - pairs);
+        b = a + (half_dim - pairs);
+    }
+}
+
+// cos and sin of pair i's angle at token t (1 and 0 past the rotated pairs).
+__device__ __forceinline__ float2 turn_of(const Params& p, int t, int i) {
+    if (i >= p.pairs) {
+        return make_float2(1.0F, 0.0F);
+    }
+    int axis = 0;
+    while (axis + 1 < p.rotary.axes && i >= p.rotary.first[axis + 1]) {
+        ++axis;
+    }
+    const long long position = p.positions[axis * p.position_stride + t];
+    const uint64_t fraction = static_cast<uint64_t>(position) * p.rotary.turns[i];
+    // The top 32 bits as a signed number of half turns in [-1, 1): within 2^-25 of a half turn.
+    const float half_turns =
+        static_cast<float>(static_cast<int>(fraction >> 32)) * 4.656612873077393e-10F;
+    float s, c;
+    sincospif(half_turns, &s, &c);
+    return make_float2(c, s);
+}
+
+__device__ __forceinline__ float warp_sum(float value) {
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) {
+        value += __shfl_xor_sync(0xFFFFFFFFu, value, offset);
+    }
+    return value;
+}
+
+// Any even head_dim and any alignment: one warp per head, scalar loads.
+template <typename T, int Norm>
+__global__ void __launch_bounds__(kThreads) qk_scalar_kernel(const __grid_constant__ Params p) {
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+    const int lane = threadIdx.x % 32;
+    const int heads = p.side[0].heads + p.side[1].heads;
+    const long long item = static_cast<long long>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
+    const int t = static_cast<int>(item / heads);
+    if (t >= p.tokens) {
+        return; // the whole warp
+    }
+    int head = static_cast<int>(item - static_cast<long long>(t) * heads);
+    const Side& side = head < p.side[0].heads ? p.side[0] : p.side[1];
+    head -= head < p.side[0].heads ? 0 : p.side[0].heads;
+    const T* const in = static_cast<const T*>(side.in) + t * side.in_stride +
+                        static_cast<long long>(head) * p.head_dim;
+    T* const out = static_cast<T*>(side.out) + t * side.out_stride +
+                   static_cast<long long>(head) * p.head_dim;
+    const int half = p.head_dim / 2;
+    constexpr int kPer = kMaxHeadDim / 2 / 32;
+    float x[kPer], y[kPer];
+    float sum = 0.0F;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = lane + 32 * j;
+        x[j] = y[j] = 0.0F;
+        if (i < half) {
+            int a, b;
+            pair_elements(i, p.pairs, half, p.adjacent, a, b);
+            x[j] = load_value(in + a);
+            y[j] = load_value(in + b);
+        }
+        sum += x[j] + y[j];
+    }
+    if constexpr (Norm != kNormNone) {
+        float mean = 0.0F;
+        if constexpr (Norm == CUVIT_NORM_LAYER) {
+            mean = warp_sum(sum) / static_cast<float>(p.head_dim);
+        }
+        float squares = 0.0F;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (lane + 32 * j < half) {
+                x[j] -= mean;
+                y[j] -= mean;
+                squares = fmaf(x[j], x[j], fmaf(y[j], y[j], squares));
+            }
+        }
+        squares = warp_sum(squares);
+        const float scale = 1.0F / sqrtf(squares / static_cast<float>(p.head_dim) + p.epsilon);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = lane + 32 * j;
+            if (i < half) {
+                int a, b;
+                pair_elements(i, p.pairs, half, p.adjacent, a, b);
+                x[j] = x[j] * scale * (side.gamma != nullptr ? side.gamma[a] : 1.0F) +
+                       (side.beta != nullptr ? side.beta[a] : 0.0F);
+                y[j] = y[j] * scale * (side.gamma != nullptr ? side.gamma[b] : 1.0F) +
+                       (side.beta != nullptr ? side.beta[b] : 0.0F);
+            }
+        }
+    }
+    __syncwarp(); // every lane has read its elements before any is written over (in place)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = lane + 32 * j;
+        if (i < half) {
+            int a, b;
+            pair_elements(i, p.pairs, half, p.adjacent, a, b);
+            if (i < p.pairs) {
+                const float2 turn = turn_of(p, t, i);
+                store_value(out + a, x[j] * turn.x - y[j] * turn.y);
+                store_value(out + b, fmaf(x[j], turn.y, y[j] * turn.x));
+            } else {
+                store_value(out + a, x[j]);
+                store_value(out + b, y[j]);
+            }
+        }
+    }
+}
+
+template <typename T, int Norm>
+int launch_scalar(const Params& p, cudaStream_t stream) {
+    const long long heads = p.side[0].heads + p.side[1].heads;
+    const long long blocks = (heads * p.tokens + kThreads / 32 - 1) / (kThreads / 32);
+    if (blocks > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "rotary launch exceeds the CUDA grid limit");
+    }
+    host::pdl_launch(qk_scalar_kernel<T, Norm>, dim3(static_cast<unsigned>(blocks)),
+                     dim3(kThreads), 0, stream, p);
+    return host::after_launch("qk_scalar_kernel");
+}
+
+template <typename T>
+int launch_typed(const Params& p, int norm, cudaStream_t stream) {
+    switch (norm) {
+    case CUVIT_NORM_RMS:
+        return launch_scalar<T, CUVIT_NORM_RMS>(p, stream);
+    case CUVIT_NORM_LAYER:
+        return launch_scalar<T, CUVIT_NORM_LAYER>(p, stream);
+    default:
+        return launch_scalar<T, kNormNone>(p, stream);
+    }
+}
+
+int check_rotary(const cuvit_rotary& r, int head_dim) {
+    bool ok = r.axes >= 1 && r.axes <= CUVIT_ROTARY_MAX_AXES && r.first[0] == 0 &&
+              (r.pairing == CUVIT_ROTARY_HALVES || r.pairing == CUVIT_ROTARY_ADJACENT);
+    for (int a = 0; ok && a < r.axes; ++a) {
+        ok = r.first[a + 1] >= r.first[a] && r.first[a + 1] <= CUVIT_ROTARY_MAX_PAIRS;
+    }
+    if (!ok || r.first[r.axes] < 1) {
+        return host::fail(CUVIT_INVALID_ARGUMENT,
+                          "the rotary axes were not set up by cuvit_rotary_init()");
+    }
+    if (2 * r.first[r.axes] > head_dim) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "the rotary axes turn more pairs than a head has");
+    }
+    return CUVIT_OK;
+}
+
+int run(const void* q, const void* k, void* q_out, void* k_out, const cuvit_qk_norm* norm,
+        const int32_t* positions, const cuvit_rotary* rotary, const cuvit_qk_problem* problem,
+        cudaStream_t stream) {
+    if (problem == nullptr) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "query / key problem cannot be null");
+    }
+    const cuvit_qk_problem& c = *problem;
+    if (c.tokens < 0 || c.q_heads < 0 || c.k_heads < 0) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "query / key dimensions cannot be negative");
+    }
+    if (c.head_dim < 2 || c.head_dim > kMaxHeadDim || c.head_dim % 2 != 0) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "head_dim must be even, from 2 to 256");
+    }
+    if (c.dtype != CUVIT_DTYPE_F32 && c.dtype != CUVIT_DTYPE_BF16) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "queries and keys must be F32 or BF16");
+    }
+    if (rotary != nullptr) {
+        CUVIT_TRY(check_rotary(*rotary, c.head_dim));
+    }
+    if (norm != nullptr && ((norm->kind != CUVIT_NORM_RMS && norm->kind != CUVIT_NORM_LAYER) ||
+                            !(norm->epsilon >= 0.0F) || std::isinf(norm->epsilon))) {
+        return host::fail(CUVIT_INVALID_ARGUMENT,
+                          "unknown norm, or an epsilon that is negative or not finite");
+    }
+    if (c.tokens == 0 || (c.q_heads == 0 && c.k_heads == 0)) {
+        return CUVIT_OK;
+    }
+    if (rotary != nullptr && positions == nullptr) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "positions cannot be null");
+    }
+
+    Params p{};
+    p.tokens = c.tokens;
+    p.head_dim = c.head_dim;
+    const int element = c.dtype == CUVIT_DTYPE_BF16 ? 2 : 4;
+    const void* const ins[2] = {q, k};
+    void* const outs[2] = {q_out, k_out};
+    const int heads[2] = {c.q_heads, c.k_heads};
+    const int64_t in_strides[2] = {c.q_stride, c.k_stride};
+    const int64_t out_strides[2] = {c.q_out_stride, c.k_out_stride};
+    host::RowSpan in_spans[2]{}, out_spans[2]{};
+    for (int s = 0; s < 2; ++s) {
+        Side& side = p.side[s];
+        side.heads = heads[s];
+        if (heads[s] == 0) {
+            continue;
+        }
+        if (ins[s] == nullptr || outs[s] == nullptr) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "queries and keys cannot be null");
+        }
+        if (reinterpret_cast<uintptr_t>(ins[s]) % element != 0 ||
+            reinterpret_cast<uintptr_t>(outs[s]) % element != 0) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "queries and keys must be aligned to their type");
+        }
+        const int64_t width = static_cast<int64_t>(heads[s]) * c.head_dim;
+        side.in = ins[s];
+        side.out = outs[s];
+        side.in_stride = in_strides[s] != 0 ? in_strides[s] : width;
+        side.out_stride = out_strides[s] != 0 ? out_strides[s] : width;
+        if (side.in_stride < width || side.out_stride < width) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "a token stride is smaller than its heads");
+        }
+        const int64_t limit = (int64_t{1} << 58) / c.tokens;
+        if (side.in_stride > limit || side.out_stride > limit) {
+            return host::fail(CUVIT_LENGTH_ERROR, "a token stride is too large");
+        }
+        in_spans[s] = {ins[s], c.tokens, width * element, side.in_stride * element};
+        out_spans[s] = {outs[s], c.tokens, width * element, side.out_stride * element};
+        if (norm != nullptr) {
+            side.gamma = s == 0 ? norm->q_gamma : norm->k_gamma;
+            side.beta = s == 0 ? norm->q_beta : norm->k_beta;
+            if (reinterpret_cast<uintptr_t>(side.gamma) % 4 != 0 ||
+                reinterpret_cast<uintptr_t>(side.beta) % 4 != 0) {
+                return host::fail(CUVIT_INVALID_ARGUMENT,
+                                  "norm gains and offsets must be aligned to their type");
+            }
+        }
+    }
+    for (int o = 0; o < 2; ++o) {
+        for (int i = 0; i < 2; ++i) {
+            const bool in_place = o == i && ins[i] == outs[o] &&
+                                  p.side[i].in_stride == p.side[i].out_stride;
+            if (!in_place && host::rows_overlap(out_spans[o], in_spans[i])) {
+                return host::fail(CUVIT_INVALID_ARGUMENT,
+                                  "an output overlaps an input that is not its own");
+            }
+        }
+    }
+    if (host::rows_overlap(out_spans[0], out_spans[1])) {
+        return host::fail(CUVIT_INVALID_ARGUMENT, "the outputs overlap");
+    }
+    p.epsilon = norm != nullptr ? norm->epsilon : 0.0F;
+    if (rotary != nullptr) {
+        p.rotary = *rotary;
+        p.pairs = rotary->first[rotary->axes];
+        p.adjacent = rotary->pairing == CUVIT_ROTARY_ADJACENT ? 1 : 0;
+        p.positions = positions;
+        p.position_stride = c.position_stride != 0 ? c.position_stride : c.tokens;
+        if (p.position_stride < 0 || p.position_stride > (int64_t{1} << 58)) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "the position stride is out of range");
+        }
+        if (reinterpret_cast<uintptr_t>(positions) % 4 != 0) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "positions must be aligned to their type");
+        }
+    }
+    const host::DeviceContext* context = nullptr;
+    CUVIT_TRY(host::current_context(&context));
+    CUVIT_TRY(host::check_operands({p.side[0].in, p.side[0].out, p.side[1].in, p.side[1].out,
+                                    p.positions, p.side[0].gamma, p.side[0].beta, p.side[1].gamma,
+                                    p.side[1].beta}));
+    const int kind = norm != nullptr ? norm->kind : kNormNone;
+    return c.dtype == CUVIT_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(p, kind, stream)
+                                       : launch_typed<float>(p, kind, stream);
+}
+
+} // namespace
+} // namespace cuvit::rotary
+
+extern "C" {
+
+int cuvit_rotary_init(cuvit_rotary* rotary, int axes, const int* sections, double base,
+                      int pairing, int ladder) {
+    return cuvit::host::guarded([&]() {
+        using cuvit::host::fail;
+        if (rotary == nullptr || sections == nullptr) {
+            return fail(CUVIT_INVALID_ARGUMENT, "rotary axes and sections cannot be null");
+        }
+        if (axes < 1 || axes > CUVIT_ROTARY_MAX_AXES) {
+            return fail(CUVIT_INVALID_ARGUMENT, "rotary positions have 1 to 4 axes");
+        }
+        int total = 0;
+        for (int a = 0; a < axes; ++a) {
+            if (sections[a] < 0 || sections[a] > CUVIT_ROTARY_MAX_PAIRS - total) {
+                return fail(CUVIT_INVALID_ARGUMENT,
+                            "rotary sections must be at least 0 and hold at most 128 pairs in all");
+            }
+            total += sections[a];
+        }
+        if (total == 0) {
+            return fail(CUVIT_INVALID_ARGUMENT, "the rotary axes turn no pair");
+        }
+        if (!std::isfinite(base) || base < 1.0) {
+            return fail(CUVIT_INVALID_ARGUMENT, "the rotary base must be finite and at least 1");
+        }
+        if ((pairing != CUVIT_ROTARY_HALVES && pairing != CUVIT_ROTARY_ADJACENT) ||
+            (ladder != CUVIT_ROTARY_LADDER_AXIS && ladder != CUVIT_ROTARY_LADDER_SHARED)) {
+            return fail(CUVIT_INVALID_ARGUMENT, "unknown rotary pairing or ladder");
+        }
+        cuvit_rotary r{};
+        r.axes = axes;
+        r.pairing = pairing;
+        constexpr long double kTwoPi = 6.283185307179586476925286766559L;
+        for (int a = 0; a < axes; ++a) {
+            r.first[a + 1] = r.first[a] + sections[a];
+            for (int j = 0; j < sections[a]; ++j) {
+                const int i = r.first[a] + j;
+                const long double exponent =
+                    ladder == CUVIT_ROTARY_LADDER_AXIS
+                        ? static_cast<long double>(j) / sections[a]
+                        : static_cast<long double>(i) / total;
+                // A rate is at most 1 radian a step, so the fraction of a turn is below 1/6.
+                const long double rate = powl(static_cast<long double>(base), -exponent);
+                r.turns[i] = static_cast<uint64_t>(ldexpl(rate / kTwoPi, 64));
+            }
+        }
+        for (int a = axes; a < CUVIT_ROTARY_MAX_AXES; ++a) {
+            r.first[a + 1] = r.first[axes];
+        }
+        *rotary = r;
+        return static_cast<int>(CUVIT_OK);
+    });
+}
+
+int cuvit_rotary_qk(const void* q, const void* k, void* q_out, void* k_out,
+                    const int32_t* positions, const cuvit_rotary* rotary,
+                    const cuvit_qk_problem* problem, cuvit_stream_t stream) {
+    return cuvit::host::guarded([&]() {
+        if (rotary == nullptr) {
+            return cuvit::host::fail(CUVIT_INVALID_ARGUMENT, "rotary axes cannot be null");
+        }
+        return cuvit::rotary::run(q, k, q_out, k_out, nullptr, positions, rotary, problem,
+                                  reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+int cuvit_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out,
+                         const cuvit_qk_norm* norm, const int32_t* positions,
+                         const cuvit_rotary* rotary, const cuvit_qk_problem* problem,
+                         cuvit_stream_t stream) {
+    return cuvit::host::guarded([&]() {
+        if (norm == nullptr) {
+            return cuvit::host::fail(CUVIT_INVALID_ARGUMENT, "the norm cannot be null");
+        }
+        return cuvit::rotary::run(q, k, q_out, k_out, norm, positions, rotary, problem,
+                                  reinterpret_cast<cudaStream_t>(stream));
+    });
+}
+
+} // extern "C"

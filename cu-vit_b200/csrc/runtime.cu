@@ -170,6 +170,47 @@ DependentLaunch::DependentLaunch(bool enable) : previous_(t_dependent_launch) {
 
 DependentLaunch::~DependentLaunch() { t_dependent_launch = previous_; }
 
+int check_operands(std::initializer_list<const void*> operands) {
+    int device = 0;
+    CUVIT_TRY_CUDA(cudaGetDevice(&device));
+    for (const void* operand : operands) {
+        if (operand == nullptr) {
+            continue;
+        }
+        cudaPointerAttributes attributes{};
+        CUVIT_TRY_CUDA(cudaPointerGetAttributes(&attributes, operand));
+        if (attributes.type == cudaMemoryTypeUnregistered) {
+            return fail(CUVIT_INVALID_ARGUMENT, "an operand is not device memory");
+        }
+        if (attributes.type == cudaMemoryTypeDevice && attributes.device != device) {
+            return fail(CUVIT_INVALID_ARGUMENT,
+                        "an operand is in the memory of another device than the current one");
+        }
+    }
+    return CUVIT_OK;
+}
+
+bool rows_overlap(const RowSpan& a, const RowSpan& b) {
+    if (a.rows <= 0 || b.rows <= 0 || a.width_bytes <= 0 || b.width_bytes <= 0) {
+        return false;
+    }
+    const auto a0 = reinterpret_cast<uintptr_t>(a.base);
+    const auto b0 = reinterpret_cast<uintptr_t>(b.base);
+    const uintptr_t a1 = a0 + static_cast<uintptr_t>((a.rows - 1) * a.stride_bytes + a.width_bytes);
+    const uintptr_t b1 = b0 + static_cast<uintptr_t>((b.rows - 1) * b.stride_bytes + b.width_bytes);
+    if (a1 <= b0 || b1 <= a0) {
+        return false;
+    }
+    if (a.stride_bytes != b.stride_bytes || a.stride_bytes <= 0) {
+        return true;
+    }
+    // b's first column within a's rows.
+    const int64_t stride = a.stride_bytes;
+    const int64_t difference = static_cast<int64_t>(b0 - a0) % stride;
+    const int64_t column = difference < 0 ? difference + stride : difference;
+    return column < a.width_bytes || column + b.width_bytes > stride;
+}
+
 int tensor_map_encoder(TensorMapEncodeFn* function) {
     static TensorMapEncodeFn cached = nullptr;
     static std::once_flag once;

@@ -10,6 +10,7 @@
 
 #include <cstdint>
 #include <functional>
+#include <initializer_list>
 #include <string>
 #include <utility>
 
@@ -124,6 +125,33 @@ cudaError_t once_per_device(const void* key, const std::function<cudaError_t(int
 // Raises kernel's dynamic shared-memory limit to `bytes` on the current device (once per
 // device).
 cudaError_t allow_dynamic_smem(const void* kernel, int bytes);
+
+// Refuses (CUVIT_INVALID_ARGUMENT) operands the current device does not hold: memory of another
+// device, or host memory CUDA does not know. Null entries are skipped.
+int check_operands(std::initializer_list<const void*> operands);
+
+// A matrix of `rows` rows of width_bytes, stride_bytes apart.
+struct RowSpan {
+    const void* base;
+    int64_t rows;
+    int64_t width_bytes;
+    int64_t stride_bytes;
+};
+
+// Whether two row matrices may share a byte: exact for equal strides (interleaved columns of one
+// buffer do not), else by their address ranges.
+bool rows_overlap(const RowSpan& a, const RowSpan& b);
+
+// Runs an entry point's body, turning a C++ exception (an allocation that failed while a
+// message was built) into CUVIT_OUT_OF_MEMORY instead of letting it cross the C ABI.
+template <typename Body>
+int guarded(const Body& body) noexcept {
+    try {
+        return body();
+    } catch (...) {
+        return CUVIT_OUT_OF_MEMORY;
+    }
+}
 
 using TensorMapEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                        const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,

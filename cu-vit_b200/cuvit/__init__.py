@@ -8,10 +8,12 @@ from . import cvw, errors, kernels
 from ._lib import LIBRARY_PATH, library
 from .errors import (CudaError, CuvitError, DeviceTimeout, InvalidArgument, LengthError,
                      Unsupported, WeightError)
-from .kernels import (GemmBatch, GemmEpilogue, GemmProblem, gemm_problem, launch_add,
-                      launch_add_broadcast, launch_attention, launch_broadcast,
-                      launch_extract_patches, launch_gelu, launch_gemm, launch_gemm_ex,
-                      launch_layer_norm, launch_softmax)
+from .kernels import (AttentionProblem, GemmBatch, GemmEpilogue, GemmProblem, LinearProblem,
+                      QkNorm, QkProblem, attention_varlen_workspace, gemm_problem, launch_add,
+                      launch_add_broadcast, launch_attention, launch_attention_varlen,
+                      launch_broadcast, launch_extract_patches, launch_gelu, launch_gemm,
+                      launch_gemm_ex, launch_layer_norm, launch_linear, launch_qk_norm_rotary,
+                      launch_rotary, launch_softmax, rotary_axes)
 from .vit import (PRECISION_BF16, PRECISION_FP32, PRECISION_TF32, VisionTransformer, VitConfig,
                   random_weights, tensor_specs)
 
@@ -21,6 +23,9 @@ __all__ = [
     "WeightError", "GemmBatch", "GemmEpilogue", "GemmProblem", "gemm_problem", "launch_add",
     "launch_add_broadcast", "launch_attention", "launch_broadcast", "launch_extract_patches",
     "launch_gelu", "launch_gemm", "launch_gemm_ex", "launch_layer_norm", "launch_softmax",
+    "AttentionProblem", "LinearProblem", "QkNorm", "QkProblem", "attention_varlen_workspace",
+    "launch_attention_varlen", "launch_linear", "launch_qk_norm_rotary", "launch_rotary",
+    "rotary_axes",
     "PRECISION_BF16", "PRECISION_FP32", "PRECISION_TF32", "VisionTransformer", "VitConfig",
     "random_weights", "tensor_specs",
 ]

@@ -34,6 +34,18 @@ DTYPE_TF32 = 2
 MATH_FP32 = 0
 MATH_TF32 = 1
 MATH_BF16 = 2
+ROTARY_HALVES = 0
+ROTARY_ADJACENT = 1
+ROTARY_LADDER_AXIS = 0
+ROTARY_LADDER_SHARED = 1
+ROTARY_MAX_AXES = 4
+ROTARY_MAX_PAIRS = 128
+NORM_RMS = 0
+NORM_LAYER = 1
+ACTIVATION_NONE = 0
+ACTIVATION_GELU = 1
+ACTIVATION_GELU_TANH = 2
+ACTIVATION_SILU = 3
 
 
 class GemmBatchC(ctypes.Structure):
@@ -97,6 +109,37 @@ class PreprocessingC(ctypes.Structure):
                 ("mean", ctypes.c_float * 3), ("stddev", ctypes.c_float * 3)]
 
 
+class RotaryC(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int), ("pairing", ctypes.c_int),
+                ("first", ctypes.c_int * (ROTARY_MAX_AXES + 1)),
+                ("turns", ctypes.c_uint64 * ROTARY_MAX_PAIRS)]
+
+
+class QkProblemC(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "tokens", "q_heads", "k_heads", "head_dim", "dtype")] + [
+            (name, ctypes.c_int64) for name in (
+                "q_stride", "k_stride", "q_out_stride", "k_out_stride", "position_stride")]
+
+
+class QkNormC(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("epsilon", ctypes.c_float)] + [
+        (name, ctypes.c_void_p) for name in ("q_gamma", "q_beta", "k_gamma", "k_beta")]
+
+
+class AttentionProblemC(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "batch", "q_tokens", "kv_tokens", "q_heads", "kv_heads", "head_dim", "dtype",
+        "causal")] + [("scale", ctypes.c_float)] + [
+            (name, ctypes.c_int64) for name in (
+                "q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class LinearProblemC(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int) for name in (
+        "m", "n", "k", "math", "out_dtype", "activation", "gated", "ldx", "ldw", "ldr", "ldo")]
+
+
 class TimelineRecordC(ctypes.Structure):
     _fields_ = [(name, ctypes.c_ulonglong) for name in (
         "grid", "first_ns", "last_ns", "warps", "cta0_entry_ns", "cta0_exit_ns",
@@ -137,6 +180,17 @@ SIGNATURES = {
     "cuvit_round_to_tf32": (_i, [_vp, _vp, _i64, _vp]),
     "cuvit_logits_top_k": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "cuvit_attention": (_i, [_vp, _vp, _i, _i, _i, _i, _i, _f, _vp]),
+    "cuvit_rotary_init": (_i, [ctypes.POINTER(RotaryC), _i, ctypes.POINTER(_i),
+                               ctypes.c_double, _i, _i]),
+    "cuvit_rotary_qk": (_i, [_vp, _vp, _vp, _vp, _vp, ctypes.POINTER(RotaryC),
+                             ctypes.POINTER(QkProblemC), _vp]),
+    "cuvit_qk_norm_rotary": (_i, [_vp, _vp, _vp, _vp, ctypes.POINTER(QkNormC), _vp,
+                                  ctypes.POINTER(RotaryC), ctypes.POINTER(QkProblemC), _vp]),
+    "cuvit_attention_varlen": (_i, [_vp, _vp, _vp, _vp, _vp, _vp,
+                                    ctypes.POINTER(AttentionProblemC), _vp, _sz, _vp]),
+    "cuvit_attention_varlen_workspace": (_i, [ctypes.POINTER(AttentionProblemC),
+                                              ctypes.POINTER(_sz)]),
+    "cuvit_linear": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(LinearProblemC), _vp]),
     "cuvit_device_status": (_i, [ctypes.POINTER(ctypes.c_uint)]),
     "cuvit_launch_count": (ctypes.c_longlong, []),
     "cuvit_selftest_bounded_wait": (_i, [ctypes.c_ulonglong]),

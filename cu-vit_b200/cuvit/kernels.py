@@ -24,6 +24,16 @@ DTYPE_TF32 = _lib.DTYPE_TF32
 MATH_FP32 = _lib.MATH_FP32
 MATH_TF32 = _lib.MATH_TF32
 MATH_BF16 = _lib.MATH_BF16
+ROTARY_HALVES = _lib.ROTARY_HALVES
+ROTARY_ADJACENT = _lib.ROTARY_ADJACENT
+ROTARY_LADDER_AXIS = _lib.ROTARY_LADDER_AXIS
+ROTARY_LADDER_SHARED = _lib.ROTARY_LADDER_SHARED
+NORM_RMS = _lib.NORM_RMS
+NORM_LAYER = _lib.NORM_LAYER
+ACTIVATION_NONE = _lib.ACTIVATION_NONE
+ACTIVATION_GELU = _lib.ACTIVATION_GELU
+ACTIVATION_GELU_TANH = _lib.ACTIVATION_GELU_TANH
+ACTIVATION_SILU = _lib.ACTIVATION_SILU
 
 
 def _ptr(value) -> ctypes.c_void_p:
@@ -225,6 +235,162 @@ def launch_preprocess(pixels, tensor, batch: int, width: int, height: int, size:
     check(_lib.library().cuvit_preprocess(_ptr(pixels), batch, width, height, image_stride,
                                           ctypes.byref(settings), _ptr(tensor),
                                           _stream(stream)))
+
+
+# ---- encoder blocks over packed images and videos ------------------------------------------
+
+
+@dataclasses.dataclass
+class QkProblem:
+    """cuvit_qk_problem: queries [tokens, q_heads, head_dim] and keys [tokens, k_heads,
+    head_dim], strides in elements between tokens (0 = packed)."""
+
+    tokens: int = 0
+    q_heads: int = 0
+    k_heads: int = 0
+    head_dim: int = 0
+    dtype: int = DTYPE_BF16
+    q_stride: int = 0
+    k_stride: int = 0
+    q_out_stride: int = 0
+    k_out_stride: int = 0
+    position_stride: int = 0
+
+    def to_c(self) -> _lib.QkProblemC:
+        return _lib.QkProblemC(self.tokens, self.q_heads, self.k_heads, self.head_dim, self.dtype,
+                               self.q_stride, self.k_stride, self.q_out_stride,
+                               self.k_out_stride, self.position_stride)
+
+
+@dataclasses.dataclass
+class QkNorm:
+    """cuvit_qk_norm: per-head norms; gains and offsets are float32 [head_dim] device arrays
+    shared by a side's heads, None for 1 and 0."""
+
+    kind: int = NORM_RMS
+    epsilon: float = 1.0e-6
+    q_gamma: object = None
+    q_beta: object = None
+    k_gamma: object = None
+    k_beta: object = None
+
+    def to_c(self) -> _lib.QkNormC:
+        return _lib.QkNormC(self.kind, self.epsilon, _ptr(self.q_gamma), _ptr(self.q_beta),
+                            _ptr(self.k_gamma), _ptr(self.k_beta))
+
+
+@dataclasses.dataclass
+class AttentionProblem:
+    """cuvit_attention_problem: packed sequences, strides in elements between rows
+    (0 = packed)."""
+
+    batch: int = 0
+    q_tokens: int = 0
+    kv_tokens: int = 0
+    q_heads: int = 0
+    kv_heads: int = 0
+    head_dim: int = 0
+    dtype: int = DTYPE_BF16
+    causal: bool = False
+    scale: float = 1.0
+    q_stride: int = 0
+    k_stride: int = 0
+    v_stride: int = 0
+    out_stride: int = 0
+
+    def to_c(self) -> _lib.AttentionProblemC:
+        return _lib.AttentionProblemC(self.batch, self.q_tokens, self.kv_tokens, self.q_heads,
+                                      self.kv_heads, self.head_dim, self.dtype,
+                                      int(self.causal), self.scale, self.q_stride,
+                                      self.k_stride, self.v_stride, self.out_stride)
+
+
+@dataclasses.dataclass
+class LinearProblem:
+    """cuvit_linear_problem: x [m, k], weight [n, k] (gated: [2n, k], gate rows first)."""
+
+    m: int = 0
+    n: int = 0
+    k: int = 0
+    math: int = MATH_BF16
+    out_dtype: int = DTYPE_BF16
+    activation: int = ACTIVATION_NONE
+    gated: bool = False
+    ldx: int = 0
+    ldw: int = 0
+    ldr: int = 0
+    ldo: int = 0
+
+    def to_c(self) -> _lib.LinearProblemC:
+        return _lib.LinearProblemC(self.m, self.n, self.k, self.math, self.out_dtype,
+                                   self.activation, int(self.gated), self.ldx, self.ldw, self.ldr,
+                                   self.ldo)
+
+
+def rotary_axes(sections, base: float = 10000.0, pairing: int = ROTARY_HALVES,
+                ladder: int = ROTARY_LADDER_AXIS) -> _lib.RotaryC:
+    """The rotation plan of position axes turning sections[a] pairs each, made once and passed
+    to launch_rotary / launch_qk_norm_rotary."""
+    rotary = _lib.RotaryC()
+    sections = list(sections)
+    check(_lib.library().cuvit_rotary_init(ctypes.byref(rotary), len(sections),
+                                           (ctypes.c_int * len(sections))(*sections), base,
+                                           pairing, ladder))
+    return rotary
+
+
+def _optional(value):
+    return None if value is None else ctypes.byref(value)
+
+
+def launch_rotary(q, k, q_out, k_out, positions, rotary: _lib.RotaryC, problem: QkProblem,
+                  stream=None) -> None:
+    """Turns query and key pairs by their positions (int32 [axes, tokens])."""
+    p = problem.to_c()
+    check(_lib.library().cuvit_rotary_qk(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out),
+                                         _ptr(positions), _optional(rotary), ctypes.byref(p),
+                                         _stream(stream)))
+
+
+def launch_qk_norm_rotary(q, k, q_out, k_out, norm: QkNorm, positions,
+                          rotary: _lib.RotaryC | None, problem: QkProblem, stream=None) -> None:
+    """Per-head norms of queries and keys, then (rotary not None) the rotation, in one pass."""
+    p = problem.to_c()
+    n = norm.to_c()
+    check(_lib.library().cuvit_qk_norm_rotary(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out),
+                                              ctypes.byref(n), _ptr(positions),
+                                              _optional(rotary), ctypes.byref(p),
+                                              _stream(stream)))
+
+
+def attention_varlen_workspace(problem: AttentionProblem) -> int:
+    """Bytes of workspace with which launch_attention_varlen may split long key ranges (0: the
+    problem is not split)."""
+    p = problem.to_c()
+    size = ctypes.c_size_t(0)
+    check(_lib.library().cuvit_attention_varlen_workspace(ctypes.byref(p), ctypes.byref(size)))
+    return size.value
+
+
+def launch_attention_varlen(q, k, v, out, q_offsets, kv_offsets, problem: AttentionProblem,
+                            workspace=None, workspace_bytes: int = 0, stream=None) -> None:
+    """Attention over packed sequences given by int32 device offsets [batch + 1]; kv_offsets
+    None: the queries' own."""
+    p = problem.to_c()
+    check(_lib.library().cuvit_attention_varlen(_ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                                                _ptr(q_offsets), _ptr(kv_offsets),
+                                                ctypes.byref(p), _ptr(workspace),
+                                                workspace_bytes, _stream(stream)))
+
+
+def launch_linear(x, weight, bias, scale, residual, out, problem: LinearProblem,
+                  stream=None) -> None:
+    """out = residual + scale * activation(x weight^T + bias), with a gate when gated; bias,
+    scale and residual may be None."""
+    p = problem.to_c()
+    check(_lib.library().cuvit_linear(_ptr(x), _ptr(weight), _ptr(bias), _ptr(scale),
+                                      _ptr(residual), _ptr(out), ctypes.byref(p),
+                                      _stream(stream)))
 
 
 def device_status() -> int:

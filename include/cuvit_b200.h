@@ -261,6 +261,169 @@ int cuvit_preprocess(const uint8_t* pixels, int batch, int width, int height,
 int cuvit_attention(const void* qkv, void* context, int dtype, int batch, int tokens,
                     int heads, int head_dim, float scale, cuvit_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Encoder blocks over packed images and videos of any size (no reference counterpart: the
+ * reference's images all have one size, its positions are a learned table and its norms span
+ * the whole embedding). Rows of several images stand one behind another in one matrix; the
+ * operators below turn and normalise queries and keys, attend within each image, and run the
+ * linear layers around them. Like the rest of the ABI they allocate nothing, check their
+ * arguments on the host before any launch, and work on the current device: an operand that the
+ * current device does not hold (memory of another GPU, pageable host memory) is refused with
+ * CUVIT_INVALID_ARGUMENT.
+ * ------------------------------------------------------------------------------------- */
+
+/* Which elements of a head's first 2 * pairs elements turn together. */
+typedef enum cuvit_rotary_pairing {
+    CUVIT_ROTARY_HALVES = 0,  /* element i with element i + pairs */
+    CUVIT_ROTARY_ADJACENT = 1 /* element 2i with element 2i + 1 */
+} cuvit_rotary_pairing;
+
+/* The angular rate of pair j (0-based) of an axis with s pairs, the axis starting at pair f of
+ * the P pairs of all axes. */
+typedef enum cuvit_rotary_ladder {
+    CUVIT_ROTARY_LADDER_AXIS = 0,  /* base^(-j / s): each axis runs through all rates */
+    CUVIT_ROTARY_LADDER_SHARED = 1 /* base^(-(f + j) / P): the axes share one ladder */
+} cuvit_rotary_ladder;
+
+#define CUVIT_ROTARY_MAX_AXES 4
+#define CUVIT_ROTARY_MAX_PAIRS 128
+
+/* How positions turn pairs; filled by cuvit_rotary_init() and kept by the caller. Axis a turns
+ * pairs first[a] .. first[a + 1] - 1. turns[i] is pair i's rate in units of 2^-64 of a full
+ * turn per step, so that position * turns[i] modulo 2^64 is the angle's fraction of a turn,
+ * exact for every 32-bit position. */
+typedef struct cuvit_rotary {
+    int axes;
+    int pairing; /* cuvit_rotary_pairing */
+    int first[CUVIT_ROTARY_MAX_AXES + 1];
+    uint64_t turns[CUVIT_ROTARY_MAX_PAIRS];
+} cuvit_rotary;
+
+/* axes in 1..4 with sections[a] >= 0 pairs each, 1 to 128 in all; base finite and >= 1. */
+int cuvit_rotary_init(cuvit_rotary* rotary, int axes, const int* sections, double base,
+                      int pairing, int ladder);
+
+/* Queries [tokens, q_heads, head_dim] and keys [tokens, k_heads, head_dim], each token's heads
+ * contiguous and tokens *_stride elements apart (0 = packed). Either may have no heads.
+ * head_dim is even, 2..256; positions are [axes][tokens], axes position_stride apart
+ * (0 = tokens). */
+typedef struct cuvit_qk_problem {
+    int tokens;
+    int q_heads;
+    int k_heads;
+    int head_dim;
+    int dtype; /* CUVIT_DTYPE_F32 or CUVIT_DTYPE_BF16, inputs and outputs */
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t q_out_stride;
+    int64_t k_out_stride;
+    int64_t position_stride;
+} cuvit_qk_problem;
+
+/* Turns pair (x, y) of every head of token t by the angle positions[a][t] * rate:
+ * (x cos - y sin, x sin + y cos), in FP32 with one rounding at the store; elements past the
+ * rotated pairs are copied. An output may be its own input (same pointer and stride); any other
+ * overlap is refused. */
+int cuvit_rotary_qk(const void* q, const void* k, void* q_out, void* k_out,
+                    const int32_t* positions, const cuvit_rotary* rotary,
+                    const cuvit_qk_problem* problem, cuvit_stream_t stream);
+
+typedef enum cuvit_norm_kind {
+    CUVIT_NORM_RMS = 0,  /* x / sqrt(mean(x^2) + eps) * gamma + beta */
+    CUVIT_NORM_LAYER = 1 /* (x - mean) / sqrt(var + eps) * gamma + beta, biased variance */
+} cuvit_norm_kind;
+
+/* Norms over each head's head_dim elements; the float [head_dim] gains and offsets are shared
+ * by the heads of a side and may be null (1 and 0). */
+typedef struct cuvit_qk_norm {
+    int kind; /* cuvit_norm_kind */
+    float epsilon;
+    const float* q_gamma;
+    const float* q_beta;
+    const float* k_gamma;
+    const float* k_beta;
+} cuvit_qk_norm;
+
+/* The norm of each query and key head, then the rotation of cuvit_rotary_qk, in one pass (the
+ * normalised values stay in FP32 until the store). rotary may be null: norm alone. */
+int cuvit_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out,
+                         const cuvit_qk_norm* norm, const int32_t* positions,
+                         const cuvit_rotary* rotary, const cuvit_qk_problem* problem,
+                         cuvit_stream_t stream);
+
+/* Attention over packed sequences. Sequence b has query rows q_offsets[b] .. q_offsets[b+1]-1
+ * and key / value rows kv_offsets[b] .. kv_offsets[b+1]-1 of the packed matrices; both arrays
+ * are device int32 [batch + 1], not decreasing, within 0 .. q_tokens / kv_tokens. (The kernels
+ * clamp offsets into that range, so wrong ones give wrong rows but no access outside the
+ * operands.) Rows are heads of head_dim contiguous elements, *_stride elements apart
+ * (0 = packed); query head h reads key head h / (q_heads / kv_heads). */
+typedef struct cuvit_attention_problem {
+    int batch;
+    int q_tokens;
+    int kv_tokens;
+    int q_heads;
+    int kv_heads; /* divides q_heads */
+    int head_dim; /* 1..128 */
+    int dtype;    /* CUVIT_DTYPE_F32 or CUVIT_DTYPE_BF16 */
+    int causal;   /* query i of n sees keys j <= i + (keys - n): aligned at the ends */
+    float scale;  /* finite and > 0 */
+    int64_t q_stride;
+    int64_t k_stride;
+    int64_t v_stride;
+    int64_t out_stride;
+} cuvit_attention_problem;
+
+/* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] per head, over the keys query i sees; a
+ * query that sees none gets zeros. Softmax statistics and sums are FP32; BF16 rounds the
+ * weights to bfloat16 for the product with v, F32 is FP32 throughout. Rows of out outside every
+ * sequence are not written, and rows of q, k and v outside a sequence may hold anything, NaN
+ * included, without reaching it. (Within a sequence a causal query's weight for a later key is
+ * zero, but zero times a NaN or infinite value is NaN, as in the plain product.) kv_offsets null: q_offsets (self-attention). out must not
+ * overlap q, k or v.
+ * The workspace (device, 16-byte aligned, cuvit_attention_varlen_workspace() bytes, contents
+ * irrelevant before and after) lets calls with few query rows split long key ranges over the
+ * whole GPU; calls that may run at the same time need one each. Null: no split. */
+int cuvit_attention_varlen(const void* q, const void* k, const void* v, void* out,
+                           const int32_t* q_offsets, const int32_t* kv_offsets,
+                           const cuvit_attention_problem* problem, void* workspace,
+                           size_t workspace_bytes, cuvit_stream_t stream);
+
+/* Workspace of a problem on the current device, 0 where it is not split. */
+int cuvit_attention_varlen_workspace(const cuvit_attention_problem* problem, size_t* bytes);
+
+typedef enum cuvit_activation {
+    CUVIT_ACTIVATION_NONE = 0,
+    CUVIT_ACTIVATION_GELU = 1,      /* x Phi(x), the erf form */
+    CUVIT_ACTIVATION_GELU_TANH = 2, /* x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2 */
+    CUVIT_ACTIVATION_SILU = 3       /* x / (1 + exp(-x)) */
+} cuvit_activation;
+
+/* A linear layer: x [m, k], weight [n, k] (gated: [2n, k], gate rows first), out and residual
+ * [m, n]; ld* are row distances in elements, 0 = packed. */
+typedef struct cuvit_linear_problem {
+    int m;
+    int n;
+    int k;
+    int math;       /* CUVIT_MATH_BF16: bfloat16 x and weight; CUVIT_MATH_FP32 / TF32: float */
+    int out_dtype;  /* cuvit_dtype of out, and the storage type of residual */
+    int activation; /* cuvit_activation */
+    int gated;
+    int ldx;
+    int ldw;
+    int ldr;
+    int ldo;
+} cuvit_linear_problem;
+
+/* y = x weight^T + bias (FP32 accumulation), then
+ *   out = residual + scale * activation(y)                        plain
+ *   out = residual + scale * activation(y[:, :n]) * y[:, n:]      gated
+ * with one rounding at the store. bias float [n] (gated [2n]), scale float [n] and residual may
+ * be null. out may be residual itself (same pointer and row distance); any other overlap of
+ * out with an operand is refused. */
+int cuvit_linear(const void* x, const void* weight, const float* bias, const float* scale,
+                 const void* residual, void* out, const cuvit_linear_problem* problem,
+                 cuvit_stream_t stream);
+
 /* Reads and clears the device status word of the current device, after synchronizing it.
  * *flags receives the bits set since the last call (0 = clean). Returns
  * CUVIT_DEVICE_TIMEOUT when a kernel gave up on a bounded wait.

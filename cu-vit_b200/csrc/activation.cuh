@@ -32,4 +32,77 @@ __device__ __forceinline__ float activate_exact(int activation, float x) {
     }
 }
 
+// ---- for bfloat16 outputs: errors far below the store's 2^-9 -------------------------------
+
+// 1 / (1 + 2^t) with the hardware's exponential and reciprocal (2^-21 relative).
+__device__ __forceinline__ float logistic_of_exp2(float t) {
+    return rcp_approx(1.0F + ex2_approx(t));
+}
+
+__device__ __forceinline__ float silu_fast(float x) {
+    return x * logistic_of_exp2(-1.4426950408889634F * x);
+}
+
+__device__ __forceinline__ float gelu_tanh_fast(float x) {
+    // exp(-2u) with 2 sqrt(2/pi) log2(e) folded into the cubic.
+    const float x2 = x * x;
+    return x * logistic_of_exp2(x * fmaf(-0.1029432397F, x2, -2.3022081985F));
+}
+
+// x Phi(x) = max(x, 0) - |x| Q(|x|), Q(z) = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) t P(t) with
+// t = 1 / (1 + 0.375 z) and P of degree 4, fitted here for minimax relative error on [0, 13.5]
+// (2.9e-5 in FP32; beyond, Q is below the smallest float). Two values, the multiply-adds packed.
+__device__ __forceinline__ float2 gelu_fast2(float x0, float x1) {
+    const float m0 = fabsf(x0);
+    const float m1 = fabsf(x1);
+    const uint64_t m = f32x2(m0, m1);
+    const float2 den = f32x2_split(fma_f32x2(f32x2(0.375F, 0.375F), m, f32x2(1.0F, 1.0F)));
+    const uint64_t t = f32x2(rcp_approx(den.x), rcp_approx(den.y));
+    // The polynomial's negative, so that its product is added to max(x, 0).
+    uint64_t poly = fma_f32x2(t, f32x2(0.0909852013F, 0.0909852013F),
+                              f32x2(-0.201043248F, -0.201043248F));
+    poly = fma_f32x2(t, poly, f32x2(-0.0829740912F, -0.0829740912F));
+    poly = fma_f32x2(t, poly, f32x2(-0.157920063F, -0.157920063F));
+    poly = fma_f32x2(t, poly, f32x2(-0.149041131F, -0.149041131F));
+    poly = mul_f32x2(poly, mul_f32x2(m, t));
+    const uint64_t x = f32x2(x0, x1);
+    constexpr float kHalfLog2e = -0.5F * 1.4426950408889634F;
+    const float2 arg = f32x2_split(mul_f32x2(x, mul_f32x2(x, f32x2(kHalfLog2e, kHalfLog2e))));
+    const uint64_t tail = f32x2(ex2_approx(arg.x), ex2_approx(arg.y));
+    return f32x2_split(fma_f32x2(poly, tail, f32x2(fmaxf(x0, 0.0F), fmaxf(x1, 0.0F))));
+}
+
+// The activation on N values: the forms above (Fast), or the exact ones.
+template <bool Fast, int N>
+__device__ __forceinline__ void activate(int activation, float (&v)[N]) {
+    if (activation == CUVIT_ACTIVATION_NONE) {
+        return;
+    }
+    if constexpr (Fast) {
+        if (activation == CUVIT_ACTIVATION_SILU) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[j] = silu_fast(v[j]);
+            }
+        } else if (activation == CUVIT_ACTIVATION_GELU) {
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const float2 g = gelu_fast2(v[j], v[j + 1]);
+                v[j] = g.x;
+                v[j + 1] = g.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                v[j] = gelu_tanh_fast(v[j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = activate_exact(activation, v[j]);
+        }
+    }
+}
+
 } // namespace cuvit::dev

@@ -1,0 +1,447 @@
+// Attention of a few query rows per sequence over many keys (pooling by one query, one new token
+// of each sequence), and the kernel that joins the parts of calls that split their keys.
+//
+// Bound by HBM: every key and value is used for a handful of multiply-adds per byte. A group of
+// lanes holds one key at a time, 16 bytes a lane (the query rows' same elements stay in
+// registers), and keeps its own running maximum, sum and output for its share of the keys, so
+// the only exchange while streaming is the butterfly of each score; groups, warps and splits are
+// merged at the end. Rows that share a key head (grouped heads, several queries) are taken
+// together, so keys are read once for them.
+#include "attention_varlen.hpp"
+#include "ptx.cuh"
+#include "varlen.cuh"
+
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+namespace cuvit::attn {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+// Keys a lane group has in flight (registers bound it: 8 rows hold 64 of queries and 64 of output).
+template <int Rows>
+constexpr int kUnrollOf = Rows >= 8 ? 2 : 4;
+
+// One lane's 16 bytes of a row as floats.
+template <typename T>
+struct Lane {
+    static constexpr int kElems = 16 / sizeof(T);
+
+    static __device__ __forceinline__ uint4 load(const T* p) {
+        return __ldg(reinterpret_cast<const uint4*>(p));
+    }
+
+    static __device__ __forceinline__ void unpack(const uint4& raw, float (&out)[kElems]) {
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                out[2 * i] = __uint_as_float(words[i] << 16);
+                out[2 * i + 1] = __uint_as_float(words[i] & 0xFFFF0000u);
+            } else {
+                out[i] = __uint_as_float(words[i]);
+            }
+        }
+    }
+};
+
+// Merges (m, l, o) with another part's; a part without a key has m = -inf and l = 0.
+__device__ __forceinline__ void merge_factors(float m, float other, float& top, float& mine,
+                                              float& theirs) {
+    top = fmaxf(m, other);
+    const float base = top == -INFINITY ? 0.0F : top;
+    mine = exp2f(m - base);
+    theirs = exp2f(other - base);
+}
+
+template <typename T, int Lanes, int Rows>
+__global__ void __launch_bounds__(kThreads)
+    attention_rows_kernel(const VarlenParams p, int queries_per_block, int head_chunks) {
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+    constexpr int kElems = Lane<T>::kElems;
+    constexpr int kUnroll = kUnrollOf<Rows>;
+    constexpr int kGroups = kThreads / Lanes; // key streams of the block
+    __shared__ float merged_out[kWarps][Rows][Lanes * kElems];
+    __shared__ float2 merged_stats[kWarps][Rows];
+
+    // Item: block of queries, key head, chunk of its query heads, split (fastest: the splits of
+    // one range run together).
+    long long item = blockIdx.x;
+    const int split = static_cast<int>(item % p.splits);
+    item /= p.splits;
+    const int chunk = static_cast<int>(item % head_chunks);
+    item /= head_chunks;
+    const int kv_head = static_cast<int>(item % p.kv_heads);
+    const Sequence s = find_block(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
+                                  item / p.kv_heads, queries_per_block);
+    if (s.index < 0) {
+        return;
+    }
+    const int heads = min(Rows / queries_per_block, p.group - chunk * (Rows / queries_per_block));
+    const int head0 = kv_head * p.group + chunk * (Rows / queries_per_block);
+    const int queries = min(queries_per_block, s.q_end - s.q_first);
+    const int rows = heads * queries; // row r: query r / heads, head r % heads
+    const int keys = s.kv_end - s.kv_begin;
+    int first_key, end_key;
+    split_keys(keys, split, p.splits, first_key, end_key);
+
+    const int lane = threadIdx.x % Lanes;
+    const int group = threadIdx.x / Lanes;
+    const int element = lane * kElems;
+    const bool in_row = element < p.head_dim;
+
+    float q[Rows][kElems];
+    int limit[Rows]; // keys row r sees
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        const int query = r / heads;
+        const int head = head0 + r - query * heads;
+#pragma unroll
+        for (int j = 0; j < kElems; ++j) {
+            q[r][j] = 0.0F;
+        }
+        limit[r] = 0;
+        if (r < rows) {
+            if (in_row) {
+                Lane<T>::unpack(Lane<T>::load(static_cast<const T*>(p.q) +
+                                              (s.q_first + query) * p.q_stride +
+                                              static_cast<long long>(head) * p.head_dim + element),
+                                q[r]);
+            }
+#pragma unroll
+            for (int j = 0; j < kElems; ++j) {
+                q[r][j] *= p.scale_log2;
+            }
+            const long long last = static_cast<long long>(s.q_first - s.q_begin) + query + 1 +
+                                   keys - (s.q_end - s.q_begin);
+            limit[r] = p.causal ? static_cast<int>(max(
+                                      0LL, min(static_cast<long long>(end_key), last)))
+                                : end_key;
+        }
+    }
+    const T* const k = static_cast<const T*>(p.k) + s.kv_begin * p.k_stride +
+                       static_cast<long long>(kv_head) * p.head_dim + element;
+    const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
+                       static_cast<long long>(kv_head) * p.head_dim + element;
+
+    float o[Rows][kElems] = {};
+    float top[Rows], sum[Rows];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        top[r] = -INFINITY;
+        sum[r] = 0.0F;
+    }
+    // Whole warps go round together (the butterflies need every lane).
+    const int warp_group0 = (threadIdx.x / 32) * (32 / Lanes);
+    for (int base = first_key; base + warp_group0 < end_key; base += kGroups * kUnroll) {
+        uint4 k_raw[kUnroll], v_raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int key = base + u * kGroups + group;
+            const bool live = key < end_key && in_row;
+            k_raw[u] = live ? Lane<T>::load(k + key * p.k_stride) : make_uint4(0, 0, 0, 0);
+            v_raw[u] = live ? Lane<T>::load(v + key * p.v_stride) : make_uint4(0, 0, 0, 0);
+        }
+        float score[Rows][kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float kf[kElems];
+            Lane<T>::unpack(k_raw[u], kf);
+#pragma unroll
+            for (int r = 0; r < Rows; ++r) {
+                float dot = 0.0F;
+#pragma unroll
+                for (int j = 0; j < kElems; ++j) {
+                    dot = fmaf(q[r][j], kf[j], dot);
+                }
+                score[r][u] = dot;
+            }
+        }
+#pragma unroll
+        for (int offset = Lanes / 2; offset > 0; offset /= 2) {
+#pragma unroll
+            for (int r = 0; r < Rows; ++r) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    score[r][u] += __shfl_xor_sync(0xFFFFFFFFu, score[r][u], offset);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < Rows; ++r) {
+            float raised = top[r];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const int key = base + u * kGroups + group;
+                score[r][u] = key < limit[r] ? score[r][u] : -INFINITY;
+                raised = fmaxf(raised, score[r][u]);
+            }
+            // Without a key so far, any finite stand-in keeps 2^(-inf - m) at zero.
+            const float stand = raised == -INFINITY ? 0.0F : raised;
+            const float factor = exp2f(top[r] - stand);
+            top[r] = raised;
+            sum[r] *= factor;
+#pragma unroll
+            for (int j = 0; j < kElems; ++j) {
+                o[r][j] *= factor;
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                score[r][u] = exp2f(score[r][u] - stand);
+                sum[r] += score[r][u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float vf[kElems];
+            Lane<T>::unpack(v_raw[u], vf);
+#pragma unroll
+            for (int r = 0; r < Rows; ++r) {
+#pragma unroll
+                for (int j = 0; j < kElems; ++j) {
+                    o[r][j] = fmaf(score[r][u], vf[j], o[r][j]);
+                }
+            }
+        }
+    }
+
+    // Lane groups of a warp, then the warps, in a fixed order.
+#pragma unroll
+    for (int offset = Lanes; offset < 32; offset *= 2) {
+#pragma unroll
+        for (int r = 0; r < Rows; ++r) {
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, top[r], offset);
+            const float other_sum = __shfl_xor_sync(0xFFFFFFFFu, sum[r], offset);
+            float raised, mine, theirs;
+            merge_factors(top[r], other, raised, mine, theirs);
+            top[r] = raised;
+            sum[r] = sum[r] * mine + other_sum * theirs;
+#pragma unroll
+            for (int j = 0; j < kElems; ++j) {
+                const float other_o = __shfl_xor_sync(0xFFFFFFFFu, o[r][j], offset);
+                o[r][j] = o[r][j] * mine + other_o * theirs;
+            }
+        }
+    }
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x % 32 < Lanes) {
+#pragma unroll
+        for (int r = 0; r < Rows; ++r) {
+            if (lane == 0) {
+                merged_stats[warp][r] = make_float2(top[r], sum[r]);
+            }
+#pragma unroll
+            for (int j = 0; j < kElems; ++j) {
+                merged_out[warp][r][element + j] = o[r][j];
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * p.head_dim; i += kThreads) {
+        const int r = i / p.head_dim;
+        const int e = i - r * p.head_dim;
+        float raised = merged_stats[0][r].x;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            raised = fmaxf(raised, merged_stats[w][r].x);
+        }
+        const float stand = raised == -INFINITY ? 0.0F : raised;
+        float total = 0.0F, value = 0.0F;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float factor = exp2f(merged_stats[w][r].x - stand);
+            total = fmaf(factor, merged_stats[w][r].y, total);
+            value = fmaf(factor, merged_out[w][r][e], value);
+        }
+        const int query = r / heads;
+        const int head = head0 + r - query * heads;
+        const long long row = s.q_first + query;
+        if (p.splits > 1) {
+            const long long at = (static_cast<long long>(split) * p.q_tokens + row) * p.q_heads +
+                                 head;
+            p.part_out[at * p.head_dim + e] = value;
+            if (e == 0) {
+                p.part_stats[at] = make_float2(raised, total);
+            }
+        } else {
+            value = total == 0.0F ? 0.0F : value / total;
+            T* const out = static_cast<T*>(p.out) + row * p.out_stride +
+                           static_cast<long long>(head) * p.head_dim + e;
+            if constexpr (sizeof(T) == 2) {
+                *out = __float2bfloat16_rn(value);
+            } else {
+                *out = value;
+            }
+        }
+    }
+}
+
+// One warp per (query row, head); lanes hold every 32nd element.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const VarlenParams p) {
+    dev::grid_dependency_wait(); // the parts
+    dev::grid_launch_dependents();
+    const long long item = static_cast<long long>(blockIdx.x) * kWarps + threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    const long long row = item / p.q_heads;
+    const int head = static_cast<int>(item - row * p.q_heads);
+    // Rows outside every sequence stay as they were.
+    if (row < clamped_offset(p.q_offsets, 0, p.q_tokens) ||
+        row >= clamped_offset(p.q_offsets, p.batch, p.q_tokens)) {
+        return; // the whole warp
+    }
+    const long long pitch = static_cast<long long>(p.q_tokens) * p.q_heads;
+    const float2* const stats = p.part_stats + row * p.q_heads + head;
+    float top = -INFINITY;
+    for (int i = lane; i < p.splits; i += 32) {
+        top = fmaxf(top, stats[i * pitch].x);
+    }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) {
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
+    }
+    const float stand = top == -INFINITY ? 0.0F : top;
+    const float* const parts = p.part_out + (row * p.q_heads + head) * p.head_dim;
+    float total = 0.0F;
+    float value[4] = {};
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i) {
+        const float2 stat = stats[i * pitch];
+        const float factor = exp2f(stat.x - stand);
+        total = fmaf(factor, stat.y, total);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = lane + 32 * j;
+            if (e < p.head_dim) {
+                value[j] = fmaf(factor, parts[i * pitch * p.head_dim + e], value[j]);
+            }
+        }
+    }
+    const float inverse = total == 0.0F ? 0.0F : 1.0F / total;
+    T* const out = static_cast<T*>(p.out) + row * p.out_stride +
+                   static_cast<long long>(head) * p.head_dim;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = lane + 32 * j;
+        if (e < p.head_dim) {
+            if constexpr (sizeof(T) == 2) {
+                out[e] = __float2bfloat16_rn(value[j] * inverse);
+            } else {
+                out[e] = value[j] * inverse;
+            }
+        }
+    }
+}
+
+int queries_per_block(const VarlenParams& p) {
+    const int rows = rows_kernel_rows(p);
+    return rows > p.group ? rows / p.group : 1;
+}
+
+int head_chunks(const VarlenParams& p) {
+    const int heads = rows_kernel_rows(p) / queries_per_block(p);
+    return (p.group + heads - 1) / heads;
+}
+
+template <typename T, int Lanes>
+int launch_lanes(const VarlenParams& p, cudaStream_t stream) {
+    const long long blocks = rows_kernel_items(p) * p.splits;
+    if (blocks > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
+    }
+    const auto start = [&](auto* kernel) {
+        host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p,
+                         queries_per_block(p), head_chunks(p));
+        return host::after_launch("attention_rows_kernel");
+    };
+    switch (rows_kernel_rows(p)) {
+    case 1:
+        return start(&attention_rows_kernel<T, Lanes, 1>);
+    case 2:
+        return start(&attention_rows_kernel<T, Lanes, 2>);
+    case 4:
+        return start(&attention_rows_kernel<T, Lanes, 4>);
+    default:
+        return start(&attention_rows_kernel<T, Lanes, 8>);
+    }
+}
+
+template <typename T>
+int launch_typed(const VarlenParams& p, cudaStream_t stream) {
+    const int chunks = p.head_dim / Lane<T>::kElems;
+    if (chunks <= 4) {
+        return launch_lanes<T, 4>(p, stream);
+    }
+    if (chunks <= 8) {
+        return launch_lanes<T, 8>(p, stream);
+    }
+    if (chunks <= 16) {
+        return launch_lanes<T, 16>(p, stream);
+    }
+    if constexpr (sizeof(T) == 4) {
+        return launch_lanes<T, 32>(p, stream);
+    }
+    return host::fail(CUVIT_RUNTIME_ERROR, "attention head_dim out of range");
+}
+
+} // namespace
+
+// Rows of one key head taken together: as many as an average sequence has, up to kMaxRows.
+int rows_kernel_rows(const VarlenParams& p) {
+    const long long queries = (p.q_tokens + static_cast<long long>(p.batch) - 1) / p.batch;
+    int rows = 1;
+    while (rows < kMaxRows && rows < queries * p.group) {
+        rows *= 2;
+    }
+    return rows;
+}
+
+long long rows_kernel_items(const VarlenParams& p) {
+    return (p.q_tokens / queries_per_block(p) + static_cast<long long>(p.batch)) * p.kv_heads *
+           head_chunks(p);
+}
+
+// 16-byte rows of q, k and v heads, and on average no more rows than the kernel takes at once.
+bool rows_kernel_takes(const VarlenParams& p) {
+    const int size = p.bf16 ? 2 : 4;
+    const auto fits = [size](const void* base, long long stride) {
+        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride * size % 16 == 0;
+    };
+    return static_cast<long long>(p.q_tokens) * p.group <=
+               static_cast<long long>(kMaxRows) * p.batch &&
+           p.head_dim * size % 16 == 0 && fits(p.q, p.q_stride) && fits(p.k, p.k_stride) &&
+           fits(p.v, p.v_stride);
+}
+
+int launch_rows(const VarlenParams& p, cudaStream_t stream) {
+    return p.bf16 ? launch_typed<__nv_bfloat16>(p, stream) : launch_typed<float>(p, stream);
+}
+
+int launch_join(const VarlenParams& p, cudaStream_t stream) {
+    const long long items = static_cast<long long>(p.q_tokens) * p.q_heads;
+    const long long blocks = (items + kWarps - 1) / kWarps;
+    if (blocks > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
+    }
+    // Always a dependent launch: the kernel before it is this call's own, which lets its
+    // dependents start early, and the join waits for its end before reading the parts.
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(blocks));
+    config.blockDim = dim3(kThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config,
+                       p.bf16 ? &attention_join_kernel<__nv_bfloat16>
+                              : &attention_join_kernel<float>,
+                       p);
+    return host::after_launch("attention_join_kernel");
+}
+
+} // namespace cuvit::attn

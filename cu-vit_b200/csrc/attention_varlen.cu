@@ -50,10 +50,12 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
     float* const ps = vs + kSimtKeys * DPad;      // [keys][pitch], key-major
     constexpr int kChunks = DPad / 64;
 
-    const long long block = blockIdx.x / p.q_heads;
-    const int head = static_cast<int>(blockIdx.x - block * p.q_heads);
-    const Sequence s = find_block<kSimtRows>(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens,
-                                             p.kv_tokens, block);
+    const int item = static_cast<int>(blockIdx.x) / p.splits;
+    const int split = static_cast<int>(blockIdx.x) - item * p.splits;
+    const int block = item / p.q_heads;
+    const int head = item - block * p.q_heads;
+    const Sequence s = find_block(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
+                                  block, kSimtRows);
     if (s.index < 0) {
         return;
     }
@@ -62,9 +64,11 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
     // Query row r of this block sees keys j <= r + reach.
     const long long reach =
         static_cast<long long>(s.q_first - s.q_begin) + keys - (s.q_end - s.q_begin);
-    const int last_key = p.causal ? static_cast<int>(min(static_cast<long long>(keys),
-                                                         max(0LL, reach + rows)))
-                                  : keys;
+    int first_key, last_key;
+    split_keys(keys, split, p.splits, first_key, last_key);
+    if (p.causal) {
+        last_key = static_cast<int>(min(static_cast<long long>(last_key), max(0LL, reach + rows)));
+    }
     const int d = p.head_dim;
     const T* const q = static_cast<const T*>(p.q) + s.q_first * p.q_stride +
                        static_cast<long long>(head) * d;
@@ -87,7 +91,7 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
         maximum[r] = -INFINITY;
         sum[r] = 0.0F;
     }
-    for (int first = 0; first < last_key; first += kSimtKeys) {
+    for (int first = first_key; first < last_key; first += kSimtKeys) {
         __syncthreads();
         for (int i = threadIdx.x; i < kSimtKeys * DPad; i += kSimtThreads) {
             const int j = i / DPad;
@@ -177,7 +181,22 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
         }
         const float inverse = sum[r] == 0.0F ? 0.0F : 1.0F / sum[r];
         const int row = 4 * ty + r;
-        if (row < rows) {
+        if (row < rows && p.splits > 1) {
+            const long long at =
+                (static_cast<long long>(split) * p.q_tokens + s.q_first + row) * p.q_heads + head;
+            if (tx == 0) {
+                p.part_stats[at] = make_float2(maximum[r], sum[r]);
+            }
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    if (64 * c + 4 * tx + x < d) {
+                        p.part_out[at * d + 64 * c + 4 * tx + x] = o[r][4 * c + x];
+                    }
+                }
+            }
+        } else if (row < rows) {
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
@@ -197,12 +216,16 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
     }
 }
 
+long long simt_items(const VarlenParams& p) {
+    return (static_cast<long long>(p.q_tokens) / kSimtRows + p.batch) * p.q_heads;
+}
+
 template <typename T, int DPad>
 int launch_simt(const VarlenParams& p, cudaStream_t stream) {
     auto* kernel = &attention_varlen_simt<T, DPad>;
     constexpr int kBytes = simt_smem_bytes<DPad>();
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
-    const long long blocks = (static_cast<long long>(p.q_tokens) / kSimtRows + p.batch) * p.q_heads;
+    const long long blocks = simt_items(p) * p.splits;
     if (blocks > 0x7FFFFFFFLL) {
         return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
     }
@@ -249,6 +272,8 @@ int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* emp
     p.group = c.q_heads / c.kv_heads;
     p.head_dim = c.head_dim;
     p.causal = c.causal ? 1 : 0;
+    p.bf16 = c.dtype == CUVIT_DTYPE_BF16 ? 1 : 0;
+    p.splits = 1;
     p.scale_log2 = c.scale * 1.4426950408889634F;
     const int64_t q_width = static_cast<int64_t>(c.q_heads) * c.head_dim;
     const int64_t kv_width = static_cast<int64_t>(c.kv_heads) * c.head_dim;
@@ -268,6 +293,52 @@ int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* emp
     }
     *out = p;
     return CUVIT_OK;
+}
+
+// Splits of the keys that give every SM `per_sm` blocks when the query rows alone do not, each
+// split with at least min_keys of an average sequence's keys.
+int choose_splits(const VarlenParams& p, long long items, int per_sm, int min_keys, int sm_count) {
+    constexpr int kMaxSplits = 64;
+    const long long wanted = (static_cast<long long>(sm_count) * per_sm) / (items > 0 ? items : 1);
+    const long long most = p.kv_tokens / static_cast<long long>(p.batch) / min_keys;
+    const long long splits = wanted < most ? wanted : most;
+    return static_cast<int>(splits < 1 ? 1 : (splits > kMaxSplits ? kMaxSplits : splits));
+}
+
+enum class Kernel { kSimt, kRows };
+
+// The splits of a call through each kernel, were a workspace given.
+int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
+    switch (kernel) {
+    case Kernel::kRows:
+        // About half of the launch's bound on blocks have rows (varlen.cuh).
+        return choose_splits(p, rows_kernel_items(p) / 2, 6, 128, sm_count);
+    default:
+        return choose_splits(p, simt_items(p), 2, 256, sm_count);
+    }
+}
+
+Kernel choose(const VarlenParams& p) {
+    return rows_kernel_takes(p) ? Kernel::kRows : Kernel::kSimt;
+}
+
+size_t workspace_bytes_of(const VarlenParams& p) {
+    if (p.splits <= 1) {
+        return 0;
+    }
+    return static_cast<size_t>(p.splits) * static_cast<size_t>(p.q_tokens) *
+           static_cast<size_t>(p.q_heads) * (static_cast<size_t>(p.head_dim) + 2) * sizeof(float);
+}
+
+// Enough for every kernel the operands' alignments may select.
+size_t workspace_bytes_at_most(VarlenParams p, int sm_count) {
+    size_t most = 0;
+    for (const Kernel kernel : {Kernel::kSimt, Kernel::kRows}) {
+        p.splits = splits_of(kernel, p, sm_count);
+        const size_t bytes = workspace_bytes_of(p);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 int run(const void* q, const void* k, const void* v, void* out, const int32_t* q_offsets,
@@ -310,8 +381,6 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
         host::rows_overlap(out_span, {v, p.kv_tokens, kv_width, p.v_stride * element})) {
         return host::fail(CUVIT_INVALID_ARGUMENT, "the attention output overlaps an operand");
     }
-    (void)workspace;
-    (void)workspace_bytes;
     p.q = q;
     p.k = k;
     p.v = v;
@@ -321,12 +390,42 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
     const host::DeviceContext* context = nullptr;
     CUVIT_TRY(host::current_context(&context));
     CUVIT_TRY(host::check_operands({q, k, v, out, q_offsets, kv_offsets}));
-    if (bf16) {
-        return p.head_dim <= 64 ? launch_simt<__nv_bfloat16, 64>(p, stream)
-                                : launch_simt<__nv_bfloat16, 128>(p, stream);
+    const Kernel kernel = choose(p);
+    p.splits = workspace != nullptr ? splits_of(kernel, p, context->sm_count) : 1;
+    if (p.splits > 1) {
+        const size_t needed = workspace_bytes_of(p);
+        if (workspace_bytes < needed || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+            return host::fail(CUVIT_INVALID_ARGUMENT,
+                              "the attention workspace is too small or not 16-byte aligned");
+        }
+        const int64_t area = static_cast<int64_t>(needed);
+        const host::RowSpan span{workspace, 1, area, area};
+        if (host::rows_overlap(span, {q, p.q_tokens, q_width, p.q_stride * element}) ||
+            host::rows_overlap(span, {k, p.kv_tokens, kv_width, p.k_stride * element}) ||
+            host::rows_overlap(span, {v, p.kv_tokens, kv_width, p.v_stride * element}) ||
+            host::rows_overlap(span, out_span)) {
+            return host::fail(CUVIT_INVALID_ARGUMENT, "the attention workspace overlaps an operand");
+        }
+        CUVIT_TRY(host::check_operands({workspace}));
+        const size_t rows = static_cast<size_t>(p.splits) * static_cast<size_t>(p.q_tokens) *
+                            static_cast<size_t>(p.q_heads);
+        p.part_stats = static_cast<float2*>(workspace);
+        p.part_out = reinterpret_cast<float*>(p.part_stats + rows);
     }
-    return p.head_dim <= 64 ? launch_simt<float, 64>(p, stream)
-                            : launch_simt<float, 128>(p, stream);
+    int status = CUVIT_OK;
+    if (kernel == Kernel::kRows) {
+        status = launch_rows(p, stream);
+    } else if (bf16) {
+        status = p.head_dim <= 64 ? launch_simt<__nv_bfloat16, 64>(p, stream)
+                                  : launch_simt<__nv_bfloat16, 128>(p, stream);
+    } else {
+        status = p.head_dim <= 64 ? launch_simt<float, 64>(p, stream)
+                                  : launch_simt<float, 128>(p, stream);
+    }
+    if (status == CUVIT_OK && p.splits > 1) {
+        status = launch_join(p, stream);
+    }
+    return status;
 }
 
 } // namespace
@@ -352,7 +451,14 @@ int cuvit_attention_varlen_workspace(const cuvit_attention_problem* problem, siz
         *bytes = 0;
         cuvit::attn::VarlenParams p{};
         bool empty = false;
-        return cuvit::attn::resolve(problem, &p, &empty);
+        CUVIT_TRY(cuvit::attn::resolve(problem, &p, &empty));
+        if (empty) {
+            return static_cast<int>(CUVIT_OK);
+        }
+        const cuvit::host::DeviceContext* context = nullptr;
+        CUVIT_TRY(cuvit::host::current_context(&context));
+        *bytes = cuvit::attn::workspace_bytes_at_most(p, context->sm_count);
+        return static_cast<int>(CUVIT_OK);
     });
 }
 

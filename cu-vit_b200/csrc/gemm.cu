@@ -213,6 +213,8 @@ bool add_batch_dims(const cuvit_gemm_batch& batch, long long stride, long long o
     return true;
 }
 
+} // namespace
+
 // Tile width: the one whose tiles finish soonest, counting whole waves of tiles over the SMs
 // (tiles = 128-row blocks x column tiles x batch entries), each wave as long as its tile is
 // wide, with a preference for wide tiles (fewer re-reads of A, fewer shared-memory and L2
@@ -244,8 +246,6 @@ int choose_block_n(long long row_blocks, int n, bool split, bool bf16, int sm_co
     }
     return best;
 }
-
-} // namespace
 
 int resolve(const void* a, const void* b, const float* bias, void* c, int c_dtype, int math,
             const cuvit_gemm_problem& problem, Resolved* out, bool* empty) {

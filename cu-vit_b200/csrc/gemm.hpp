@@ -65,5 +65,7 @@ int launch_tc_pair(const Plan& plan, cudaStream_t stream);
 // CUVIT_GEMM_PAIRS=0 (which keeps every GEMM on the one-CTA kernel).
 bool pairs_enabled();
 
+// The tile width (64, 128 or 256 columns) whose waves of tiles over the SMs finish soonest.
+int choose_block_n(long long row_blocks, int n, bool split, bool bf16, int sm_count);
 
 } // namespace cuvit::gemm

@@ -41,6 +41,8 @@ constexpr int kEpilogueThreads = 32 * kEpilogueWarps;
 constexpr int kSlabBytes = 32 * kSwizzleBytes; // one warp's 32 output rows x 128 bytes
 
 struct TcParams {
+    // Parameters of a derived kind select another epilogue (and, when gated, another B).
+    static constexpr bool kLinear = false;
     int m, n, k;
     int m_tiles, n_tiles, k_blocks;
     int total_tiles;
@@ -59,6 +61,13 @@ struct TcParams {
     int reverse; // walk the output tiles from the last to the first
     unsigned* status;
 };
+
+// The epilogue of linear layers (linear_tc.cuh).
+struct LinearParams;
+template <int BN, bool Split>
+__device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uint32_t tmem_cols,
+                            int n_block, int row_base, int half, uint8_t* slab, uint32_t slab_addr,
+                            uint32_t residual_bar, uint32_t& residual_phase, int lane);
 
 // The output tile a CTA's t-th tile index stands for, in the launch's sweep order.
 __device__ __forceinline__ int ordered_tile(const TcParams& p, int t) {
@@ -85,7 +94,9 @@ struct TcShape {
     static constexpr int kBarrierOffset = kSlabOffset + kEpilogueWarps * kSlabBytes;
     // barriers: full, empty, converted (split) per stage; tmem full/empty x2; drain
     static constexpr int kBarrierBytes = (3 * kStages + 5) * 8 + 16;
-    static constexpr int kSmemBytes = 1024 + kBarrierOffset + kBarrierBytes;
+    // Linear layers: one barrier per epilogue warp for the residual's loads.
+    static constexpr int kResidualOffset = kBarrierOffset + kBarrierBytes;
+    static constexpr int kSmemBytes = 1024 + kResidualOffset + 8 * kEpilogueWarps;
     static_assert(kStages >= 2, "at least two pipeline stages");
     static_assert(BN % 64 == 0 && BN >= 64 && BN <= 256, "BN must be 64, 128 or 256");
     static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
@@ -313,11 +324,15 @@ __device__ __forceinline__ void epilogue_tma(const TcParams& p, const CUtensorMa
     }
 }
 
-template <int ElemBytes, int BN, bool BMnMajor, bool Split>
+// Params: TcParams, or LinearParams (linear_tc.cuh), whose epilogue is linear_tile(). A gated
+// linear layer's tile holds BN / 2 output columns: its B is BN / 2 gate rows of the weight, then
+// the BN / 2 rows n further on that multiply them, so its accumulator holds both.
+template <int ElemBytes, int BN, bool BMnMajor, bool Split, class Params = TcParams>
 __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
     tc_gemm_kernel(const __grid_constant__ CUtensorMap tma_a,
                    const __grid_constant__ CUtensorMap tma_b,
-                   const __grid_constant__ CUtensorMap tma_c, const TcParams p) {
+                   const __grid_constant__ CUtensorMap tma_c,
+                   const __grid_constant__ Params p) {
     dev::timeline_enter();
     using Shape = TcShape<ElemBytes, BN, Split>;
     constexpr int kStages = Shape::kStages;
@@ -367,6 +382,11 @@ __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
             dev::mbar_init(tempty_bar(a), kEpilogueThreads);
         }
         dev::mbar_init(drain_bar, 1);
+        if constexpr (Params::kLinear) {
+            for (int e = 0; e < kEpilogueWarps; ++e) {
+                dev::mbar_init(base + Shape::kResidualOffset + 8u * e, 1);
+            }
+        }
         dev::fence_barrier_init();
     }
     if (warp == 2) {
@@ -411,7 +431,19 @@ __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
                 if (p.a_has_index) ca[r++] = index;
                 if (p.a_has_outer) ca[r++] = outer;
                 dev::tma_load(stage_a(stage), &tma_a, full_bar(stage), p.a_rank, ca);
-                if constexpr (!BMnMajor) {
+                bool loaded = false;
+                if constexpr (Params::kLinear) {
+                    if (p.gated) {
+                        const int gate[2] = {k0, n_block * (BN / 2)};
+                        const int up[2] = {k0, p.n + n_block * (BN / 2)};
+                        dev::tma_load(stage_b(stage), &tma_b, full_bar(stage), 2, gate);
+                        dev::tma_load(stage_b(stage) + Shape::kBBytes / 2, &tma_b,
+                                      full_bar(stage), 2, up);
+                        loaded = true;
+                    }
+                }
+                if (loaded) {
+                } else if constexpr (!BMnMajor) {
                     int cb[4] = {k0, n_block * BN, 0, 0};
                     int rb = 2;
                     if (p.b_has_index) cb[rb++] = index;
@@ -527,6 +559,7 @@ __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
         if (p.c_tma && lane == 0) {
             dev::tma_prefetch_descriptor(&tma_c);
         }
+        [[maybe_unused]] uint32_t residual_phase = 0;
         int local = 0;
         for (int tile = blockIdx.x; tile < p.total_tiles; tile += gridDim.x, ++local) {
             const int ordered = ordered_tile(p, tile);
@@ -547,6 +580,13 @@ __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
                 tmem_base + lane_field + static_cast<uint32_t>(acc * Shape::kAccColumns);
             const int first = half * kHalf;
             const int col_base = n_block * BN;
+            if constexpr (Params::kLinear) {
+                if (!linear_tile<BN, Split>(p, &tma_c, tmem_cols, n_block, row_base, half, slab,
+                                            slab_addr, base + Shape::kResidualOffset + 8u * e,
+                                            residual_phase, lane)) {
+                    break;
+                }
+            } else
             // A BF16 chunk is 64 columns (128 bytes); with BN = 64 a half tile is narrower,
             // so that combination always takes the direct path (the host never sets c_tma).
             if (p.c_tma && (p.c_kind != 1 || kHalf >= 64)) {

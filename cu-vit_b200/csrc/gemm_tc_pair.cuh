@@ -41,17 +41,20 @@ struct PairShape {
     static constexpr int kBarrierOffset = kSlabOffset + kEpilogueWarps * kSlabBytes;
     // barriers: full, empty, relay per stage; accumulator full/empty x2; drain
     static constexpr int kBarrierBytes = (3 * kStages + 5) * 8 + 16;
-    static constexpr int kSmemBytes = 1024 + kBarrierOffset + kBarrierBytes;
+    // Linear layers: one barrier per epilogue warp for the residual's loads.
+    static constexpr int kResidualOffset = kBarrierOffset + kBarrierBytes;
+    static constexpr int kSmemBytes = 1024 + kResidualOffset + 8 * kEpilogueWarps;
     static_assert(BN == 128 || BN == 256, "pair tiles are 256 x 128 or 256 x 256");
     static_assert(kStages >= 2, "at least two pipeline stages");
     static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 };
 
-template <int BN>
+template <int BN, class Params = TcParams>
 __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
     tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a,
                         const __grid_constant__ CUtensorMap tma_b,
-                        const __grid_constant__ CUtensorMap tma_c, const TcParams p) {
+                        const __grid_constant__ CUtensorMap tma_c,
+                        const __grid_constant__ Params p) {
     dev::timeline_enter();
     using Shape = PairShape<BN>;
     constexpr int kStages = Shape::kStages;
@@ -99,6 +102,11 @@ __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
             dev::mbar_init(tempty_bar(a), 2 * kEpilogueWarps);
         }
         dev::mbar_init(drain_bar, 1);
+        if constexpr (Params::kLinear) {
+            for (int e = 0; e < kEpilogueWarps; ++e) {
+                dev::mbar_init(base + Shape::kResidualOffset + 8u * e, 1);
+            }
+        }
         dev::fence_barrier_init();
     }
     if (warp == 2) {
@@ -148,6 +156,11 @@ __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
                 if (p.a_has_outer) ca[r++] = outer;
                 dev::tma_load(stage_a(stage), &tma_a, full_bar(stage), p.a_rank, ca);
                 int cb[4] = {k0, n_block * BN + static_cast<int>(rank) * (BN / 2), 0, 0};
+                if constexpr (Params::kLinear) {
+                    if (p.gated) { // rank 0 the gate's rows, rank 1 the rows they multiply
+                        cb[1] = static_cast<int>(rank) * p.n + n_block * (BN / 2);
+                    }
+                }
                 int rb = 2;
                 if (p.b_has_index) cb[rb++] = index;
                 if (p.b_has_outer) cb[rb++] = outer;
@@ -242,6 +255,7 @@ __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
         if (p.c_tma && lane == 0) {
             dev::tma_prefetch_descriptor(&tma_c);
         }
+        [[maybe_unused]] uint32_t residual_phase = 0;
         int local = 0;
         for (int tile = pair_id; tile < p.total_tiles; tile += pair_count, ++local) {
             const int ordered = ordered_tile(p, tile);
@@ -262,7 +276,13 @@ __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
                 tmem_base + lane_field + static_cast<uint32_t>(acc * BN);
             const int first = half * kHalf;
             const int col_base = n_block * BN;
-            if (p.c_tma && (p.c_kind != 1 || kHalf >= 64)) {
+            if constexpr (Params::kLinear) {
+                if (!linear_tile<BN, false>(p, &tma_c, tmem_cols, n_block, row_base, half, slab,
+                                            slab_addr, base + Shape::kResidualOffset + 8u * e,
+                                            residual_phase, lane)) {
+                    break;
+                }
+            } else if (p.c_tma && (p.c_kind != 1 || kHalf >= 64)) {
                 if (p.c_kind == 1) {
                     epilogue_tma<64, BN, false>(p, &tma_c, tmem_cols, first, first + kHalf,
                                                 col_base, row_base, index, outer, slab,

@@ -1,10 +1,7 @@
 // Linear layers: out = residual + scale * act(x W^T + b), or with a gate act(x Wg^T + bg) *
 // (x Wu^T + bu). Argument checks, choice of kernel, and the FP32 kernel for operands TMA cannot
 // describe.
-#include "activation.cuh"
-#include "cuvit_b200.h"
-#include "ptx.cuh"
-#include "runtime.hpp"
+#include "linear.hpp"
 
 #include <cuda_bf16.h>
 
@@ -12,20 +9,6 @@
 
 namespace cuvit::linear {
 namespace {
-
-struct Params {
-    const void* x;
-    const void* w;
-    const float* bias;
-    const float* scale;
-    const void* residual;
-    void* out;
-    int m, n, k;
-    int out_kind; // cuvit_dtype
-    int activation;
-    int gated;
-    long long ldx, ldw, ldr, ldo;
-};
 
 constexpr int kTile = 64;
 constexpr int kTileK = 16;
@@ -37,31 +20,6 @@ __device__ __forceinline__ float load_value(const T* p) {
         return __bfloat162float(*p);
     } else {
         return *p;
-    }
-}
-
-// out[row][col] from the sums of its gate (or only) column and its upper column.
-__device__ __forceinline__ void finish(const Params& p, int row, int col, float gate, float up) {
-    float value = p.bias != nullptr ? gate + p.bias[col] : gate;
-    value = dev::activate_exact(p.activation, value);
-    if (p.gated) {
-        value *= p.bias != nullptr ? up + p.bias[p.n + col] : up;
-    }
-    if (p.scale != nullptr) {
-        value *= p.scale[col];
-    }
-    if (p.out_kind == CUVIT_DTYPE_BF16) {
-        if (p.residual != nullptr) {
-            value += __bfloat162float(
-                static_cast<const __nv_bfloat16*>(p.residual)[row * p.ldr + col]);
-        }
-        static_cast<__nv_bfloat16*>(p.out)[row * p.ldo + col] = __float2bfloat16_rn(value);
-    } else {
-        if (p.residual != nullptr) {
-            value += static_cast<const float*>(p.residual)[row * p.ldr + col];
-        }
-        static_cast<float*>(p.out)[row * p.ldo + col] =
-            p.out_kind == CUVIT_DTYPE_TF32 ? dev::round_to_tf32(value) : value;
     }
 }
 
@@ -134,6 +92,114 @@ int launch_simt(const Params& p, cudaStream_t stream) {
     host::pdl_launch(p.gated ? linear_simt_kernel<T, true> : linear_simt_kernel<T, false>,
                      dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
     return host::after_launch("linear_simt_kernel");
+}
+
+// Bytes per access that every row of a matrix allows, from 16 down to an element.
+int access_bytes(const void* base, long long pitch_bytes) {
+    int bytes = 16;
+    while (reinterpret_cast<uintptr_t>(base) % bytes != 0 || pitch_bytes % bytes != 0) {
+        bytes /= 2;
+    }
+    return bytes;
+}
+
+// A row-major matrix as a TMA tensor of boxes of box_rows rows of 128 bytes.
+bool describe(const void* base, bool bf16, long long columns, long long rows, long long pitch,
+              int box_rows, CUtensorMap* map) {
+    host::TmaTensor t;
+    t.base = base;
+    t.type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    t.element_bytes = bf16 ? 2 : 4;
+    t.rank = 2;
+    t.dims[0] = static_cast<uint64_t>(columns);
+    t.dims[1] = static_cast<uint64_t>(rows);
+    t.strides_bytes[0] = static_cast<uint64_t>(pitch) * t.element_bytes;
+    t.box[0] = static_cast<uint32_t>(gemm::kSwizzleBytes / t.element_bytes);
+    t.box[1] = static_cast<uint32_t>(box_rows);
+    if (!host::tma_describable(t) || host::encode_tma(t, map) != CUVIT_OK) {
+        host::clear_error(); // another path serves what TMA cannot
+        return false;
+    }
+    return true;
+}
+
+// Plans a tensor-core launch; false where TMA cannot describe x or the weight, or k is 0.
+bool prepare(const Params& p, int math, const host::DeviceContext& context, TcPlan* plan) {
+    if (!host::is_blackwell(context) || p.k == 0) {
+        return false;
+    }
+    const bool bf16 = math == CUVIT_MATH_BF16;
+    const bool split = math == CUVIT_MATH_FP32;
+    const long long row_blocks = (p.m + gemm::kBlockM - 1LL) / gemm::kBlockM;
+    const long long weight_rows = static_cast<long long>(p.n) * (p.gated ? 2 : 1);
+    int bn = gemm::choose_block_n(row_blocks, static_cast<int>(weight_rows), split, bf16,
+                                  context.sm_count);
+    if (p.gated && bn < 128) {
+        bn = 128; // a half tile's columns of one operand stay a whole 32-column step
+    }
+    const int columns = p.gated ? bn / 2 : bn; // output columns of a tile
+    const long long n_tiles = (p.n + columns - 1) / columns;
+    const long long pair_rows = (p.m + 2LL * gemm::kBlockM - 1) / (2 * gemm::kBlockM);
+    plan->pair = bf16 && bn == 256 && gemm::pairs_enabled() &&
+                 pair_rows * n_tiles >= context.sm_count;
+    const long long m_tiles = plan->pair ? pair_rows : row_blocks;
+    const long long total = m_tiles * n_tiles;
+    const int b_rows = plan->pair || p.gated ? bn / 2 : bn;
+    if (total > 0x7FFFFFFFLL ||
+        !describe(p.x, bf16, p.k, p.m, p.ldx, gemm::kBlockM, &plan->map_x) ||
+        !describe(p.w, bf16, p.k, weight_rows, p.ldw, b_rows, &plan->map_w)) {
+        return false;
+    }
+    const auto aligned16 = [](const void* pointer) {
+        return reinterpret_cast<uintptr_t>(pointer) % 16 == 0 ? 1 : 0;
+    };
+    gemm::LinearParams& q = plan->params;
+    const int element = bf16 ? 2 : 4;
+    q.m = p.m;
+    q.n = p.n;
+    q.k = p.k;
+    q.m_tiles = static_cast<int>(m_tiles);
+    q.n_tiles = static_cast<int>(n_tiles);
+    q.k_blocks = (p.k + gemm::kSwizzleBytes / element - 1) / (gemm::kSwizzleBytes / element);
+    q.total_tiles = static_cast<int>(total);
+    q.count = 1;
+    q.a_rank = q.b_rank = q.c_rank = 2;
+    q.alpha = 1.0F;
+    q.bias = p.bias;
+    q.bias_vector_ok = aligned16(p.bias);
+    q.up_vector_ok = p.bias != nullptr ? aligned16(p.bias + p.n) : 0;
+    q.scale = p.scale;
+    q.scale_vector_ok = aligned16(p.scale);
+    q.c = p.out;
+    q.ldc = p.ldo;
+    q.c_kind = p.out_kind;
+    q.reverse = host::reverse_sweep() ? 1 : 0;
+    q.status = context.status;
+    q.activation = p.activation;
+    q.gated = p.gated;
+    q.residual = p.residual;
+    q.ldr = p.ldr;
+    // Whole slab rows (128 bytes: 64 bfloat16 or 32 float columns) go by TMA.
+    const bool out_bf16 = p.out_kind == CUVIT_DTYPE_BF16;
+    const int out_bytes = out_bf16 ? 2 : 4;
+    const bool whole = !out_bf16 || columns / 2 >= 64;
+    q.c_tma = whole && describe(p.out, out_bf16, p.n, p.m, p.ldo, 32, &plan->map_out) ? 1 : 0;
+    q.residual_tma = p.residual != nullptr && whole &&
+                             describe(p.residual, out_bf16, p.n, p.m, p.ldr, 32, &q.map_residual)
+                         ? 1
+                         : 0;
+    q.out_vector = access_bytes(p.out, p.ldo * out_bytes);
+    q.residual_vector = p.residual != nullptr ? access_bytes(p.residual, p.ldr * out_bytes) : 16;
+    plan->block_n = bn;
+    plan->grid = static_cast<int>(total < context.sm_count ? total : context.sm_count);
+    if (plan->pair) {
+        int resident = 0;
+        if (pair_resident(&resident) != CUVIT_OK) {
+            return false;
+        }
+        plan->grid = 2 * static_cast<int>(total < resident ? total : resident);
+    }
+    return true;
 }
 
 int run(const void* x, const void* weight, const float* bias, const float* scale,
@@ -220,8 +286,17 @@ int run(const void* x, const void* weight, const float* bias, const float* scale
     const host::DeviceContext* context = nullptr;
     CUVIT_TRY(host::current_context(&context));
     CUVIT_TRY(host::check_operands({x, weight, bias, scale, residual, out}));
-    return c.math == CUVIT_MATH_BF16 ? launch_simt<__nv_bfloat16>(p, stream)
-                                     : launch_simt<float>(p, stream);
+    const bool bf16 = c.math == CUVIT_MATH_BF16;
+    if (rows_kernel_takes(p, bf16)) {
+        return launch_rows(p, bf16, context->sm_count, stream);
+    }
+    TcPlan plan;
+    if (prepare(p, c.math, *context, &plan)) {
+        return bf16 ? launch_tc_bf16(plan, stream)
+                    : (c.math == CUVIT_MATH_FP32 ? launch_tc_split(plan, stream)
+                                                 : launch_tc_tf32(plan, stream));
+    }
+    return bf16 ? launch_simt<__nv_bfloat16>(p, stream) : launch_simt<float>(p, stream);
 }
 
 } // namespace

@@ -190,6 +190,246 @@ __global__ void __launch_bounds__(kThreads) qk_scalar_kernel(const __grid_consta
     }
 }
 
+// ---- vector kernel ------------------------------------------------------------------------
+//
+// Bound by HBM (each element read once and written once). A lane holds V pairs of one head: two
+// vectors of V elements that turn together (V elements apart by the pairing, or next to each
+// other), so the rotation needs no exchange between lanes and a norm one butterfly over the
+// `lanes` lanes of a head. A block takes a few tokens with all their heads and first fills a
+// table of their turns in shared memory: one sine and cosine per (token, pair), however many
+// heads share it. Lanes past the last chunk of a head (head_dim / 2 / V not a power of two) idle.
+constexpr int kTableVectors = 512; // float4 of two turns each: 8 KB
+
+struct VectorShape {
+    int lanes;        // lanes per head, a power of two
+    int lanes_log2;
+    int chunks;       // vectors of pairs per head, <= lanes
+    int block_tokens; // tokens per block
+    unsigned magic[2]; // ceil(2^32 / heads) of each side
+};
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T value[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&out)[V]) {
+    const Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        out[j] = load_value(&raw.value[j]);
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
+    Vec<T, V> raw;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        store_value(&raw.value[j], in[j]);
+    }
+    *reinterpret_cast<Vec<T, V>*>(p) = raw;
+}
+
+template <typename T, int V, int Norm>
+__global__ void __launch_bounds__(kThreads)
+    qk_vector_kernel(const __grid_constant__ Params p, const VectorShape s) {
+    __shared__ float4 table[kTableVectors];
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+    const int token0 = static_cast<int>(blockIdx.x) * s.block_tokens;
+    const int tokens = min(s.block_tokens, p.tokens - token0);
+    const int half = p.head_dim / 2;
+    // Two neighbouring pairs of a token per float4, placed so that the lanes of a head read
+    // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c.
+    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+        const int t = i / half;
+        const int pair = i - t * half;
+        const int chunk = pair / V;
+        const int within = pair - chunk * V;
+        reinterpret_cast<float2*>(
+            table)[(t * (half / 2) + (within / 2) * s.chunks + chunk) * 2 + (within & 1)] =
+            turn_of(p, token0 + t, pair);
+    }
+    __syncthreads();
+
+    const int lane = threadIdx.x & (s.lanes - 1);
+    const int group = threadIdx.x >> s.lanes_log2;
+    const int groups = kThreads >> s.lanes_log2;
+    const bool in_head = lane < s.chunks;
+    const int chunk = in_head ? lane : 0;
+    int first, second; // this lane's elements
+    if (p.adjacent) {
+        first = 2 * V * chunk;
+        second = first + V;
+    } else {
+        pair_elements(V * chunk, p.pairs, half, 0, first, second);
+    }
+    const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+        const Side& side = p.side[k];
+        if (side.heads == 0) {
+            continue;
+        }
+        float gamma[2][V], beta[2][V];
+        if constexpr (Norm != kNormNone) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                gamma[0][j] = side.gamma != nullptr ? side.gamma[first + j] : 1.0F;
+                gamma[1][j] = side.gamma != nullptr ? side.gamma[second + j] : 1.0F;
+                beta[0][j] = side.beta != nullptr ? side.beta[first + j] : 0.0F;
+                beta[1][j] = side.beta != nullptr ? side.beta[second + j] : 0.0F;
+            }
+        }
+        const int items = tokens * side.heads;
+        // Whole warps go round together: the butterflies need every lane.
+        for (int base = 0; base < items; base += groups) {
+            const int item = base + group;
+            const bool live = item < items && in_head;
+            const int t = item < items
+                              ? (side.heads == 1 ? item
+                                                 : static_cast<int>(__umulhi(
+                                                       static_cast<unsigned>(item), s.magic[k])))
+                              : 0;
+            const int head = item < items ? item - t * side.heads : 0;
+            const long long row = token0 + t;
+            const T* const in = static_cast<const T*>(side.in) + row * side.in_stride +
+                                head * p.head_dim;
+            float x[V], y[V];
+            if (live) {
+                load_vec<T, V>(in + first, x);
+                load_vec<T, V>(in + second, y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    x[j] = y[j] = 0.0F;
+                }
+            }
+            if constexpr (Norm != kNormNone) {
+                float mean = 0.0F;
+                if constexpr (Norm == CUVIT_NORM_LAYER) {
+                    float sum = 0.0F;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        sum += x[j] + y[j];
+                    }
+                    for (int offset = s.lanes / 2; offset > 0; offset /= 2) {
+                        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
+                    }
+                    mean = sum * inverse_dim;
+                }
+                float squares = 0.0F;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    x[j] -= mean;
+                    y[j] -= mean;
+                    squares = fmaf(x[j], x[j], fmaf(y[j], y[j], squares));
+                }
+                squares = in_head ? squares : 0.0F;
+                for (int offset = s.lanes / 2; offset > 0; offset /= 2) {
+                    squares += __shfl_xor_sync(0xFFFFFFFFu, squares, offset);
+                }
+                const float scale = 1.0F / sqrtf(squares * inverse_dim + p.epsilon);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    x[j] = fmaf(x[j] * scale, gamma[0][j], beta[0][j]);
+                    y[j] = fmaf(y[j] * scale, gamma[1][j], beta[1][j]);
+                }
+            }
+            if (live) {
+                float turns[2 * V]; // cos, sin of each pair
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) {
+                    const float4 two = table[t * (half / 2) + q * s.chunks + chunk];
+                    turns[4 * q] = two.x;
+                    turns[4 * q + 1] = two.y;
+                    turns[4 * q + 2] = two.z;
+                    turns[4 * q + 3] = two.w;
+                }
+                // Pair j of the chunk: (x[j], y[j]), or elements 2j and 2j + 1 of x followed by y.
+                const auto turn = [&](float& a, float& b, int j) {
+                    const float c = turns[2 * j];
+                    const float d = turns[2 * j + 1];
+                    const float first_new = a * c - b * d;
+                    b = fmaf(a, d, b * c);
+                    a = first_new;
+                };
+                if (p.adjacent) {
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) {
+                        turn(x[2 * j], x[2 * j + 1], j);
+                        turn(y[2 * j], y[2 * j + 1], V / 2 + j);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        turn(x[j], y[j], j);
+                    }
+                }
+                T* const out = static_cast<T*>(side.out) + row * side.out_stride +
+                               head * p.head_dim;
+                store_vec<T, V>(out + first, x);
+                store_vec<T, V>(out + second, y);
+            }
+        }
+    }
+}
+
+// Widest vectors the sizes and alignments allow: a lane's two vectors must lie within the
+// rotated or the unrotated part of a head, start on a multiple of their size, and fit a warp.
+template <typename T>
+int vector_width(const Params& p) {
+    const int half = p.head_dim / 2;
+    for (int v = 16 / static_cast<int>(sizeof(T)); v >= 2; v /= 2) {
+        const int bytes = v * static_cast<int>(sizeof(T));
+        bool ok = half % v == 0 && half / v <= 32 && half / 2 <= kTableVectors;
+        ok = ok && (p.adjacent || (p.pairs % v == 0 && (half - p.pairs) % v == 0));
+        for (const Side& side : p.side) {
+            if (side.heads == 0) {
+                continue;
+            }
+            const auto fits = [bytes](const void* base, long long stride) {
+                return reinterpret_cast<uintptr_t>(base) % bytes == 0 &&
+                       stride * static_cast<long long>(sizeof(T)) % bytes == 0;
+            };
+            ok = ok && fits(side.in, side.in_stride) && fits(side.out, side.out_stride);
+            ok = ok && side.heads <= 4096; // item numbers and their reciprocals stay exact
+        }
+        if (ok) {
+            return v;
+        }
+    }
+    return 1;
+}
+
+template <typename T, int V, int Norm>
+int launch_vector(const Params& p, int sm_count, cudaStream_t stream) {
+    VectorShape s{};
+    const int half = p.head_dim / 2;
+    s.chunks = half / V;
+    s.lanes = 1;
+    while (s.lanes < s.chunks) {
+        s.lanes *= 2;
+        ++s.lanes_log2;
+    }
+    for (int k = 0; k < 2; ++k) {
+        const unsigned heads = static_cast<unsigned>(p.side[k].heads);
+        s.magic[k] = heads > 1 ? static_cast<unsigned>((0x100000000ull + heads - 1) / heads) : 0u;
+    }
+    // As many tokens as fill the table's threads and give each thread a few heads, but no more
+    // than leave two blocks for every SM.
+    int tokens = kTableVectors * 2 / half;
+    tokens = tokens > 16 ? 16 : tokens;
+    const int spread = p.tokens / (2 * sm_count);
+    s.block_tokens = tokens < spread ? tokens : (spread > 0 ? spread : 1);
+    const int blocks = (p.tokens + s.block_tokens - 1) / s.block_tokens;
+    host::pdl_launch(qk_vector_kernel<T, V, Norm>, dim3(static_cast<unsigned>(blocks)),
+                     dim3(kThreads), 0, stream, p, s);
+    return host::after_launch("qk_vector_kernel");
+}
+
 template <typename T, int Norm>
 int launch_scalar(const Params& p, cudaStream_t stream) {
     const long long heads = p.side[0].heads + p.side[1].heads;
@@ -202,15 +442,32 @@ int launch_scalar(const Params& p, cudaStream_t stream) {
     return host::after_launch("qk_scalar_kernel");
 }
 
+template <typename T, int Norm>
+int launch_norm(const Params& p, int sm_count, cudaStream_t stream) {
+    switch (vector_width<T>(p)) {
+    case 8:
+        if constexpr (sizeof(T) == 2) {
+            return launch_vector<T, 8, Norm>(p, sm_count, stream);
+        }
+        [[fallthrough]];
+    case 4:
+        return launch_vector<T, 4, Norm>(p, sm_count, stream);
+    case 2:
+        return launch_vector<T, 2, Norm>(p, sm_count, stream);
+    default:
+        return launch_scalar<T, Norm>(p, stream);
+    }
+}
+
 template <typename T>
-int launch_typed(const Params& p, int norm, cudaStream_t stream) {
+int launch_typed(const Params& p, int norm, int sm_count, cudaStream_t stream) {
     switch (norm) {
     case CUVIT_NORM_RMS:
-        return launch_scalar<T, CUVIT_NORM_RMS>(p, stream);
+        return launch_norm<T, CUVIT_NORM_RMS>(p, sm_count, stream);
     case CUVIT_NORM_LAYER:
-        return launch_scalar<T, CUVIT_NORM_LAYER>(p, stream);
+        return launch_norm<T, CUVIT_NORM_LAYER>(p, sm_count, stream);
     default:
-        return launch_scalar<T, kNormNone>(p, stream);
+        return launch_norm<T, kNormNone>(p, sm_count, stream);
     }
 }
 
@@ -341,8 +598,9 @@ int run(const void* q, const void* k, void* q_out, void* k_out, const cuvit_qk_n
                                     p.positions, p.side[0].gamma, p.side[0].beta, p.side[1].gamma,
                                     p.side[1].beta}));
     const int kind = norm != nullptr ? norm->kind : kNormNone;
-    return c.dtype == CUVIT_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(p, kind, stream)
-                                       : launch_typed<float>(p, kind, stream);
+    return c.dtype == CUVIT_DTYPE_BF16
+               ? launch_typed<__nv_bfloat16>(p, kind, context->sm_count, stream)
+               : launch_typed<float>(p, kind, context->sm_count, stream);
 }
 
 } // namespace

@@ -388,7 +388,8 @@ int cuvit_attention_varlen(const void* q, const void* k, const void* v, void* ou
                            const cuvit_attention_problem* problem, void* workspace,
                            size_t workspace_bytes, cuvit_stream_t stream);
 
-/* Workspace of a problem on the current device, 0 where it is not split. */
+/* Bytes of workspace with which a problem may be split on the current device, whatever its
+ * operands' alignments; 0 where it is not split. */
 int cuvit_attention_varlen_workspace(const cuvit_attention_problem* problem, size_t* bytes);
 
 typedef enum cuvit_activation {

@@ -1,0 +1,711 @@
+// Attention over packed sequences on the tensor cores, bfloat16 operands.
+//
+//   S = Q K^T for 128 query rows and 128 keys at a time into tensor memory; P = 2^(S scale - m);
+//   O += P V, with m and the sum of P kept per row.
+//
+// One persistent CTA per SM walks (256 query rows, head, split of the keys) items. The 256 rows
+// are two tiles of 128 whose chains alternate: while the tensor core works for one tile, the other
+// tile's rows take their maxima and exponentials, so neither waits for the other longer than it
+// must. Keys and values stream through a ring of TMA stages shared by both tiles.
+//
+//   warp 0        loads (one lane)        warp 1      MMA issue
+//   warp 2        tensor memory           warp 3      -
+//   warps 4..7    rows of tile 0          warps 8..11 rows of tile 1 (one thread per row)
+//
+// * Rescaling O when a maximum rises would put a round trip through tensor memory into every
+//   step. m therefore only follows the true maximum when that has risen by more than 2^8, and
+//   O is rescaled then: P stays below 2^8, sums below 2^8 per key, well inside FP32 and
+//   bfloat16's range, and results do not change, since m cancels in the quotient.
+// * head_dim <= 64: P has tensor memory of its own, so the next S is issued as soon as the rows
+//   have read the current one. Up to 128: P overlays S (S 2 x 128, O 2 x 128 columns fill the 512),
+//   and the next S follows P V.
+// * A sequence may end inside a tile. K rows past the end only make scores that are replaced by
+//   -inf. V rows past the end would be multiplied by P = 0, which leaves NaN where they hold NaN
+//   or infinity (they belong to other sequences, or to nobody): the at most 15 of them that the
+//   last 16-key step still reads are overwritten with zeros in shared memory first.
+#include "attention_varlen.hpp"
+#include "ptx.cuh"
+#include "varlen.cuh"
+
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+namespace cuvit::attn {
+namespace {
+
+constexpr int kTile = 128;                // query rows of a tile, keys of a step
+constexpr int kAtomBytes = kTile * 128;   // 128 rows of 64 bfloat16
+constexpr int kThreads = 384;
+constexpr float kRescaleAbove = 8.0F;     // log2
+// Above this |m scale| (log2) the plain and the exact form of P would differ by more than 2^-14.
+constexpr float kLargeMaximum = 1024.0F;
+// Registers: 384 threads are launched with 168 each; the row warps (256 threads) take 208 and
+// leave 88 to the others: 256 * 208 + 128 * 88 = 384 * 168.
+constexpr int kRowRegisters = 208;
+constexpr int kOtherRegisters = 88;
+// Exponentials of these pairs of a 32-key chunk run on the FMA pipe (see attention.cu).
+constexpr uint32_t kPolyPairs = 0xA4A4u;
+
+template <int Atoms>
+struct Shape {
+    static constexpr bool kOverlay = Atoms == 2; // P in the columns of S
+    static constexpr int kQBytes = Atoms * kAtomBytes;
+    static constexpr int kSlotBytes = Atoms * kAtomBytes;
+    static constexpr int kSlots = Atoms == 2 ? 5 : 8;
+    static constexpr int kSlotOffset = 2 * kQBytes;
+    static constexpr int kBarrierOffset = kSlotOffset + kSlots * kSlotBytes;
+    // full, empty per slot; q_full[2], q_empty, s_full[2], s_free[2], p_full[2], o_done[2], drain
+    static constexpr int kBarriers = 2 * kSlots + 12;
+    static constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 16;
+    static constexpr uint32_t kOColumn = 256;
+    static constexpr uint32_t kOPitch = Atoms == 2 ? 128 : 64;
+    static constexpr uint32_t kPColumn = Atoms == 2 ? 0 : 384;
+    static constexpr uint32_t kPPitch = Atoms == 2 ? 128 : 64;
+    static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
+};
+
+struct Item {
+    Sequence s;
+    int head;
+    int split;
+    int rows;      // query rows of the block (1..256), 0: nothing to do
+    int first_key; // this split's keys, within the sequence
+    int end_key;
+    long long reach; // row r of the block sees keys below r + reach (causal)
+    int steps[2];  // key tiles of each query tile
+};
+
+__device__ __forceinline__ Item find_item(const VarlenParams& p, long long index) {
+    Item item;
+    item.split = static_cast<int>(index % p.splits);
+    index /= p.splits;
+    item.head = static_cast<int>(index % p.q_heads);
+    index /= p.q_heads;
+    item.s = find_block(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens, index,
+                        2 * kTile);
+    const Sequence& s = item.s;
+    item.rows = s.index < 0 ? 0 : min(2 * kTile, s.q_end - s.q_first);
+    const int keys = s.kv_end - s.kv_begin;
+    // Whole tiles per split, so that only a sequence's end falls inside a tile.
+    const int tiles = (keys + kTile - 1) / kTile;
+    const int each = (tiles + p.splits - 1) / p.splits;
+    item.first_key = min(keys, min(tiles, item.split * each) * kTile);
+    item.end_key = min(keys, min(tiles, (item.split + 1) * each) * kTile);
+    item.reach = static_cast<long long>(s.q_first - s.q_begin) + 1 + keys - (s.q_end - s.q_begin);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int rows = min(kTile, item.rows - t * kTile);
+        long long end = item.end_key;
+        if (p.causal) {
+            end = min(end, item.reach + t * kTile + rows - 1);
+        }
+        item.steps[t] = rows <= 0 || end <= item.first_key
+                            ? 0
+                            : static_cast<int>((end - item.first_key + kTile - 1) / kTile);
+    }
+    return item;
+}
+
+__device__ __forceinline__ float row_maximum(const uint32_t (&s)[kTile]) {
+    float m[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        m[c] = __uint_as_float(s[c]);
+    }
+#pragma unroll
+    for (int j = 4; j + 8 <= kTile; j += 8) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            m[c] = dev::max3(m[c], __uint_as_float(s[j + c]), __uint_as_float(s[j + 4 + c]));
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        m[c] = fmaxf(m[c], __uint_as_float(s[kTile - 4 + c]));
+    }
+    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// P = 2^(scale (s - m)) of 128 scores, packed, into tensor memory, and their sum. The plain form
+// folds scale and m into one multiply-add, off by a row-wide factor 2^d, |d| <= 2^-24 |m scale|
+// (it cancels in the quotient), and takes some exponentials on the FMA pipe. The exact form, for
+// tiles with masked scores and rows with a very large m, subtracts first, so that no m overflows
+// the exponent, and keeps to the special-function unit, whose 2^-inf is zero (the polynomial's is
+// 2^-125).
+template <bool Exact>
+__device__ __forceinline__ float exponentials(const uint32_t (&s)[kTile], float scale, float m,
+                                              uint32_t p_tmem) {
+    const uint64_t scale2 = dev::f32x2(scale, scale);
+    const float minus = Exact ? -m : -m * scale;
+    const uint64_t minus2 = dev::f32x2(minus, minus);
+    uint64_t sums[2] = {dev::f32x2(0.0F, 0.0F), dev::f32x2(0.0F, 0.0F)};
+#pragma unroll
+    for (int c = 0; c < kTile / 32; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint64_t s2 = dev::f32x2(__uint_as_float(s[32 * c + 2 * j]),
+                                           __uint_as_float(s[32 * c + 2 * j + 1]));
+            const uint64_t x2 = Exact ? dev::mul_f32x2(dev::add_f32x2(s2, minus2), scale2)
+                                      : dev::fma_f32x2(s2, scale2, minus2);
+            const float2 x = dev::f32x2_split(x2);
+            float2 e;
+            if (!Exact && ((kPolyPairs >> j) & 1u)) {
+                e = dev::exp2_poly2(x.x, x.y);
+            } else {
+                e = make_float2(dev::ex2_approx(x.x), dev::ex2_approx(x.y));
+            }
+            packed[j] = dev::pack_bf16x2(e.x, e.y);
+            sums[j & 1] = dev::add_f32x2(sums[j & 1], dev::f32x2(e.x, e.y));
+        }
+        dev::tmem_store_16(p_tmem + 16 * c, packed);
+    }
+    const float2 total = dev::f32x2_split(dev::add_f32x2(sums[0], sums[1]));
+    return total.x + total.y;
+}
+
+template <int Atoms>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q,
+                           const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const VarlenParams p,
+                           const long long items, unsigned* const status) {
+    using S = Shape<Atoms>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = dev::smem_u32(smem_raw);
+    const uint32_t base = (raw_base + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw_base);
+    const auto q_smem = [&](int t) -> uint32_t { return base + t * S::kQBytes; };
+    const auto slot_smem = [&](int i) -> uint32_t {
+        return base + S::kSlotOffset + i * S::kSlotBytes;
+    };
+    const uint32_t bars = base + S::kBarrierOffset;
+    const auto full = [&](int i) -> uint32_t { return bars + 8u * i; };
+    const auto empty = [&](int i) -> uint32_t { return bars + 8u * (S::kSlots + i); };
+    const uint32_t more = bars + 16u * S::kSlots;
+    const auto q_full = [&](int t) -> uint32_t { return more + 8u * t; };
+    const uint32_t q_empty = more + 16;
+    const auto s_full = [&](int t) -> uint32_t { return more + 24 + 8u * t; };
+    const auto s_free = [&](int t) -> uint32_t { return more + 40 + 8u * t; };
+    const auto p_full = [&](int t) -> uint32_t { return more + 56 + 8u * t; };
+    const auto o_done = [&](int t) -> uint32_t { return more + 72 + 8u * t; };
+    const uint32_t drain = more + 88;
+    uint32_t* const tmem_slot =
+        reinterpret_cast<uint32_t*>(smem + S::kBarrierOffset + 8 * S::kBarriers);
+
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kSlots; ++i) {
+            dev::mbar_init(full(i), 1);
+            dev::mbar_init(empty(i), 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            dev::mbar_init(q_full(t), 1);
+            dev::mbar_init(s_full(t), 1);
+            dev::mbar_init(s_free(t), kTile);
+            dev::mbar_init(p_full(t), kTile);
+            dev::mbar_init(o_done(t), 1);
+        }
+        dev::mbar_init(q_empty, 1);
+        dev::mbar_init(drain, 1);
+        dev::fence_barrier_init();
+    }
+    if (warp == 2) {
+        dev::tmem_alloc(dev::smem_u32(tmem_slot), 512);
+        dev::tmem_relinquish();
+    }
+    dev::tc_fence_before();
+    __syncthreads();
+    dev::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+        if (warp == 0 && lane == 0) {
+            // ---------------- loads ----------------
+            dev::tma_prefetch_descriptor(&map_q);
+            dev::tma_prefetch_descriptor(&map_k);
+            dev::tma_prefetch_descriptor(&map_v);
+            int slot = 0;
+            uint32_t phase = 0;
+            uint32_t q_phase = 0;     // items with keys so far
+            uint32_t q_loads[2] = {}; // loads of each query tile so far
+            bool ok = true;
+            const auto load_kv = [&](const CUtensorMap* map, int kv_head, int row) {
+                if (!dev::mbar_wait(empty(slot), phase ^ 1u, status)) {
+                    ok = false;
+                    return;
+                }
+                dev::mbar_arrive_expect_tx(full(slot), S::kSlotBytes);
+                for (int a = 0; a < Atoms; ++a) {
+                    const int c[3] = {64 * a, kv_head, row};
+                    dev::tma_load(slot_smem(slot) + a * kAtomBytes, map, full(slot), 3, c);
+                }
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            };
+            for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
+                const Item item = find_item(p, index);
+                const int steps = max(item.steps[0], item.steps[1]);
+                if (steps == 0) {
+                    continue;
+                }
+                if (!dev::mbar_wait(q_empty, (q_phase & 1u) ^ 1u, status)) {
+                    ok = false;
+                    break;
+                }
+                ++q_phase;
+                for (int t = 0; t < 2; ++t) {
+                    if (item.steps[t] > 0) {
+                        ++q_loads[t];
+                        dev::mbar_arrive_expect_tx(q_full(t), S::kQBytes);
+                        for (int a = 0; a < Atoms; ++a) {
+                            const int c[3] = {64 * a, item.head, item.s.q_first + t * kTile};
+                            dev::tma_load(q_smem(t) + a * kAtomBytes, &map_q, q_full(t), 3, c);
+                        }
+                    }
+                }
+                const int kv_head = item.head / p.group;
+                const int row = item.s.kv_begin + item.first_key;
+                // In the order the MMA warp takes them.
+                load_kv(&map_k, kv_head, row);
+                for (int j = 0; j < steps && ok; ++j) {
+                    if (S::kOverlay) {
+                        load_kv(&map_v, kv_head, row + j * kTile);
+                    }
+                    if (ok && j + 1 < steps) {
+                        load_kv(&map_k, kv_head, row + (j + 1) * kTile);
+                    }
+                    if (ok && !S::kOverlay) {
+                        load_kv(&map_v, kv_head, row + j * kTile);
+                    }
+                }
+            }
+            if (!ok) {
+                // Every load issued lands before the CTA's shared memory goes.
+                for (int i = 0; i < S::kSlots; ++i) {
+                    dev::mbar_drain_wait(full(i), phase ^ (i < slot ? 0u : 1u));
+                }
+                for (int t = 0; t < 2; ++t) {
+                    if (q_loads[t] > 0) {
+                        dev::mbar_drain_wait(q_full(t), (q_loads[t] - 1) & 1u);
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            // ---------------- MMA issue (the warp together, one lane issuing) ----------------
+            const int k_steps = (p.head_dim + 15) / 16;
+            const uint32_t idesc_o =
+                dev::make_idesc(1u, kTile, 16 * k_steps, false, true);
+            int slot = 0;
+            uint32_t phase = 0;
+            uint32_t q_phase[2] = {};
+            uint32_t free_phase[2] = {};
+            uint32_t p_phase[2] = {};
+            bool ok = true;
+            const auto next_slot = [&]() {
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+            };
+            // Keys of a tile, rounded up to whole 16-key steps.
+            const auto scores = [&](int t, uint32_t k_smem, int keys16) {
+                const uint32_t idesc = dev::make_idesc(1u, kTile, keys16, false, false);
+                for (int kk = 0; kk < k_steps; ++kk) {
+                    const uint32_t offset = (kk >> 2) * kAtomBytes + (kk & 3) * 32;
+                    dev::mma_ss<dev::MmaKind::kF16>(
+                        tmem + t * kTile, dev::smem_desc_sw128(q_smem(t) + offset, 16, 1024),
+                        dev::smem_desc_sw128(k_smem + offset, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+                }
+                dev::tc_commit(s_full(t));
+            };
+            for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
+                const Item item = find_item(p, index);
+                const int steps = max(item.steps[0], item.steps[1]);
+                if (steps == 0) {
+                    continue;
+                }
+                const int keys = item.end_key - item.first_key;
+                const auto keys_of = [&](int j) { return min(kTile, keys - j * kTile); };
+                const auto round16 = [](int n) { return (n + 15) & ~15; };
+                // The first scores.
+                ok = dev::mbar_wait_warp(full(slot), phase, status);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (item.steps[t] > 0) {
+                        ok = dev::mbar_wait_warp(q_full(t), q_phase[t], status);
+                        q_phase[t] ^= 1u;
+                        if (ok && lane == 0) {
+                            dev::tc_fence_after();
+                            scores(t, slot_smem(slot), round16(keys_of(0)));
+                        }
+                    }
+                }
+                if (!ok) {
+                    break;
+                }
+                if (lane == 0) {
+                    dev::tc_commit(empty(slot));
+                    if (steps == 1) {
+                        dev::tc_commit(q_empty);
+                    }
+                }
+                next_slot();
+                for (int j = 0; j < steps && ok; ++j) {
+                    // Slots of this step: the next keys and these values, in the loads' order.
+                    const bool more_keys = j + 1 < steps;
+                    int v_slot, k_slot;
+                    uint32_t v_phase, k_phase;
+                    if (!S::kOverlay && more_keys) {
+                        k_slot = slot;
+                        k_phase = phase;
+                        next_slot();
+                    }
+                    v_slot = slot;
+                    v_phase = phase;
+                    next_slot();
+                    if (S::kOverlay && more_keys) {
+                        k_slot = slot;
+                        k_phase = phase;
+                        next_slot();
+                    }
+                    if (!S::kOverlay && more_keys) {
+                        // The next scores as soon as the rows have read these.
+                        ok = dev::mbar_wait_warp(full(k_slot), k_phase, status);
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            if (j + 1 < item.steps[t]) {
+                                ok = dev::mbar_wait_warp(s_free(t), free_phase[t], status);
+                                if (ok && lane == 0) {
+                                    dev::tc_fence_after();
+                                    scores(t, slot_smem(k_slot), round16(keys_of(j + 1)));
+                                }
+                            }
+                        }
+                        if (!ok) {
+                            break;
+                        }
+                        if (lane == 0) {
+                            dev::tc_commit(empty(k_slot));
+                        }
+                    }
+                    // s_free completes once per step of a tile, whether or not more scores follow.
+                    for (int t = 0; t < 2; ++t) {
+                        free_phase[t] ^= j < item.steps[t] ? 1u : 0u;
+                    }
+                    ok = dev::mbar_wait_warp(full(v_slot), v_phase, status);
+                    if (!ok) {
+                        break;
+                    }
+                    const int live = keys_of(j);
+                    const int live16 = round16(live);
+                    if (live < live16) {
+                        // Values behind the sequence's end that the last 16-key step reads.
+                        uint8_t* const v_bytes = smem + (slot_smem(v_slot) - base);
+                        const int vectors = (live16 - live) * 8;
+                        for (int i = lane; i < vectors * Atoms; i += 32) {
+                            const int a = i / vectors;
+                            reinterpret_cast<uint4*>(v_bytes + a * kAtomBytes +
+                                                     live * 128)[i - a * vectors] =
+                                make_uint4(0, 0, 0, 0);
+                        }
+                        dev::fence_proxy_async_shared();
+                        __syncwarp();
+                    }
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j >= item.steps[t]) {
+                            continue;
+                        }
+                        ok = dev::mbar_wait_warp(p_full(t), p_phase[t], status);
+                        p_phase[t] ^= 1u;
+                        if (ok && lane == 0) {
+                            dev::tc_fence_after();
+                            for (int kk = 0; kk < live16 / 16; ++kk) {
+                                dev::mma_ts<dev::MmaKind::kF16>(
+                                    tmem + S::kOColumn + t * S::kOPitch,
+                                    tmem + S::kPColumn + t * S::kPPitch + 8 * kk,
+                                    dev::smem_desc(slot_smem(v_slot) + kk * 2048, kAtomBytes, 1024,
+                                                   dev::kLayoutSwizzle128),
+                                    idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+                            }
+                            dev::tc_commit(o_done(t));
+                        }
+                        if (ok && S::kOverlay && j + 1 < item.steps[t]) {
+                            ok = dev::mbar_wait_warp(full(k_slot), k_phase, status);
+                            if (ok && lane == 0) {
+                                dev::tc_fence_after();
+                                scores(t, slot_smem(k_slot), round16(keys_of(j + 1)));
+                            }
+                        }
+                    }
+                    if (!ok) {
+                        break;
+                    }
+                    if (lane == 0) {
+                        dev::tc_commit(empty(v_slot));
+                        if (S::kOverlay && more_keys) {
+                            dev::tc_commit(empty(k_slot));
+                        }
+                        if (j + 2 == steps) {
+                            dev::tc_commit(q_empty); // the last scores have been issued
+                        }
+                    }
+                }
+            }
+            // Every MMA issued has finished before the CTA's shared and tensor memory go.
+            if (lane == 0) {
+                dev::tc_commit(drain);
+                dev::mbar_drain_wait(drain, 0);
+            }
+        }
+    } else {
+        // ---------------- rows ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
+        const int t = (warp - 4) / 4;
+        const int quarter = warp & 3; // the tensor memory lanes this warp may access
+        const int row = quarter * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_tmem = tmem + lanes + t * kTile;
+        const uint32_t p_tmem = tmem + lanes + S::kPColumn + t * S::kPPitch;
+        const uint32_t o_tmem = tmem + lanes + S::kOColumn + t * S::kOPitch;
+        const int o_columns = 16 * ((p.head_dim + 15) / 16);
+        uint32_t s_phase = 0;
+        uint32_t o_phase = 0; // of the tile's next P V to complete
+        bool ok = true;
+        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
+            const Item item = find_item(p, index);
+            const int rows = item.rows - t * kTile; // may be 0 or less
+            if (rows <= 0) {
+                continue;
+            }
+            const int steps = item.steps[t];
+            const bool live_warp = quarter * 32 < rows;
+            // Keys this row sees, from the split's first on.
+            long long end = item.end_key;
+            if (p.causal) {
+                end = max(0LL, min(end, item.reach + t * kTile + row));
+            }
+            const int row_keys = static_cast<int>(max(0LL, end - item.first_key));
+            float m = 0.0F; // unscaled
+            float sum = 0.0F;
+            for (int j = 0; j < steps; ++j) {
+                ok = dev::mbar_wait_warp(s_full(t), s_phase, status);
+                s_phase ^= 1u;
+                if (!ok) {
+                    break;
+                }
+                dev::tc_fence_after();
+                uint32_t s[kTile];
+                if (live_warp) {
+#pragma unroll
+                    for (int c = 0; c < kTile / 32; ++c) {
+                        dev::tmem_load_32(s_tmem + 32 * c,
+                                          *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                    }
+                    dev::tmem_wait_load();
+                }
+                if (!S::kOverlay) {
+                    dev::tc_fence_before();
+                    dev::mbar_arrive(s_free(t));
+                    if (j > 0) {
+                        // P V of the previous step has read P and written O.
+                        ok = dev::mbar_wait_warp(o_done(t), o_phase, status);
+                        o_phase ^= 1u;
+                        if (!ok) {
+                            break;
+                        }
+                        dev::tc_fence_after();
+                    }
+                }
+                if (live_warp) {
+                    const int limit = row_keys - j * kTile;
+                    if (__any_sync(0xFFFFFFFFu, limit < kTile)) {
+#pragma unroll
+                        for (int c = 0; c < kTile; ++c) {
+                            s[c] = c < limit ? s[c] : 0xFF800000u; // -inf
+                        }
+                    }
+                    const float top = row_maximum(s);
+                    if (j == 0) {
+                        m = top == -INFINITY ? 0.0F : top;
+                    } else {
+                        const bool raise = (top - m) * p.scale_log2 > kRescaleAbove;
+                        if (__any_sync(0xFFFFFFFFu, raise)) {
+                            const float raised = raise ? top : m;
+                            const float factor = dev::ex2_approx((m - raised) * p.scale_log2);
+                            m = raised;
+                            sum *= factor;
+                            for (int c = 0; c < o_columns; c += 16) {
+                                uint32_t o[16];
+                                dev::tmem_load_16(o_tmem + c, o);
+                                dev::tmem_wait_load();
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) {
+                                    o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
+                                }
+                                dev::tmem_store_16(o_tmem + c, o);
+                            }
+                        }
+                    }
+                    const bool exact = limit < kTile || fabsf(m * p.scale_log2) > kLargeMaximum;
+                    sum += __any_sync(0xFFFFFFFFu, exact)
+                               ? exponentials<true>(s, p.scale_log2, m, p_tmem)
+                               : exponentials<false>(s, p.scale_log2, m, p_tmem);
+                    dev::tmem_wait_store();
+                }
+                dev::tc_fence_before();
+                dev::mbar_arrive(p_full(t));
+            }
+            if (!ok) {
+                break;
+            }
+            if (steps > 0) {
+                // The last P V of this tile. With the overlay the phases of the earlier ones were
+                // not waited for: each later S came after them.
+                if (S::kOverlay) {
+                    o_phase ^= static_cast<uint32_t>(steps - 1) & 1u;
+                }
+                ok = dev::mbar_wait_warp(o_done(t), o_phase, status);
+                o_phase ^= 1u;
+                if (!ok) {
+                    break;
+                }
+                dev::tc_fence_after();
+            }
+            if (!live_warp) {
+                continue;
+            }
+            const bool live = row < rows;
+            const long long token = item.s.q_first + t * kTile + row;
+            const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
+            const long long part =
+                (static_cast<long long>(item.split) * p.q_tokens + token) * p.q_heads + item.head;
+            if (live && p.splits > 1) {
+                p.part_stats[part] = make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
+            }
+            for (int c = 0; c < o_columns; c += 16) {
+                uint32_t o[16];
+                if (steps > 0) {
+                    dev::tmem_load_16(o_tmem + c, o);
+                    dev::tmem_wait_load();
+                }
+                if (sum == 0.0F) { // no keys: what tensor memory holds is nobody's
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        o[x] = 0u;
+                    }
+                }
+                if (!live) {
+                    continue;
+                }
+                if (p.splits > 1) {
+                    float4* const out =
+                        reinterpret_cast<float4*>(p.part_out + part * p.head_dim + c);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        if (c + 4 * x < p.head_dim) {
+                            out[x] = make_float4(
+                                __uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                                __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+                        }
+                    }
+                } else {
+                    uint4* const out = reinterpret_cast<uint4*>(
+                        static_cast<__nv_bfloat16*>(p.out) + token * p.out_stride +
+                        static_cast<long long>(item.head) * p.head_dim + c);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        if (c + 8 * x < p.head_dim) {
+                            uint32_t words[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {
+                                words[y] = dev::pack_bf16x2(
+                                    __uint_as_float(o[8 * x + 2 * y]) * inverse,
+                                    __uint_as_float(o[8 * x + 2 * y + 1]) * inverse);
+                            }
+                            out[x] = make_uint4(words[0], words[1], words[2], words[3]);
+                        }
+                    }
+                }
+            }
+            // O has been read before the next item's first P V, which follows this tile's p_full.
+            dev::tc_fence_before();
+        }
+    }
+
+    __syncthreads();
+    if (warp == 2) {
+        dev::tc_fence_after();
+        dev::tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int Atoms>
+int launch_atoms(const VarlenParams& p, const host::DeviceContext& context,
+                 const CUtensorMap (&maps)[3], cudaStream_t stream) {
+    auto* kernel = &attention_tiles_kernel<Atoms>;
+    constexpr int kBytes = Shape<Atoms>::kSmemBytes;
+    CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
+    const long long items = tiles_kernel_items(p) * p.splits;
+    const long long grid = items < context.sm_count ? items : context.sm_count;
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kBytes, stream,
+                     maps[0], maps[1], maps[2], p, items, context.status);
+    return host::after_launch("attention_tiles_kernel");
+}
+
+// [rows][heads][head_dim] with boxes of 64 elements of one head of 128 rows.
+bool describe(const void* base, int head_dim, int heads, long long rows, long long stride,
+              CUtensorMap* map) {
+    host::TmaTensor t;
+    t.base = base;
+    t.type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    t.element_bytes = 2;
+    t.rank = 3;
+    t.dims[0] = static_cast<uint64_t>(head_dim);
+    t.dims[1] = static_cast<uint64_t>(heads);
+    t.dims[2] = static_cast<uint64_t>(rows);
+    t.strides_bytes[0] = static_cast<uint64_t>(head_dim) * 2;
+    t.strides_bytes[1] = static_cast<uint64_t>(stride) * 2;
+    t.box[0] = 64;
+    t.box[1] = 1;
+    t.box[2] = kTile;
+    if (!host::tma_describable(t) || (map != nullptr && host::encode_tma(t, map) != CUVIT_OK)) {
+        host::clear_error(); // another kernel serves what TMA cannot
+        return false;
+    }
+    return true;
+}
+
+} // namespace
+
+long long tiles_kernel_items(const VarlenParams& p) {
+    return (p.q_tokens / (2 * kTile) + static_cast<long long>(p.batch)) * p.q_heads;
+}
+
+bool tiles_kernel_takes(const VarlenParams& p) {
+    return p.bf16 && p.kv_tokens > 0 && p.head_dim % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % 8 == 0 &&
+           describe(p.q, p.head_dim, p.q_heads, p.q_tokens, p.q_stride, nullptr) &&
+           describe(p.k, p.head_dim, p.kv_heads, p.kv_tokens, p.k_stride, nullptr) &&
+           describe(p.v, p.head_dim, p.kv_heads, p.kv_tokens, p.v_stride, nullptr);
+}
+
+int launch_tiles(const VarlenParams& p, cudaStream_t stream) {
+    const host::DeviceContext* context = nullptr;
+    CUVIT_TRY(host::current_context(&context));
+    CUtensorMap maps[3];
+    if (!describe(p.q, p.head_dim, p.q_heads, p.q_tokens, p.q_stride, &maps[0]) ||
+        !describe(p.k, p.head_dim, p.kv_heads, p.kv_tokens, p.k_stride, &maps[1]) ||
+        !describe(p.v, p.head_dim, p.kv_heads, p.kv_tokens, p.v_stride, &maps[2])) {
+        return host::fail(CUVIT_CUDA_ERROR, "the attention operands' TMA descriptors failed");
+    }
+    return p.head_dim <= 64 ? launch_atoms<1>(p, *context, maps, stream)
+                            : launch_atoms<2>(p, *context, maps, stream);
+}
+
+} // namespace cuvit::attn

@@ -305,7 +305,7 @@ int choose_splits(const VarlenParams& p, long long items, int per_sm, int min_ke
     return static_cast<int>(splits < 1 ? 1 : (splits > kMaxSplits ? kMaxSplits : splits));
 }
 
-enum class Kernel { kSimt, kRows };
+enum class Kernel { kSimt, kRows, kTiles };
 
 // The splits of a call through each kernel, were a workspace given.
 int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
@@ -313,27 +313,38 @@ int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
     case Kernel::kRows:
         // About half of the launch's bound on blocks have rows (varlen.cuh).
         return choose_splits(p, rows_kernel_items(p) / 2, 6, 128, sm_count);
+    case Kernel::kTiles:
+        return choose_splits(p, tiles_kernel_items(p), 1, 512, sm_count);
     default:
         return choose_splits(p, simt_items(p), 2, 256, sm_count);
     }
 }
 
 Kernel choose(const VarlenParams& p) {
-    return rows_kernel_takes(p) ? Kernel::kRows : Kernel::kSimt;
+    if (rows_kernel_takes(p)) {
+        return Kernel::kRows;
+    }
+    return tiles_kernel_takes(p) ? Kernel::kTiles : Kernel::kSimt;
+}
+
+// The parts' outputs, rounded up to whole 16-byte vectors, then their statistics.
+size_t part_rows(const VarlenParams& p) {
+    return static_cast<size_t>(p.splits) * static_cast<size_t>(p.q_tokens) *
+           static_cast<size_t>(p.q_heads);
+}
+
+size_t part_out_bytes(const VarlenParams& p) {
+    return (part_rows(p) * static_cast<size_t>(p.head_dim) * sizeof(float) + 15) / 16 * 16;
 }
 
 size_t workspace_bytes_of(const VarlenParams& p) {
-    if (p.splits <= 1) {
-        return 0;
-    }
-    return static_cast<size_t>(p.splits) * static_cast<size_t>(p.q_tokens) *
-           static_cast<size_t>(p.q_heads) * (static_cast<size_t>(p.head_dim) + 2) * sizeof(float);
+    return p.splits <= 1 ? 0 : part_out_bytes(p) + part_rows(p) * sizeof(float2);
 }
 
 // Enough for every kernel the operands' alignments may select.
 size_t workspace_bytes_at_most(VarlenParams p, int sm_count) {
     size_t most = 0;
-    for (const Kernel kernel : {Kernel::kSimt, Kernel::kRows}) {
+    for (const Kernel kernel : {Kernel::kSimt, Kernel::kRows, Kernel::kTiles}) {
         p.splits = splits_of(kernel, p, sm_count);
         const size_t bytes = workspace_bytes_of(p);
         most = bytes > most ? bytes : most;
@@ -407,14 +418,14 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
             return host::fail(CUVIT_INVALID_ARGUMENT, "the attention workspace overlaps an operand");
         }
         CUVIT_TRY(host::check_operands({workspace}));
-        const size_t rows = static_cast<size_t>(p.splits) * static_cast<size_t>(p.q_tokens) *
-                            static_cast<size_t>(p.q_heads);
-        p.part_stats = static_cast<float2*>(workspace);
-        p.part_out = reinterpret_cast<float*>(p.part_stats + rows);
+        p.part_out = static_cast<float*>(workspace);
+        p.part_stats = reinterpret_cast<float2*>(static_cast<char*>(workspace) + part_out_bytes(p));
     }
     int status = CUVIT_OK;
     if (kernel == Kernel::kRows) {
         status = launch_rows(p, stream);
+    } else if (kernel == Kernel::kTiles) {
+        status = launch_tiles(p, stream);
     } else if (bf16) {
         status = p.head_dim <= 64 ? launch_simt<__nv_bfloat16, 64>(p, stream)
                                   : launch_simt<__nv_bfloat16, 128>(p, stream);

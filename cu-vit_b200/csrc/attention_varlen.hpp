@@ -48,6 +48,11 @@ int rows_kernel_rows(const VarlenParams& p);
 long long rows_kernel_items(const VarlenParams& p); // blocks of a launch per split
 int launch_rows(const VarlenParams& p, cudaStream_t stream);
 
+// bfloat16 on the tensor cores (attention_tiles.cu).
+bool tiles_kernel_takes(const VarlenParams& p);
+long long tiles_kernel_items(const VarlenParams& p); // work items per split
+int launch_tiles(const VarlenParams& p, cudaStream_t stream);
+
 // Joins the splits: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 int launch_join(const VarlenParams& p, cudaStream_t stream);
 

@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+constexpr int kStages = 3; // of keys and values in flight: 48 KB a block, four blocks an SM
 // Keys a lane group has in flight (registers bound it: 8 rows hold 64 of queries and 64 of output).
 template <int Rows>
 constexpr int kUnrollOf = Rows >= 8 ? 2 : 4;
@@ -31,6 +32,13 @@ struct Lane {
 
     static __device__ __forceinline__ uint4 load(const T* p) {
         return __ldg(reinterpret_cast<const uint4*>(p));
+    }
+
+    // Copies 16 bytes to shared memory asynchronously, or zeros.
+    static __device__ __forceinline__ void copy(uint4* to, const T* p, bool live) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dev::smem_u32(to)),
+                     "l"(p), "r"(live ? 16 : 0)
+                     : "memory");
     }
 
     static __device__ __forceinline__ void unpack(const uint4& raw, float (&out)[kElems]) {
@@ -64,8 +72,18 @@ __global__ void __launch_bounds__(kThreads)
     constexpr int kElems = Lane<T>::kElems;
     constexpr int kUnroll = kUnrollOf<Rows>;
     constexpr int kGroups = kThreads / Lanes; // key streams of the block
-    __shared__ float merged_out[kWarps][Rows][Lanes * kElems];
-    __shared__ float2 merged_stats[kWarps][Rows];
+    // Keys and values in flight; each lane reads back only what it copied itself, so the ring
+    // needs no barrier. Afterwards the warps' parts.
+    struct Parts {
+        float out[kWarps][Rows][Lanes * kElems];
+        float2 stats[kWarps][Rows];
+    };
+    __shared__ union {
+        uint4 ring[kStages][kUnroll][2][kThreads];
+        Parts parts;
+    } shared;
+    auto& merged_out = shared.parts.out;
+    auto& merged_stats = shared.parts.stats;
 
     // Item: block of queries, key head, chunk of its query heads, split (fastest: the splits of
     // one range run together).
@@ -122,6 +140,7 @@ __global__ void __launch_bounds__(kThreads)
                                 : end_key;
         }
     }
+    const T* const k0 = static_cast<const T*>(p.q); // never read: copies of no bytes name it
     const T* const k = static_cast<const T*>(p.k) + s.kv_begin * p.k_stride +
                        static_cast<long long>(kv_head) * p.head_dim + element;
     const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
@@ -136,14 +155,33 @@ __global__ void __launch_bounds__(kThreads)
     }
     // Whole warps go round together (the butterflies need every lane).
     const int warp_group0 = (threadIdx.x / 32) * (32 / Lanes);
-    for (int base = first_key; base + warp_group0 < end_key; base += kGroups * kUnroll) {
-        uint4 k_raw[kUnroll], v_raw[kUnroll];
+    const int step = kGroups * kUnroll;
+    const auto fetch = [&](int stage, int base) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int key = base + u * kGroups + group;
             const bool live = key < end_key && in_row;
-            k_raw[u] = live ? Lane<T>::load(k + key * p.k_stride) : make_uint4(0, 0, 0, 0);
-            v_raw[u] = live ? Lane<T>::load(v + key * p.v_stride) : make_uint4(0, 0, 0, 0);
+            const long long row = live ? key : 0;
+            Lane<T>::copy(&shared.ring[stage][u][0][threadIdx.x], live ? k + row * p.k_stride : k0,
+                          live);
+            Lane<T>::copy(&shared.ring[stage][u][1][threadIdx.x], live ? v + row * p.v_stride : k0,
+                          live);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (first_key + i * step + warp_group0 < end_key) {
+            fetch(i, first_key + i * step);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int stage = 0;
+    for (int base = first_key; base + warp_group0 < end_key; base += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        uint4 k_raw[kUnroll], v_raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            k_raw[u] = shared.ring[stage][u][0][threadIdx.x];
         }
         float score[Rows][kUnroll];
 #pragma unroll
@@ -197,6 +235,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             float vf[kElems];
+            v_raw[u] = shared.ring[stage][u][1][threadIdx.x];
             Lane<T>::unpack(v_raw[u], vf);
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
@@ -206,7 +245,17 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
+        // Into the stage read in the previous round: its values have been used by now.
+        const int ahead = stage == 0 ? kStages - 1 : stage - 1;
+        const int next = base + (kStages - 1) * step;
+        if (next + warp_group0 < end_key) {
+            fetch(ahead, next);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        stage = stage + 1 == kStages ? 0 : stage + 1;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads(); // the ring becomes the parts
 
     // Lane groups of a warp, then the warps, in a fixed order.
 #pragma unroll
@@ -279,59 +328,78 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// One warp per (query row, head); lanes hold every 32nd element.
+// One block per (query row, head): its warps take every fourth split, lanes every 32nd element,
+// and the warps' sums are added in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const VarlenParams p) {
+    __shared__ float sums[kWarps][128];
     dev::grid_dependency_wait(); // the parts
     dev::grid_launch_dependents();
-    const long long item = static_cast<long long>(blockIdx.x) * kWarps + threadIdx.x / 32;
+    const long long row = blockIdx.x / p.q_heads;
+    const int head = static_cast<int>(blockIdx.x - row * p.q_heads);
+    const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
-    const long long row = item / p.q_heads;
-    const int head = static_cast<int>(item - row * p.q_heads);
     // Rows outside every sequence stay as they were.
     if (row < clamped_offset(p.q_offsets, 0, p.q_tokens) ||
         row >= clamped_offset(p.q_offsets, p.batch, p.q_tokens)) {
-        return; // the whole warp
+        return; // the whole block
     }
     const long long pitch = static_cast<long long>(p.q_tokens) * p.q_heads;
     const float2* const stats = p.part_stats + row * p.q_heads + head;
-    float top = -INFINITY;
-    for (int i = lane; i < p.splits; i += 32) {
-        top = fmaxf(top, stats[i * pitch].x);
+    static_assert(kMaxSplits <= 64, "two splits' statistics per lane");
+    float2 stat[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int at = lane + 32 * i;
+        stat[i] = at < p.splits ? stats[at * pitch] : make_float2(-INFINITY, 0.0F);
     }
+    float top = fmaxf(stat[0].x, stat[1].x);
 #pragma unroll
     for (int offset = 16; offset > 0; offset /= 2) {
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
     }
     const float stand = top == -INFINITY ? 0.0F : top;
-    const float* const parts = p.part_out + (row * p.q_heads + head) * p.head_dim;
-    float total = 0.0F;
-    float value[4] = {};
-#pragma unroll 4
-    for (int i = 0; i < p.splits; ++i) {
-        const float2 stat = stats[i * pitch];
-        const float factor = exp2f(stat.x - stand);
-        total = fmaf(factor, stat.y, total);
+    const float factor[2] = {exp2f(stat[0].x - stand), exp2f(stat[1].x - stand)};
+    float total = factor[0] * stat[0].y + factor[1] * stat[1].y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = lane + 32 * j;
-            if (e < p.head_dim) {
-                value[j] = fmaf(factor, parts[i * pitch * p.head_dim + e], value[j]);
+    for (int offset = 16; offset > 0; offset /= 2) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
+    }
+    const float* const parts = p.part_out + (row * p.q_heads + head) * p.head_dim;
+    float value[4] = {};
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / kWarps; ++i) {
+        const int at = warp + kWarps * i;
+        const float weight = __shfl_sync(0xFFFFFFFFu, factor[at / 32], at % 32);
+        if (at < p.splits) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = lane + 32 * j;
+                if (e < p.head_dim) {
+                    value[j] = fmaf(weight, parts[at * pitch * p.head_dim + e], value[j]);
+                }
             }
         }
     }
-    const float inverse = total == 0.0F ? 0.0F : 1.0F / total;
-    T* const out = static_cast<T*>(p.out) + row * p.out_stride +
-                   static_cast<long long>(head) * p.head_dim;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int e = lane + 32 * j;
-        if (e < p.head_dim) {
-            if constexpr (sizeof(T) == 2) {
-                out[e] = __float2bfloat16_rn(value[j] * inverse);
-            } else {
-                out[e] = value[j] * inverse;
-            }
+        sums[warp][lane + 32 * j] = value[j];
+    }
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e < p.head_dim) {
+        float sum = sums[0][e];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) {
+            sum += sums[w][e];
+        }
+        sum = total == 0.0F ? 0.0F : sum / total;
+        T* const out = static_cast<T*>(p.out) + row * p.out_stride +
+                       static_cast<long long>(head) * p.head_dim + e;
+        if constexpr (sizeof(T) == 2) {
+            *out = __float2bfloat16_rn(sum);
+        } else {
+            *out = sum;
         }
     }
 }
@@ -421,8 +489,7 @@ int launch_rows(const VarlenParams& p, cudaStream_t stream) {
 }
 
 int launch_join(const VarlenParams& p, cudaStream_t stream) {
-    const long long items = static_cast<long long>(p.q_tokens) * p.q_heads;
-    const long long blocks = (items + kWarps - 1) / kWarps;
+    const long long blocks = static_cast<long long>(p.q_tokens) * p.q_heads;
     if (blocks > 0x7FFFFFFFLL) {
         return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
     }

@@ -298,7 +298,6 @@ int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* emp
 // Splits of the keys that give every SM `per_sm` blocks when the query rows alone do not, each
 // split with at least min_keys of an average sequence's keys.
 int choose_splits(const VarlenParams& p, long long items, int per_sm, int min_keys, int sm_count) {
-    constexpr int kMaxSplits = 64;
     const long long wanted = (static_cast<long long>(sm_count) * per_sm) / (items > 0 ? items : 1);
     const long long most = p.kv_tokens / static_cast<long long>(p.batch) / min_keys;
     const long long splits = wanted < most ? wanted : most;

@@ -9,6 +9,8 @@
 
 namespace cuvit::attn {
 
+constexpr int kMaxSplits = 64;
+
 // Rows are heads * head_dim elements, strides in elements, defaults resolved.
 struct VarlenParams {
     const void* q;

@@ -60,28 +60,41 @@ __global__ void __launch_bounds__(kThreads)
     const T* const x = static_cast<const T*>(p.x);
     float acc[Rows][kColumns] = {};
     const int step = warps_per_columns * 32 * kElems;
-#pragma unroll 2
-    for (int k = (part * 32 + lane) * kElems; k < p.k; k += step) {
-        uint4 raw[kColumns];
+    // kPieces pieces of every column are loaded before the first is used.
+    constexpr int kPieces = Rows <= 2 ? 4 : (Rows <= 4 ? 2 : 1);
+    for (int k0 = (part * 32 + lane) * kElems; k0 < p.k; k0 += kPieces * step) {
+        uint4 raw[kPieces][kColumns];
 #pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-            raw[c] = __ldg(reinterpret_cast<const uint4*>(w[c] + k));
-        }
-        float wf[kColumns][kElems];
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-            Piece<T>::unpack(raw[c], wf[c]);
-        }
-#pragma unroll
-        for (int r = 0; r < Rows; ++r) {
-            const int row = min(r, p.m - 1); // rows past the end are not stored
-            float xf[kElems];
-            Piece<T>::unpack(__ldg(reinterpret_cast<const uint4*>(x + row * p.ldx + k)), xf);
+        for (int i = 0; i < kPieces; ++i) {
+            const int k = k0 + i * step;
 #pragma unroll
             for (int c = 0; c < kColumns; ++c) {
+                raw[i][c] = k < p.k ? __ldg(reinterpret_cast<const uint4*>(w[c] + k))
+                                    : make_uint4(0, 0, 0, 0);
+            }
+        }
 #pragma unroll
-                for (int j = 0; j < kElems; ++j) {
-                    acc[r][c] = fmaf(xf[j], wf[c][j], acc[r][c]);
+        for (int i = 0; i < kPieces; ++i) {
+            const int k = k0 + i * step;
+            if (k < p.k) { // x may hold anything past its rows' ends
+                float wf[kColumns][kElems];
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) {
+                    Piece<T>::unpack(raw[i][c], wf[c]);
+                }
+#pragma unroll
+                for (int r = 0; r < Rows; ++r) {
+                    const int row = min(r, p.m - 1); // rows past the end are not stored
+                    float xf[kElems];
+                    Piece<T>::unpack(__ldg(reinterpret_cast<const uint4*>(x + row * p.ldx + k)),
+                                     xf);
+#pragma unroll
+                    for (int c = 0; c < kColumns; ++c) {
+#pragma unroll
+                        for (int j = 0; j < kElems; ++j) {
+                            acc[r][c] = fmaf(xf[j], wf[c][j], acc[r][c]);
+                        }
+                    }
                 }
             }
         }

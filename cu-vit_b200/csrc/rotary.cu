@@ -194,18 +194,21 @@ __global__ void __launch_bounds__(kThreads) qk_scalar_kernel(const __grid_consta
 //
 // Bound by HBM (each element read once and written once). A lane holds V pairs of one head: two
 // vectors of V elements that turn together (V elements apart by the pairing, or next to each
-// other), so the rotation needs no exchange between lanes and a norm one butterfly over the
-// `lanes` lanes of a head. A block takes a few tokens with all their heads and first fills a
-// table of their turns in shared memory: one sine and cosine per (token, pair), however many
-// heads share it. Lanes past the last chunk of a head (head_dim / 2 / V not a power of two) idle.
+// other), so the rotation needs no exchange between lanes and a norm one sum over the `chunks`
+// lanes of a head, as many heads side by side in a warp as fit (6 of 5 lanes for head_dim 80; with
+// heads padded to 8 lanes 3 in 8 would idle). A block takes a few tokens with all their query and
+// key heads and first fills a table of their turns in shared memory: one sine and cosine per
+// (token, pair), however many heads share it. The next head's vectors are loaded before the
+// current one's are used: at HBM's latency a block's threads have to keep 64 bytes each in flight.
+constexpr int kWarps = kThreads / 32;
 constexpr int kTableVectors = 512; // float4 of two turns each: 8 KB
+constexpr int kMaxHeads = 8192;    // of both sides: item numbers and their reciprocal stay exact
 
 struct VectorShape {
-    int lanes;        // lanes per head, a power of two
-    int lanes_log2;
-    int chunks;       // vectors of pairs per head, <= lanes
+    int chunks;       // lanes per head
+    int warp_groups;  // heads side by side in a warp: 32 / chunks
     int block_tokens; // tokens per block
-    unsigned magic[2]; // ceil(2^32 / heads) of each side
+    unsigned magic;   // ceil(2^32 / heads of both sides)
 };
 
 template <typename T, int V>
@@ -214,8 +217,7 @@ struct alignas(sizeof(T) * V) Vec {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&out)[V]) {
-    const Vec<T, V> raw = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ __forceinline__ void unpack(const Vec<T, V>& raw, float (&out)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         out[j] = load_value(&raw.value[j]);
@@ -232,33 +234,47 @@ __device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
     *reinterpret_cast<Vec<T, V>*>(p) = raw;
 }
 
+// Sum over the `count` lanes from lane `first` on, of which this is number `position`: windows of
+// 1, 2, 4, ... lanes (around the group's end) and from them the sum of `count`.
+__device__ __forceinline__ float group_sum(float value, int first, int position, int count) {
+    const auto from = [&](float v, int distance) {
+        int at = position + distance;
+        at -= at >= count ? count : 0;
+        return __shfl_sync(0xFFFFFFFFu, v, first + at);
+    };
+    float total = 0.0F;
+    int covered = 0;
+    for (int width = 1; width <= count; width *= 2) {
+        if (count & width) {
+            total = covered == 0 ? value : total + from(value, covered);
+            covered += width;
+        }
+        if (2 * width <= count) {
+            value += from(value, width);
+        }
+    }
+    return total;
+}
+
 template <typename T, int V, int Norm>
 __global__ void __launch_bounds__(kThreads)
     qk_vector_kernel(const __grid_constant__ Params p, const VectorShape s) {
     __shared__ float4 table[kTableVectors];
+    __shared__ __align__(16) float gains[Norm == kNormNone ? 1 : 4][kMaxHeadDim];
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
     const int token0 = static_cast<int>(blockIdx.x) * s.block_tokens;
     const int tokens = min(s.block_tokens, p.tokens - token0);
     const int half = p.head_dim / 2;
-    // Two neighbouring pairs of a token per float4, placed so that the lanes of a head read
-    // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c.
-    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
-        const int t = i / half;
-        const int pair = i - t * half;
-        const int chunk = pair / V;
-        const int within = pair - chunk * V;
-        reinterpret_cast<float2*>(
-            table)[(t * (half / 2) + (within / 2) * s.chunks + chunk) * 2 + (within & 1)] =
-            turn_of(p, token0 + t, pair);
-    }
-    __syncthreads();
 
-    const int lane = threadIdx.x & (s.lanes - 1);
-    const int group = threadIdx.x >> s.lanes_log2;
-    const int groups = kThreads >> s.lanes_log2;
-    const bool in_head = lane < s.chunks;
-    const int chunk = in_head ? lane : 0;
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    const int group_of_warp = lane / s.chunks;
+    const int chunk = lane - group_of_warp * s.chunks;
+    const bool in_group = group_of_warp < s.warp_groups;
+    const int first_lane = group_of_warp * s.chunks;
+    const int group = warp * s.warp_groups + group_of_warp;
+    const int groups = kWarps * s.warp_groups;
     int first, second; // this lane's elements
     if (p.adjacent) {
         first = 2 * V * chunk;
@@ -266,113 +282,122 @@ __global__ void __launch_bounds__(kThreads)
     } else {
         pair_elements(V * chunk, p.pairs, half, 0, first, second);
     }
-    const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-        const Side& side = p.side[k];
-        if (side.heads == 0) {
-            continue;
+    const int q_heads = p.side[0].heads;
+    const int heads = q_heads + p.side[1].heads;
+    const int items = tokens * heads; // heads of a token, queries first
+    const auto token_of = [&](int item) {
+        return heads == 1 ? item : static_cast<int>(__umulhi(static_cast<unsigned>(item), s.magic));
+    };
+    const auto load_item = [&](int item, Vec<T, V>& x, Vec<T, V>& y) {
+        if (item < items && in_group) {
+            const int t = token_of(item);
+            const int head = item - t * heads;
+            const bool key = head >= q_heads;
+            const Side& side = p.side[key ? 1 : 0];
+            const T* const in = static_cast<const T*>(side.in) + (token0 + t) * side.in_stride +
+                                (head - (key ? q_heads : 0)) * p.head_dim;
+            x = *reinterpret_cast<const Vec<T, V>*>(in + first);
+            y = *reinterpret_cast<const Vec<T, V>*>(in + second);
         }
-        float gamma[2][V], beta[2][V];
+    };
+    Vec<T, V> x_next{}, y_next{};
+    load_item(group, x_next, y_next);
+
+    // Two neighbouring pairs of a token per float4, placed so that the lanes of a head read
+    // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c.
+    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+        const int t = i / half;
+        const int pair = i - t * half;
+        const int c = pair / V;
+        const int within = pair - c * V;
+        reinterpret_cast<float2*>(
+            table)[(t * (half / 2) + (within / 2) * s.chunks + c) * 2 + (within & 1)] =
+            turn_of(p, token0 + t, pair);
+    }
+    if constexpr (Norm != kNormNone) {
+        for (int i = threadIdx.x; i < 2 * p.head_dim; i += kThreads) {
+            const int k = i >= p.head_dim ? 1 : 0;
+            const int e = i - k * p.head_dim;
+            gains[2 * k][e] = p.side[k].gamma != nullptr ? p.side[k].gamma[e] : 1.0F;
+            gains[2 * k + 1][e] = p.side[k].beta != nullptr ? p.side[k].beta[e] : 0.0F;
+        }
+    }
+    __syncthreads();
+
+    const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
+    // Whole warps go round together: the sums need every lane of a group.
+    for (int base = 0; base < items; base += groups) {
+        const int item = base + group;
+        const bool live = item < items && in_group;
+        float x[V], y[V];
+        unpack(x_next, x);
+        unpack(y_next, y);
+        load_item(item + groups, x_next, y_next);
+        const int t = live ? token_of(item) : 0;
+        const int head = live ? item - t * heads : 0;
+        const int key = head >= q_heads ? 1 : 0;
         if constexpr (Norm != kNormNone) {
+            float mean = 0.0F;
+            if constexpr (Norm == CUVIT_NORM_LAYER) {
+                float sum = 0.0F;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    sum += x[j] + y[j];
+                }
+                mean = group_sum(sum, first_lane, chunk, s.chunks) * inverse_dim;
+            }
+            float squares = 0.0F;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                gamma[0][j] = side.gamma != nullptr ? side.gamma[first + j] : 1.0F;
-                gamma[1][j] = side.gamma != nullptr ? side.gamma[second + j] : 1.0F;
-                beta[0][j] = side.beta != nullptr ? side.beta[first + j] : 0.0F;
-                beta[1][j] = side.beta != nullptr ? side.beta[second + j] : 0.0F;
+                x[j] -= mean;
+                y[j] -= mean;
+                squares = fmaf(x[j], x[j], fmaf(y[j], y[j], squares));
+            }
+            squares = group_sum(squares, first_lane, chunk, s.chunks);
+            const float scale = 1.0F / sqrtf(squares * inverse_dim + p.epsilon);
+            const float* const gamma = gains[2 * key];
+            const float* const beta = gains[2 * key + 1];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                x[j] = fmaf(x[j] * scale, gamma[first + j], beta[first + j]);
+                y[j] = fmaf(y[j] * scale, gamma[second + j], beta[second + j]);
             }
         }
-        const int items = tokens * side.heads;
-        // Whole warps go round together: the butterflies need every lane.
-        for (int base = 0; base < items; base += groups) {
-            const int item = base + group;
-            const bool live = item < items && in_head;
-            const int t = item < items
-                              ? (side.heads == 1 ? item
-                                                 : static_cast<int>(__umulhi(
-                                                       static_cast<unsigned>(item), s.magic[k])))
-                              : 0;
-            const int head = item < items ? item - t * side.heads : 0;
-            const long long row = token0 + t;
-            const T* const in = static_cast<const T*>(side.in) + row * side.in_stride +
-                                head * p.head_dim;
-            float x[V], y[V];
-            if (live) {
-                load_vec<T, V>(in + first, x);
-                load_vec<T, V>(in + second, y);
+        if (live) {
+            float turns[2 * V]; // cos, sin of each pair
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) {
+                const float4 two = table[t * (half / 2) + q * s.chunks + chunk];
+                turns[4 * q] = two.x;
+                turns[4 * q + 1] = two.y;
+                turns[4 * q + 2] = two.z;
+                turns[4 * q + 3] = two.w;
+            }
+            // Pair j of the chunk: (x[j], y[j]), or elements 2j and 2j + 1 of x followed by y.
+            const auto turn = [&](float& a, float& b, int j) {
+                const float c = turns[2 * j];
+                const float d = turns[2 * j + 1];
+                const float turned = a * c - b * d;
+                b = fmaf(a, d, b * c);
+                a = turned;
+            };
+            if (p.adjacent) {
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    turn(x[2 * j], x[2 * j + 1], j);
+                    turn(y[2 * j], y[2 * j + 1], V / 2 + j);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    x[j] = y[j] = 0.0F;
+                    turn(x[j], y[j], j);
                 }
             }
-            if constexpr (Norm != kNormNone) {
-                float mean = 0.0F;
-                if constexpr (Norm == CUVIT_NORM_LAYER) {
-                    float sum = 0.0F;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        sum += x[j] + y[j];
-                    }
-                    for (int offset = s.lanes / 2; offset > 0; offset /= 2) {
-                        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, offset);
-                    }
-                    mean = sum * inverse_dim;
-                }
-                float squares = 0.0F;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    x[j] -= mean;
-                    y[j] -= mean;
-                    squares = fmaf(x[j], x[j], fmaf(y[j], y[j], squares));
-                }
-                squares = in_head ? squares : 0.0F;
-                for (int offset = s.lanes / 2; offset > 0; offset /= 2) {
-                    squares += __shfl_xor_sync(0xFFFFFFFFu, squares, offset);
-                }
-                const float scale = 1.0F / sqrtf(squares * inverse_dim + p.epsilon);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    x[j] = fmaf(x[j] * scale, gamma[0][j], beta[0][j]);
-                    y[j] = fmaf(y[j] * scale, gamma[1][j], beta[1][j]);
-                }
-            }
-            if (live) {
-                float turns[2 * V]; // cos, sin of each pair
-#pragma unroll
-                for (int q = 0; q < V / 2; ++q) {
-                    const float4 two = table[t * (half / 2) + q * s.chunks + chunk];
-                    turns[4 * q] = two.x;
-                    turns[4 * q + 1] = two.y;
-                    turns[4 * q + 2] = two.z;
-                    turns[4 * q + 3] = two.w;
-                }
-                // Pair j of the chunk: (x[j], y[j]), or elements 2j and 2j + 1 of x followed by y.
-                const auto turn = [&](float& a, float& b, int j) {
-                    const float c = turns[2 * j];
-                    const float d = turns[2 * j + 1];
-                    const float first_new = a * c - b * d;
-                    b = fmaf(a, d, b * c);
-                    a = first_new;
-                };
-                if (p.adjacent) {
-#pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {
-                        turn(x[2 * j], x[2 * j + 1], j);
-                        turn(y[2 * j], y[2 * j + 1], V / 2 + j);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        turn(x[j], y[j], j);
-                    }
-                }
-                T* const out = static_cast<T*>(side.out) + row * side.out_stride +
-                               head * p.head_dim;
-                store_vec<T, V>(out + first, x);
-                store_vec<T, V>(out + second, y);
-            }
+            const Side& side = p.side[key];
+            T* const out = static_cast<T*>(side.out) + (token0 + t) * side.out_stride +
+                           (head - (key ? q_heads : 0)) * p.head_dim;
+            store_vec<T, V>(out + first, x);
+            store_vec<T, V>(out + second, y);
         }
     }
 }
@@ -384,7 +409,8 @@ int vector_width(const Params& p) {
     const int half = p.head_dim / 2;
     for (int v = 16 / static_cast<int>(sizeof(T)); v >= 2; v /= 2) {
         const int bytes = v * static_cast<int>(sizeof(T));
-        bool ok = half % v == 0 && half / v <= 32 && half / 2 <= kTableVectors;
+        bool ok = half % v == 0 && half / v <= 32 &&
+                  p.side[0].heads <= kMaxHeads / 2 && p.side[1].heads <= kMaxHeads / 2;
         ok = ok && (p.adjacent || (p.pairs % v == 0 && (half - p.pairs) % v == 0));
         for (const Side& side : p.side) {
             if (side.heads == 0) {
@@ -395,7 +421,6 @@ int vector_width(const Params& p) {
                        stride * static_cast<long long>(sizeof(T)) % bytes == 0;
             };
             ok = ok && fits(side.in, side.in_stride) && fits(side.out, side.out_stride);
-            ok = ok && side.heads <= 4096; // item numbers and their reciprocals stay exact
         }
         if (ok) {
             return v;
@@ -409,20 +434,14 @@ int launch_vector(const Params& p, int sm_count, cudaStream_t stream) {
     VectorShape s{};
     const int half = p.head_dim / 2;
     s.chunks = half / V;
-    s.lanes = 1;
-    while (s.lanes < s.chunks) {
-        s.lanes *= 2;
-        ++s.lanes_log2;
-    }
-    for (int k = 0; k < 2; ++k) {
-        const unsigned heads = static_cast<unsigned>(p.side[k].heads);
-        s.magic[k] = heads > 1 ? static_cast<unsigned>((0x100000000ull + heads - 1) / heads) : 0u;
-    }
-    // As many tokens as fill the table's threads and give each thread a few heads, but no more
-    // than leave two blocks for every SM.
+    s.warp_groups = 32 / s.chunks;
+    const unsigned heads = static_cast<unsigned>(p.side[0].heads + p.side[1].heads);
+    s.magic = heads > 1 ? static_cast<unsigned>((0x100000000ull + heads - 1) / heads) : 0u;
+    // As many tokens as the table holds, up to 8 (more leave too few blocks to balance), but no
+    // more than give every SM 12 blocks.
     int tokens = kTableVectors * 2 / half;
-    tokens = tokens > 16 ? 16 : tokens;
-    const int spread = p.tokens / (2 * sm_count);
+    tokens = tokens > 8 ? 8 : tokens;
+    const int spread = p.tokens / (12 * sm_count);
     s.block_tokens = tokens < spread ? tokens : (spread > 0 ? spread : 1);
     const int blocks = (p.tokens + s.block_tokens - 1) / s.block_tokens;
     host::pdl_launch(qk_vector_kernel<T, V, Norm>, dim3(static_cast<unsigned>(blocks)),

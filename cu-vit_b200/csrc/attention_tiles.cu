@@ -8,10 +8,15 @@
 // tile's rows take their maxima and exponentials, so neither waits for the other longer than it
 // must. Keys and values stream through a ring of TMA stages shared by both tiles.
 //
-//   warp 0        loads (one lane)        warp 1      MMA issue
-//   warp 2        tensor memory           warp 3      -
-//   warps 4..7    rows of tile 0          warps 8..11 rows of tile 1 (one thread per row)
+//   warps 0..15   rows: warp w has tile w / 8, half (w / 4) % 2 of the tile's keys and tensor
+//                 memory lanes 32 (w % 4) .. + 31, so two threads share a row and every SM
+//                 sub-partition runs one warp of each (tile, half)
+//   warp 16       loads (one lane)
+//   warp 17       MMA issue (one lane)
+//   warp 18       tensor memory
 //
+// * The two threads of a row exchange their maxima through shared memory every step, over an
+//   mbarrier with bounded waits.
 // * Rescaling O when a maximum rises would put a round trip through tensor memory into every
 //   step. m therefore only follows the true maximum when that has risen by more than 2^8, and
 //   O is rescaled then: P stays below 2^8, sums below 2^8 per key, well inside FP32 and
@@ -23,6 +28,9 @@
 //   -inf. V rows past the end would be multiplied by P = 0, which leaves NaN where they hold NaN
 //   or infinity (they belong to other sequences, or to nobody): the at most 15 of them that the
 //   last 16-key step still reads are overwritten with zeros in shared memory first.
+// * Tensor memory is read and written by whole warps (.sync.aligned): no lane leaves or skips
+//   ahead in the row warps' loops, and stores that only some lanes make are followed by a
+//   __syncwarp.
 #include "attention_varlen.hpp"
 #include "ptx.cuh"
 #include "varlen.cuh"
@@ -34,16 +42,17 @@
 namespace cuvit::attn {
 namespace {
 
-constexpr int kTile = 128;                // query rows of a tile, keys of a step
-constexpr int kAtomBytes = kTile * 128;   // 128 rows of 64 bfloat16
-constexpr int kThreads = 384;
-constexpr float kRescaleAbove = 8.0F;     // log2
+constexpr int kTile = 128;              // query rows of a tile, keys of a step
+constexpr int kHalf = 64;               // keys of a row thread
+constexpr int kAtomBytes = kTile * 128; // 128 rows of 64 bfloat16
+constexpr int kRowWarps = 16;
+constexpr int kLoadWarp = 16;
+constexpr int kMmaWarp = 17;
+constexpr int kTmemWarp = 18;
+constexpr int kThreads = 640;
+constexpr float kRescaleAbove = 8.0F; // log2
 // Above this |m scale| (log2) the plain and the exact form of P would differ by more than 2^-14.
 constexpr float kLargeMaximum = 1024.0F;
-// Registers: 384 threads are launched with 168 each; the row warps (256 threads) take 208 and
-// leave 88 to the others: 256 * 208 + 128 * 88 = 384 * 168.
-constexpr int kRowRegisters = 208;
-constexpr int kOtherRegisters = 88;
 // Exponentials of these pairs of a 32-key chunk run on the FMA pipe (see attention.cu).
 constexpr uint32_t kPolyPairs = 0xA4A4u;
 
@@ -52,16 +61,24 @@ struct Shape {
     static constexpr bool kOverlay = Atoms == 2; // P in the columns of S
     static constexpr int kQBytes = Atoms * kAtomBytes;
     static constexpr int kSlotBytes = Atoms * kAtomBytes;
-    static constexpr int kSlots = Atoms == 2 ? 5 : 8;
+    static constexpr int kSlots = Atoms == 2 ? 4 : 8;
     static constexpr int kSlotOffset = 2 * kQBytes;
-    static constexpr int kBarrierOffset = kSlotOffset + kSlots * kSlotBytes;
-    // full, empty per slot; q_full[2], q_empty, s_full[2], s_free[2], p_full[2], o_done[2], drain
-    static constexpr int kBarriers = 2 * kSlots + 12;
-    static constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 16;
+    // Maxima and sums of a row's halves: [step parity][tile][half][row].
+    static constexpr int kExchangeOffset = kSlotOffset + kSlots * kSlotBytes;
+    static constexpr int kExchangeBytes = 2 * 2 * 2 * kTile * 4;
+    static constexpr int kBarrierOffset = kExchangeOffset + kExchangeBytes;
+    // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2],
+    // exchange[tile][quarter]
+    static constexpr int kBarriers = 2 * kSlots + 12 + 8;
+    static constexpr int kTmemSlotOffset = kBarrierOffset + 8 * kBarriers;
+    static constexpr int kSmemBytes = 1024 + kTmemSlotOffset + 16;
     static constexpr uint32_t kOColumn = 256;
     static constexpr uint32_t kOPitch = Atoms == 2 ? 128 : 64;
+    // P of a tile's first half of keys, and from there to the second half's: the overlay puts each
+    // half into the columns of the scores its own warps have read.
     static constexpr uint32_t kPColumn = Atoms == 2 ? 0 : 384;
     static constexpr uint32_t kPPitch = Atoms == 2 ? 128 : 64;
+    static constexpr uint32_t kPHalf = Atoms == 2 ? 64 : 32;
     static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 };
 
@@ -73,8 +90,20 @@ struct Item {
     int first_key; // this split's keys, within the sequence
     int end_key;
     long long reach; // row r of the block sees keys below r + reach (causal)
-    int steps[2];  // key tiles of each query tile
+    int steps0;      // key tiles of each query tile
+    int steps1;
 };
+
+__device__ __forceinline__ int tile_steps(const VarlenParams& p, const Item& item, int t) {
+    const int rows = min(kTile, item.rows - t * kTile);
+    long long end = item.end_key;
+    if (p.causal) {
+        end = min(end, item.reach + t * kTile + rows - 1);
+    }
+    return rows <= 0 || end <= item.first_key
+               ? 0
+               : static_cast<int>((end - item.first_key + kTile - 1) / kTile);
+}
 
 __device__ __forceinline__ Item find_item(const VarlenParams& p, long long index) {
     Item item;
@@ -93,106 +122,137 @@ __device__ __forceinline__ Item find_item(const VarlenParams& p, long long index
     item.first_key = min(keys, min(tiles, item.split * each) * kTile);
     item.end_key = min(keys, min(tiles, (item.split + 1) * each) * kTile);
     item.reach = static_cast<long long>(s.q_first - s.q_begin) + 1 + keys - (s.q_end - s.q_begin);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int rows = min(kTile, item.rows - t * kTile);
-        long long end = item.end_key;
-        if (p.causal) {
-            end = min(end, item.reach + t * kTile + rows - 1);
-        }
-        item.steps[t] = rows <= 0 || end <= item.first_key
-                            ? 0
-                            : static_cast<int>((end - item.first_key + kTile - 1) / kTile);
-    }
+    item.steps0 = tile_steps(p, item, 0);
+    item.steps1 = tile_steps(p, item, 1);
     return item;
 }
 
-__device__ __forceinline__ float row_maximum(const uint32_t (&s)[kTile]) {
-    float m[4];
+// Scores at or past `limit` become -inf.
+__device__ __forceinline__ void mask(uint32_t (&s)[32], int limit) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        m[c] = __uint_as_float(s[c]);
+    for (int c = 0; c < 32; ++c) {
+        s[c] = c < limit ? s[c] : 0xFF800000u;
     }
-#pragma unroll
-    for (int j = 4; j + 8 <= kTile; j += 8) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            m[c] = dev::max3(m[c], __uint_as_float(s[j + c]), __uint_as_float(s[j + 4 + c]));
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        m[c] = fmaxf(m[c], __uint_as_float(s[kTile - 4 + c]));
-    }
-    return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// P = 2^(scale (s - m)) of 128 scores, packed, into tensor memory, and their sum. The plain form
+__device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
+    float m[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        m[c] = __uint_as_float(s[16 * c]);
+#pragma unroll
+        for (int j = 1; j < 15; j += 2) {
+            m[c] = dev::max3(m[c], __uint_as_float(s[16 * c + j]),
+                             __uint_as_float(s[16 * c + j + 1]));
+        }
+        m[c] = fmaxf(m[c], __uint_as_float(s[16 * c + 15]));
+    }
+    return fmaxf(m[0], m[1]);
+}
+
+// P = 2^(scale (s - m)) of 32 scores, packed, into tensor memory, and their sum. The plain form
 // folds scale and m into one multiply-add, off by a row-wide factor 2^d, |d| <= 2^-24 |m scale|
 // (it cancels in the quotient), and takes some exponentials on the FMA pipe. The exact form, for
 // tiles with masked scores and rows with a very large m, subtracts first, so that no m overflows
 // the exponent, and keeps to the special-function unit, whose 2^-inf is zero (the polynomial's is
 // 2^-125).
 template <bool Exact>
-__device__ __forceinline__ float exponentials(const uint32_t (&s)[kTile], float scale, float m,
+__device__ __forceinline__ float exponentials(const uint32_t (&s)[32], float scale, float m,
                                               uint32_t p_tmem) {
     const uint64_t scale2 = dev::f32x2(scale, scale);
     const float minus = Exact ? -m : -m * scale;
     const uint64_t minus2 = dev::f32x2(minus, minus);
     uint64_t sums[2] = {dev::f32x2(0.0F, 0.0F), dev::f32x2(0.0F, 0.0F)};
+    uint32_t packed[16];
 #pragma unroll
-    for (int c = 0; c < kTile / 32; ++c) {
-        uint32_t packed[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const uint64_t s2 = dev::f32x2(__uint_as_float(s[32 * c + 2 * j]),
-                                           __uint_as_float(s[32 * c + 2 * j + 1]));
-            const uint64_t x2 = Exact ? dev::mul_f32x2(dev::add_f32x2(s2, minus2), scale2)
-                                      : dev::fma_f32x2(s2, scale2, minus2);
-            const float2 x = dev::f32x2_split(x2);
-            float2 e;
-            if (!Exact && ((kPolyPairs >> j) & 1u)) {
-                e = dev::exp2_poly2(x.x, x.y);
-            } else {
-                e = make_float2(dev::ex2_approx(x.x), dev::ex2_approx(x.y));
-            }
-            packed[j] = dev::pack_bf16x2(e.x, e.y);
-            sums[j & 1] = dev::add_f32x2(sums[j & 1], dev::f32x2(e.x, e.y));
+    for (int j = 0; j < 16; ++j) {
+        const uint64_t s2 = dev::f32x2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
+        const uint64_t x2 = Exact ? dev::mul_f32x2(dev::add_f32x2(s2, minus2), scale2)
+                                  : dev::fma_f32x2(s2, scale2, minus2);
+        const float2 x = dev::f32x2_split(x2);
+        float2 e;
+        if (!Exact && ((kPolyPairs >> j) & 1u)) {
+            e = dev::exp2_poly2(x.x, x.y);
+        } else {
+            e = make_float2(dev::ex2_approx(x.x), dev::ex2_approx(x.y));
         }
-        dev::tmem_store_16(p_tmem + 16 * c, packed);
+        packed[j] = dev::pack_bf16x2(e.x, e.y);
+        sums[j & 1] = dev::add_f32x2(sums[j & 1], dev::f32x2(e.x, e.y));
     }
+    dev::tmem_store_16(p_tmem, packed);
     const float2 total = dev::f32x2_split(dev::add_f32x2(sums[0], sums[1]));
     return total.x + total.y;
+}
+
+// S = Q K^T: k_steps steps of 16 elements, 4 to an atom.
+template <int Atoms>
+__device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc,
+                                             uint32_t idesc, int k_steps) {
+    constexpr uint64_t kAtomStep = kAtomBytes >> 4; // descriptors count 16-byte units
+    if (k_steps == 4 * Atoms) {
+#pragma unroll
+        for (int kk = 0; kk < 4 * Atoms; ++kk) {
+            const uint64_t at = static_cast<uint64_t>(kk >> 2) * kAtomStep + 2u * (kk & 3);
+            dev::mma_ss<dev::MmaKind::kF16>(d_tmem, q_desc + at, k_desc + at, idesc,
+                                            kk > 0 ? 1u : 0u);
+        }
+    } else {
+#pragma unroll 1
+        for (int kk = 0; kk < k_steps; ++kk) {
+            const uint64_t at = static_cast<uint64_t>(kk >> 2) * kAtomStep + 2u * (kk & 3);
+            dev::mma_ss<dev::MmaKind::kF16>(d_tmem, q_desc + at, k_desc + at, idesc,
+                                            kk > 0 ? 1u : 0u);
+        }
+    }
+}
+
+// O (+)= P V: v_steps steps of 16 keys, the first 4 in P's first half.
+template <int Atoms>
+__device__ __forceinline__ void issue_outputs(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc,
+                                              uint32_t idesc, int v_steps, uint32_t accumulate) {
+    if (v_steps == kTile / 16) {
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk) {
+            dev::mma_ts<dev::MmaKind::kF16>(
+                d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+                v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
+                kk > 0 ? 1u : accumulate);
+        }
+    } else {
+#pragma unroll 1
+        for (int kk = 0; kk < v_steps; ++kk) {
+            dev::mma_ts<dev::MmaKind::kF16>(
+                d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+                v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
+                kk > 0 ? 1u : accumulate);
+        }
+    }
 }
 
 template <int Atoms>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q,
                            const __grid_constant__ CUtensorMap map_k,
-                           const __grid_constant__ CUtensorMap map_v, const VarlenParams p,
-                           const long long items, unsigned* const status) {
+                           const __grid_constant__ CUtensorMap map_v,
+                           const __grid_constant__ VarlenParams p, const long long items,
+                           unsigned* const status) {
     using S = Shape<Atoms>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = dev::smem_u32(smem_raw);
     const uint32_t base = (raw_base + 1023u) & ~1023u;
     uint8_t* const smem = smem_raw + (base - raw_base);
-    const auto q_smem = [&](int t) -> uint32_t { return base + t * S::kQBytes; };
-    const auto slot_smem = [&](int i) -> uint32_t {
-        return base + S::kSlotOffset + i * S::kSlotBytes;
-    };
     const uint32_t bars = base + S::kBarrierOffset;
     const auto full = [&](int i) -> uint32_t { return bars + 8u * i; };
     const auto empty = [&](int i) -> uint32_t { return bars + 8u * (S::kSlots + i); };
     const uint32_t more = bars + 16u * S::kSlots;
-    const auto q_full = [&](int t) -> uint32_t { return more + 8u * t; };
+    const uint32_t q_full = more;        // + 8 t
     const uint32_t q_empty = more + 16;
-    const auto s_full = [&](int t) -> uint32_t { return more + 24 + 8u * t; };
-    const auto s_free = [&](int t) -> uint32_t { return more + 40 + 8u * t; };
-    const auto p_full = [&](int t) -> uint32_t { return more + 56 + 8u * t; };
-    const auto o_done = [&](int t) -> uint32_t { return more + 72 + 8u * t; };
-    const uint32_t drain = more + 88;
-    uint32_t* const tmem_slot =
-        reinterpret_cast<uint32_t*>(smem + S::kBarrierOffset + 8 * S::kBarriers);
+    const uint32_t drain = more + 24;
+    const uint32_t s_full = more + 32;   // + 8 t
+    const uint32_t s_free = more + 48;   // + 8 t
+    const uint32_t p_full = more + 64;   // + 8 t
+    const uint32_t o_done = more + 80;   // + 8 t
+    const uint32_t exchange = more + 96; // + 8 (4 t + quarter)
 
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
@@ -201,336 +261,358 @@ __global__ void __launch_bounds__(kThreads, 1)
             dev::mbar_init(full(i), 1);
             dev::mbar_init(empty(i), 1);
         }
-        for (int t = 0; t < 2; ++t) {
-            dev::mbar_init(q_full(t), 1);
-            dev::mbar_init(s_full(t), 1);
-            dev::mbar_init(s_free(t), kTile);
-            dev::mbar_init(p_full(t), kTile);
-            dev::mbar_init(o_done(t), 1);
+        for (uint32_t t = 0; t < 2; ++t) {
+            dev::mbar_init(q_full + 8 * t, 1);
+            dev::mbar_init(s_full + 8 * t, 1);
+            dev::mbar_init(s_free + 8 * t, kRowWarps / 2);
+            dev::mbar_init(p_full + 8 * t, kRowWarps / 2);
+            dev::mbar_init(o_done + 8 * t, 1);
+        }
+        for (uint32_t i = 0; i < 8; ++i) {
+            dev::mbar_init(exchange + 8 * i, 2); // the two warps of a tile's lane quarter
         }
         dev::mbar_init(q_empty, 1);
         dev::mbar_init(drain, 1);
         dev::fence_barrier_init();
     }
-    if (warp == 2) {
-        dev::tmem_alloc(dev::smem_u32(tmem_slot), 512);
+    if (warp == kTmemWarp) {
+        dev::tmem_alloc(base + S::kTmemSlotOffset, 512);
         dev::tmem_relinquish();
     }
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = *reinterpret_cast<const uint32_t*>(smem + S::kTmemSlotOffset);
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
 
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-        if (warp == 0 && lane == 0) {
-            // ---------------- loads ----------------
-            dev::tma_prefetch_descriptor(&map_q);
-            dev::tma_prefetch_descriptor(&map_k);
-            dev::tma_prefetch_descriptor(&map_v);
-            int slot = 0;
-            uint32_t phase = 0;
-            uint32_t q_phase = 0;     // items with keys so far
-            uint32_t q_loads[2] = {}; // loads of each query tile so far
-            bool ok = true;
-            const auto load_kv = [&](const CUtensorMap* map, int kv_head, int row) {
-                if (!dev::mbar_wait(empty(slot), phase ^ 1u, status)) {
-                    ok = false;
-                    return;
+    if (warp == kLoadWarp && lane == 0) {
+        // ---------------- loads ----------------
+        dev::tma_prefetch_descriptor(&map_q);
+        dev::tma_prefetch_descriptor(&map_k);
+        dev::tma_prefetch_descriptor(&map_v);
+        int slot = 0;
+        uint32_t phase = 0;
+        uint32_t q_phase = 0;                 // items with keys so far
+        uint32_t q_loads0 = 0, q_loads1 = 0;  // loads of each query tile so far
+        bool ok = true;
+        const auto load_kv = [&](const CUtensorMap* map, int kv_head, int row) {
+            if (!dev::mbar_wait(empty(slot), phase ^ 1u, status)) {
+                ok = false;
+                return;
+            }
+            dev::mbar_arrive_expect_tx(full(slot), S::kSlotBytes);
+            for (int a = 0; a < Atoms; ++a) {
+                const int c[3] = {64 * a, kv_head, row};
+                dev::tma_load(base + S::kSlotOffset + slot * S::kSlotBytes + a * kAtomBytes, map,
+                              full(slot), 3, c);
+            }
+            if (++slot == S::kSlots) {
+                slot = 0;
+                phase ^= 1u;
+            }
+        };
+        const auto load_q = [&](int t, int head, int row) {
+            dev::mbar_arrive_expect_tx(q_full + 8 * t, S::kQBytes);
+            for (int a = 0; a < Atoms; ++a) {
+                const int c[3] = {64 * a, head, row};
+                dev::tma_load(base + t * S::kQBytes + a * kAtomBytes, &map_q, q_full + 8 * t, 3, c);
+            }
+        };
+        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
+            const Item item = find_item(p, index);
+            const int steps = max(item.steps0, item.steps1);
+            if (steps == 0) {
+                continue;
+            }
+            if (!dev::mbar_wait(q_empty, (q_phase & 1u) ^ 1u, status)) {
+                ok = false;
+                break;
+            }
+            ++q_phase;
+            if (item.steps0 > 0) {
+                ++q_loads0;
+                load_q(0, item.head, item.s.q_first);
+            }
+            if (item.steps1 > 0) {
+                ++q_loads1;
+                load_q(1, item.head, item.s.q_first + kTile);
+            }
+            const int kv_head = item.head / p.group;
+            const int row = item.s.kv_begin + item.first_key;
+            // In the order the MMA warp takes them.
+            load_kv(&map_k, kv_head, row);
+            for (int j = 0; j < steps && ok; ++j) {
+                if (S::kOverlay) {
+                    load_kv(&map_v, kv_head, row + j * kTile);
                 }
-                dev::mbar_arrive_expect_tx(full(slot), S::kSlotBytes);
-                for (int a = 0; a < Atoms; ++a) {
-                    const int c[3] = {64 * a, kv_head, row};
-                    dev::tma_load(slot_smem(slot) + a * kAtomBytes, map, full(slot), 3, c);
+                if (ok && j + 1 < steps) {
+                    load_kv(&map_k, kv_head, row + (j + 1) * kTile);
                 }
-                if (++slot == S::kSlots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-            };
-            for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
-                const Item item = find_item(p, index);
-                const int steps = max(item.steps[0], item.steps[1]);
-                if (steps == 0) {
-                    continue;
-                }
-                if (!dev::mbar_wait(q_empty, (q_phase & 1u) ^ 1u, status)) {
-                    ok = false;
-                    break;
-                }
-                ++q_phase;
-                for (int t = 0; t < 2; ++t) {
-                    if (item.steps[t] > 0) {
-                        ++q_loads[t];
-                        dev::mbar_arrive_expect_tx(q_full(t), S::kQBytes);
-                        for (int a = 0; a < Atoms; ++a) {
-                            const int c[3] = {64 * a, item.head, item.s.q_first + t * kTile};
-                            dev::tma_load(q_smem(t) + a * kAtomBytes, &map_q, q_full(t), 3, c);
-                        }
-                    }
-                }
-                const int kv_head = item.head / p.group;
-                const int row = item.s.kv_begin + item.first_key;
-                // In the order the MMA warp takes them.
-                load_kv(&map_k, kv_head, row);
-                for (int j = 0; j < steps && ok; ++j) {
-                    if (S::kOverlay) {
-                        load_kv(&map_v, kv_head, row + j * kTile);
-                    }
-                    if (ok && j + 1 < steps) {
-                        load_kv(&map_k, kv_head, row + (j + 1) * kTile);
-                    }
-                    if (ok && !S::kOverlay) {
-                        load_kv(&map_v, kv_head, row + j * kTile);
-                    }
+                if (ok && !S::kOverlay) {
+                    load_kv(&map_v, kv_head, row + j * kTile);
                 }
             }
-            if (!ok) {
-                // Every load issued lands before the CTA's shared memory goes.
-                for (int i = 0; i < S::kSlots; ++i) {
-                    dev::mbar_drain_wait(full(i), phase ^ (i < slot ? 0u : 1u));
-                }
-                for (int t = 0; t < 2; ++t) {
-                    if (q_loads[t] > 0) {
-                        dev::mbar_drain_wait(q_full(t), (q_loads[t] - 1) & 1u);
-                    }
-                }
+        }
+        if (!ok) {
+            // Every load issued lands before the CTA's shared memory goes.
+            for (int i = 0; i < S::kSlots; ++i) {
+                dev::mbar_drain_wait(full(i), phase ^ (i < slot ? 0u : 1u));
             }
-        } else if (warp == 1) {
-            // ---------------- MMA issue (the warp together, one lane issuing) ----------------
-            const int k_steps = (p.head_dim + 15) / 16;
-            const uint32_t idesc_o =
-                dev::make_idesc(1u, kTile, 16 * k_steps, false, true);
-            int slot = 0;
-            uint32_t phase = 0;
-            uint32_t q_phase[2] = {};
-            uint32_t free_phase[2] = {};
-            uint32_t p_phase[2] = {};
-            bool ok = true;
-            const auto next_slot = [&]() {
-                if (++slot == S::kSlots) {
-                    slot = 0;
-                    phase ^= 1u;
-                }
-            };
-            // Keys of a tile, rounded up to whole 16-key steps.
-            const auto scores = [&](int t, uint32_t k_smem, int keys16) {
+            if (q_loads0 > 0) {
+                dev::mbar_drain_wait(q_full, (q_loads0 - 1) & 1u);
+            }
+            if (q_loads1 > 0) {
+                dev::mbar_drain_wait(q_full + 8, (q_loads1 - 1) & 1u);
+            }
+        }
+    } else if (warp == kMmaWarp && lane == 0) {
+        // ---------------- MMA issue ----------------
+        const int k_steps = (p.head_dim + 15) / 16;
+        const uint32_t idesc_o = dev::make_idesc(1u, kTile, 16 * k_steps, false, true);
+        // Descriptors are built once and stepped by adding to their start-address field.
+        const uint64_t q_desc0 = dev::smem_desc_sw128(base, 16, 1024);
+        const uint64_t k_desc0 = dev::smem_desc_sw128(base + S::kSlotOffset, 16, 1024);
+        const uint64_t v_desc0 = dev::smem_desc(base + S::kSlotOffset, kAtomBytes, 1024,
+                                                dev::kLayoutSwizzle128);
+        constexpr uint64_t kSlotStep = S::kSlotBytes >> 4;
+        constexpr uint64_t kQStep = S::kQBytes >> 4;
+        int slot = 0;
+        uint32_t phase = 0;
+        uint32_t q_phase[2] = {0u, 0u};
+        uint32_t free_phase[2] = {0u, 0u};
+        uint32_t p_phase[2] = {0u, 0u};
+        bool ok = true;
+        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
+            const Item item = find_item(p, index);
+            const int tile_steps[2] = {item.steps0, item.steps1};
+            const int steps = max(item.steps0, item.steps1);
+            if (steps == 0) {
+                continue;
+            }
+            const int keys = item.end_key - item.first_key;
+            // The first scores.
+            {
+                const int keys16 = (min(kTile, keys) + 15) & ~15;
                 const uint32_t idesc = dev::make_idesc(1u, kTile, keys16, false, false);
-                for (int kk = 0; kk < k_steps; ++kk) {
-                    const uint32_t offset = (kk >> 2) * kAtomBytes + (kk & 3) * 32;
-                    dev::mma_ss<dev::MmaKind::kF16>(
-                        tmem + t * kTile, dev::smem_desc_sw128(q_smem(t) + offset, 16, 1024),
-                        dev::smem_desc_sw128(k_smem + offset, 16, 1024), idesc, kk > 0 ? 1u : 0u);
-                }
-                dev::tc_commit(s_full(t));
-            };
-            for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
-                const Item item = find_item(p, index);
-                const int steps = max(item.steps[0], item.steps[1]);
-                if (steps == 0) {
-                    continue;
-                }
-                const int keys = item.end_key - item.first_key;
-                const auto keys_of = [&](int j) { return min(kTile, keys - j * kTile); };
-                const auto round16 = [](int n) { return (n + 15) & ~15; };
-                // The first scores.
-                ok = dev::mbar_wait_warp(full(slot), phase, status);
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (item.steps[t] > 0) {
-                        ok = dev::mbar_wait_warp(q_full(t), q_phase[t], status);
+                ok = dev::mbar_wait(full(slot), phase, status);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (ok && tile_steps[t] > 0) {
+                        ok = dev::mbar_wait(q_full + 8 * t, q_phase[t], status);
                         q_phase[t] ^= 1u;
-                        if (ok && lane == 0) {
+                        if (ok) {
                             dev::tc_fence_after();
-                            scores(t, slot_smem(slot), round16(keys_of(0)));
+                            issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
+                                                k_desc0 + slot * kSlotStep, idesc, k_steps);
+                            dev::tc_commit(s_full + 8 * t);
                         }
                     }
                 }
                 if (!ok) {
                     break;
                 }
-                if (lane == 0) {
-                    dev::tc_commit(empty(slot));
-                    if (steps == 1) {
-                        dev::tc_commit(q_empty);
-                    }
+                dev::tc_commit(empty(slot));
+                if (steps == 1) {
+                    dev::tc_commit(q_empty);
                 }
-                next_slot();
-                for (int j = 0; j < steps && ok; ++j) {
-                    // Slots of this step: the next keys and these values, in the loads' order.
-                    const bool more_keys = j + 1 < steps;
-                    int v_slot, k_slot;
-                    uint32_t v_phase, k_phase;
-                    if (!S::kOverlay && more_keys) {
-                        k_slot = slot;
-                        k_phase = phase;
-                        next_slot();
-                    }
-                    v_slot = slot;
-                    v_phase = phase;
-                    next_slot();
-                    if (S::kOverlay && more_keys) {
-                        k_slot = slot;
-                        k_phase = phase;
-                        next_slot();
-                    }
-                    if (!S::kOverlay && more_keys) {
-                        // The next scores as soon as the rows have read these.
-                        ok = dev::mbar_wait_warp(full(k_slot), k_phase, status);
-                        for (int t = 0; t < 2 && ok; ++t) {
-                            if (j + 1 < item.steps[t]) {
-                                ok = dev::mbar_wait_warp(s_free(t), free_phase[t], status);
-                                if (ok && lane == 0) {
-                                    dev::tc_fence_after();
-                                    scores(t, slot_smem(k_slot), round16(keys_of(j + 1)));
-                                }
-                            }
-                        }
-                        if (!ok) {
-                            break;
-                        }
-                        if (lane == 0) {
-                            dev::tc_commit(empty(k_slot));
-                        }
-                    }
-                    // s_free completes once per step of a tile, whether or not more scores follow.
-                    for (int t = 0; t < 2; ++t) {
-                        free_phase[t] ^= j < item.steps[t] ? 1u : 0u;
-                    }
-                    ok = dev::mbar_wait_warp(full(v_slot), v_phase, status);
-                    if (!ok) {
-                        break;
-                    }
-                    const int live = keys_of(j);
-                    const int live16 = round16(live);
-                    if (live < live16) {
-                        // Values behind the sequence's end that the last 16-key step reads.
-                        uint8_t* const v_bytes = smem + (slot_smem(v_slot) - base);
-                        const int vectors = (live16 - live) * 8;
-                        for (int i = lane; i < vectors * Atoms; i += 32) {
-                            const int a = i / vectors;
-                            reinterpret_cast<uint4*>(v_bytes + a * kAtomBytes +
-                                                     live * 128)[i - a * vectors] =
-                                make_uint4(0, 0, 0, 0);
-                        }
-                        dev::fence_proxy_async_shared();
-                        __syncwarp();
-                    }
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        if (j >= item.steps[t]) {
-                            continue;
-                        }
-                        ok = dev::mbar_wait_warp(p_full(t), p_phase[t], status);
-                        p_phase[t] ^= 1u;
-                        if (ok && lane == 0) {
-                            dev::tc_fence_after();
-                            for (int kk = 0; kk < live16 / 16; ++kk) {
-                                dev::mma_ts<dev::MmaKind::kF16>(
-                                    tmem + S::kOColumn + t * S::kOPitch,
-                                    tmem + S::kPColumn + t * S::kPPitch + 8 * kk,
-                                    dev::smem_desc(slot_smem(v_slot) + kk * 2048, kAtomBytes, 1024,
-                                                   dev::kLayoutSwizzle128),
-                                    idesc_o, j > 0 || kk > 0 ? 1u : 0u);
-                            }
-                            dev::tc_commit(o_done(t));
-                        }
-                        if (ok && S::kOverlay && j + 1 < item.steps[t]) {
-                            ok = dev::mbar_wait_warp(full(k_slot), k_phase, status);
-                            if (ok && lane == 0) {
-                                dev::tc_fence_after();
-                                scores(t, slot_smem(k_slot), round16(keys_of(j + 1)));
-                            }
-                        }
-                    }
-                    if (!ok) {
-                        break;
-                    }
-                    if (lane == 0) {
-                        dev::tc_commit(empty(v_slot));
-                        if (S::kOverlay && more_keys) {
-                            dev::tc_commit(empty(k_slot));
-                        }
-                        if (j + 2 == steps) {
-                            dev::tc_commit(q_empty); // the last scores have been issued
-                        }
-                    }
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
                 }
             }
-            // Every MMA issued has finished before the CTA's shared and tensor memory go.
-            if (lane == 0) {
-                dev::tc_commit(drain);
-                dev::mbar_drain_wait(drain, 0);
+            for (int j = 0; j < steps; ++j) {
+                // Slots of this step: these values and the next keys, in the loads' order.
+                const bool next = j + 1 < steps;
+                int slot2 = slot + 1;
+                uint32_t phase2 = phase;
+                if (slot2 == S::kSlots) {
+                    slot2 = 0;
+                    phase2 ^= 1u;
+                }
+                const bool keys_first = !S::kOverlay && next;
+                const int v_slot = keys_first ? slot2 : slot;
+                const uint32_t v_phase = keys_first ? phase2 : phase;
+                const int k_slot = keys_first ? slot : slot2;
+                const uint32_t k_phase = keys_first ? phase : phase2;
+                const int next16 = (min(kTile, keys - (j + 1) * kTile) + 15) & ~15;
+                const uint32_t idesc_next =
+                    dev::make_idesc(1u, kTile, next ? next16 : 16, false, false);
+                if (keys_first) {
+                    // The next scores as soon as the rows have read these.
+                    ok = dev::mbar_wait(full(k_slot), k_phase, status);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (ok && j + 1 < tile_steps[t]) {
+                            ok = dev::mbar_wait(s_free + 8 * t, free_phase[t], status);
+                            if (ok) {
+                                dev::tc_fence_after();
+                                issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
+                                                    k_desc0 + k_slot * kSlotStep, idesc_next,
+                                                    k_steps);
+                                dev::tc_commit(s_full + 8 * t);
+                            }
+                        }
+                    }
+                    if (!ok) {
+                        break;
+                    }
+                    dev::tc_commit(empty(k_slot));
+                }
+                // s_free completes once per step of a tile, whether or not more scores follow.
+                free_phase[0] ^= j < tile_steps[0] ? 1u : 0u;
+                free_phase[1] ^= j < tile_steps[1] ? 1u : 0u;
+                ok = dev::mbar_wait(full(v_slot), v_phase, status);
+                if (!ok) {
+                    break;
+                }
+                const int live = min(kTile, keys - j * kTile);
+                const int live16 = (live + 15) & ~15;
+                if (live < live16) {
+                    // Values behind the sequence's end that the last 16-key step reads.
+                    const float zero[4] = {0.0F, 0.0F, 0.0F, 0.0F};
+                    for (int a = 0; a < Atoms; ++a) {
+                        const uint32_t rows = base + S::kSlotOffset + v_slot * S::kSlotBytes +
+                                              a * kAtomBytes + live * 128;
+#pragma unroll 4
+                        for (int i = 0; i < (live16 - live) * 8; ++i) {
+                            dev::st_shared_v4(rows + 16 * i, zero);
+                        }
+                    }
+                    dev::fence_proxy_async_shared();
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (ok && j < tile_steps[t]) {
+                        ok = dev::mbar_wait(p_full + 8 * t, p_phase[t], status);
+                        p_phase[t] ^= 1u;
+                        if (ok) {
+                            dev::tc_fence_after();
+                            issue_outputs<Atoms>(tmem + S::kOColumn + t * S::kOPitch,
+                                                 tmem + S::kPColumn + t * S::kPPitch,
+                                                 v_desc0 + v_slot * kSlotStep, idesc_o, live16 / 16,
+                                                 j > 0 ? 1u : 0u);
+                            dev::tc_commit(o_done + 8 * t);
+                        }
+                        if (S::kOverlay && ok && j + 1 < tile_steps[t]) {
+                            ok = dev::mbar_wait(full(k_slot), k_phase, status);
+                            if (ok) {
+                                dev::tc_fence_after();
+                                issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
+                                                    k_desc0 + k_slot * kSlotStep, idesc_next,
+                                                    k_steps);
+                                dev::tc_commit(s_full + 8 * t);
+                            }
+                        }
+                    }
+                }
+                if (!ok) {
+                    break;
+                }
+                dev::tc_commit(empty(v_slot));
+                if (S::kOverlay && next) {
+                    dev::tc_commit(empty(k_slot));
+                }
+                if (j + 2 == steps) {
+                    dev::tc_commit(q_empty); // the last scores have been issued
+                }
+                // This step took the values' slot and, if keys followed, theirs.
+                slot = next ? slot2 : slot;
+                phase = next ? phase2 : phase;
+                if (++slot == S::kSlots) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
             }
         }
-    } else {
+        // Every MMA issued has finished before the CTA's shared and tensor memory go.
+        dev::tc_commit(drain);
+        dev::mbar_drain_wait(drain, 0);
+    } else if (warp < kRowWarps) {
         // ---------------- rows ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegisters));
-        const int t = (warp - 4) / 4;
+        const int t = warp >> 3;
+        const int half = (warp >> 2) & 1;
         const int quarter = warp & 3; // the tensor memory lanes this warp may access
         const int row = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_tmem = tmem + lanes + t * kTile;
-        const uint32_t p_tmem = tmem + lanes + S::kPColumn + t * S::kPPitch;
+        const uint32_t s_tmem = tmem + lanes + t * kTile + half * kHalf;
+        const uint32_t p_tmem = tmem + lanes + S::kPColumn + t * S::kPPitch + half * S::kPHalf;
         const uint32_t o_tmem = tmem + lanes + S::kOColumn + t * S::kOPitch;
-        const int o_columns = 16 * ((p.head_dim + 15) / 16);
+        const int o_chunks = (p.head_dim + 15) / 16; // of 16 columns; the halves take alternate ones
+        const uint32_t exchange_bar = exchange + 8u * static_cast<uint32_t>(4 * t + quarter);
+        float* const mine = reinterpret_cast<float*>(smem + S::kExchangeOffset) +
+                            (2 * t + half) * kTile + row;
+        const float* const theirs = reinterpret_cast<const float*>(smem + S::kExchangeOffset) +
+                                    (2 * t + (half ^ 1)) * kTile + row;
+        constexpr int kParity = 4 * kTile; // floats between the two exchange buffers
         uint32_t s_phase = 0;
-        uint32_t o_phase = 0; // of the tile's next P V to complete
+        uint32_t o_phase = 0;     // of the tile's next P V to complete
+        uint32_t exchanges = 0;   // so far
         bool ok = true;
+        // Gives `value` to the row's other thread and returns that thread's.
+        const auto swap = [&](float value) -> float {
+            const int at = (exchanges & 1u) ? kParity : 0;
+            mine[at] = value;
+            __syncwarp();
+            if (lane == 0) {
+                dev::mbar_arrive(exchange_bar);
+            }
+            ok = dev::mbar_wait_warp(exchange_bar, exchanges & 1u, status);
+            ++exchanges;
+            return theirs[at];
+        };
         for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
             const Item item = find_item(p, index);
             const int rows = item.rows - t * kTile; // may be 0 or less
             if (rows <= 0) {
                 continue;
             }
-            const int steps = item.steps[t];
+            const int steps = t == 0 ? item.steps0 : item.steps1;
             const bool live_warp = quarter * 32 < rows;
-            // Keys this row sees, from the split's first on.
+            // Keys of this thread's half that its row sees, from the split's first on.
             long long end = item.end_key;
             if (p.causal) {
                 end = max(0LL, min(end, item.reach + t * kTile + row));
             }
-            const int row_keys = static_cast<int>(max(0LL, end - item.first_key));
+            const int row_keys = static_cast<int>(max(0LL, end - item.first_key)) - half * kHalf;
             float m = 0.0F; // unscaled
             float sum = 0.0F;
-            for (int j = 0; j < steps; ++j) {
-                ok = dev::mbar_wait_warp(s_full(t), s_phase, status);
+            for (int j = 0; j < steps && ok; ++j) {
+                ok = dev::mbar_wait_warp(s_full + 8 * t, s_phase, status);
                 s_phase ^= 1u;
                 if (!ok) {
                     break;
                 }
                 dev::tc_fence_after();
-                uint32_t s[kTile];
                 if (live_warp) {
+                    // Scores are read 32 at a time, once for the maximum and once for the
+                    // exponentials: 64 held over both would not fit the 96 registers.
+                    const int limit = row_keys - j * kTile;
+                    const bool masked = __any_sync(0xFFFFFFFFu, limit < kHalf);
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < kTile / 32; ++c) {
-                        dev::tmem_load_32(s_tmem + 32 * c,
-                                          *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t s[32];
+                        dev::tmem_load_32(s_tmem + 32 * c, s);
+                        dev::tmem_wait_load();
+                        if (masked) {
+                            mask(s, limit - 32 * c);
+                        }
+                        top = fmaxf(top, maximum(s));
                     }
-                    dev::tmem_wait_load();
-                }
-                if (!S::kOverlay) {
-                    dev::tc_fence_before();
-                    dev::mbar_arrive(s_free(t));
-                    if (j > 0) {
+                    top = fmaxf(top, swap(top));
+                    if (!ok) {
+                        break;
+                    }
+                    if (!S::kOverlay && j > 0) {
                         // P V of the previous step has read P and written O.
-                        ok = dev::mbar_wait_warp(o_done(t), o_phase, status);
+                        ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
                         o_phase ^= 1u;
                         if (!ok) {
                             break;
                         }
                         dev::tc_fence_after();
                     }
-                }
-                if (live_warp) {
-                    const int limit = row_keys - j * kTile;
-                    if (__any_sync(0xFFFFFFFFu, limit < kTile)) {
-#pragma unroll
-                        for (int c = 0; c < kTile; ++c) {
-                            s[c] = c < limit ? s[c] : 0xFF800000u; // -inf
-                        }
-                    }
-                    const float top = row_maximum(s);
                     if (j == 0) {
                         m = top == -INFINITY ? 0.0F : top;
                     } else {
@@ -540,26 +622,58 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float factor = dev::ex2_approx((m - raised) * p.scale_log2);
                             m = raised;
                             sum *= factor;
-                            for (int c = 0; c < o_columns; c += 16) {
+#pragma unroll 1
+                            for (int c = half; c < o_chunks; c += 2) {
                                 uint32_t o[16];
-                                dev::tmem_load_16(o_tmem + c, o);
+                                dev::tmem_load_16(o_tmem + 16 * c, o);
                                 dev::tmem_wait_load();
 #pragma unroll
                                 for (int x = 0; x < 16; ++x) {
                                     o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
                                 }
-                                dev::tmem_store_16(o_tmem + c, o);
+                                dev::tmem_store_16(o_tmem + 16 * c, o);
                             }
                         }
                     }
-                    const bool exact = limit < kTile || fabsf(m * p.scale_log2) > kLargeMaximum;
-                    sum += __any_sync(0xFFFFFFFFu, exact)
-                               ? exponentials<true>(s, p.scale_log2, m, p_tmem)
-                               : exponentials<false>(s, p.scale_log2, m, p_tmem);
+                    const bool exact =
+                        masked || __any_sync(0xFFFFFFFFu,
+                                             fabsf(m * p.scale_log2) > kLargeMaximum);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t s[32];
+                        dev::tmem_load_32(s_tmem + 32 * c, s);
+                        dev::tmem_wait_load();
+                        if (!S::kOverlay && c == 1) {
+                            dev::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                dev::mbar_arrive(s_free + 8 * t);
+                            }
+                            __syncwarp();
+                        }
+                        if (exact) {
+                            if (masked) {
+                                mask(s, limit - 32 * c);
+                            }
+                            sum += exponentials<true>(s, p.scale_log2, m, p_tmem + 16 * c);
+                        } else {
+                            sum += exponentials<false>(s, p.scale_log2, m, p_tmem + 16 * c);
+                        }
+                    }
                     dev::tmem_wait_store();
+                } else if (!S::kOverlay) {
+                    __syncwarp();
+                    if (lane == 0) {
+                        dev::mbar_arrive(s_free + 8 * t);
+                    }
+                    o_phase ^= j > 0 ? 1u : 0u;
                 }
                 dev::tc_fence_before();
-                dev::mbar_arrive(p_full(t));
+                __syncwarp();
+                if (lane == 0) {
+                    dev::mbar_arrive(p_full + 8 * t);
+                }
+                __syncwarp();
             }
             if (!ok) {
                 break;
@@ -570,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (S::kOverlay) {
                     o_phase ^= static_cast<uint32_t>(steps - 1) & 1u;
                 }
-                ok = dev::mbar_wait_warp(o_done(t), o_phase, status);
+                ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
                 o_phase ^= 1u;
                 if (!ok) {
                     break;
@@ -578,20 +692,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::tc_fence_after();
             }
             if (!live_warp) {
-                continue;
+                continue; // the whole warp
+            }
+            sum += swap(sum);
+            if (!ok) {
+                break;
             }
             const bool live = row < rows;
-            const long long token = item.s.q_first + t * kTile + row;
+            const long long token = static_cast<long long>(item.s.q_first) + t * kTile + row;
             const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
             const long long part =
                 (static_cast<long long>(item.split) * p.q_tokens + token) * p.q_heads + item.head;
-            if (live && p.splits > 1) {
-                p.part_stats[part] = make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
+            if (live && half == 0 && p.splits > 1) {
+                p.part_stats[part] =
+                    make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
             }
-            for (int c = 0; c < o_columns; c += 16) {
+#pragma unroll 1
+            for (int c = half; c < o_chunks; c += 2) {
                 uint32_t o[16];
+                // The read is warp-wide: lanes that store below, and those that do not, meet first.
+                __syncwarp();
                 if (steps > 0) {
-                    dev::tmem_load_16(o_tmem + c, o);
+                    dev::tmem_load_16(o_tmem + 16 * c, o);
                     dev::tmem_wait_load();
                 }
                 if (sum == 0.0F) { // no keys: what tensor memory holds is nobody's
@@ -600,27 +722,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                         o[x] = 0u;
                     }
                 }
-                if (!live) {
-                    continue;
-                }
-                if (p.splits > 1) {
+                if (live && p.splits > 1) {
                     float4* const out =
-                        reinterpret_cast<float4*>(p.part_out + part * p.head_dim + c);
+                        reinterpret_cast<float4*>(p.part_out + part * p.head_dim + 16 * c);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        if (c + 4 * x < p.head_dim) {
+                        if (16 * c + 4 * x < p.head_dim) {
                             out[x] = make_float4(
                                 __uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
                                 __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
                         }
                     }
-                } else {
+                } else if (live) {
                     uint4* const out = reinterpret_cast<uint4*>(
                         static_cast<__nv_bfloat16*>(p.out) + token * p.out_stride +
-                        static_cast<long long>(item.head) * p.head_dim + c);
+                        static_cast<long long>(item.head) * p.head_dim + 16 * c);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        if (c + 8 * x < p.head_dim) {
+                        if (16 * c + 8 * x < p.head_dim) {
                             uint32_t words[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {
@@ -633,13 +752,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            __syncwarp();
             // O has been read before the next item's first P V, which follows this tile's p_full.
             dev::tc_fence_before();
         }
     }
 
     __syncthreads();
-    if (warp == 2) {
+    if (warp == kTmemWarp) {
         dev::tc_fence_after();
         dev::tmem_dealloc(tmem, 512);
     }

@@ -178,6 +178,7 @@ __device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uin
 #pragma unroll 1
         for (int s = 0; s < chunk; s += 32) {
             float v[32];
+            __syncwarp(); // the accumulator's reads are warp-wide
             load_accumulator<32, BN, Split>(tmem_cols + c + s, v);
             if (p.bias != nullptr) {
                 apply_columns<false>(v, p.bias, col0 + s, p.n, p.bias_vector_ok);

@@ -12,15 +12,18 @@
 //                 memory lanes 32 (w % 4) .. + 31, so two threads share a row and every SM
 //                 sub-partition runs one warp of each (tile, half)
 //   warp 16       loads (one lane)
-//   warp 17       MMA issue (one lane)
+//   warp 17       MMA issue for both tiles in turn: P V and the next S of tile 0, then of tile 1,
+//                 which is what keeps the tiles' chains half a step apart (with an issuer each they
+//                 run in phase, and tensor core and exponentials wait for each other)
 //   warp 18       tensor memory
 //
-// * The two threads of a row exchange their maxima through shared memory every step, over an
-//   mbarrier with bounded waits.
-// * Rescaling O when a maximum rises would put a round trip through tensor memory into every
-//   step. m therefore only follows the true maximum when that has risen by more than 2^8, and
-//   O is rescaled then: P stays below 2^8, sums below 2^8 per key, well inside FP32 and
-//   bfloat16's range, and results do not change, since m cancels in the quotient.
+// * m follows the true maximum only when that has risen by more than 2^8: P stays below 2^8, sums
+//   below 2^8 per key, well inside FP32's and bfloat16's range, and results do not change, since m
+//   cancels in the quotient. So a step takes its exponentials with the m it has, one read of the
+//   scores giving both them and their maximum; only where a maximum turns out too high (and in the
+//   first step) do the row's threads exchange maxima, rescale O and the sums, and read the scores
+//   again. Whether to is the only thing two warps tell each other every step, over an mbarrier
+//   with bounded waits, and they do so before the second half of their exponentials.
 // * head_dim <= 64: P has tensor memory of its own, so the next S is issued as soon as the rows
 //   have read the current one. Up to 128: P overlays S (S 2 x 128, O 2 x 128 columns fill the 512),
 //   and the next S follows P V.
@@ -54,7 +57,7 @@ constexpr float kRescaleAbove = 8.0F; // log2
 // Above this |m scale| (log2) the plain and the exact form of P would differ by more than 2^-14.
 constexpr float kLargeMaximum = 1024.0F;
 // Exponentials of these pairs of a 32-key chunk run on the FMA pipe (see attention.cu).
-constexpr uint32_t kPolyPairs = 0xA4A4u;
+constexpr uint32_t kPolyPairs = 0x8888u;
 
 template <int Atoms>
 struct Shape {
@@ -66,7 +69,10 @@ struct Shape {
     // Maxima and sums of a row's halves: [step parity][tile][half][row].
     static constexpr int kExchangeOffset = kSlotOffset + kSlots * kSlotBytes;
     static constexpr int kExchangeBytes = 2 * 2 * 2 * kTile * 4;
-    static constexpr int kBarrierOffset = kExchangeOffset + kExchangeBytes;
+    // Whether a maximum is too high: [step parity][tile][half][quarter].
+    static constexpr int kFlagOffset = kExchangeOffset + kExchangeBytes;
+    static constexpr int kFlagBytes = 2 * 2 * 2 * 4 * 4;
+    static constexpr int kBarrierOffset = kFlagOffset + kFlagBytes;
     // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2],
     // exchange[tile][quarter]
     static constexpr int kBarriers = 2 * kSlots + 12 + 8;
@@ -150,7 +156,7 @@ __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
     return fmaxf(m[0], m[1]);
 }
 
-// P = 2^(scale (s - m)) of 32 scores, packed, into tensor memory, and their sum. The plain form
+// P = 2^(scale (s - m)) of 32 scores, packed, and their sum. The plain form
 // folds scale and m into one multiply-add, off by a row-wide factor 2^d, |d| <= 2^-24 |m scale|
 // (it cancels in the quotient), and takes some exponentials on the FMA pipe. The exact form, for
 // tiles with masked scores and rows with a very large m, subtracts first, so that no m overflows
@@ -158,12 +164,11 @@ __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
 // 2^-125).
 template <bool Exact>
 __device__ __forceinline__ float exponentials(const uint32_t (&s)[32], float scale, float m,
-                                              uint32_t p_tmem) {
+                                              uint32_t (&packed)[16]) {
     const uint64_t scale2 = dev::f32x2(scale, scale);
     const float minus = Exact ? -m : -m * scale;
     const uint64_t minus2 = dev::f32x2(minus, minus);
     uint64_t sums[2] = {dev::f32x2(0.0F, 0.0F), dev::f32x2(0.0F, 0.0F)};
-    uint32_t packed[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const uint64_t s2 = dev::f32x2(__uint_as_float(s[2 * j]), __uint_as_float(s[2 * j + 1]));
@@ -179,12 +184,11 @@ __device__ __forceinline__ float exponentials(const uint32_t (&s)[32], float sca
         packed[j] = dev::pack_bf16x2(e.x, e.y);
         sums[j & 1] = dev::add_f32x2(sums[j & 1], dev::f32x2(e.x, e.y));
     }
-    dev::tmem_store_16(p_tmem, packed);
     const float2 total = dev::f32x2_split(dev::add_f32x2(sums[0], sums[1]));
     return total.x + total.y;
 }
 
-// S = Q K^T: k_steps steps of 16 elements, 4 to an atom.
+// S = Q K^T: k_steps steps of 16 elements, 4 to an atom. By the whole warp.
 template <int Atoms>
 __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint64_t q_desc, uint64_t k_desc,
                                              uint32_t idesc, int k_steps) {
@@ -193,38 +197,34 @@ __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint64_t q_desc, u
 #pragma unroll
         for (int kk = 0; kk < 4 * Atoms; ++kk) {
             const uint64_t at = static_cast<uint64_t>(kk >> 2) * kAtomStep + 2u * (kk & 3);
-            dev::mma_ss<dev::MmaKind::kF16>(d_tmem, q_desc + at, k_desc + at, idesc,
-                                            kk > 0 ? 1u : 0u);
+            dev::mma_ss_f16_warp(d_tmem, q_desc + at, k_desc + at, idesc, kk > 0 ? 1u : 0u);
         }
     } else {
 #pragma unroll 1
         for (int kk = 0; kk < k_steps; ++kk) {
             const uint64_t at = static_cast<uint64_t>(kk >> 2) * kAtomStep + 2u * (kk & 3);
-            dev::mma_ss<dev::MmaKind::kF16>(d_tmem, q_desc + at, k_desc + at, idesc,
-                                            kk > 0 ? 1u : 0u);
+            dev::mma_ss_f16_warp(d_tmem, q_desc + at, k_desc + at, idesc, kk > 0 ? 1u : 0u);
         }
     }
 }
 
-// O (+)= P V: v_steps steps of 16 keys, the first 4 in P's first half.
+// O (+)= P V: v_steps steps of 16 keys, the first 4 in P's first half. By the whole warp.
 template <int Atoms>
 __device__ __forceinline__ void issue_outputs(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc,
                                               uint32_t idesc, int v_steps, uint32_t accumulate) {
     if (v_steps == kTile / 16) {
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk) {
-            dev::mma_ts<dev::MmaKind::kF16>(
-                d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
-                v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
-                kk > 0 ? 1u : accumulate);
+            dev::mma_ts_f16_warp(d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+                                 v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
+                                 kk > 0 ? 1u : accumulate);
         }
     } else {
 #pragma unroll 1
         for (int kk = 0; kk < v_steps; ++kk) {
-            dev::mma_ts<dev::MmaKind::kF16>(
-                d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
-                v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
-                kk > 0 ? 1u : accumulate);
+            dev::mma_ts_f16_warp(d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+                                 v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
+                                 kk > 0 ? 1u : accumulate);
         }
     }
 }
@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_done = more + 80;   // + 8 t
     const uint32_t exchange = more + 96; // + 8 (4 t + quarter)
 
-    const int warp = threadIdx.x / 32;
+    // Through a shuffle, so that the compiler knows it is the same for the warp.
+    const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) / 32, 0);
     const int lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kSlots; ++i) {
@@ -282,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev::tc_fence_before();
     __syncthreads();
     dev::tc_fence_after();
-    const uint32_t tmem = *reinterpret_cast<const uint32_t*>(smem + S::kTmemSlotOffset);
+    const uint32_t tmem = __shfl_sync(
+        0xFFFFFFFFu, *reinterpret_cast<const uint32_t*>(smem + S::kTmemSlotOffset), 0);
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
 
@@ -366,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::mbar_drain_wait(q_full + 8, (q_loads1 - 1) & 1u);
             }
         }
-    } else if (warp == kMmaWarp && lane == 0) {
-        // ---------------- MMA issue ----------------
+    } else if (warp == kMmaWarp) {
+        // ---------------- MMA issue (the whole warp, one lane issuing) ----------------
         const int k_steps = (p.head_dim + 15) / 16;
         const uint32_t idesc_o = dev::make_idesc(1u, kTile, 16 * k_steps, false, true);
         // Descriptors are built once and stepped by adding to their start-address field.
@@ -385,36 +387,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
             const Item item = find_item(p, index);
-            const int tile_steps[2] = {item.steps0, item.steps1};
-            const int steps = max(item.steps0, item.steps1);
+            const auto uniform = [](int value) { return __shfl_sync(0xFFFFFFFFu, value, 0); };
+            const int tile_steps[2] = {uniform(item.steps0), uniform(item.steps1)};
+            const int steps = max(tile_steps[0], tile_steps[1]);
             if (steps == 0) {
                 continue;
             }
-            const int keys = item.end_key - item.first_key;
+            const int keys = uniform(item.end_key - item.first_key);
             // The first scores.
             {
                 const int keys16 = (min(kTile, keys) + 15) & ~15;
                 const uint32_t idesc = dev::make_idesc(1u, kTile, keys16, false, false);
-                ok = dev::mbar_wait(full(slot), phase, status);
+                ok = dev::mbar_wait_warp(full(slot), phase, status);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     if (ok && tile_steps[t] > 0) {
-                        ok = dev::mbar_wait(q_full + 8 * t, q_phase[t], status);
+                        ok = dev::mbar_wait_warp(q_full + 8 * t, q_phase[t], status);
                         q_phase[t] ^= 1u;
                         if (ok) {
                             dev::tc_fence_after();
                             issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
                                                 k_desc0 + slot * kSlotStep, idesc, k_steps);
-                            dev::tc_commit(s_full + 8 * t);
+                            dev::tc_commit_warp(s_full + 8 * t);
                         }
                     }
                 }
                 if (!ok) {
                     break;
                 }
-                dev::tc_commit(empty(slot));
+                dev::tc_commit_warp(empty(slot));
                 if (steps == 1) {
-                    dev::tc_commit(q_empty);
+                    dev::tc_commit_warp(q_empty);
                 }
                 if (++slot == S::kSlots) {
                     slot = 0;
@@ -438,31 +441,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int next16 = (min(kTile, keys - (j + 1) * kTile) + 15) & ~15;
                 const uint32_t idesc_next =
                     dev::make_idesc(1u, kTile, next ? next16 : 16, false, false);
-                if (keys_first) {
-                    // The next scores as soon as the rows have read these.
-                    ok = dev::mbar_wait(full(k_slot), k_phase, status);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (ok && j + 1 < tile_steps[t]) {
-                            ok = dev::mbar_wait(s_free + 8 * t, free_phase[t], status);
-                            if (ok) {
-                                dev::tc_fence_after();
-                                issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
-                                                    k_desc0 + k_slot * kSlotStep, idesc_next,
-                                                    k_steps);
-                                dev::tc_commit(s_full + 8 * t);
-                            }
-                        }
-                    }
-                    if (!ok) {
-                        break;
-                    }
-                    dev::tc_commit(empty(k_slot));
+                ok = dev::mbar_wait_warp(full(v_slot), v_phase, status);
+                if (ok && next) {
+                    ok = dev::mbar_wait_warp(full(k_slot), k_phase, status);
                 }
-                // s_free completes once per step of a tile, whether or not more scores follow.
-                free_phase[0] ^= j < tile_steps[0] ? 1u : 0u;
-                free_phase[1] ^= j < tile_steps[1] ? 1u : 0u;
-                ok = dev::mbar_wait(full(v_slot), v_phase, status);
                 if (!ok) {
                     break;
                 }
@@ -474,47 +456,59 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int a = 0; a < Atoms; ++a) {
                         const uint32_t rows = base + S::kSlotOffset + v_slot * S::kSlotBytes +
                                               a * kAtomBytes + live * 128;
-#pragma unroll 4
-                        for (int i = 0; i < (live16 - live) * 8; ++i) {
+                        for (int i = lane; i < (live16 - live) * 8; i += 32) {
                             dev::st_shared_v4(rows + 16 * i, zero);
                         }
                     }
                     dev::fence_proxy_async_shared();
+                    __syncwarp();
                 }
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (ok && j < tile_steps[t]) {
-                        ok = dev::mbar_wait(p_full + 8 * t, p_phase[t], status);
-                        p_phase[t] ^= 1u;
-                        if (ok) {
-                            dev::tc_fence_after();
-                            issue_outputs<Atoms>(tmem + S::kOColumn + t * S::kOPitch,
-                                                 tmem + S::kPColumn + t * S::kPPitch,
-                                                 v_desc0 + v_slot * kSlotStep, idesc_o, live16 / 16,
-                                                 j > 0 ? 1u : 0u);
-                            dev::tc_commit(o_done + 8 * t);
-                        }
-                        if (S::kOverlay && ok && j + 1 < tile_steps[t]) {
-                            ok = dev::mbar_wait(full(k_slot), k_phase, status);
+                    if (!ok || j >= tile_steps[t]) {
+                        continue;
+                    }
+                    const bool more_scores = j + 1 < tile_steps[t];
+                    const auto next_scores = [&]() {
+                        dev::tc_fence_after();
+                        issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
+                                            k_desc0 + k_slot * kSlotStep, idesc_next, k_steps);
+                        dev::tc_commit_warp(s_full + 8 * t);
+                    };
+                    if (!S::kOverlay) {
+                        // The next scores as soon as the rows have read these. (s_free completes
+                        // once per step, whether or not more scores follow.)
+                        if (more_scores) {
+                            ok = dev::mbar_wait_warp(s_free + 8 * t, free_phase[t], status);
                             if (ok) {
-                                dev::tc_fence_after();
-                                issue_scores<Atoms>(tmem + t * kTile, q_desc0 + t * kQStep,
-                                                    k_desc0 + k_slot * kSlotStep, idesc_next,
-                                                    k_steps);
-                                dev::tc_commit(s_full + 8 * t);
+                                next_scores();
                             }
+                        }
+                        free_phase[t] ^= 1u;
+                    }
+                    ok = ok && dev::mbar_wait_warp(p_full + 8 * t, p_phase[t], status);
+                    p_phase[t] ^= 1u;
+                    if (ok) {
+                        dev::tc_fence_after();
+                        issue_outputs<Atoms>(tmem + S::kOColumn + t * S::kOPitch,
+                                             tmem + S::kPColumn + t * S::kPPitch,
+                                             v_desc0 + v_slot * kSlotStep, idesc_o, live16 / 16,
+                                             j > 0 ? 1u : 0u);
+                        dev::tc_commit_warp(o_done + 8 * t);
+                        if (S::kOverlay && more_scores) {
+                            next_scores();
                         }
                     }
                 }
                 if (!ok) {
                     break;
                 }
-                dev::tc_commit(empty(v_slot));
-                if (S::kOverlay && next) {
-                    dev::tc_commit(empty(k_slot));
+                dev::tc_commit_warp(empty(v_slot));
+                if (next) {
+                    dev::tc_commit_warp(empty(k_slot));
                 }
                 if (j + 2 == steps) {
-                    dev::tc_commit(q_empty); // the last scores have been issued
+                    dev::tc_commit_warp(q_empty); // the last scores have been issued
                 }
                 // This step took the values' slot and, if keys followed, theirs.
                 slot = next ? slot2 : slot;
@@ -526,8 +520,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // Every MMA issued has finished before the CTA's shared and tensor memory go.
-        dev::tc_commit(drain);
+        dev::tc_commit_warp(drain);
         dev::mbar_drain_wait(drain, 0);
+        __syncwarp();
     } else if (warp < kRowWarps) {
         // ---------------- rows ----------------
         const int t = warp >> 3;
@@ -545,10 +540,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float* const theirs = reinterpret_cast<const float*>(smem + S::kExchangeOffset) +
                                     (2 * t + (half ^ 1)) * kTile + row;
         constexpr int kParity = 4 * kTile; // floats between the two exchange buffers
+        int* const my_flag = reinterpret_cast<int*>(smem + S::kFlagOffset) + (2 * t + half) * 4 +
+                             quarter;
+        const int* const their_flag = reinterpret_cast<const int*>(smem + S::kFlagOffset) +
+                                      (2 * t + (half ^ 1)) * 4 + quarter;
+        constexpr int kFlagParity = 16;
         uint32_t s_phase = 0;
         uint32_t o_phase = 0;     // of the tile's next P V to complete
         uint32_t exchanges = 0;   // so far
         bool ok = true;
+        // Tells the other warp of these rows whether this one needs higher maxima.
+        const auto offer_flag = [&](bool raise) {
+            if (lane == 0) {
+                my_flag[(exchanges & 1u) ? kFlagParity : 0] = raise ? 1 : 0;
+                dev::mbar_arrive(exchange_bar);
+            }
+            __syncwarp();
+        };
+        const auto take_flag = [&]() -> bool {
+            const int at = (exchanges & 1u) ? kFlagParity : 0;
+            ok = dev::mbar_wait_warp(exchange_bar, exchanges & 1u, status);
+            ++exchanges;
+            return ok && their_flag[at] != 0;
+        };
         // Gives `value` to the row's other thread and returns that thread's.
         const auto swap = [&](float value) -> float {
             const int at = (exchanges & 1u) ? kParity : 0;
@@ -585,24 +599,47 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 dev::tc_fence_after();
                 if (live_warp) {
-                    // Scores are read 32 at a time, once for the maximum and once for the
-                    // exponentials: 64 held over both would not fit the 96 registers.
                     const int limit = row_keys - j * kTile;
                     const bool masked = __any_sync(0xFFFFFFFFu, limit < kHalf);
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t s[32];
+                    const auto read = [&](uint32_t (&s)[32], int c) {
                         dev::tmem_load_32(s_tmem + 32 * c, s);
                         dev::tmem_wait_load();
                         if (masked) {
                             mask(s, limit - 32 * c);
                         }
+                    };
+                    const auto weigh = [&](const uint32_t (&s)[32], bool exact,
+                                           uint32_t (&packed)[16]) -> float {
+                        return exact ? exponentials<true>(s, p.scale_log2, m, packed)
+                                     : exponentials<false>(s, p.scale_log2, m, packed);
+                    };
+                    uint32_t packed[2][16];
+                    float top = -INFINITY;
+                    bool raise = j == 0;
+                    if (j > 0) {
+                        const bool exact =
+                            masked || __any_sync(0xFFFFFFFFu,
+                                                 fabsf(m * p.scale_log2) > kLargeMaximum);
+                        uint32_t s[32];
+                        read(s, 0);
+                        top = maximum(s);
+                        float added = weigh(s, exact, packed[0]);
+                        read(s, 1);
                         top = fmaxf(top, maximum(s));
-                    }
-                    top = fmaxf(top, swap(top));
-                    if (!ok) {
-                        break;
+                        raise = __any_sync(0xFFFFFFFFu, (top - m) * p.scale_log2 > kRescaleAbove);
+                        offer_flag(raise);
+                        added += weigh(s, exact, packed[1]);
+                        raise = take_flag() || raise;
+                        if (!ok) {
+                            break;
+                        }
+                        sum += raise ? 0.0F : added;
+                    } else {
+                        uint32_t s[32];
+                        read(s, 0);
+                        top = maximum(s);
+                        read(s, 1);
+                        top = fmaxf(top, maximum(s));
                     }
                     if (!S::kOverlay && j > 0) {
                         // P V of the previous step has read P and written O.
@@ -613,12 +650,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         dev::tc_fence_after();
                     }
-                    if (j == 0) {
-                        m = top == -INFINITY ? 0.0F : top;
-                    } else {
-                        const bool raise = (top - m) * p.scale_log2 > kRescaleAbove;
-                        if (__any_sync(0xFFFFFFFFu, raise)) {
-                            const float raised = raise ? top : m;
+                    if (raise) {
+                        top = fmaxf(top, swap(top));
+                        if (!ok) {
+                            break;
+                        }
+                        if (j == 0) {
+                            m = top == -INFINITY ? 0.0F : top;
+                        } else {
+                            const float raised =
+                                (top - m) * p.scale_log2 > kRescaleAbove ? top : m;
                             const float factor = dev::ex2_approx((m - raised) * p.scale_log2);
                             m = raised;
                             sum *= factor;
@@ -634,32 +675,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 dev::tmem_store_16(o_tmem + 16 * c, o);
                             }
                         }
-                    }
-                    const bool exact =
-                        masked || __any_sync(0xFFFFFFFFu,
-                                             fabsf(m * p.scale_log2) > kLargeMaximum);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
                         uint32_t s[32];
-                        dev::tmem_load_32(s_tmem + 32 * c, s);
-                        dev::tmem_wait_load();
-                        if (!S::kOverlay && c == 1) {
-                            dev::tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) {
-                                dev::mbar_arrive(s_free + 8 * t);
-                            }
-                            __syncwarp();
-                        }
-                        if (exact) {
-                            if (masked) {
-                                mask(s, limit - 32 * c);
-                            }
-                            sum += exponentials<true>(s, p.scale_log2, m, p_tmem + 16 * c);
-                        } else {
-                            sum += exponentials<false>(s, p.scale_log2, m, p_tmem + 16 * c);
-                        }
+                        read(s, 0);
+                        sum += weigh(s, true, packed[0]);
+                        read(s, 1);
+                        sum += weigh(s, true, packed[1]);
                     }
+                    if (!S::kOverlay) {
+                        dev::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            dev::mbar_arrive(s_free + 8 * t);
+                        }
+                        __syncwarp();
+                    }
+                    dev::tmem_store_16(p_tmem, packed[0]);
+                    dev::tmem_store_16(p_tmem + 16, packed[1]);
                     dev::tmem_wait_store();
                 } else if (!S::kOverlay) {
                     __syncwarp();

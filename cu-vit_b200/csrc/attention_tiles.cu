@@ -8,22 +8,22 @@
 // tile's rows take their maxima and exponentials, so neither waits for the other longer than it
 // must. Keys and values stream through a ring of TMA stages shared by both tiles.
 //
-//   warps 0..15   rows: warp w has tile w / 8, half (w / 4) % 2 of the tile's keys and tensor
-//                 memory lanes 32 (w % 4) .. + 31, so two threads share a row and every SM
-//                 sub-partition runs one warp of each (tile, half)
-//   warp 16       loads (one lane)
-//   warp 17       MMA issue for both tiles in turn: P V and the next S of tile 0, then of tile 1,
+//   warps 0..7    rows: one thread per row, warp w with tile w / 4 and tensor memory lanes
+//                 32 (w % 4) .. + 31, so that every SM sub-partition runs one warp of each tile
+//   warp 8        loads (one lane)
+//   warp 9        MMA issue for both tiles in turn: P V and the next S of tile 0, then of tile 1,
 //                 which is what keeps the tiles' chains half a step apart (with an issuer each they
 //                 run in phase, and tensor core and exponentials wait for each other)
-//   warp 18       tensor memory
+//   warp 10       tensor memory
 //
 // * m follows the true maximum only when that has risen by more than 2^8: P stays below 2^8, sums
 //   below 2^8 per key, well inside FP32's and bfloat16's range, and results do not change, since m
 //   cancels in the quotient. So a step takes its exponentials with the m it has, one read of the
 //   scores giving both them and their maximum; only where a maximum turns out too high (and in the
-//   first step) do the row's threads exchange maxima, rescale O and the sums, and read the scores
-//   again. Whether to is the only thing two warps tell each other every step, over an mbarrier
-//   with bounded waits, and they do so before the second half of their exponentials.
+//   first step) are O and the sums rescaled and the scores read again.
+// * Scores are read 32 at a time, the next 32 in flight meanwhile. Two threads per row (64 scores
+//   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes %CLIP%
+//   (16384 tokens, 16 heads of 128): their exchanges cost more than the shorter rows saved.
 // * head_dim <= 64: P has tensor memory of its own, so the next S is issued as soon as the rows
 //   have read the current one. Up to 128: P overlays S (S 2 x 128, O 2 x 128 columns fill the 512),
 //   and the next S follows P V.
@@ -41,18 +41,18 @@
 #include <cuda_bf16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace cuvit::attn {
 namespace {
 
 constexpr int kTile = 128;              // query rows of a tile, keys of a step
-constexpr int kHalf = 64;               // keys of a row thread
 constexpr int kAtomBytes = kTile * 128; // 128 rows of 64 bfloat16
-constexpr int kRowWarps = 16;
-constexpr int kLoadWarp = 16;
-constexpr int kMmaWarp = 17;
-constexpr int kTmemWarp = 18;
-constexpr int kThreads = 640;
+constexpr int kRowWarps = 8;
+constexpr int kLoadWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kTmemWarp = 10;
+constexpr int kThreads = 352;
 constexpr float kRescaleAbove = 8.0F; // log2
 // Above this |m scale| (log2) the plain and the exact form of P would differ by more than 2^-14.
 constexpr float kLargeMaximum = 1024.0F;
@@ -64,27 +64,17 @@ struct Shape {
     static constexpr bool kOverlay = Atoms == 2; // P in the columns of S
     static constexpr int kQBytes = Atoms * kAtomBytes;
     static constexpr int kSlotBytes = Atoms * kAtomBytes;
-    static constexpr int kSlots = Atoms == 2 ? 4 : 8;
+    static constexpr int kSlots = Atoms == 2 ? 5 : 8;
     static constexpr int kSlotOffset = 2 * kQBytes;
-    // Maxima and sums of a row's halves: [step parity][tile][half][row].
-    static constexpr int kExchangeOffset = kSlotOffset + kSlots * kSlotBytes;
-    static constexpr int kExchangeBytes = 2 * 2 * 2 * kTile * 4;
-    // Whether a maximum is too high: [step parity][tile][half][quarter].
-    static constexpr int kFlagOffset = kExchangeOffset + kExchangeBytes;
-    static constexpr int kFlagBytes = 2 * 2 * 2 * 4 * 4;
-    static constexpr int kBarrierOffset = kFlagOffset + kFlagBytes;
-    // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2],
-    // exchange[tile][quarter]
-    static constexpr int kBarriers = 2 * kSlots + 12 + 8;
+    static constexpr int kBarrierOffset = kSlotOffset + kSlots * kSlotBytes;
+    // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2]
+    static constexpr int kBarriers = 2 * kSlots + 12;
     static constexpr int kTmemSlotOffset = kBarrierOffset + 8 * kBarriers;
     static constexpr int kSmemBytes = 1024 + kTmemSlotOffset + 16;
     static constexpr uint32_t kOColumn = 256;
     static constexpr uint32_t kOPitch = Atoms == 2 ? 128 : 64;
-    // P of a tile's first half of keys, and from there to the second half's: the overlay puts each
-    // half into the columns of the scores its own warps have read.
     static constexpr uint32_t kPColumn = Atoms == 2 ? 0 : 384;
     static constexpr uint32_t kPPitch = Atoms == 2 ? 128 : 64;
-    static constexpr uint32_t kPHalf = Atoms == 2 ? 64 : 32;
     static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 };
 
@@ -208,21 +198,20 @@ __device__ __forceinline__ void issue_scores(uint32_t d_tmem, uint64_t q_desc, u
     }
 }
 
-// O (+)= P V: v_steps steps of 16 keys, the first 4 in P's first half. By the whole warp.
-template <int Atoms>
+// O (+)= P V: v_steps steps of 16 keys. By the whole warp.
 __device__ __forceinline__ void issue_outputs(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc,
                                               uint32_t idesc, int v_steps, uint32_t accumulate) {
     if (v_steps == kTile / 16) {
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk) {
-            dev::mma_ts_f16_warp(d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+            dev::mma_ts_f16_warp(d_tmem, p_tmem + 8 * kk,
                                  v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
                                  kk > 0 ? 1u : accumulate);
         }
     } else {
 #pragma unroll 1
         for (int kk = 0; kk < v_steps; ++kk) {
-            dev::mma_ts_f16_warp(d_tmem, p_tmem + (kk >> 2) * Shape<Atoms>::kPHalf + 8 * (kk & 3),
+            dev::mma_ts_f16_warp(d_tmem, p_tmem + 8 * kk,
                                  v_desc + static_cast<uint64_t>(kk) * (2048 >> 4), idesc,
                                  kk > 0 ? 1u : accumulate);
         }
@@ -252,7 +241,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_free = more + 48;   // + 8 t
     const uint32_t p_full = more + 64;   // + 8 t
     const uint32_t o_done = more + 80;   // + 8 t
-    const uint32_t exchange = more + 96; // + 8 (4 t + quarter)
 
     // Through a shuffle, so that the compiler knows it is the same for the warp.
     const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) / 32, 0);
@@ -268,9 +256,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             dev::mbar_init(s_free + 8 * t, kRowWarps / 2);
             dev::mbar_init(p_full + 8 * t, kRowWarps / 2);
             dev::mbar_init(o_done + 8 * t, 1);
-        }
-        for (uint32_t i = 0; i < 8; ++i) {
-            dev::mbar_init(exchange + 8 * i, 2); // the two warps of a tile's lane quarter
         }
         dev::mbar_init(q_empty, 1);
         dev::mbar_init(drain, 1);
@@ -490,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     p_phase[t] ^= 1u;
                     if (ok) {
                         dev::tc_fence_after();
-                        issue_outputs<Atoms>(tmem + S::kOColumn + t * S::kOPitch,
+                        issue_outputs(tmem + S::kOColumn + t * S::kOPitch,
                                              tmem + S::kPColumn + t * S::kPPitch,
                                              v_desc0 + v_slot * kSlotStep, idesc_o, live16 / 16,
                                              j > 0 ? 1u : 0u);
@@ -525,55 +510,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp < kRowWarps) {
         // ---------------- rows ----------------
-        const int t = warp >> 3;
-        const int half = (warp >> 2) & 1;
+        const int t = warp >> 2;
         const int quarter = warp & 3; // the tensor memory lanes this warp may access
         const int row = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_tmem = tmem + lanes + t * kTile + half * kHalf;
-        const uint32_t p_tmem = tmem + lanes + S::kPColumn + t * S::kPPitch + half * S::kPHalf;
+        const uint32_t s_tmem = tmem + lanes + t * kTile;
+        const uint32_t p_tmem = tmem + lanes + S::kPColumn + t * S::kPPitch;
         const uint32_t o_tmem = tmem + lanes + S::kOColumn + t * S::kOPitch;
-        const int o_chunks = (p.head_dim + 15) / 16; // of 16 columns; the halves take alternate ones
-        const uint32_t exchange_bar = exchange + 8u * static_cast<uint32_t>(4 * t + quarter);
-        float* const mine = reinterpret_cast<float*>(smem + S::kExchangeOffset) +
-                            (2 * t + half) * kTile + row;
-        const float* const theirs = reinterpret_cast<const float*>(smem + S::kExchangeOffset) +
-                                    (2 * t + (half ^ 1)) * kTile + row;
-        constexpr int kParity = 4 * kTile; // floats between the two exchange buffers
-        int* const my_flag = reinterpret_cast<int*>(smem + S::kFlagOffset) + (2 * t + half) * 4 +
-                             quarter;
-        const int* const their_flag = reinterpret_cast<const int*>(smem + S::kFlagOffset) +
-                                      (2 * t + (half ^ 1)) * 4 + quarter;
-        constexpr int kFlagParity = 16;
+        const int o_columns = 16 * ((p.head_dim + 15) / 16);
         uint32_t s_phase = 0;
-        uint32_t o_phase = 0;     // of the tile's next P V to complete
-        uint32_t exchanges = 0;   // so far
+        uint32_t o_phase = 0; // of the tile's next P V to complete
         bool ok = true;
-        // Tells the other warp of these rows whether this one needs higher maxima.
-        const auto offer_flag = [&](bool raise) {
-            if (lane == 0) {
-                my_flag[(exchanges & 1u) ? kFlagParity : 0] = raise ? 1 : 0;
-                dev::mbar_arrive(exchange_bar);
-            }
-            __syncwarp();
-        };
-        const auto take_flag = [&]() -> bool {
-            const int at = (exchanges & 1u) ? kFlagParity : 0;
-            ok = dev::mbar_wait_warp(exchange_bar, exchanges & 1u, status);
-            ++exchanges;
-            return ok && their_flag[at] != 0;
-        };
-        // Gives `value` to the row's other thread and returns that thread's.
-        const auto swap = [&](float value) -> float {
-            const int at = (exchanges & 1u) ? kParity : 0;
-            mine[at] = value;
+        // One arrival for the warp's tensor memory accesses so far.
+        const auto arrive = [&](uint32_t bar) {
+            dev::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                dev::mbar_arrive(exchange_bar);
+                dev::mbar_arrive(bar);
             }
-            ok = dev::mbar_wait_warp(exchange_bar, exchanges & 1u, status);
-            ++exchanges;
-            return theirs[at];
+            __syncwarp();
         };
         for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
             const Item item = find_item(p, index);
@@ -583,12 +538,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int steps = t == 0 ? item.steps0 : item.steps1;
             const bool live_warp = quarter * 32 < rows;
-            // Keys of this thread's half that its row sees, from the split's first on.
+            // Keys this row sees, from the split's first on.
             long long end = item.end_key;
             if (p.causal) {
                 end = max(0LL, min(end, item.reach + t * kTile + row));
             }
-            const int row_keys = static_cast<int>(max(0LL, end - item.first_key)) - half * kHalf;
+            const int row_keys = static_cast<int>(max(0LL, end - item.first_key));
             float m = 0.0F; // unscaled
             float sum = 0.0F;
             for (int j = 0; j < steps && ok; ++j) {
@@ -600,61 +555,63 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::tc_fence_after();
                 if (live_warp) {
                     const int limit = row_keys - j * kTile;
-                    const bool masked = __any_sync(0xFFFFFFFFu, limit < kHalf);
-                    const auto read = [&](uint32_t (&s)[32], int c) {
-                        dev::tmem_load_32(s_tmem + 32 * c, s);
-                        dev::tmem_wait_load();
-                        if (masked) {
-                            mask(s, limit - 32 * c);
-                        }
-                    };
-                    const auto weigh = [&](const uint32_t (&s)[32], bool exact,
-                                           uint32_t (&packed)[16]) -> float {
-                        return exact ? exponentials<true>(s, p.scale_log2, m, packed)
-                                     : exponentials<false>(s, p.scale_log2, m, packed);
-                    };
-                    uint32_t packed[2][16];
+                    const bool masked = __any_sync(0xFFFFFFFFu, limit < kTile);
+                    uint32_t packed[4][16];
+                    float added = 0.0F;
                     float top = -INFINITY;
-                    bool raise = j == 0;
+                    bool raise = true;
                     if (j > 0) {
-                        const bool exact =
-                            masked || __any_sync(0xFFFFFFFFu,
-                                                 fabsf(m * p.scale_log2) > kLargeMaximum);
-                        uint32_t s[32];
-                        read(s, 0);
-                        top = maximum(s);
-                        float added = weigh(s, exact, packed[0]);
-                        read(s, 1);
-                        top = fmaxf(top, maximum(s));
+                        // Without branches inside, so that one chunk's maxima run under another's
+                        // exponentials: a warp has its scheduler almost to itself here.
+                        const auto weigh = [&](auto exact) {
+                            uint32_t s[2][32];
+                            dev::tmem_load_32(s_tmem, s[0]);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                dev::tmem_wait_load_of(s[c & 1]);
+                                if (c < 3) {
+                                    dev::tmem_load_32(s_tmem + 32 * (c + 1), s[(c + 1) & 1]);
+                                }
+                                if constexpr (exact.value) {
+                                    mask(s[c & 1], limit - 32 * c);
+                                }
+                                top = fmaxf(top, maximum(s[c & 1]));
+                                added += exponentials<exact.value>(s[c & 1], p.scale_log2, m,
+                                                                   packed[c]);
+                            }
+                        };
+                        if (masked || __any_sync(0xFFFFFFFFu,
+                                                 fabsf(m * p.scale_log2) > kLargeMaximum)) {
+                            weigh(std::true_type{});
+                        } else {
+                            weigh(std::false_type{});
+                        }
                         raise = __any_sync(0xFFFFFFFFu, (top - m) * p.scale_log2 > kRescaleAbove);
-                        offer_flag(raise);
-                        added += weigh(s, exact, packed[1]);
-                        raise = take_flag() || raise;
-                        if (!ok) {
-                            break;
+                        if (!S::kOverlay && !raise) {
+                            arrive(s_free + 8 * t);
                         }
-                        sum += raise ? 0.0F : added;
+                        if (!S::kOverlay) {
+                            // P V of the previous step has read P and written O.
+                            ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
+                            o_phase ^= 1u;
+                            if (!ok) {
+                                break;
+                            }
+                            dev::tc_fence_after();
+                        }
                     } else {
-                        uint32_t s[32];
-                        read(s, 0);
-                        top = maximum(s);
-                        read(s, 1);
-                        top = fmaxf(top, maximum(s));
-                    }
-                    if (!S::kOverlay && j > 0) {
-                        // P V of the previous step has read P and written O.
-                        ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
-                        o_phase ^= 1u;
-                        if (!ok) {
-                            break;
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t s[32];
+                            dev::tmem_load_32(s_tmem + 32 * c, s);
+                            dev::tmem_wait_load_of(s);
+                            if (masked) {
+                                mask(s, limit - 32 * c);
+                            }
+                            top = fmaxf(top, maximum(s));
                         }
-                        dev::tc_fence_after();
                     }
                     if (raise) {
-                        top = fmaxf(top, swap(top));
-                        if (!ok) {
-                            break;
-                        }
                         if (j == 0) {
                             m = top == -INFINITY ? 0.0F : top;
                         } else {
@@ -664,47 +621,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                             m = raised;
                             sum *= factor;
 #pragma unroll 1
-                            for (int c = half; c < o_chunks; c += 2) {
+                            for (int c = 0; c < o_columns; c += 16) {
                                 uint32_t o[16];
-                                dev::tmem_load_16(o_tmem + 16 * c, o);
+                                dev::tmem_load_16(o_tmem + c, o);
                                 dev::tmem_wait_load();
 #pragma unroll
                                 for (int x = 0; x < 16; ++x) {
                                     o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);
                                 }
-                                dev::tmem_store_16(o_tmem + 16 * c, o);
+                                dev::tmem_store_16(o_tmem + c, o);
                             }
                         }
-                        uint32_t s[32];
-                        read(s, 0);
-                        sum += weigh(s, true, packed[0]);
-                        read(s, 1);
-                        sum += weigh(s, true, packed[1]);
-                    }
-                    if (!S::kOverlay) {
-                        dev::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) {
-                            dev::mbar_arrive(s_free + 8 * t);
+                        added = 0.0F;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t s[32];
+                            dev::tmem_load_32(s_tmem + 32 * c, s);
+                            dev::tmem_wait_load_of(s);
+                            if (masked) {
+                                mask(s, limit - 32 * c);
+                            }
+                            added += exponentials<true>(s, p.scale_log2, m, packed[c]);
                         }
-                        __syncwarp();
+                        if (!S::kOverlay) {
+                            arrive(s_free + 8 * t);
+                        }
                     }
-                    dev::tmem_store_16(p_tmem, packed[0]);
-                    dev::tmem_store_16(p_tmem + 16, packed[1]);
+                    sum += added;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        dev::tmem_store_16(p_tmem + 16 * c, packed[c]);
+                    }
                     dev::tmem_wait_store();
                 } else if (!S::kOverlay) {
-                    __syncwarp();
-                    if (lane == 0) {
-                        dev::mbar_arrive(s_free + 8 * t);
+                    // A warp without rows keeps the others' pace: the next scores may come before
+                    // they have handed over this step's P, and an arrival for that step would be
+                    // counted into this one.
+                    arrive(s_free + 8 * t);
+                    if (j > 0) {
+                        ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
+                        o_phase ^= 1u;
+                        if (!ok) {
+                            break;
+                        }
                     }
-                    o_phase ^= j > 0 ? 1u : 0u;
                 }
-                dev::tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    dev::mbar_arrive(p_full + 8 * t);
-                }
-                __syncwarp();
+                arrive(p_full + 8 * t);
             }
             if (!ok) {
                 break;
@@ -725,26 +687,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!live_warp) {
                 continue; // the whole warp
             }
-            sum += swap(sum);
-            if (!ok) {
-                break;
-            }
             const bool live = row < rows;
             const long long token = static_cast<long long>(item.s.q_first) + t * kTile + row;
             const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
             const long long part =
                 (static_cast<long long>(item.split) * p.q_tokens + token) * p.q_heads + item.head;
-            if (live && half == 0 && p.splits > 1) {
-                p.part_stats[part] =
-                    make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
+            if (live && p.splits > 1) {
+                p.part_stats[part] = make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
             }
 #pragma unroll 1
-            for (int c = half; c < o_chunks; c += 2) {
+            for (int c = 0; c < o_columns; c += 16) {
                 uint32_t o[16];
                 // The read is warp-wide: lanes that store below, and those that do not, meet first.
                 __syncwarp();
                 if (steps > 0) {
-                    dev::tmem_load_16(o_tmem + 16 * c, o);
+                    dev::tmem_load_16(o_tmem + c, o);
                     dev::tmem_wait_load();
                 }
                 if (sum == 0.0F) { // no keys: what tensor memory holds is nobody's
@@ -755,10 +712,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (live && p.splits > 1) {
                     float4* const out =
-                        reinterpret_cast<float4*>(p.part_out + part * p.head_dim + 16 * c);
+                        reinterpret_cast<float4*>(p.part_out + part * p.head_dim + c);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        if (16 * c + 4 * x < p.head_dim) {
+                        if (c + 4 * x < p.head_dim) {
                             out[x] = make_float4(
                                 __uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
                                 __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
@@ -767,10 +724,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else if (live) {
                     uint4* const out = reinterpret_cast<uint4*>(
                         static_cast<__nv_bfloat16*>(p.out) + token * p.out_stride +
-                        static_cast<long long>(item.head) * p.head_dim + 16 * c);
+                        static_cast<long long>(item.head) * p.head_dim + c);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        if (16 * c + 8 * x < p.head_dim) {
+                        if (c + 8 * x < p.head_dim) {
                             uint32_t words[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {

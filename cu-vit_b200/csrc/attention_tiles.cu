@@ -3,14 +3,19 @@
 //   S = Q K^T for 128 query rows and 128 keys at a time into tensor memory; P = 2^(S scale - m);
 //   O += P V, with m and the sum of P kept per row.
 //
-// One persistent CTA per SM walks (256 query rows, head, split of the keys) items. The 256 rows
+// A CTA works on (256 query rows, head, split of the keys) items: its own block index, then those of
+// blocks that have not started, which it takes over one by one (cluster launch control), so that
+// sequences of very different lengths balance over the SMs without a counter in memory. The load
+// warp asks for the next item, finds its sequence and hands it to the other warps through a ring,
+// all while they still work on the previous ones; queries that see fewer keys than others (causal)
+// come last. The 256 rows
 // are two tiles of 128 whose chains alternate: while the tensor core works for one tile, the other
 // tile's rows take their maxima and exponentials, so neither waits for the other longer than it
 // must. Keys and values stream through a ring of TMA stages shared by both tiles.
 //
 //   warps 0..7    rows: one thread per row, warp w with tile w / 4 and tensor memory lanes
 //                 32 (w % 4) .. + 31, so that every SM sub-partition runs one warp of each tile
-//   warp 8        loads (one lane)
+//   warp 8        items and loads (one lane loading)
 //   warp 9        MMA issue for both tiles in turn: P V and the next S of tile 0, then of tile 1,
 //                 which is what keeps the tiles' chains half a step apart (with an issuer each they
 //                 run in phase, and tensor core and exponentials wait for each other)
@@ -59,6 +64,11 @@ constexpr float kLargeMaximum = 1024.0F;
 // Exponentials of these pairs of a 32-key chunk run on the FMA pipe (see attention.cu).
 constexpr uint32_t kPolyPairs = 0x8888u;
 
+constexpr int kItemSlots = 2;
+// A warp may wait for its next item as long as another tile's rows take: seconds for 10^8 keys.
+constexpr unsigned long long kItemWaitNs = 60000000000ull;
+constexpr int kItemBytes = 48;
+
 template <int Atoms>
 struct Shape {
     static constexpr bool kOverlay = Atoms == 2; // P in the columns of S
@@ -67,9 +77,12 @@ struct Shape {
     static constexpr int kSlots = Atoms == 2 ? 5 : 8;
     static constexpr int kSlotOffset = 2 * kQBytes;
     static constexpr int kBarrierOffset = kSlotOffset + kSlots * kSlotBytes;
-    // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2]
-    static constexpr int kBarriers = 2 * kSlots + 12;
-    static constexpr int kTmemSlotOffset = kBarrierOffset + 8 * kBarriers;
+    // full, empty per slot; q_full[2], q_empty, drain, s_full[2], s_free[2], p_full[2], o_done[2],
+    // item_full, item_empty per item slot, the launch control's answer
+    static constexpr int kBarriers = 2 * kSlots + 12 + 2 * kItemSlots + 1;
+    static constexpr int kItemOffset = (kBarrierOffset + 8 * kBarriers + 15) / 16 * 16;
+    static constexpr int kAnswerOffset = kItemOffset + kItemSlots * kItemBytes;
+    static constexpr int kTmemSlotOffset = kAnswerOffset + 16;
     static constexpr int kSmemBytes = 1024 + kTmemSlotOffset + 16;
     static constexpr uint32_t kOColumn = 256;
     static constexpr uint32_t kOPitch = Atoms == 2 ? 128 : 64;
@@ -78,48 +91,54 @@ struct Shape {
     static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
 };
 
+// What the warps know of an item, in shared memory.
 struct Item {
-    Sequence s;
+    int rows; // query rows of the block (1..256); 0: no more items
     int head;
     int split;
-    int rows;      // query rows of the block (1..256), 0: nothing to do
-    int first_key; // this split's keys, within the sequence
-    int end_key;
-    long long reach; // row r of the block sees keys below r + reach (causal)
-    int steps0;      // key tiles of each query tile
-    int steps1;
+    int q_first;   // the block's first query row
+    int kv_first;  // the split's first key row
+    int keys;      // of the split
+    int reach;     // row r of the block sees the split's first (reach + r) keys, at least 0
+    int steps[2];  // key tiles of each query tile
+    int unused[3];
 };
+static_assert(sizeof(Item) == kItemBytes, "items are handed over as whole vectors");
 
-__device__ __forceinline__ int tile_steps(const VarlenParams& p, const Item& item, int t) {
-    const int rows = min(kTile, item.rows - t * kTile);
-    long long end = item.end_key;
-    if (p.causal) {
-        end = min(end, item.reach + t * kTile + rows - 1);
-    }
-    return rows <= 0 || end <= item.first_key
-               ? 0
-               : static_cast<int>((end - item.first_key + kTile - 1) / kTile);
+__device__ __forceinline__ int tile_steps(int rows, int keys, int reach, int t) {
+    const int live = min(kTile, rows - t * kTile);
+    const int seen = min(static_cast<long long>(keys),
+                         static_cast<long long>(reach) + t * kTile + live - 1);
+    return live <= 0 || seen <= 0 ? 0 : (seen + kTile - 1) / kTile;
 }
 
+// Item `index` by a whole warp; rows 0 where the block has none.
 __device__ __forceinline__ Item find_item(const VarlenParams& p, long long index) {
-    Item item;
+    Item item{};
     item.split = static_cast<int>(index % p.splits);
     index /= p.splits;
     item.head = static_cast<int>(index % p.q_heads);
     index /= p.q_heads;
-    item.s = find_block(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens, index,
-                        2 * kTile);
-    const Sequence& s = item.s;
+    const Sequence s = find_block_warp(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
+                                       index, 2 * kTile);
     item.rows = s.index < 0 ? 0 : min(2 * kTile, s.q_end - s.q_first);
+    item.q_first = s.q_first;
     const int keys = s.kv_end - s.kv_begin;
     // Whole tiles per split, so that only a sequence's end falls inside a tile.
     const int tiles = (keys + kTile - 1) / kTile;
     const int each = (tiles + p.splits - 1) / p.splits;
-    item.first_key = min(keys, min(tiles, item.split * each) * kTile);
-    item.end_key = min(keys, min(tiles, (item.split + 1) * each) * kTile);
-    item.reach = static_cast<long long>(s.q_first - s.q_begin) + 1 + keys - (s.q_end - s.q_begin);
-    item.steps0 = tile_steps(p, item, 0);
-    item.steps1 = tile_steps(p, item, 1);
+    const int first = min(keys, min(tiles, item.split * each) * kTile);
+    const int end = min(keys, min(tiles, (item.split + 1) * each) * kTile);
+    item.kv_first = s.kv_begin + first;
+    item.keys = end - first;
+    // The first row's share of the split's keys (rows see the split's keys at most).
+    const long long reach = static_cast<long long>(s.q_first - s.q_begin) + 1 + keys -
+                            (s.q_end - s.q_begin) - first;
+    item.reach = p.causal ? static_cast<int>(
+                                max(-4LL * kTile, min(static_cast<long long>(item.keys), reach)))
+                          : item.keys;
+    item.steps[0] = tile_steps(item.rows, item.keys, item.reach, 0);
+    item.steps[1] = tile_steps(item.rows, item.keys, item.reach, 1);
     return item;
 }
 
@@ -223,8 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q,
                            const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v,
-                           const __grid_constant__ VarlenParams p, const long long items,
-                           unsigned* const status) {
+                           const __grid_constant__ VarlenParams p, unsigned* const status) {
     using S = Shape<Atoms>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = dev::smem_u32(smem_raw);
@@ -241,6 +259,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_free = more + 48;   // + 8 t
     const uint32_t p_full = more + 64;   // + 8 t
     const uint32_t o_done = more + 80;   // + 8 t
+    const uint32_t item_full = more + 96;  // + 8 slot
+    const uint32_t item_empty = item_full + 8 * kItemSlots;
+    const uint32_t answer_full = item_empty + 8 * kItemSlots;
+    const auto item_slot = [&](int i) -> Item* {
+        return reinterpret_cast<Item*>(smem + S::kItemOffset) + i;
+    };
 
     // Through a shuffle, so that the compiler knows it is the same for the warp.
     const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) / 32, 0);
@@ -257,6 +281,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             dev::mbar_init(p_full + 8 * t, kRowWarps / 2);
             dev::mbar_init(o_done + 8 * t, 1);
         }
+        for (uint32_t i = 0; i < kItemSlots; ++i) {
+            dev::mbar_init(item_full + 8 * i, 1);
+            dev::mbar_init(item_empty + 8 * i, kRowWarps + 1); // the rows' warps and the issuer
+        }
+        dev::mbar_init(answer_full, 1);
         dev::mbar_init(q_empty, 1);
         dev::mbar_init(drain, 1);
         dev::fence_barrier_init();
@@ -273,15 +302,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
 
-    if (warp == kLoadWarp && lane == 0) {
-        // ---------------- loads ----------------
-        dev::tma_prefetch_descriptor(&map_q);
-        dev::tma_prefetch_descriptor(&map_k);
-        dev::tma_prefetch_descriptor(&map_v);
+    if (warp == kLoadWarp) {
+        // ---------------- items and loads ----------------
+        if (lane == 0) {
+            dev::tma_prefetch_descriptor(&map_q);
+            dev::tma_prefetch_descriptor(&map_k);
+            dev::tma_prefetch_descriptor(&map_v);
+        }
         int slot = 0;
         uint32_t phase = 0;
-        uint32_t q_phase = 0;                 // items with keys so far
-        uint32_t q_loads0 = 0, q_loads1 = 0;  // loads of each query tile so far
+        uint32_t q_phase = 0;                // items with keys so far
+        uint32_t q_loads0 = 0, q_loads1 = 0; // loads of each query tile so far
+        int item_at = 0;
+        uint32_t item_phase = 0;
+        uint32_t answers = 0; // taken so far
+        bool asked = false;
         bool ok = true;
         const auto load_kv = [&](const CUtensorMap* map, int kv_head, int row) {
             if (!dev::mbar_wait(empty(slot), phase ^ 1u, status)) {
@@ -306,43 +341,87 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::tma_load(base + t * S::kQBytes + a * kAtomBytes, &map_q, q_full + 8 * t, 3, c);
             }
         };
-        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
-            const Item item = find_item(p, index);
-            const int steps = max(item.steps0, item.steps1);
-            if (steps == 0) {
-                continue;
+        uint32_t index = blockIdx.x;
+        bool more_items = true;
+        while (true) {
+            Item item{};
+            if (more_items) {
+                // Asked for while this item's loads wait for room.
+                if (lane == 0) {
+                    dev::mbar_arrive_expect_tx(answer_full, 16);
+                    dev::launch_control_try_cancel(base + S::kAnswerOffset, answer_full);
+                }
+                __syncwarp();
+                asked = true;
+                item = find_item(p, p.causal ? gridDim.x - 1 - index : index);
             }
-            if (!dev::mbar_wait(q_empty, (q_phase & 1u) ^ 1u, status)) {
-                ok = false;
+            if (!more_items || item.rows > 0) {
+                ok = dev::mbar_wait_warp(item_empty + 8 * item_at, item_phase ^ 1u, status, kItemWaitNs);
+                if (!ok) {
+                    break;
+                }
+                if (lane == 0) {
+                    *item_slot(item_at) = item;
+                    dev::mbar_arrive(item_full + 8 * item_at);
+                }
+                __syncwarp();
+                if (++item_at == kItemSlots) {
+                    item_at = 0;
+                    item_phase ^= 1u;
+                }
+                if (!more_items) {
+                    break;
+                }
+            }
+            const int steps = max(item.steps[0], item.steps[1]);
+            if (item.rows > 0 && steps > 0) {
+                if (lane == 0) {
+                    ok = dev::mbar_wait(q_empty, (q_phase & 1u) ^ 1u, status);
+                    if (ok && item.steps[0] > 0) {
+                        load_q(0, item.head, item.q_first);
+                    }
+                    if (ok && item.steps[1] > 0) {
+                        load_q(1, item.head, item.q_first + kTile);
+                    }
+                    q_loads0 += ok && item.steps[0] > 0 ? 1u : 0u;
+                    q_loads1 += ok && item.steps[1] > 0 ? 1u : 0u;
+                    const int kv_head = item.head / p.group;
+                    const int row = item.kv_first;
+                    // In the order the MMA warp takes them.
+                    if (ok) {
+                        load_kv(&map_k, kv_head, row);
+                    }
+                    for (int j = 0; j < steps && ok; ++j) {
+                        if (S::kOverlay) {
+                            load_kv(&map_v, kv_head, row + j * kTile);
+                        }
+                        if (ok && j + 1 < steps) {
+                            load_kv(&map_k, kv_head, row + (j + 1) * kTile);
+                        }
+                        if (ok && !S::kOverlay) {
+                            load_kv(&map_v, kv_head, row + j * kTile);
+                        }
+                    }
+                }
+                ++q_phase;
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) {
+                    break;
+                }
+            }
+            ok = dev::mbar_wait_warp(answer_full, answers & 1u, status);
+            if (!ok) {
                 break;
             }
-            ++q_phase;
-            if (item.steps0 > 0) {
-                ++q_loads0;
-                load_q(0, item.head, item.s.q_first);
-            }
-            if (item.steps1 > 0) {
-                ++q_loads1;
-                load_q(1, item.head, item.s.q_first + kTile);
-            }
-            const int kv_head = item.head / p.group;
-            const int row = item.s.kv_begin + item.first_key;
-            // In the order the MMA warp takes them.
-            load_kv(&map_k, kv_head, row);
-            for (int j = 0; j < steps && ok; ++j) {
-                if (S::kOverlay) {
-                    load_kv(&map_v, kv_head, row + j * kTile);
-                }
-                if (ok && j + 1 < steps) {
-                    load_kv(&map_k, kv_head, row + (j + 1) * kTile);
-                }
-                if (ok && !S::kOverlay) {
-                    load_kv(&map_v, kv_head, row + j * kTile);
-                }
-            }
+            ++answers;
+            asked = false;
+            more_items = dev::launch_control_answer(base + S::kAnswerOffset, &index);
+            // The answer has been read before the next one may be written.
+            dev::fence_proxy_async_shared();
+            __syncwarp();
         }
-        if (!ok) {
-            // Every load issued lands before the CTA's shared memory goes.
+        if (!ok && lane == 0) {
+            // Every copy asked for lands before the CTA's shared memory goes.
             for (int i = 0; i < S::kSlots; ++i) {
                 dev::mbar_drain_wait(full(i), phase ^ (i < slot ? 0u : 1u));
             }
@@ -352,7 +431,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (q_loads1 > 0) {
                 dev::mbar_drain_wait(q_full + 8, (q_loads1 - 1) & 1u);
             }
+            if (asked) {
+                dev::mbar_drain_wait(answer_full, answers & 1u);
+            }
         }
+        __syncwarp();
     } else if (warp == kMmaWarp) {
         // ---------------- MMA issue (the whole warp, one lane issuing) ----------------
         const int k_steps = (p.head_dim + 15) / 16;
@@ -370,15 +453,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t free_phase[2] = {0u, 0u};
         uint32_t p_phase[2] = {0u, 0u};
         bool ok = true;
-        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
-            const Item item = find_item(p, index);
+        int item_at = 0;
+        uint32_t item_phase = 0;
+        while (ok) {
+            ok = dev::mbar_wait_warp(item_full + 8 * item_at, item_phase, status, kItemWaitNs);
+            if (!ok) {
+                break;
+            }
             const auto uniform = [](int value) { return __shfl_sync(0xFFFFFFFFu, value, 0); };
-            const int tile_steps[2] = {uniform(item.steps0), uniform(item.steps1)};
+            const Item* const item = item_slot(item_at);
+            const int rows = uniform(item->rows);
+            const int tile_steps[2] = {uniform(item->steps[0]), uniform(item->steps[1])};
+            const int keys = uniform(item->keys);
+            if (lane == 0) {
+                dev::mbar_arrive(item_empty + 8 * item_at);
+            }
+            __syncwarp();
+            if (++item_at == kItemSlots) {
+                item_at = 0;
+                item_phase ^= 1u;
+            }
+            if (rows == 0) {
+                break;
+            }
             const int steps = max(tile_steps[0], tile_steps[1]);
             if (steps == 0) {
                 continue;
             }
-            const int keys = uniform(item.end_key - item.first_key);
             // The first scores.
             {
                 const int keys16 = (min(kTile, keys) + 15) & ~15;
@@ -530,20 +631,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         };
-        for (long long index = blockIdx.x; index < items && ok; index += gridDim.x) {
-            const Item item = find_item(p, index);
-            const int rows = item.rows - t * kTile; // may be 0 or less
+        int item_at = 0;
+        uint32_t item_phase = 0;
+        while (ok) {
+            ok = dev::mbar_wait_warp(item_full + 8 * item_at, item_phase, status, kItemWaitNs);
+            if (!ok) {
+                break;
+            }
+            const Item* const item = item_slot(item_at);
+            const int block_rows = item->rows;
+            const int head = item->head;
+            const int split = item->split;
+            const int steps = item->steps[t];
+            // Keys of the split that this row sees.
+            const int row_keys = max(0, min(item->keys, item->reach + t * kTile + row));
+            const long long token = static_cast<long long>(item->q_first) + t * kTile + row;
+            __syncwarp();
+            if (lane == 0) {
+                dev::mbar_arrive(item_empty + 8 * item_at);
+            }
+            __syncwarp();
+            if (++item_at == kItemSlots) {
+                item_at = 0;
+                item_phase ^= 1u;
+            }
+            if (block_rows == 0) {
+                break;
+            }
+            const int rows = block_rows - t * kTile; // may be 0 or less
             if (rows <= 0) {
                 continue;
             }
-            const int steps = t == 0 ? item.steps0 : item.steps1;
             const bool live_warp = quarter * 32 < rows;
-            // Keys this row sees, from the split's first on.
-            long long end = item.end_key;
-            if (p.causal) {
-                end = max(0LL, min(end, item.reach + t * kTile + row));
-            }
-            const int row_keys = static_cast<int>(max(0LL, end - item.first_key));
             float m = 0.0F; // unscaled
             float sum = 0.0F;
             for (int j = 0; j < steps && ok; ++j) {
@@ -688,25 +807,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue; // the whole warp
             }
             const bool live = row < rows;
-            const long long token = static_cast<long long>(item.s.q_first) + t * kTile + row;
             const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
             const long long part =
-                (static_cast<long long>(item.split) * p.q_tokens + token) * p.q_heads + item.head;
+                (static_cast<long long>(split) * p.q_tokens + token) * p.q_heads + head;
             if (live && p.splits > 1) {
                 p.part_stats[part] = make_float2(sum == 0.0F ? -INFINITY : m * p.scale_log2, sum);
             }
 #pragma unroll 1
-            for (int c = 0; c < o_columns; c += 16) {
-                uint32_t o[16];
+            for (int c = 0; c < p.head_dim; c += 32) {
+                uint32_t o[32];
                 // The read is warp-wide: lanes that store below, and those that do not, meet first.
+                // (Columns past the last 16-column step hold anything and are not stored.)
                 __syncwarp();
                 if (steps > 0) {
-                    dev::tmem_load_16(o_tmem + c, o);
-                    dev::tmem_wait_load();
+                    dev::tmem_load_32(o_tmem + c, o);
+                    dev::tmem_wait_load_of(o);
                 }
                 if (sum == 0.0F) { // no keys: what tensor memory holds is nobody's
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
+                    for (int x = 0; x < 32; ++x) {
                         o[x] = 0u;
                     }
                 }
@@ -714,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float4* const out =
                         reinterpret_cast<float4*>(p.part_out + part * p.head_dim + c);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
+                    for (int x = 0; x < 8; ++x) {
                         if (c + 4 * x < p.head_dim) {
                             out[x] = make_float4(
                                 __uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
@@ -724,9 +843,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 } else if (live) {
                     uint4* const out = reinterpret_cast<uint4*>(
                         static_cast<__nv_bfloat16*>(p.out) + token * p.out_stride +
-                        static_cast<long long>(item.head) * p.head_dim + c);
+                        static_cast<long long>(head) * p.head_dim + c);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
+                    for (int x = 0; x < 4; ++x) {
                         if (c + 8 * x < p.head_dim) {
                             uint32_t words[4];
 #pragma unroll
@@ -760,9 +879,11 @@ int launch_atoms(const VarlenParams& p, const host::DeviceContext& context,
     constexpr int kBytes = Shape<Atoms>::kSmemBytes;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
     const long long items = tiles_kernel_items(p) * p.splits;
-    const long long grid = items < context.sm_count ? items : context.sm_count;
-    host::pdl_launch(kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kBytes, stream,
-                     maps[0], maps[1], maps[2], p, items, context.status);
+    if (items > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
+    }
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(items)), dim3(kThreads), kBytes, stream,
+                     maps[0], maps[1], maps[2], p, context.status);
     return host::after_launch("attention_tiles_kernel");
 }
 

@@ -96,8 +96,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigne
 // mbar_wait by all 32 lanes of a warp, succeeding or failing for the whole warp, so that a
 // warp-wide instruction after it (tcgen05.ld / st are .sync.aligned) never runs with some lanes
 // gone: lanes of one warp can disagree when the wait runs out.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, unsigned* status) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, status));
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, unsigned* status,
+                                               unsigned long long limit_ns = kWaitLimitNs) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, status, limit_ns));
 }
 
 // Waits up to limit_ns for a phase regardless of the status word: used after a failure to
@@ -152,6 +153,36 @@ __device__ __forceinline__ void cluster_sync() {
 // after that wait.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Cluster launch control: asks for the index of a block of this grid that has not started, which
+// then never starts (the running block does its work instead). The 16-byte answer arrives in
+// shared memory, completing transaction bytes on the mbarrier. Not to be asked again after an
+// answer without a block.
+__device__ __forceinline__ void launch_control_try_cancel(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes."
+                 "b128 [%0], [%1];" ::"r"(answer),
+                 "r"(bar)
+                 : "memory");
+}
+
+// Whether an answer names a block, and its blockIdx.x.
+__device__ __forceinline__ bool launch_control_answer(uint32_t answer, uint32_t* index) {
+    uint32_t x = 0, valid;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b128 h;\n\t"
+        "ld.shared.b128 h, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+        "selp.u32 %1, 1, 0, p;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, h;\n\t"
+        "}\n"
+        : "+r"(x), "=r"(valid)
+        : "r"(answer)
+        : "memory");
+    *index = x;
+    return valid != 0;
 }
 
 // Programmatic dependent launch: kernels are launched so that they may start while the

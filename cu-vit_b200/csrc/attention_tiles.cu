@@ -7,8 +7,8 @@
 // blocks that have not started, which it takes over one by one (cluster launch control), so that
 // sequences of very different lengths balance over the SMs without a counter in memory. The load
 // warp asks for the next item, finds its sequence and hands it to the other warps through a ring,
-// all while they still work on the previous ones; queries that see fewer keys than others (causal)
-// come last. The 256 rows
+// all while they still work on the previous ones. Items with most keys come first (up to 32
+// sequences are ordered by their lengths; causal: a sequence's last rows first). The 256 rows
 // are two tiles of 128 whose chains alternate: while the tensor core works for one tile, the other
 // tile's rows take their maxima and exponentials, so neither waits for the other longer than it
 // must. Keys and values stream through a ring of TMA stages shared by both tiles.
@@ -112,15 +112,22 @@ __device__ __forceinline__ int tile_steps(int rows, int keys, int reach, int t) 
     return live <= 0 || seen <= 0 ? 0 : (seen + kTile - 1) / kTile;
 }
 
-// Item `index` by a whole warp; rows 0 where the block has none.
-__device__ __forceinline__ Item find_item(const VarlenParams& p, long long index) {
+// Item `index` by a whole warp; rows 0 where the block has none. Up to 32 sequences come in the
+// order of their work, more in their own order (causal: backwards, rows that see most first).
+__device__ __forceinline__ Item find_item(const VarlenParams& p, const Order& order,
+                                          long long index, long long items) {
     Item item{};
+    const bool ordered = p.batch <= 32;
+    index = p.causal && !ordered ? items - 1 - index : index;
     item.split = static_cast<int>(index % p.splits);
     index /= p.splits;
     item.head = static_cast<int>(index % p.q_heads);
     index /= p.q_heads;
-    const Sequence s = find_block_warp(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
-                                       index, 2 * kTile);
+    const Sequence s =
+        ordered ? find_ordered_block(order, p.q_offsets, p.kv_offsets, p.batch, p.q_tokens,
+                                     p.kv_tokens, index, 2 * kTile, p.causal != 0)
+                : find_block_warp(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
+                                  index, 2 * kTile);
     item.rows = s.index < 0 ? 0 : min(2 * kTile, s.q_end - s.q_first);
     item.q_first = s.q_first;
     const int keys = s.kv_end - s.kv_begin;
@@ -341,6 +348,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::tma_load(base + t * S::kQBytes + a * kAtomBytes, &map_q, q_full + 8 * t, 3, c);
             }
         };
+        Order order{};
+        if (p.batch <= 32) {
+            order = order_sequences(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
+                                    2 * kTile);
+        }
         uint32_t index = blockIdx.x;
         bool more_items = true;
         while (true) {
@@ -353,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
                 asked = true;
-                item = find_item(p, p.causal ? gridDim.x - 1 - index : index);
+                item = find_item(p, order, index, gridDim.x);
             }
             if (!more_items || item.rows > 0) {
                 ok = dev::mbar_wait_warp(item_empty + 8 * item_at, item_phase ^ 1u, status, kItemWaitNs);

@@ -18,10 +18,10 @@
 namespace cuvit::attn {
 namespace {
 
-constexpr int kSimtRows = 64;
+constexpr int kSimtRows = 128;
 constexpr int kSimtKeys = 64;
-constexpr int kSimtThreads = 256;
-constexpr int kSimtPitch = kSimtKeys + 4;
+constexpr int kRowPitch = kSimtRows + 4; // floats; consecutive keys' rows start 4 banks apart
+constexpr int kKeyPitch = kSimtKeys + 4;
 
 template <typename T>
 __device__ __forceinline__ float load_value(const T* p) {
@@ -32,23 +32,73 @@ __device__ __forceinline__ float load_value(const T* p) {
     }
 }
 
-template <int DPad>
-constexpr int simt_smem_bytes() {
-    return 4 * (2 * DPad * kSimtPitch + kSimtKeys * DPad + kSimtKeys * kSimtPitch);
+// Elements e .. e + 3 of a row of d, zeros past its end; `vector`: rows are whole aligned float4s.
+template <typename T>
+__device__ __forceinline__ float4 load_four(const T* row, int e, int d, bool vector) {
+    if constexpr (sizeof(T) == 4) {
+        if (vector) {
+            return e < d ? *reinterpret_cast<const float4*>(row + e)
+                         : make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+        }
+    }
+    return make_float4(e < d ? load_value(row + e) : 0.0F,
+                       e + 1 < d ? load_value(row + e + 1) : 0.0F,
+                       e + 2 < d ? load_value(row + e + 2) : 0.0F,
+                       e + 3 < d ? load_value(row + e + 3) : 0.0F);
 }
 
-// 64 query rows of one head per block, keys in tiles of 64; thread (ty, tx) has rows 4 ty .. + 3
-// and, of the scores, keys 4 tx .. + 3, of the output, elements 4 tx .. + 3 of every 64.
+// Threads along the keys and elements of a tile (kX); each has 8 of its elements, and 8 or 4 of its
+// keys, for 8 rows.
+template <int DPad>
+struct SimtShape {
+    static constexpr int kX = DPad / 8;
+    static constexpr int kCols = DPad / kX / 4; // element groups of four
+    static constexpr int kThreads = 16 * kX;
+    static constexpr int kKeyGroups = kSimtKeys / kX / 4; // of four keys
+    static constexpr int kSmemBytes =
+        4 * (DPad * (kRowPitch + kKeyPitch) + kSimtKeys * DPad + kSimtKeys * kRowPitch);
+};
+
+// acc[r][j] += a[r] * b[j] for 8 rows, contiguous in shared memory.
+__device__ __forceinline__ void outer(const float* rows, const float4& b, float (&acc)[8][4]) {
+    const float4 low = reinterpret_cast<const float4*>(rows)[0];
+    const float4 high = reinterpret_cast<const float4*>(rows)[1];
+    const float a[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+    const float c[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[r][j] = fmaf(a[r], c[j], acc[r][j]);
+        }
+    }
+}
+
+// 128 query rows of one head per block, keys in tiles of 64. Thread (ty, tx) of 16 x kX has rows
+// 8 ty .. + 7 and, of the scores, the keys tx + kX m, of the output, elements 4 tx .. + 3 of every
+// 4 kX. Operands come from shared memory as whole vectors (Q and P with rows contiguous): for heads
+// up to 64, 64 multiply-adds share four loads, and two blocks fit an SM and load under each other's
+// arithmetic. 4096 tokens, 8 heads of 64: 954 us, 36 TFLOP/s of the FP32 pipe's 74. (8 x 4 products a
+// thread on twice the threads: 990 us, shared memory then takes as many cycles as the arithmetic;
+// packed multiply-adds on pairs of rows: 1050 us, since doubling the other operand takes moves on
+// the same pipe. Heads up to 128 use 8 x 4 for the scores: the outputs take the registers.) A tile's
+// keys lie in the order the threads read them, kX apart, which also lets a warp write its weights
+// without bank conflicts.
 template <typename T, int DPad>
-__global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const VarlenParams p) {
+__global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
+    attention_varlen_simt(const VarlenParams p, const int vector) {
+    using Shape = SimtShape<DPad>;
+    constexpr int kX = Shape::kX;
+    constexpr int kThreads = Shape::kThreads;
+    constexpr int kGroups = Shape::kKeyGroups;
+    constexpr int kCols = Shape::kCols;
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
     extern __shared__ __align__(16) float smem[];
-    float* const qs = smem;                       // [DPad][pitch], element-major
-    float* const ks = qs + DPad * kSimtPitch;     // [DPad][pitch]
-    float* const vs = ks + DPad * kSimtPitch;     // [keys][DPad]
-    float* const ps = vs + kSimtKeys * DPad;      // [keys][pitch], key-major
-    constexpr int kChunks = DPad / 64;
+    float* const qs = smem;                  // [DPad][row pitch], element-major
+    float* const ks = qs + DPad * kRowPitch; // [DPad][key pitch], element-major
+    float* const vs = ks + DPad * kKeyPitch; // [keys][DPad]
+    float* const ps = vs + kSimtKeys * DPad; // [keys][row pitch]
 
     const int item = static_cast<int>(blockIdx.x) / p.splits;
     const int split = static_cast<int>(blockIdx.x) - item * p.splits;
@@ -76,139 +126,142 @@ __global__ void __launch_bounds__(kSimtThreads) attention_varlen_simt(const Varl
                        static_cast<long long>(head / p.group) * d;
     const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
                        static_cast<long long>(head / p.group) * d;
+    const auto zeros = []() { return make_float4(0.0F, 0.0F, 0.0F, 0.0F); };
 
-    for (int i = threadIdx.x; i < kSimtRows * DPad; i += kSimtThreads) {
-        const int r = i / DPad;
-        const int e = i - r * DPad;
-        qs[e * kSimtPitch + r] = r < rows && e < d ? load_value(q + r * p.q_stride + e) : 0.0F;
+    for (int i = threadIdx.x; i < kSimtRows * DPad / 4; i += kThreads) {
+        const int r = i % kSimtRows;
+        const int e = i / kSimtRows * 4;
+        const float4 x = r < rows ? load_four(q + r * p.q_stride, e, d, vector != 0) : zeros();
+        qs[e * kRowPitch + r] = x.x;
+        qs[(e + 1) * kRowPitch + r] = x.y;
+        qs[(e + 2) * kRowPitch + r] = x.z;
+        qs[(e + 3) * kRowPitch + r] = x.w;
     }
-    const int tx = threadIdx.x % 16;
-    const int ty = threadIdx.x / 16;
-    float o[4][4 * kChunks] = {};
-    float maximum[4], sum[4];
+    const int tx = threadIdx.x % kX;
+    const int ty = threadIdx.x / kX;
+    float o[kCols][8][4] = {}; // element group, row, element
+    float maximum[8], sum[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 8; ++r) {
         maximum[r] = -INFINITY;
         sum[r] = 0.0F;
     }
     for (int first = first_key; first < last_key; first += kSimtKeys) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kSimtKeys * DPad; i += kSimtThreads) {
-            const int j = i / DPad;
-            const int e = i - j * DPad;
-            const bool live = first + j < last_key && e < d;
-            const long long row = first + j;
-            ks[e * kSimtPitch + j] = live ? load_value(k + row * p.k_stride + e) : 0.0F;
-            vs[j * DPad + e] = live ? load_value(v + row * p.v_stride + e) : 0.0F;
+        __syncthreads(); // the previous tile has been used
+        const int live = min(kSimtKeys, last_key - first);
+        for (int i = threadIdx.x; i < kSimtKeys * DPad / 4; i += kThreads) {
+            const int j = i % kSimtKeys;
+            const int e = i / kSimtKeys * 4;
+            const long long row = static_cast<long long>(first) + j;
+            const float4 x = j < live ? load_four(k + row * p.k_stride, e, d, vector != 0) : zeros();
+            const int m = j / kX;
+            const int at = m / 4 * (4 * kX) + j % kX * 4 + m % 4;
+            ks[e * kKeyPitch + at] = x.x;
+            ks[(e + 1) * kKeyPitch + at] = x.y;
+            ks[(e + 2) * kKeyPitch + at] = x.z;
+            ks[(e + 3) * kKeyPitch + at] = x.w;
+        }
+        for (int i = threadIdx.x; i < kSimtKeys * DPad / 4; i += kThreads) {
+            const int j = i / (DPad / 4);
+            const int e = i % (DPad / 4) * 4;
+            const long long row = static_cast<long long>(first) + j;
+            *reinterpret_cast<float4*>(vs + j * DPad + e) =
+                j < live ? load_four(v + row * p.v_stride, e, d, vector != 0) : zeros();
         }
         __syncthreads();
-        float sc[4][4] = {};
-#pragma unroll 8
+        float score[kGroups][8][4] = {}; // key group, row, key
+#pragma unroll 4
         for (int e = 0; e < d; ++e) {
-            const float4 a = *reinterpret_cast<const float4*>(qs + e * kSimtPitch + 4 * ty);
-            const float4 b = *reinterpret_cast<const float4*>(ks + e * kSimtPitch + 4 * tx);
-            const float av[4] = {a.x, a.y, a.z, a.w};
-            const float bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    sc[r][j] = fmaf(av[r], bv[j], sc[r][j]);
-                }
+            for (int g = 0; g < kGroups; ++g) {
+                outer(qs + e * kRowPitch + 8 * ty,
+                      *reinterpret_cast<const float4*>(ks + e * kKeyPitch + 4 * kX * g + 4 * tx),
+                      score[g]);
             }
         }
+        float factor[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const long long limit = p.causal ? min(static_cast<long long>(last_key),
-                                                   reach + 4 * ty + r + 1)
-                                             : static_cast<long long>(last_key);
+        for (int r = 0; r < 8; ++r) {
+            const int limit = static_cast<int>(
+                p.causal ? min(static_cast<long long>(live), reach + 8 * ty + r + 1 - first)
+                         : static_cast<long long>(live));
             float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sc[r][j] = first + 4 * tx + j < limit ? sc[r][j] * p.scale_log2 : -INFINITY;
-                top = fmaxf(top, sc[r][j]);
+            for (int j = 0; j < 4 * kGroups; ++j) {
+                score[j / 4][r][j % 4] = tx + kX * j < limit ? score[j / 4][r][j % 4] * p.scale_log2 : -INFINITY;
+                top = fmaxf(top, score[j / 4][r][j % 4]);
             }
 #pragma unroll
-            for (int offset = 8; offset > 0; offset /= 2) {
+            for (int offset = kX / 2; offset > 0; offset /= 2) {
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
             }
             const float raised = fmaxf(maximum[r], top);
             // A row without a key so far: any finite stand-in keeps 2^(-inf - m) at zero.
-            const float base = raised == -INFINITY ? 0.0F : raised;
-            const float factor = exp2f(maximum[r] - base);
+            const float stand = raised == -INFINITY ? 0.0F : raised;
+            factor[r] = exp2f(maximum[r] - stand);
             maximum[r] = raised;
-            float part = 0.0F;
+            sum[r] *= factor[r];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sc[r][j] = exp2f(sc[r][j] - base);
-                part += sc[r][j];
-                ps[(4 * tx + j) * kSimtPitch + 4 * ty + r] = sc[r][j];
-            }
-            sum[r] = fmaf(sum[r], factor, part);
-#pragma unroll
-            for (int c = 0; c < 4 * kChunks; ++c) {
-                o[r][c] *= factor;
+            for (int j = 0; j < 4 * kGroups; ++j) {
+                score[j / 4][r][j % 4] = exp2f(score[j / 4][r][j % 4] - stand);
+                sum[r] += score[j / 4][r][j % 4];
             }
         }
-        __syncwarp(); // a row's 16 threads are in one warp
-        const int live = min(kSimtKeys, last_key - first);
+#pragma unroll
+        for (int j = 0; j < 4 * kGroups; ++j) {
+            float4* const at =
+                reinterpret_cast<float4*>(ps + (tx + kX * j) * kRowPitch + 8 * ty);
+            at[0] = make_float4(score[j / 4][0][j % 4], score[j / 4][1][j % 4], score[j / 4][2][j % 4], score[j / 4][3][j % 4]);
+            at[1] = make_float4(score[j / 4][4][j % 4], score[j / 4][5][j % 4], score[j / 4][6][j % 4], score[j / 4][7][j % 4]);
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    o[c][r][j] *= factor[r];
+                }
+            }
+        }
+        __syncwarp(); // the threads of a row are in one warp
 #pragma unroll 4
         for (int j = 0; j < live; ++j) {
-            const float4 a = *reinterpret_cast<const float4*>(ps + j * kSimtPitch + 4 * ty);
-            const float av[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const float4 b =
-                    *reinterpret_cast<const float4*>(vs + j * DPad + 64 * c + 4 * tx);
-                const float bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        o[r][4 * c + x] = fmaf(av[r], bv[x], o[r][4 * c + x]);
-                    }
-                }
+            for (int c = 0; c < kCols; ++c) {
+                outer(ps + j * kRowPitch + 8 * ty,
+                      *reinterpret_cast<const float4*>(vs + j * DPad + 4 * kX * c + 4 * tx), o[c]);
             }
         }
     }
     T* const out = static_cast<T*>(p.out) + s.q_first * p.out_stride +
                    static_cast<long long>(head) * d;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 8; ++r) {
 #pragma unroll
-        for (int offset = 8; offset > 0; offset /= 2) {
+        for (int offset = kX / 2; offset > 0; offset /= 2) {
             sum[r] += __shfl_xor_sync(0xFFFFFFFFu, sum[r], offset);
         }
         const float inverse = sum[r] == 0.0F ? 0.0F : 1.0F / sum[r];
-        const int row = 4 * ty + r;
-        if (row < rows && p.splits > 1) {
-            const long long at =
-                (static_cast<long long>(split) * p.q_tokens + s.q_first + row) * p.q_heads + head;
-            if (tx == 0) {
-                p.part_stats[at] = make_float2(maximum[r], sum[r]);
-            }
+        const int row = 8 * ty + r;
+        const long long at =
+            (static_cast<long long>(split) * p.q_tokens + s.q_first + row) * p.q_heads + head;
+        if (row < rows && p.splits > 1 && tx == 0) {
+            p.part_stats[at] = make_float2(maximum[r], sum[r]);
+        }
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < kCols; ++c) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    if (64 * c + 4 * tx + x < d) {
-                        p.part_out[at * d + 64 * c + 4 * tx + x] = o[r][4 * c + x];
-                    }
-                }
-            }
-        } else if (row < rows) {
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int e = 64 * c + 4 * tx + x;
-                    if (e < d) {
-                        const float value = o[r][4 * c + x] * inverse;
-                        if constexpr (sizeof(T) == 2) {
-                            out[row * p.out_stride + e] = __float2bfloat16_rn(value);
-                        } else {
-                            out[row * p.out_stride + e] = value;
-                        }
+            for (int j = 0; j < 4; ++j) {
+                const int e = 4 * kX * c + 4 * tx + j;
+                const float value = o[c][r][j];
+                if (row < rows && e < d) {
+                    if (p.splits > 1) {
+                        p.part_out[at * d + e] = value;
+                    } else if constexpr (sizeof(T) == 2) {
+                        out[row * p.out_stride + e] = __float2bfloat16_rn(value * inverse);
+                    } else {
+                        out[row * p.out_stride + e] = value * inverse;
                     }
                 }
             }
@@ -223,14 +276,21 @@ long long simt_items(const VarlenParams& p) {
 template <typename T, int DPad>
 int launch_simt(const VarlenParams& p, cudaStream_t stream) {
     auto* kernel = &attention_varlen_simt<T, DPad>;
-    constexpr int kBytes = simt_smem_bytes<DPad>();
+    constexpr int kBytes = SimtShape<DPad>::kSmemBytes;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
     const long long blocks = simt_items(p) * p.splits;
     if (blocks > 0x7FFFFFFFLL) {
         return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
     }
-    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSimtThreads), kBytes,
-                     stream, p);
+    const auto whole = [&](const void* base, long long stride) {
+        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride % 4 == 0;
+    };
+    const int vector = p.head_dim % 4 == 0 && whole(p.q, p.q_stride) && whole(p.k, p.k_stride) &&
+                               whole(p.v, p.v_stride)
+                           ? 1
+                           : 0;
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(SimtShape<DPad>::kThreads),
+                     kBytes, stream, p, vector);
     return host::after_launch("attention_varlen_simt");
 }
 

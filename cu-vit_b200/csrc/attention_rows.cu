@@ -2,11 +2,18 @@
 // of each sequence), and the kernel that joins the parts of calls that split their keys.
 //
 // Bound by HBM: every key and value is used for a handful of multiply-adds per byte. A group of
-// lanes holds one key at a time, 16 bytes a lane (the query rows' same elements stay in
-// registers), and keeps its own running maximum, sum and output for its share of the keys, so
-// the only exchange while streaming is the butterfly of each score; groups, warps and splits are
-// merged at the end. Rows that share a key head (grouped heads, several queries) are taken
-// together, so keys are read once for them.
+// lanes takes a few keys at a time, 16 bytes of each a lane (the query rows' same elements stay in
+// registers), and keeps its own running maximum, sum and output for its share of the keys; groups,
+// warps and splits are merged at the end. Rows that share a key head (grouped heads, several
+// queries) are taken together, so keys are read once for them.
+//
+// What is left to spend is issue slots: 4 rows over heads of 128 at 24 bytes a cycle and SM leave
+// about 40 instructions a key and warp. So the lanes' partial scores of all (row, key) pairs are
+// summed by halving, each step leaving a lane with half the pairs (15 shuffles for 16 sums over 16
+// lanes, where a butterfly for each takes 64), every weight is computed once, by the lane that ends
+// up with its score, and handed back by one shuffle, products run as packed pairs, and outputs are
+// rescaled only when a maximum has risen by more than 2^8 (weights stay below 2^8; the quotient
+// does not change).
 #include "attention_varlen.hpp"
 #include "ptx.cuh"
 #include "varlen.cuh"
@@ -41,15 +48,54 @@ struct Lane {
                      : "memory");
     }
 
-    static __device__ __forceinline__ void unpack(const uint4& raw, float (&out)[kElems]) {
+    static __device__ __forceinline__ void unpack(const uint4& raw, uint64_t (&out)[kElems / 2]) {
         const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 2) {
-                out[2 * i] = __uint_as_float(words[i] << 16);
-                out[2 * i + 1] = __uint_as_float(words[i] & 0xFFFF0000u);
+            for (int i = 0; i < 4; ++i) {
+                out[i] = dev::f32x2(__uint_as_float(words[i] << 16),
+                                    __uint_as_float(words[i] & 0xFFFF0000u));
+            }
+        } else {
+            out[0] = dev::f32x2(__uint_as_float(words[0]), __uint_as_float(words[1]));
+            out[1] = dev::f32x2(__uint_as_float(words[2]), __uint_as_float(words[3]));
+        }
+    }
+};
+
+__host__ __device__ constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
+
+// Which of a group's N = Rows * Unroll sums (sum r * Unroll + u is row r's of key u) a lane ends up
+// with after halving: kHeld consecutive ones, from kHeld * (lane / kCopies) on.
+template <int Lanes, int Rows, int Unroll>
+struct Halving {
+    static constexpr int kSums = Rows * Unroll;
+    static constexpr int kSteps =
+        log2_of(kSums) < log2_of(Lanes) ? log2_of(kSums) : log2_of(Lanes);
+    static constexpr int kHeld = kSums >> kSteps;
+    static constexpr int kCopies = Lanes >> kSteps; // lanes with the same sums
+    static constexpr int kHeldRows = kHeld > Unroll ? kHeld / Unroll : 1;
+    static constexpr int kHeldKeys = kHeld > Unroll ? Unroll : kHeld;
+
+    // The lane of a group that holds sum i, and where.
+    static __host__ __device__ constexpr int lane_of(int i) { return i / kHeld * kCopies; }
+    static __host__ __device__ constexpr int place_of(int i) { return i % kHeld; }
+
+    static __device__ __forceinline__ void reduce(float (&v)[kSums], int lane) {
+#pragma unroll
+        for (int step = 0; step < log2_of(Lanes); ++step) {
+            const int offset = Lanes >> (step + 1);
+            if (step < kSteps) {
+                const int n = kSums >> (step + 1);
+                const bool upper = (lane & offset) != 0;
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const float send = upper ? v[i] : v[i + n];
+                    const float keep = upper ? v[i + n] : v[i];
+                    v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, send, offset);
+                }
             } else {
-                out[i] = __uint_as_float(words[i]);
+                v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], offset);
             }
         }
     }
@@ -70,7 +116,9 @@ __global__ void __launch_bounds__(kThreads)
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
     constexpr int kElems = Lane<T>::kElems;
+    constexpr int kPairs = kElems / 2;
     constexpr int kUnroll = kUnrollOf<Rows>;
+    using Halves = Halving<Lanes, Rows, kUnroll>;
     constexpr int kGroups = kThreads / Lanes; // key streams of the block
     // Keys and values in flight; each lane reads back only what it copied itself, so the ring
     // needs no barrier. Afterwards the warps' parts.
@@ -111,34 +159,44 @@ __global__ void __launch_bounds__(kThreads)
     const int element = lane * kElems;
     const bool in_row = element < p.head_dim;
 
-    float q[Rows][kElems];
-    int limit[Rows]; // keys row r sees
+    uint64_t q[Rows][kPairs];
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
         const int query = r / heads;
         const int head = head0 + r - query * heads;
 #pragma unroll
-        for (int j = 0; j < kElems; ++j) {
-            q[r][j] = 0.0F;
+        for (int j = 0; j < kPairs; ++j) {
+            q[r][j] = 0u;
         }
-        limit[r] = 0;
-        if (r < rows) {
-            if (in_row) {
-                Lane<T>::unpack(Lane<T>::load(static_cast<const T*>(p.q) +
-                                              (s.q_first + query) * p.q_stride +
-                                              static_cast<long long>(head) * p.head_dim + element),
-                                q[r]);
-            }
+        if (r < rows && in_row) {
+            Lane<T>::unpack(Lane<T>::load(static_cast<const T*>(p.q) +
+                                          (s.q_first + query) * p.q_stride +
+                                          static_cast<long long>(head) * p.head_dim + element),
+                            q[r]);
+            const uint64_t scale = dev::f32x2(p.scale_log2, p.scale_log2);
 #pragma unroll
-            for (int j = 0; j < kElems; ++j) {
-                q[r][j] *= p.scale_log2;
+            for (int j = 0; j < kPairs; ++j) {
+                q[r][j] = dev::mul_f32x2(q[r][j], scale);
             }
-            const long long last = static_cast<long long>(s.q_first - s.q_begin) + query + 1 +
-                                   keys - (s.q_end - s.q_begin);
-            limit[r] = p.causal ? static_cast<int>(max(
-                                      0LL, min(static_cast<long long>(end_key), last)))
-                                : end_key;
         }
+    }
+    // What this lane holds of the group's scores: rows from held_row on, keys from held_key on.
+    const int held = lane / Halves::kCopies * Halves::kHeld;
+    const int held_row = held / kUnroll;
+    const int held_key = held % kUnroll;
+    int limit[Halves::kHeldRows]; // keys a held row sees
+    float top[Halves::kHeldRows]; // its maximum, at most 2^8 below the true one
+    float sum[Halves::kHeldRows]; // its weights, of the keys held here
+#pragma unroll
+    for (int h = 0; h < Halves::kHeldRows; ++h) {
+        const int r = held_row + h;
+        const long long last = static_cast<long long>(s.q_first - s.q_begin) + r / heads + 1 +
+                               keys - (s.q_end - s.q_begin);
+        limit[h] = p.causal ? static_cast<int>(max(0LL, min(static_cast<long long>(end_key), last)))
+                            : end_key;
+        limit[h] = r < rows ? limit[h] : 0;
+        top[h] = -INFINITY;
+        sum[h] = 0.0F;
     }
     const T* const k0 = static_cast<const T*>(p.q); // never read: copies of no bytes name it
     const T* const k = static_cast<const T*>(p.k) + s.kv_begin * p.k_stride +
@@ -146,14 +204,19 @@ __global__ void __launch_bounds__(kThreads)
     const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
                        static_cast<long long>(kv_head) * p.head_dim + element;
 
-    float o[Rows][kElems] = {};
-    float top[Rows], sum[Rows];
+    uint64_t o[Rows][kPairs];
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
-        top[r] = -INFINITY;
-        sum[r] = 0.0F;
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+            o[r][j] = 0u;
+        }
     }
-    // Whole warps go round together (the butterflies need every lane).
+    const int group_lane0 = threadIdx.x % 32 / Lanes * Lanes;
+    const auto from_lane = [&](float value, int lane_of_group) {
+        return __shfl_sync(0xFFFFFFFFu, value, group_lane0 + lane_of_group);
+    };
+    // Whole warps go round together (the sums need every lane).
     const int warp_group0 = (threadIdx.x / 32) * (32 / Lanes);
     const int step = kGroups * kUnroll;
     const auto fetch = [&](int stage, int base) {
@@ -178,70 +241,88 @@ __global__ void __launch_bounds__(kThreads)
     int stage = 0;
     for (int base = first_key; base + warp_group0 < end_key; base += step) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-        uint4 k_raw[kUnroll], v_raw[kUnroll];
+        float score[Halves::kSums];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            k_raw[u] = shared.ring[stage][u][0][threadIdx.x];
-        }
-        float score[Rows][kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float kf[kElems];
-            Lane<T>::unpack(k_raw[u], kf);
+            uint64_t kf[kPairs];
+            Lane<T>::unpack(shared.ring[stage][u][0][threadIdx.x], kf);
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
-                float dot = 0.0F;
+                uint64_t dot = dev::mul_f32x2(q[r][0], kf[0]);
 #pragma unroll
-                for (int j = 0; j < kElems; ++j) {
-                    dot = fmaf(q[r][j], kf[j], dot);
+                for (int j = 1; j < kPairs; ++j) {
+                    dot = dev::fma_f32x2(q[r][j], kf[j], dot);
                 }
-                score[r][u] = dot;
+                const float2 both = dev::f32x2_split(dot);
+                score[r * kUnroll + u] = both.x + both.y;
             }
         }
+        Halves::reduce(score, lane);
+        // The held scores' weights.
+        bool raise = false;
+        float high[Halves::kHeldRows];
 #pragma unroll
-        for (int offset = Lanes / 2; offset > 0; offset /= 2) {
+        for (int h = 0; h < Halves::kHeldRows; ++h) {
+            high[h] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < Halves::kHeldKeys; ++i) {
+                float& value = score[h * Halves::kHeldKeys + i];
+                const int key = base + (held_key + i) * kGroups + group;
+                value = key < limit[h] ? value : -INFINITY;
+                high[h] = fmaxf(high[h], value);
+            }
+            // Over the lanes that hold the row's other keys.
+#pragma unroll
+            for (int keys_held = Halves::kHeldKeys; keys_held < kUnroll; keys_held *= 2) {
+                high[h] = fmaxf(high[h],
+                                __shfl_xor_sync(0xFFFFFFFFu, high[h],
+                                                keys_held / Halves::kHeld * Halves::kCopies));
+            }
+            raise = raise || high[h] > top[h] + 8.0F;
+        }
+        if (__any_sync(0xFFFFFFFFu, raise)) {
+            float factor[Halves::kHeldRows];
+#pragma unroll
+            for (int h = 0; h < Halves::kHeldRows; ++h) {
+                // Without a key so far, any finite stand-in keeps 2^(-inf - m) at zero.
+                const float raised = fmaxf(top[h], high[h]);
+                factor[h] = exp2f(top[h] - (raised == -INFINITY ? 0.0F : raised));
+                top[h] = raised;
+                sum[h] *= factor[h];
+            }
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
+                const float f = from_lane(factor[Halves::place_of(r * kUnroll) / kUnroll],
+                                          Halves::lane_of(r * kUnroll));
+                const uint64_t f2 = dev::f32x2(f, f);
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    score[r][u] += __shfl_xor_sync(0xFFFFFFFFu, score[r][u], offset);
+                for (int j = 0; j < kPairs; ++j) {
+                    o[r][j] = dev::mul_f32x2(o[r][j], f2);
                 }
             }
         }
 #pragma unroll
-        for (int r = 0; r < Rows; ++r) {
-            float raised = top[r];
+        for (int h = 0; h < Halves::kHeldRows; ++h) {
+            const float stand = top[h] == -INFINITY ? 0.0F : top[h];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int key = base + u * kGroups + group;
-                score[r][u] = key < limit[r] ? score[r][u] : -INFINITY;
-                raised = fmaxf(raised, score[r][u]);
-            }
-            // Without a key so far, any finite stand-in keeps 2^(-inf - m) at zero.
-            const float stand = raised == -INFINITY ? 0.0F : raised;
-            const float factor = exp2f(top[r] - stand);
-            top[r] = raised;
-            sum[r] *= factor;
-#pragma unroll
-            for (int j = 0; j < kElems; ++j) {
-                o[r][j] *= factor;
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                score[r][u] = exp2f(score[r][u] - stand);
-                sum[r] += score[r][u];
+            for (int i = 0; i < Halves::kHeldKeys; ++i) {
+                float& value = score[h * Halves::kHeldKeys + i];
+                value = dev::ex2_approx(value - stand);
+                sum[h] += value;
             }
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float vf[kElems];
-            v_raw[u] = shared.ring[stage][u][1][threadIdx.x];
-            Lane<T>::unpack(v_raw[u], vf);
+            uint64_t vf[kPairs];
+            Lane<T>::unpack(shared.ring[stage][u][1][threadIdx.x], vf);
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
+                const float weight = from_lane(score[Halves::place_of(r * kUnroll + u)],
+                                               Halves::lane_of(r * kUnroll + u));
+                const uint64_t weight2 = dev::f32x2(weight, weight);
 #pragma unroll
-                for (int j = 0; j < kElems; ++j) {
-                    o[r][j] = fmaf(score[r][u], vf[j], o[r][j]);
+                for (int j = 0; j < kPairs; ++j) {
+                    o[r][j] = dev::fma_f32x2(weight2, vf[j], o[r][j]);
                 }
             }
         }
@@ -257,21 +338,40 @@ __global__ void __launch_bounds__(kThreads)
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads(); // the ring becomes the parts
 
-    // Lane groups of a warp, then the warps, in a fixed order.
+    // Every lane gets its group's maxima and sums, then lane groups of a warp and the warps are
+    // merged, in a fixed order.
+    float row_top[Rows], row_sum[Rows];
+    float part[Rows][kElems];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        const int slot = Halves::place_of(r * kUnroll) / kUnroll;
+        row_top[r] = from_lane(top[slot], Halves::lane_of(r * kUnroll));
+        row_sum[r] = 0.0F;
+#pragma unroll
+        for (int u = 0; u < kUnroll; u += Halves::kHeldKeys) {
+            row_sum[r] += from_lane(sum[slot], Halves::lane_of(r * kUnroll + u));
+        }
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+            const float2 pair = dev::f32x2_split(o[r][j]);
+            part[r][2 * j] = pair.x;
+            part[r][2 * j + 1] = pair.y;
+        }
+    }
 #pragma unroll
     for (int offset = Lanes; offset < 32; offset *= 2) {
 #pragma unroll
         for (int r = 0; r < Rows; ++r) {
-            const float other = __shfl_xor_sync(0xFFFFFFFFu, top[r], offset);
-            const float other_sum = __shfl_xor_sync(0xFFFFFFFFu, sum[r], offset);
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, row_top[r], offset);
+            const float other_sum = __shfl_xor_sync(0xFFFFFFFFu, row_sum[r], offset);
             float raised, mine, theirs;
-            merge_factors(top[r], other, raised, mine, theirs);
-            top[r] = raised;
-            sum[r] = sum[r] * mine + other_sum * theirs;
+            merge_factors(row_top[r], other, raised, mine, theirs);
+            row_top[r] = raised;
+            row_sum[r] = row_sum[r] * mine + other_sum * theirs;
 #pragma unroll
             for (int j = 0; j < kElems; ++j) {
-                const float other_o = __shfl_xor_sync(0xFFFFFFFFu, o[r][j], offset);
-                o[r][j] = o[r][j] * mine + other_o * theirs;
+                const float other_o = __shfl_xor_sync(0xFFFFFFFFu, part[r][j], offset);
+                part[r][j] = part[r][j] * mine + other_o * theirs;
             }
         }
     }
@@ -280,11 +380,11 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int r = 0; r < Rows; ++r) {
             if (lane == 0) {
-                merged_stats[warp][r] = make_float2(top[r], sum[r]);
+                merged_stats[warp][r] = make_float2(row_top[r], row_sum[r]);
             }
 #pragma unroll
             for (int j = 0; j < kElems; ++j) {
-                merged_out[warp][r][element + j] = o[r][j];
+                merged_out[warp][r][element + j] = part[r][j];
             }
         }
     }

@@ -16,6 +16,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 
 namespace cuvit::rotary {
 namespace {
@@ -216,24 +217,6 @@ struct alignas(sizeof(T) * V) Vec {
     T value[V];
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void unpack(const Vec<T, V>& raw, float (&out)[V]) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        out[j] = load_value(&raw.value[j]);
-    }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
-    Vec<T, V> raw;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        store_value(&raw.value[j], in[j]);
-    }
-    *reinterpret_cast<Vec<T, V>*>(p) = raw;
-}
-
 // Sum over the `count` lanes from lane `first` on, of which this is number `position`: windows of
 // 1, 2, 4, ... lanes (around the group's end) and from them the sum of `count`.
 __device__ __forceinline__ float group_sum(float value, int first, int position, int count) {
@@ -256,13 +239,61 @@ __device__ __forceinline__ float group_sum(float value, int first, int position,
     return total;
 }
 
-template <typename T, int V, int Norm>
+// A lane's V elements as V / 2 packed pairs.
+template <typename T, int V>
+__device__ __forceinline__ void unpack2(const Vec<T, V>& raw, uint64_t (&out)[V / 2]) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t word;
+            memcpy(&word, &raw.value[2 * j], 4);
+            out[j] = dev::f32x2(__uint_as_float(word << 16), __uint_as_float(word & 0xFFFF0000u));
+        } else {
+            out[j] = dev::f32x2(raw.value[2 * j], raw.value[2 * j + 1]);
+        }
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store2(T* p, const uint64_t (&in)[V / 2]) {
+    Vec<T, V> raw;
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+        const float2 pair = dev::f32x2_split(in[j]);
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t word = dev::pack_bf16x2(pair.x, pair.y);
+            memcpy(&raw.value[2 * j], &word, 4);
+        } else {
+            raw.value[2 * j] = pair.x;
+            raw.value[2 * j + 1] = pair.y;
+        }
+    }
+    *reinterpret_cast<Vec<T, V>*>(p) = raw;
+}
+
+// V consecutive floats of shared memory as pairs.
+template <int V>
+__device__ __forceinline__ void shared_pairs(const float* p, uint64_t (&out)[V / 2]) {
+    if constexpr (V >= 4) {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const ulonglong2 two = reinterpret_cast<const ulonglong2*>(p)[j];
+            out[2 * j] = two.x;
+            out[2 * j + 1] = two.y;
+        }
+    } else {
+        out[0] = *reinterpret_cast<const uint64_t*>(p);
+    }
+}
+
+template <typename T, int V, int Norm, bool Adjacent>
 __global__ void __launch_bounds__(kThreads)
     qk_vector_kernel(const __grid_constant__ Params p, const VectorShape s) {
     __shared__ float4 table[kTableVectors];
     __shared__ __align__(16) float gains[Norm == kNormNone ? 1 : 4][kMaxHeadDim];
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
+    constexpr int kPairs = V / 2;
     const int token0 = static_cast<int>(blockIdx.x) * s.block_tokens;
     const int tokens = min(s.block_tokens, p.tokens - token0);
     const int half = p.head_dim / 2;
@@ -276,7 +307,7 @@ __global__ void __launch_bounds__(kThreads)
     const int group = warp * s.warp_groups + group_of_warp;
     const int groups = kWarps * s.warp_groups;
     int first, second; // this lane's elements
-    if (p.adjacent) {
+    if constexpr (Adjacent) {
         first = 2 * V * chunk;
         second = first + V;
     } else {
@@ -288,31 +319,39 @@ __global__ void __launch_bounds__(kThreads)
     const auto token_of = [&](int item) {
         return heads == 1 ? item : static_cast<int>(__umulhi(static_cast<unsigned>(item), s.magic));
     };
+    const T* const in[2] = {
+        static_cast<const T*>(p.side[0].in) + token0 * p.side[0].in_stride,
+        static_cast<const T*>(p.side[1].in) + token0 * p.side[1].in_stride -
+            static_cast<long long>(q_heads) * p.head_dim};
     const auto load_item = [&](int item, Vec<T, V>& x, Vec<T, V>& y) {
         if (item < items && in_group) {
             const int t = token_of(item);
             const int head = item - t * heads;
             const bool key = head >= q_heads;
-            const Side& side = p.side[key ? 1 : 0];
-            const T* const in = static_cast<const T*>(side.in) + (token0 + t) * side.in_stride +
-                                (head - (key ? q_heads : 0)) * p.head_dim;
-            x = *reinterpret_cast<const Vec<T, V>*>(in + first);
-            y = *reinterpret_cast<const Vec<T, V>*>(in + second);
+            const T* const at = (key ? in[1] : in[0]) +
+                                t * (key ? p.side[1].in_stride : p.side[0].in_stride) +
+                                head * p.head_dim;
+            x = *reinterpret_cast<const Vec<T, V>*>(at + first);
+            y = *reinterpret_cast<const Vec<T, V>*>(at + second);
         }
     };
     Vec<T, V> x_next{}, y_next{};
     load_item(group, x_next, y_next);
 
     // Two neighbouring pairs of a token per float4, placed so that the lanes of a head read
-    // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c.
+    // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c, as cos, cos, sin, sin for
+    // pairs in two halves (whose elements are packed with their neighbours) and cos, sin, cos, sin
+    // for adjacent ones.
     for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
         const int t = i / half;
         const int pair = i - t * half;
         const int c = pair / V;
         const int within = pair - c * V;
-        reinterpret_cast<float2*>(
-            table)[(t * (half / 2) + (within / 2) * s.chunks + c) * 2 + (within & 1)] =
-            turn_of(p, token0 + t, pair);
+        float* const at = reinterpret_cast<float*>(
+            table + t * (half / 2) + (within / 2) * s.chunks + c);
+        const float2 turn = turn_of(p, token0 + t, pair);
+        at[Adjacent ? 2 * (within & 1) : within & 1] = turn.x;
+        at[Adjacent ? 2 * (within & 1) + 1 : 2 + (within & 1)] = turn.y;
     }
     if constexpr (Norm != kNormNone) {
         for (int i = threadIdx.x; i < 2 * p.head_dim; i += kThreads) {
@@ -324,80 +363,112 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncthreads();
 
+    const bool offsets = p.side[0].beta != nullptr || p.side[1].beta != nullptr;
     const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
     // Whole warps go round together: the sums need every lane of a group.
     for (int base = 0; base < items; base += groups) {
         const int item = base + group;
         const bool live = item < items && in_group;
-        float x[V], y[V];
-        unpack(x_next, x);
-        unpack(y_next, y);
+        uint64_t x[kPairs], y[kPairs];
+        unpack2(x_next, x);
+        unpack2(y_next, y);
         load_item(item + groups, x_next, y_next);
         const int t = live ? token_of(item) : 0;
         const int head = live ? item - t * heads : 0;
-        const int key = head >= q_heads ? 1 : 0;
+        const bool key = head >= q_heads;
         if constexpr (Norm != kNormNone) {
-            float mean = 0.0F;
             if constexpr (Norm == CUVIT_NORM_LAYER) {
-                float sum = 0.0F;
+                uint64_t sums = dev::add_f32x2(x[0], y[0]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    sum += x[j] + y[j];
+                for (int j = 1; j < kPairs; ++j) {
+                    sums = dev::add_f32x2(sums, dev::add_f32x2(x[j], y[j]));
                 }
-                mean = group_sum(sum, first_lane, chunk, s.chunks) * inverse_dim;
-            }
-            float squares = 0.0F;
+                const float2 both = dev::f32x2_split(sums);
+                const float mean =
+                    group_sum(both.x + both.y, first_lane, chunk, s.chunks) * inverse_dim;
+                const uint64_t mean2 = dev::f32x2(mean, mean);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                x[j] -= mean;
-                y[j] -= mean;
-                squares = fmaf(x[j], x[j], fmaf(y[j], y[j], squares));
+                for (int j = 0; j < kPairs; ++j) {
+                    x[j] = dev::sub_f32x2(x[j], mean2);
+                    y[j] = dev::sub_f32x2(y[j], mean2);
+                }
             }
-            squares = group_sum(squares, first_lane, chunk, s.chunks);
-            const float scale = 1.0F / sqrtf(squares * inverse_dim + p.epsilon);
-            const float* const gamma = gains[2 * key];
-            const float* const beta = gains[2 * key + 1];
+            uint64_t squares2 = dev::mul_f32x2(x[0], x[0]);
+            squares2 = dev::fma_f32x2(y[0], y[0], squares2);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                x[j] = fmaf(x[j] * scale, gamma[first + j], beta[first + j]);
-                y[j] = fmaf(y[j] * scale, gamma[second + j], beta[second + j]);
+            for (int j = 1; j < kPairs; ++j) {
+                squares2 = dev::fma_f32x2(x[j], x[j], squares2);
+                squares2 = dev::fma_f32x2(y[j], y[j], squares2);
+            }
+            const float2 both = dev::f32x2_split(squares2);
+            const float squares = group_sum(both.x + both.y, first_lane, chunk, s.chunks);
+            const float scale = rsqrtf(fmaf(squares, inverse_dim, p.epsilon));
+            const uint64_t scale2 = dev::f32x2(scale, scale);
+            const float* const gamma = gains[key ? 2 : 0];
+            uint64_t gain[kPairs];
+            shared_pairs<V>(gamma + first, gain);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                x[j] = dev::mul_f32x2(dev::mul_f32x2(x[j], scale2), gain[j]);
+            }
+            shared_pairs<V>(gamma + second, gain);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+                y[j] = dev::mul_f32x2(dev::mul_f32x2(y[j], scale2), gain[j]);
+            }
+            if (offsets) {
+                const float* const beta = gains[key ? 3 : 1];
+                shared_pairs<V>(beta + first, gain);
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    x[j] = dev::add_f32x2(x[j], gain[j]);
+                }
+                shared_pairs<V>(beta + second, gain);
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    y[j] = dev::add_f32x2(y[j], gain[j]);
+                }
             }
         }
         if (live) {
-            float turns[2 * V]; // cos, sin of each pair
+            const float4* const turns = table + t * (half / 2) + chunk;
+            if constexpr (Adjacent) {
+                // Pair j of the chunk is element pair j of x followed by y: with the turn (c, s),
+                // (a, b) becomes (a c - b s, b c + a s).
+                const auto turn = [](uint64_t pair, float c, float d) {
+                    const float2 v = dev::f32x2_split(pair);
+                    return dev::fma_f32x2(dev::f32x2(-v.y, v.x), dev::f32x2(d, d),
+                                          dev::mul_f32x2(pair, dev::f32x2(c, c)));
+                };
+                constexpr int kQuarter = kPairs / 2;
 #pragma unroll
-            for (int q = 0; q < V / 2; ++q) {
-                const float4 two = table[t * (half / 2) + q * s.chunks + chunk];
-                turns[4 * q] = two.x;
-                turns[4 * q + 1] = two.y;
-                turns[4 * q + 2] = two.z;
-                turns[4 * q + 3] = two.w;
-            }
-            // Pair j of the chunk: (x[j], y[j]), or elements 2j and 2j + 1 of x followed by y.
-            const auto turn = [&](float& a, float& b, int j) {
-                const float c = turns[2 * j];
-                const float d = turns[2 * j + 1];
-                const float turned = a * c - b * d;
-                b = fmaf(a, d, b * c);
-                a = turned;
-            };
-            if (p.adjacent) {
-#pragma unroll
-                for (int j = 0; j < V / 2; ++j) {
-                    turn(x[2 * j], x[2 * j + 1], j);
-                    turn(y[2 * j], y[2 * j + 1], V / 2 + j);
+                for (int q = 0; q < kPairs; ++q) {
+                    const float4 two = turns[q * s.chunks];
+                    if constexpr (kQuarter > 0) {
+                        uint64_t* const at = q < kQuarter ? &x[2 * q] : &y[2 * (q - kQuarter)];
+                        at[0] = turn(at[0], two.x, two.y);
+                        at[1] = turn(at[1], two.z, two.w);
+                    } else {
+                        x[0] = turn(x[0], two.x, two.y);
+                        y[0] = turn(y[0], two.z, two.w);
+                    }
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    turn(x[j], y[j], j);
+                for (int j = 0; j < kPairs; ++j) {
+                    const ulonglong2 two =
+                        *reinterpret_cast<const ulonglong2*>(turns + j * s.chunks);
+                    const uint64_t turned = dev::sub_f32x2(dev::mul_f32x2(x[j], two.x),
+                                                           dev::mul_f32x2(y[j], two.y));
+                    y[j] = dev::fma_f32x2(x[j], two.y, dev::mul_f32x2(y[j], two.x));
+                    x[j] = turned;
                 }
             }
-            const Side& side = p.side[key];
+            const Side& side = p.side[key ? 1 : 0];
             T* const out = static_cast<T*>(side.out) + (token0 + t) * side.out_stride +
                            (head - (key ? q_heads : 0)) * p.head_dim;
-            store_vec<T, V>(out + first, x);
-            store_vec<T, V>(out + second, y);
+            store2<T, V>(out + first, x);
+            store2<T, V>(out + second, y);
         }
     }
 }
@@ -444,8 +515,9 @@ int launch_vector(const Params& p, int sm_count, cudaStream_t stream) {
     const int spread = p.tokens / (12 * sm_count);
     s.block_tokens = tokens < spread ? tokens : (spread > 0 ? spread : 1);
     const int blocks = (p.tokens + s.block_tokens - 1) / s.block_tokens;
-    host::pdl_launch(qk_vector_kernel<T, V, Norm>, dim3(static_cast<unsigned>(blocks)),
-                     dim3(kThreads), 0, stream, p, s);
+    host::pdl_launch(p.adjacent ? qk_vector_kernel<T, V, Norm, true>
+                                : qk_vector_kernel<T, V, Norm, false>,
+                     dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p, s);
     return host::after_launch("qk_vector_kernel");
 }
 

@@ -465,25 +465,49 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const VarlenPa
     for (int offset = 16; offset > 0; offset /= 2) {
         total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
     }
+    // Lane's elements: 4 lane .. + 3 as one vector, or lane, lane + 32, ... where rows are not whole
+    // vectors. Eight splits' loads are in flight at a time.
     const float* const parts = p.part_out + (row * p.q_heads + head) * p.head_dim;
+    const bool vector = p.head_dim % 4 == 0;
+    constexpr int kBatch = 8;
     float value[4] = {};
+#pragma unroll 1
+    for (int first = 0; first < p.splits; first += kBatch * kWarps) {
+        float4 loaded[kBatch];
+        float weight[kBatch];
 #pragma unroll
-    for (int i = 0; i < kMaxSplits / kWarps; ++i) {
-        const int at = warp + kWarps * i;
-        const float weight = __shfl_sync(0xFFFFFFFFu, factor[at / 32], at % 32);
-        if (at < p.splits) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int e = lane + 32 * j;
-                if (e < p.head_dim) {
-                    value[j] = fmaf(weight, parts[at * pitch * p.head_dim + e], value[j]);
+        for (int i = 0; i < kBatch; ++i) {
+            const int at = first + warp + kWarps * i;
+            weight[i] = __shfl_sync(0xFFFFFFFFu, at < 32 ? factor[0] : factor[1], at % 32);
+            loaded[i] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+            if (at < p.splits) {
+                const float* const from = parts + at * pitch * p.head_dim;
+                if (vector) {
+                    if (4 * lane < p.head_dim) {
+                        loaded[i] = reinterpret_cast<const float4*>(from)[lane];
+                    }
+                } else {
+                    loaded[i].x = lane < p.head_dim ? from[lane] : 0.0F;
+                    loaded[i].y = lane + 32 < p.head_dim ? from[lane + 32] : 0.0F;
+                    loaded[i].z = lane + 64 < p.head_dim ? from[lane + 64] : 0.0F;
+                    loaded[i].w = lane + 96 < p.head_dim ? from[lane + 96] : 0.0F;
                 }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (first + warp + kWarps * i < p.splits) { // a weight past the end is a NaN's at worst
+                value[0] = fmaf(weight[i], loaded[i].x, value[0]);
+                value[1] = fmaf(weight[i], loaded[i].y, value[1]);
+                value[2] = fmaf(weight[i], loaded[i].z, value[2]);
+                value[3] = fmaf(weight[i], loaded[i].w, value[3]);
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        sums[warp][lane + 32 * j] = value[j];
+        const int e = vector ? 4 * lane + j : lane + 32 * j;
+        sums[warp][e] = value[j];
     }
     __syncthreads();
     const int e = threadIdx.x;

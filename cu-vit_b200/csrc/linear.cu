@@ -8,6 +8,34 @@
 #include <cstdint>
 
 namespace cuvit::linear {
+
+int access_bytes(const void* base, long long pitch_bytes) {
+    int bytes = 16;
+    while (reinterpret_cast<uintptr_t>(base) % bytes != 0 || pitch_bytes % bytes != 0) {
+        bytes /= 2;
+    }
+    return bytes;
+}
+
+bool describe(const void* base, bool bf16, long long columns, long long rows, long long pitch,
+              int box_rows, CUtensorMap* map) {
+    host::TmaTensor t;
+    t.base = base;
+    t.type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    t.element_bytes = bf16 ? 2 : 4;
+    t.rank = 2;
+    t.dims[0] = static_cast<uint64_t>(columns);
+    t.dims[1] = static_cast<uint64_t>(rows);
+    t.strides_bytes[0] = static_cast<uint64_t>(pitch) * t.element_bytes;
+    t.box[0] = static_cast<uint32_t>(gemm::kSwizzleBytes / t.element_bytes);
+    t.box[1] = static_cast<uint32_t>(box_rows);
+    if (!host::tma_describable(t) || host::encode_tma(t, map) != CUVIT_OK) {
+        host::clear_error(); // another path serves what TMA cannot
+        return false;
+    }
+    return true;
+}
+
 namespace {
 
 constexpr int kTile = 64;
@@ -94,45 +122,15 @@ int launch_simt(const Params& p, cudaStream_t stream) {
     return host::after_launch("linear_simt_kernel");
 }
 
-// Bytes per access that every row of a matrix allows, from 16 down to an element.
-int access_bytes(const void* base, long long pitch_bytes) {
-    int bytes = 16;
-    while (reinterpret_cast<uintptr_t>(base) % bytes != 0 || pitch_bytes % bytes != 0) {
-        bytes /= 2;
-    }
-    return bytes;
-}
-
-// A row-major matrix as a TMA tensor of boxes of box_rows rows of 128 bytes.
-bool describe(const void* base, bool bf16, long long columns, long long rows, long long pitch,
-              int box_rows, CUtensorMap* map) {
-    host::TmaTensor t;
-    t.base = base;
-    t.type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
-    t.element_bytes = bf16 ? 2 : 4;
-    t.rank = 2;
-    t.dims[0] = static_cast<uint64_t>(columns);
-    t.dims[1] = static_cast<uint64_t>(rows);
-    t.strides_bytes[0] = static_cast<uint64_t>(pitch) * t.element_bytes;
-    t.box[0] = static_cast<uint32_t>(gemm::kSwizzleBytes / t.element_bytes);
-    t.box[1] = static_cast<uint32_t>(box_rows);
-    if (!host::tma_describable(t) || host::encode_tma(t, map) != CUVIT_OK) {
-        host::clear_error(); // another path serves what TMA cannot
-        return false;
-    }
-    return true;
-}
-
 // Plans a tensor-core launch; false where TMA cannot describe x or the weight, or k is 0.
 bool prepare(const Params& p, int math, const host::DeviceContext& context, TcPlan* plan) {
     if (!host::is_blackwell(context) || p.k == 0) {
         return false;
     }
     const bool bf16 = math == CUVIT_MATH_BF16;
-    const bool split = math == CUVIT_MATH_FP32;
     const long long row_blocks = (p.m + gemm::kBlockM - 1LL) / gemm::kBlockM;
     const long long weight_rows = static_cast<long long>(p.n) * (p.gated ? 2 : 1);
-    int bn = gemm::choose_block_n(row_blocks, static_cast<int>(weight_rows), split, bf16,
+    int bn = gemm::choose_block_n(row_blocks, static_cast<int>(weight_rows), false, bf16,
                                   context.sm_count);
     if (p.gated && bn < 128) {
         bn = 128; // a half tile's columns of one operand stay a whole 32-column step
@@ -290,11 +288,13 @@ int run(const void* x, const void* weight, const float* bias, const float* scale
     if (rows_kernel_takes(p, bf16)) {
         return launch_rows(p, bf16, context->sm_count, stream);
     }
+    int result = CUVIT_OK;
+    if (c.math == CUVIT_MATH_FP32 && launch_split(p, *context, stream, &result)) {
+        return result;
+    }
     TcPlan plan;
-    if (prepare(p, c.math, *context, &plan)) {
-        return bf16 ? launch_tc_bf16(plan, stream)
-                    : (c.math == CUVIT_MATH_FP32 ? launch_tc_split(plan, stream)
-                                                 : launch_tc_tf32(plan, stream));
+    if (c.math != CUVIT_MATH_FP32 && prepare(p, c.math, *context, &plan)) {
+        return bf16 ? launch_tc_bf16(plan, stream) : launch_tc_tf32(plan, stream);
     }
     return bf16 ? launch_simt<__nv_bfloat16>(p, stream) : launch_simt<float>(p, stream);
 }

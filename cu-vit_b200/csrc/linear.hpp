@@ -55,7 +55,19 @@ constexpr int kMaxRows = 8;
 bool rows_kernel_takes(const Params& p, bool bf16);
 int launch_rows(const Params& p, bool bf16, int sm_count, cudaStream_t stream);
 
-// A prepared launch on the tensor-core kernels.
+// Bytes per access that every row of a matrix allows, from 16 down to an element.
+int access_bytes(const void* base, long long pitch_bytes);
+
+// A row-major matrix as a TMA tensor of boxes of box_rows rows of 128 bytes.
+bool describe(const void* base, bool bf16, long long columns, long long rows, long long pitch,
+              int box_rows, CUtensorMap* map);
+
+// FP32 math on the tensor cores (linear_split.cu). False where TMA cannot describe x or the
+// weight, or k is 0; else *result is the launch's status.
+bool launch_split(const Params& p, const host::DeviceContext& context, cudaStream_t stream,
+                  int* result);
+
+// A prepared launch on the tensor-core kernels of one product.
 struct TcPlan {
     CUtensorMap map_x{};
     CUtensorMap map_w{};
@@ -71,6 +83,5 @@ int pair_resident(int* pairs);
 
 int launch_tc_bf16(const TcPlan& plan, cudaStream_t stream);
 int launch_tc_tf32(const TcPlan& plan, cudaStream_t stream);
-int launch_tc_split(const TcPlan& plan, cudaStream_t stream);
 
 } // namespace cuvit::linear

@@ -672,3 +672,57 @@ def test_block_captured_and_replayed(kind, cuda):
         for state in (captured, beside):
             assert torch.equal(state["y"], eager["y"])
             assert torch.equal(state["context"], eager["context"])
+
+
+def test_linear_f32_special_values(cuda):
+    """Operands are split into TF32 values: infinities, NaN and the largest float among them."""
+    torch = cuda
+    m, n, k = 140, 150, 68
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(m, k, device="cuda", generator=gen)
+    w = torch.randn(n, k, device="cuda", generator=gen)
+    x[3, 7] = float("nan")
+    x[130, 67] = float("inf")
+    w[149, 1] = float("nan")
+    largest = torch.finfo(torch.float32).max
+    x[5] = 0.0
+    x[5, 9] = largest
+    w[:, 9] = 0.5 * torch.sign(w[:, 9])
+    out = torch.empty(m, n, device="cuda")
+    torch.cuda.synchronize()
+    kernels.launch_linear(x, w, None, None, None, out,
+                          LinearProblem(m=m, n=n, k=k, math=kernels.MATH_FP32,
+                                        out_dtype=kernels.DTYPE_F32))
+    torch.cuda.synchronize()
+    assert out[3].isnan().all() and out[:, 149].isnan().all()
+    assert not out[130, :149].isfinite().any()
+    rows = [r for r in range(m) if r not in (3, 130)]
+    assert out[rows, :149].isfinite().all()
+    # The head of the largest float is cut, not rounded to infinity: 2^-10 remain to the rest,
+    # which the tensor core holds to 2^-11 of that.
+    expected = largest * w[:149, 9].double()
+    error = (out[5, :149].double() - expected).abs()
+    assert (error <= 2.0 ** -20 * expected.abs()).all()
+
+
+@pytest.mark.parametrize("k", [60, 1000, 16388])
+def test_linear_f32_long_rows(k, cuda):
+    torch = cuda
+    m, n = 200, 170
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    # All products positive: what a summation loses in one direction adds up.
+    x = torch.rand(m, k, device="cuda", generator=gen)
+    w = torch.rand(n, k, device="cuda", generator=gen)
+    out = torch.empty(m, n, device="cuda")
+    torch.cuda.synchronize()
+    kernels.launch_linear(x, w, None, None, None, out,
+                          LinearProblem(m=m, n=n, k=k, math=kernels.MATH_FP32,
+                                        out_dtype=kernels.DTYPE_F32))
+    torch.cuda.synchronize()
+    exact = x.double() @ w.double().T
+    # Operands: 2^-23 each, and the product of the remainders, 2^-22. 64 of k in the accumulator:
+    # 24 additions, each cutting off less than 2^-23 of the partial sum, which grows from 0 to the
+    # whole: half of 24 2^-23. Then k / 64 additions rounded to 2^-24 of a sum that grows from 0
+    # to the whole: half of k / 64 2^-24, at most.
+    bound = 4 * 2.0 ** -23 + 13 * 2.0 ** -23 + (k / 128 + 1) * 2.0 ** -24
+    assert ((out.double() - exact).abs() <= bound * exact).all()

@@ -1,5 +1,5 @@
 // Attention over packed sequences of any length: argument checks, choice of kernel, and the
-// FP32 kernel for float operands and for bfloat16 ones that TMA cannot describe.
+// FP32 kernel for bfloat16 operands that TMA cannot describe.
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = 2^(scale log2(e) q_i . k_j - m_i)
 //
@@ -23,28 +23,12 @@ constexpr int kSimtKeys = 64;
 constexpr int kRowPitch = kSimtRows + 4; // floats; consecutive keys' rows start 4 banks apart
 constexpr int kKeyPitch = kSimtKeys + 4;
 
-template <typename T>
-__device__ __forceinline__ float load_value(const T* p) {
-    if constexpr (sizeof(T) == 2) {
-        return __bfloat162float(*p);
-    } else {
-        return *p;
-    }
-}
-
-// Elements e .. e + 3 of a row of d, zeros past its end; `vector`: rows are whole aligned float4s.
-template <typename T>
-__device__ __forceinline__ float4 load_four(const T* row, int e, int d, bool vector) {
-    if constexpr (sizeof(T) == 4) {
-        if (vector) {
-            return e < d ? *reinterpret_cast<const float4*>(row + e)
-                         : make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-        }
-    }
-    return make_float4(e < d ? load_value(row + e) : 0.0F,
-                       e + 1 < d ? load_value(row + e + 1) : 0.0F,
-                       e + 2 < d ? load_value(row + e + 2) : 0.0F,
-                       e + 3 < d ? load_value(row + e + 3) : 0.0F);
+// Elements e .. e + 3 of a row of d, zeros past its end.
+__device__ __forceinline__ float4 load_four(const __nv_bfloat16* row, int e, int d) {
+    return make_float4(e < d ? __bfloat162float(row[e]) : 0.0F,
+                       e + 1 < d ? __bfloat162float(row[e + 1]) : 0.0F,
+                       e + 2 < d ? __bfloat162float(row[e + 2]) : 0.0F,
+                       e + 3 < d ? __bfloat162float(row[e + 3]) : 0.0F);
 }
 
 // Threads along the keys and elements of a tile (kX); each has 8 of its elements, and 8 or 4 of its
@@ -78,15 +62,16 @@ __device__ __forceinline__ void outer(const float* rows, const float4& b, float 
 // 8 ty .. + 7 and, of the scores, the keys tx + kX m, of the output, elements 4 tx .. + 3 of every
 // 4 kX. Operands come from shared memory as whole vectors (Q and P with rows contiguous): for heads
 // up to 64, 64 multiply-adds share four loads, and two blocks fit an SM and load under each other's
-// arithmetic. 4096 tokens, 8 heads of 64: 954 us, 36 TFLOP/s of the FP32 pipe's 74. (8 x 4 products a
-// thread on twice the threads: 990 us, shared memory then takes as many cycles as the arithmetic;
+// arithmetic. 4096 tokens, 8 heads of 64: 954 us, 36 TFLOP/s of the FP32 pipe's 74. (8 x 4 products
+// a thread on twice the threads: 990 us, shared memory then takes as many cycles as the arithmetic;
 // packed multiply-adds on pairs of rows: 1050 us, since doubling the other operand takes moves on
 // the same pipe. Heads up to 128 use 8 x 4 for the scores: the outputs take the registers.) A tile's
 // keys lie in the order the threads read them, kX apart, which also lets a warp write its weights
 // without bank conflicts.
-template <typename T, int DPad>
+template <int DPad>
 __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
-    attention_varlen_simt(const VarlenParams p, const int vector) {
+    attention_varlen_simt(const VarlenParams p) {
+    using T = __nv_bfloat16;
     using Shape = SimtShape<DPad>;
     constexpr int kX = Shape::kX;
     constexpr int kThreads = Shape::kThreads;
@@ -131,7 +116,7 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
     for (int i = threadIdx.x; i < kSimtRows * DPad / 4; i += kThreads) {
         const int r = i % kSimtRows;
         const int e = i / kSimtRows * 4;
-        const float4 x = r < rows ? load_four(q + r * p.q_stride, e, d, vector != 0) : zeros();
+        const float4 x = r < rows ? load_four(q + r * p.q_stride, e, d) : zeros();
         qs[e * kRowPitch + r] = x.x;
         qs[(e + 1) * kRowPitch + r] = x.y;
         qs[(e + 2) * kRowPitch + r] = x.z;
@@ -153,7 +138,7 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
             const int j = i % kSimtKeys;
             const int e = i / kSimtKeys * 4;
             const long long row = static_cast<long long>(first) + j;
-            const float4 x = j < live ? load_four(k + row * p.k_stride, e, d, vector != 0) : zeros();
+            const float4 x = j < live ? load_four(k + row * p.k_stride, e, d) : zeros();
             const int m = j / kX;
             const int at = m / 4 * (4 * kX) + j % kX * 4 + m % 4;
             ks[e * kKeyPitch + at] = x.x;
@@ -166,7 +151,7 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
             const int e = i % (DPad / 4) * 4;
             const long long row = static_cast<long long>(first) + j;
             *reinterpret_cast<float4*>(vs + j * DPad + e) =
-                j < live ? load_four(v + row * p.v_stride, e, d, vector != 0) : zeros();
+                j < live ? load_four(v + row * p.v_stride, e, d) : zeros();
         }
         __syncthreads();
         float score[kGroups][8][4] = {}; // key group, row, key
@@ -258,10 +243,8 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
                 if (row < rows && e < d) {
                     if (p.splits > 1) {
                         p.part_out[at * d + e] = value;
-                    } else if constexpr (sizeof(T) == 2) {
-                        out[row * p.out_stride + e] = __float2bfloat16_rn(value * inverse);
                     } else {
-                        out[row * p.out_stride + e] = value * inverse;
+                        out[row * p.out_stride + e] = __float2bfloat16_rn(value * inverse);
                     }
                 }
             }
@@ -273,24 +256,17 @@ long long simt_items(const VarlenParams& p) {
     return (static_cast<long long>(p.q_tokens) / kSimtRows + p.batch) * p.q_heads;
 }
 
-template <typename T, int DPad>
+template <int DPad>
 int launch_simt(const VarlenParams& p, cudaStream_t stream) {
-    auto* kernel = &attention_varlen_simt<T, DPad>;
+    auto* kernel = &attention_varlen_simt<DPad>;
     constexpr int kBytes = SimtShape<DPad>::kSmemBytes;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
     const long long blocks = simt_items(p) * p.splits;
     if (blocks > 0x7FFFFFFFLL) {
         return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
     }
-    const auto whole = [&](const void* base, long long stride) {
-        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride % 4 == 0;
-    };
-    const int vector = p.head_dim % 4 == 0 && whole(p.q, p.q_stride) && whole(p.k, p.k_stride) &&
-                               whole(p.v, p.v_stride)
-                           ? 1
-                           : 0;
     host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(SimtShape<DPad>::kThreads),
-                     kBytes, stream, p, vector);
+                     kBytes, stream, p);
     return host::after_launch("attention_varlen_simt");
 }
 
@@ -364,7 +340,7 @@ int choose_splits(const VarlenParams& p, long long items, int per_sm, int min_ke
     return static_cast<int>(splits < 1 ? 1 : (splits > kMaxSplits ? kMaxSplits : splits));
 }
 
-enum class Kernel { kSimt, kRows, kTiles };
+enum class Kernel { kSimt, kRows, kTiles, kSplit };
 
 // The splits of a call through each kernel, were a workspace given.
 int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
@@ -374,6 +350,8 @@ int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
         return choose_splits(p, rows_kernel_items(p) / 2, 6, 128, sm_count);
     case Kernel::kTiles:
         return choose_splits(p, tiles_kernel_items(p), 1, 512, sm_count);
+    case Kernel::kSplit:
+        return choose_splits(p, split_kernel_items(p), 1, 512, sm_count);
     default:
         return choose_splits(p, simt_items(p), 2, 256, sm_count);
     }
@@ -382,6 +360,9 @@ int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
 Kernel choose(const VarlenParams& p) {
     if (rows_kernel_takes(p)) {
         return Kernel::kRows;
+    }
+    if (!p.bf16) {
+        return Kernel::kSplit;
     }
     return tiles_kernel_takes(p) ? Kernel::kTiles : Kernel::kSimt;
 }
@@ -403,7 +384,7 @@ size_t workspace_bytes_of(const VarlenParams& p) {
 // Enough for every kernel the operands' alignments may select.
 size_t workspace_bytes_at_most(VarlenParams p, int sm_count) {
     size_t most = 0;
-    for (const Kernel kernel : {Kernel::kSimt, Kernel::kRows, Kernel::kTiles}) {
+    for (const Kernel kernel : {Kernel::kSimt, Kernel::kRows, Kernel::kTiles, Kernel::kSplit}) {
         p.splits = splits_of(kernel, p, sm_count);
         const size_t bytes = workspace_bytes_of(p);
         most = bytes > most ? bytes : most;
@@ -485,12 +466,10 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
         status = launch_rows(p, stream);
     } else if (kernel == Kernel::kTiles) {
         status = launch_tiles(p, stream);
-    } else if (bf16) {
-        status = p.head_dim <= 64 ? launch_simt<__nv_bfloat16, 64>(p, stream)
-                                  : launch_simt<__nv_bfloat16, 128>(p, stream);
+    } else if (kernel == Kernel::kSplit) {
+        status = launch_split(p, context->status, stream);
     } else {
-        status = p.head_dim <= 64 ? launch_simt<float, 64>(p, stream)
-                                  : launch_simt<float, 128>(p, stream);
+        status = p.head_dim <= 64 ? launch_simt<64>(p, stream) : launch_simt<128>(p, stream);
     }
     if (status == CUVIT_OK && p.splits > 1) {
         status = launch_join(p, stream);

@@ -55,6 +55,10 @@ bool tiles_kernel_takes(const VarlenParams& p);
 long long tiles_kernel_items(const VarlenParams& p); // work items per split
 int launch_tiles(const VarlenParams& p, cudaStream_t stream);
 
+// Floats on the tensor cores, any alignment (attention_split.cu).
+long long split_kernel_items(const VarlenParams& p); // blocks of a launch per split
+int launch_split(const VarlenParams& p, unsigned* status, cudaStream_t stream);
+
 // Joins the splits: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 int launch_join(const VarlenParams& p, cudaStream_t stream);
 

@@ -1,11 +1,8 @@
 // FP32 linear layers on the tensor cores (tcgen05): out = residual + scale * act(x W^T + b)
 // [* (up + b)], each operand split into two TF32 values.
 //
-// x = hi + lo + e with hi = rn_tf32(x), lo = x - hi cut to TF32, |e| <= 2^-23 |x|, so
-//   x w = lo_x hi_w + hi_x lo_w + hi_x hi_w,
-// each product exact in the tensor core's accumulator, which does not round to nearest but cuts
-// off: a long sum kept there drifts towards zero. So it collects 64 of k at a time (24
-// instructions) and hands them to registers, where the running sum is rounded to nearest; the
+// Three products of TF32 halves make one of floats (split_tf32.cuh). The accumulator collects 64 of k
+// at a time (24 instructions) and hands them to registers, where the sum is rounded to nearest: the
 // error then hardly grows with k (relative, root mean square against FP64: 4.7e-7 for k = 384,
 // 5.4e-7 for 15360; summed in the accumulator throughout 9.4e-7 and, at k = 3840, 9e-6).
 //
@@ -30,6 +27,7 @@
 #include "activation.cuh"
 #include "linear.hpp"
 #include "ptx.cuh"
+#include "split_tf32.cuh"
 
 #include <cuda_bf16.h>
 
@@ -88,51 +86,6 @@ struct SplitParams {
     int columns_ok;      // bias and scale are 16-byte aligned
     unsigned* status;
 };
-
-// hi and lo of four values: adding half a step and masking rounds to nearest, x - hi is exact, and
-// what the tensor core cuts off lo is its 12th bit at most, 2^-23 |x| (rounding it would be a tie).
-// An infinity, a NaN or an x that rounds to infinity leaves a rest that is not finite and turns
-// `check`, otherwise zero, into a NaN; the warp that meets one takes the checked form.
-__device__ __forceinline__ void split4(float (&x)[4], float (&hi)[4], uint64_t& check) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        hi[j] = __uint_as_float((__float_as_uint(x[j]) + 0x1000u) & 0xFFFFE000u);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-        const uint64_t rest =
-            dev::sub_f32x2(dev::f32x2(x[j], x[j + 1]), dev::f32x2(hi[j], hi[j + 1]));
-        check = dev::fma_f32x2(rest, dev::f32x2(0.0F, 0.0F), check);
-        const float2 both = dev::f32x2_split(rest);
-        x[j] = both.x; // lo
-        x[j + 1] = both.y;
-    }
-}
-
-__device__ __forceinline__ bool any_special(uint64_t check) {
-    const float2 both = dev::f32x2_split(check);
-    return __any_sync(0xFFFFFFFFu, !(both.x + both.y == 0.0F));
-}
-
-// From shared memory again: lo has taken x's place.
-__device__ __forceinline__ void split4_checked(uint32_t address, float (&hi)[4], float (&lo)[4]) {
-    float x[4];
-    dev::ld_shared_v4(address, x);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        hi[j] = dev::round_to_tf32(x[j]);
-        lo[j] = (__float_as_uint(x[j]) & 0x7F800000u) == 0x7F800000u ? 0.0F : x[j] - hi[j];
-    }
-}
-
-__device__ __forceinline__ void store_words(uint32_t to, const float (&v)[4][4]) {
-    uint32_t words[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        words[j] = __float_as_uint(v[j / 4][j % 4]);
-    }
-    dev::tmem_store_16(to, words);
-}
 
 template <bool Multiply>
 __device__ __forceinline__ void with_columns(float (&v)[kGroup], const float* vector, int col0,
@@ -559,17 +512,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t check = 0u;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    split4(x[h][q], hi[q], check);
+                    dev::split4(x[h][q], hi[q], check);
                 }
-                if (any_special(check)) {
+                if (dev::any_special(check)) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        split4_checked(at(4 * h + q), hi[q], x[h][q]);
+                        float again[4]; // lo has taken x's place
+                        dev::ld_shared_v4(at(4 * h + q), again);
+                        dev::split4_checked(again, hi[q], x[h][q]);
                     }
                 }
                 const uint32_t to = halves + split * 2 * kBlockK + 16 * h;
-                store_words(to, hi);
-                store_words(to + kBlockK, x[h]);
+                dev::tmem_store_floats(to, hi);
+                dev::tmem_store_floats(to + kBlockK, x[h]);
             }
             dev::tmem_wait_store();
             dev::tc_fence_before();
@@ -629,13 +584,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint64_t check = 0u;
 #pragma unroll
                 for (int q = 0; q < kBatch; ++q) {
-                    split4(w[q], hi[q], check);
+                    dev::split4(w[q], hi[q], check);
                 }
-                if (any_special(check)) {
+                if (dev::any_special(check)) {
 #pragma unroll
                     for (int q = 0; q < kBatch; ++q) {
                         if (first + q < rounds) {
-                            split4_checked(hi_at + 2048u * (first + q), hi[q], w[q]);
+                            float again[4];
+                            dev::ld_shared_v4(hi_at + 2048u * (first + q), again);
+                            dev::split4_checked(again, hi[q], w[q]);
                         }
                     }
                 }

@@ -6,14 +6,19 @@
 // into one of two buffers there, weights go back as halves, and a tile's weighted values are added
 // to registers, so no accumulator sums more than 64 products or a head's width.
 //
-// %PERF%
+// 4096 tokens, 8 heads of 64: 320 us, 107 TFLOP/s (products in the FP32 pipe: 954 us); heads of 128
+// 760 us; 8 x 197 tokens, 12 heads 41 us (78). The tensor core would allow three times that (its
+// products take 1540 cycles of the 4700 a tile of 64 keys and 64 elements takes): what bounds it is
+// the softmax warps' chain of waits (scores, maximum, exponentials, previous sum, weights), and a
+// quarter is the loading warps' share of the issue slots. Two softmax warps a scheduler do not hide
+// the chain; a second set on alternate tiles would need more registers than an SM has.
 //
 //   warps 0-7    softmax: two threads per row, one for each half of a tile's keys; they exchange
 //                the row's maximum through shared memory, and each keeps half of the output row
-//   warps 8-15   bring keys and values in (each thread its own pieces, several tiles ahead, without
+//   warps 8-15   (wide heads: 8-11) bring keys and values in (each thread its own pieces, several tiles ahead, without
 //                any wait for one another), split them, and lay them out for the tensor core:
 //                keys as they are, values transposed
-//   warp 16      issues the products: S(0), S(1), PV(0), S(2), PV(1), ...
+//   last warp    issues the products: S(0), S(1), PV(0), S(2), PV(1), ...
 #include "attention_varlen.hpp"
 #include "ptx.cuh"
 #include "split_tf32.cuh"
@@ -26,18 +31,16 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kSoftmaxWarps = 8;
-constexpr int kLoadWarps = 8;
-constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
-constexpr int kLoaders = 32 * kLoadWarps;
-constexpr int kPieces = 4; // 16-byte pieces of a tile a loading thread has: 64 x 64 or 32 x 128
+// A tile is 1024 16-byte pieces (64 keys of 64 or 32 of 128), four to a place.
+constexpr int kPieces = 4;
+constexpr int kPlaces = 256;
 constexpr int kGroup = 16; // columns of a tensor-memory access
 
 constexpr int kHalfBytes = 16384; // a tile's hi or lo
 constexpr int kTileBytes = 2 * kHalfBytes;
 constexpr int kTiles = 4; // split tiles: the tensor core works on one, up to three wait
 constexpr int kRaw = 4;   // tiles being fetched
-constexpr int kRawBytes = kLoaders * kPieces * 16;
+constexpr int kRawBytes = kPlaces * kPieces * 16;
 constexpr int kRawOffset = kTiles * kTileBytes;
 constexpr int kTopOffset = kRawOffset + kRaw * kRawBytes; // [2][2][kRows] floats
 constexpr int kBarrierOffset = kTopOffset + 4 * kRows * 4;
@@ -57,6 +60,14 @@ struct Shape {
     static constexpr int kP = kS + 2 * kKeys;      // hi, then lo
     static constexpr int kO = kP + 2 * kKeys;
     static_assert(kO + kWidth <= kTmemColumns, "tensor memory");
+    // Loading warps. Wide heads' outputs take 32 more registers in the softmax warps: more than
+    // 16 warps a block would leave too few (4 loading warps 760 us, 8 870 us for 4096 tokens, 8
+    // heads of 128); narrow heads fit, and loading twice as wide pays (384 and 325 us for 64).
+    static constexpr int kLoadWarps = Wide ? 4 : 8;
+    static constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
+    static constexpr int kThreads = 32 * (kMmaWarp + 1);
+    static constexpr int kLoaders = 32 * kLoadWarps;
+    static constexpr int kSets = kPlaces / kLoaders; // places of a loading thread
 };
 
 struct Flags {
@@ -94,11 +105,14 @@ __device__ __forceinline__ void copy_async(uint32_t to, const float* from, bool 
 }
 
 template <bool Wide>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
     attention_split_kernel(const __grid_constant__ VarlenParams p, const Flags flags,
                            unsigned* status) {
     using S = Shape<Wide>;
     constexpr int kKeys = S::kKeys;
+    constexpr int kLoaders = S::kLoaders;
+    constexpr int kSets = S::kSets;
+    constexpr int kMmaWarp = S::kMmaWarp;
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
     const int item = static_cast<int>(blockIdx.x) / p.splits;
@@ -144,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kTiles; ++i) {
-            dev::mbar_init(tile_full(i), kLoadWarps);
+            dev::mbar_init(tile_full(i), S::kLoadWarps);
             dev::mbar_init(tile_empty(i), 1);
         }
         dev::mbar_init(q_full, kSoftmaxWarps);
@@ -269,9 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             dev::tc_fence_before();
             return true;
         };
+        // The end of the keys that the row sees, less this half's place in a tile.
+        const int seen =
+            (p.causal ? static_cast<int>(min(static_cast<long long>(last_key), max(0LL, reach + row + 1)))
+                      : last_key) -
+            half * S::kOwn;
         bool ok = true;
-        int tile = 0;
-        for (; tile < tiles; ++tile) {
+#pragma unroll 1
+        for (int tile = 0; tile < tiles; ++tile) {
             const int buffer = tile & 1;
             if (!dev::mbar_wait_warp(s_full(buffer), (tile >> 1) & 1, status)) {
                 ok = false;
@@ -295,11 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 dev::mbar_arrive(s_empty(buffer));
             }
             const int first = first_key + tile * kKeys;
-            long long seen = last_key - first;
-            if (p.causal) {
-                seen = min(seen, reach + row + 1 - first);
-            }
-            const int limit = static_cast<int>(max(seen, 0LL)) - half * S::kOwn; // of these keys
+            const int limit = seen - first; // of these keys
             if (__any_sync(0xFFFFFFFFu, limit < S::kOwn)) {
 #pragma unroll
                 for (int i = 0; i < S::kOwn; ++i) {
@@ -334,21 +349,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             pending = factor;
+            // Eight at a time: registers are short.
+            uint64_t check = 0u; // weights are at most 1, or NaN, which lo keeps
 #pragma unroll
-            for (int g = 0; g < S::kOwn / kGroup; ++g) {
-                float hi[4][4], lo[4][4];
-                uint64_t check = 0u; // weights are at most 1, or NaN, which lo keeps
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        lo[c][j] = w[4 * g + c][j];
-                    }
-                    dev::split4(lo[c], hi[c], check);
-                }
-                const uint32_t to = mine + S::kP + half * S::kOwn + g * kGroup;
-                dev::tmem_store_floats(to, hi);
-                dev::tmem_store_floats(to + kKeys, lo);
+            for (int c = 0; c < S::kOwn / 4; c += 2) {
+                float hi[2][4];
+                dev::split4(w[c], hi[0], check);
+                dev::split4(w[c + 1], hi[1], check);
+                const uint32_t to = mine + S::kP + half * S::kOwn + 4 * c;
+                dev::tmem_store_8(to, hi[0], hi[1]);
+                dev::tmem_store_8(to + kKeys, w[c], w[c + 1]);
             }
             dev::tmem_wait_store();
             dev::tc_fence_before();
@@ -414,15 +424,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Keys: piece t + 256 u of the tile, row-major. Values: a block of four keys by four
         // elements, eight lanes on consecutive key blocks, so that both the loads (a sector a
         // row) and the transposed stores (eight different bank groups) are whole.
-        int k_row[kPieces], k_element[kPieces];
+        int k_row[kSets][kPieces], k_element[kSets][kPieces];
+        int v_row[kSets], v_element[kSets];
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-            const int piece = t + kLoaders * u;
-            k_row[u] = piece / pieces;
-            k_element[u] = 4 * (piece - k_row[u] * pieces);
+        for (int n = 0; n < kSets; ++n) {
+            const int place = t + kLoaders * n;
+#pragma unroll
+            for (int u = 0; u < kPieces; ++u) {
+                const int piece = place + kPlaces * u;
+                k_row[n][u] = piece / pieces;
+                k_element[n][u] = 4 * (piece - k_row[n][u] * pieces);
+            }
+            v_row[n] = 4 * (Wide ? place % 8 : place % 8 + 8 * (place / 8 % 2));
+            v_element[n] = 4 * (Wide ? place / 8 : place / 16);
         }
-        const int v_row = 4 * (Wide ? t % 8 : t % 8 + 8 * (t / 8 % 2));
-        const int v_element = 4 * (Wide ? t / 8 : t / 16);
         const uint32_t raw0 = base + kRawOffset + 16u * t;
         const auto fetch = [&](int i) {
             if (i >= 2 * tiles) {
@@ -434,19 +449,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float* const from = tile.value ? v : k;
             const long long stride = tile.value ? p.v_stride : p.k_stride;
 #pragma unroll
-            for (int u = 0; u < kPieces; ++u) {
-                const int r = tile.value ? v_row + u : k_row[u];
-                const int e = tile.value ? v_element : k_element[u];
-                const bool live = r < kKeys && first + r < last_key && e < d;
-                const float* const at = live ? from + (first + r) * stride + e : from;
-                const uint32_t here = to + u * kLoaders * 16;
-                if (flags.in_vector) {
-                    copy_async<16>(here, at, live);
-                } else {
+            for (int n = 0; n < kSets; ++n) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const bool one = live && e + j < d;
-                        copy_async<4>(here + 4 * j, one ? at + j : from, one);
+                for (int u = 0; u < kPieces; ++u) {
+                    const int r = tile.value ? v_row[n] + u : k_row[n][u];
+                    const int e = tile.value ? v_element[n] : k_element[n][u];
+                    const bool live = r < kKeys && first + r < last_key && e < d;
+                    const float* const at = live ? from + (first + r) * stride + e : from;
+                    const uint32_t here = to + 16 * (u * kPlaces + n * kLoaders);
+                    if (flags.in_vector) {
+                        copy_async<16>(here, at, live);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const bool one = live && e + j < d;
+                            copy_async<4>(here + 4 * j, one ? at + j : from, one);
+                        }
                     }
                 }
             }
@@ -461,57 +479,68 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
             const Tile tile = tile_at(i, tiles);
             const uint32_t from = raw0 + (i % kRaw) * kRawBytes;
-            float x[kPieces][4], hi[kPieces][4];
+            const int slot = i % kTiles;
+            const uint32_t to = base + slot * kTileBytes;
+            bool free = false;
 #pragma unroll
-            for (int u = 0; u < kPieces; ++u) {
-                dev::ld_shared_v4(from + u * kLoaders * 16, x[u]);
-            }
-            uint64_t check = 0u;
-#pragma unroll
-            for (int u = 0; u < kPieces; ++u) {
-                dev::split4(x[u], hi[u], check);
-            }
-            if (dev::any_special(check)) {
+            for (int n = 0; n < kSets; ++n) {
+                float x[kPieces][4], hi[kPieces][4];
 #pragma unroll
                 for (int u = 0; u < kPieces; ++u) {
-                    float again[4]; // lo has taken x's place
-                    dev::ld_shared_v4(from + u * kLoaders * 16, again);
-                    dev::split4_checked(again, hi[u], x[u]);
+                    dev::ld_shared_v4(from + 16 * (u * kPlaces + n * kLoaders), x[u]);
                 }
+                uint64_t check = 0u;
+#pragma unroll
+                for (int u = 0; u < kPieces; ++u) {
+                    dev::split4(x[u], hi[u], check);
+                }
+                if (dev::any_special(check)) {
+#pragma unroll
+                    for (int u = 0; u < kPieces; ++u) {
+                        float again[4]; // lo has taken x's place
+                        dev::ld_shared_v4(from + 16 * (u * kPlaces + n * kLoaders), again);
+                        dev::split4_checked(again, hi[u], x[u]);
+                    }
+                }
+                if (n == 0) {
+                    free = dev::mbar_wait_warp(tile_empty(slot), ((i / kTiles) & 1) ^ 1u, status);
+                    if (!free) {
+                        break;
+                    }
+                }
+                if (tile.value) {
+                    // Row e of the transposed tile: 32 keys are 128 bytes, swizzled.
+                    if (v_element[n] < padded) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int e = v_element[n] + j;
+                            const uint32_t at = to + (v_row[n] / 32) * padded * 128 + e * 128 +
+                                                ((v_row[n] % 32 / 4 ^ (e & 7)) << 4);
+                            const float h[4] = {hi[0][j], hi[1][j], hi[2][j], hi[3][j]};
+                            const float l[4] = {x[0][j], x[1][j], x[2][j], x[3][j]};
+                            dev::st_shared_v4(at, h);
+                            dev::st_shared_v4(at + kHalfBytes, l);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kPieces; ++u) {
+                        const int r = k_row[n][u];
+                        if (r < kKeys) {
+                            const int e = k_element[n][u];
+                            const uint32_t at = to + (e / 32) * kKeys * 128 + r * 128 +
+                                                ((e % 32 / 4 ^ (r & 7)) << 4);
+                            dev::st_shared_v4(at, hi[u]);
+                            dev::st_shared_v4(at + kHalfBytes, x[u]);
+                        }
+                    }
+                }
+            }
+            if (!free) {
+                break;
             }
             fetch(i + kRaw - 1); // into the place read in the previous round
             asm volatile("cp.async.commit_group;" ::: "memory");
-            const int slot = i % kTiles;
-            if (!dev::mbar_wait_warp(tile_empty(slot), ((i / kTiles) & 1) ^ 1u, status)) {
-                break;
-            }
-            const uint32_t to = base + slot * kTileBytes;
-            if (tile.value) {
-                // Row e of the transposed tile: 32 keys are 128 bytes, swizzled.
-                if (v_element < padded) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int e = v_element + j;
-                        const uint32_t at = to + (v_row / 32) * padded * 128 + e * 128 +
-                                            ((v_row % 32 / 4 ^ (e & 7)) << 4);
-                        const float h[4] = {hi[0][j], hi[1][j], hi[2][j], hi[3][j]};
-                        const float l[4] = {x[0][j], x[1][j], x[2][j], x[3][j]};
-                        dev::st_shared_v4(at, h);
-                        dev::st_shared_v4(at + kHalfBytes, l);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int u = 0; u < kPieces; ++u) {
-                    if (k_row[u] < kKeys) {
-                        const int e = k_element[u];
-                        const uint32_t at = to + (e / 32) * kKeys * 128 + k_row[u] * 128 +
-                                            ((e % 32 / 4 ^ (k_row[u] & 7)) << 4);
-                        dev::st_shared_v4(at, hi[u]);
-                        dev::st_shared_v4(at + kHalfBytes, x[u]);
-                    }
-                }
-            }
             dev::fence_proxy_async_shared();
             __syncwarp();
             if (lane == 0) {
@@ -612,9 +641,10 @@ int launch_split(const VarlenParams& p, unsigned* status, cudaStream_t stream) {
     if (blocks > 0x7FFFFFFFLL) {
         return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
     }
-    auto* kernel = p.head_dim <= 64 ? &attention_split_kernel<false> : &attention_split_kernel<true>;
+    const bool wide = p.head_dim > 64;
+    auto* kernel = wide ? &attention_split_kernel<true> : &attention_split_kernel<false>;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmemBytes));
-    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), kSmemBytes,
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(wide ? Shape<true>::kThreads : Shape<false>::kThreads), kSmemBytes,
                      stream, p, flags, status);
     return host::after_launch("attention_split_kernel");
 }

@@ -567,6 +567,16 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
         : "memory");
 }
 
+// Eight values into 8 consecutive columns.
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const float (&a)[4],
+                                             const float (&b)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr),
+                 "f"(a[0]), "f"(a[1]), "f"(a[2]), "f"(a[3]), "f"(b[0]), "f"(b[1]), "f"(b[2]),
+                 "f"(b[3])
+                 : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_load() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }

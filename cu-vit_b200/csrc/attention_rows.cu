@@ -1,5 +1,5 @@
-// Attention of a few query rows per sequence over many keys (pooling by one query, one new token
-// of each sequence), and the kernel that joins the parts of calls that split their keys.
+// Attention of a few float query rows per sequence over many keys (pooling by one query, one new
+// token of each sequence), and the kernel that joins the parts of calls that split their keys.
 //
 // Bound by HBM: every key and value is used for a handful of multiply-adds per byte. A group of
 // lanes takes a few keys at a time, 16 bytes of each a lane (the query rows' same elements stay in
@@ -32,36 +32,21 @@ constexpr int kStages = 3; // of keys and values in flight: 48 KB a block, four 
 template <int Rows>
 constexpr int kUnrollOf = Rows >= 8 ? 2 : 4;
 
-// One lane's 16 bytes of a row as floats.
-template <typename T>
-struct Lane {
-    static constexpr int kElems = 16 / sizeof(T);
+// One lane's 16 bytes of a row.
+constexpr int kElems = 4;
+constexpr int kPairs = kElems / 2;
 
-    static __device__ __forceinline__ uint4 load(const T* p) {
-        return __ldg(reinterpret_cast<const uint4*>(p));
-    }
+__device__ __forceinline__ void unpack(const uint4& raw, uint64_t (&out)[kPairs]) {
+    out[0] = dev::f32x2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+    out[1] = dev::f32x2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+}
 
-    // Copies 16 bytes to shared memory asynchronously, or zeros.
-    static __device__ __forceinline__ void copy(uint4* to, const T* p, bool live) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dev::smem_u32(to)),
-                     "l"(p), "r"(live ? 16 : 0)
-                     : "memory");
-    }
-
-    static __device__ __forceinline__ void unpack(const uint4& raw, uint64_t (&out)[kElems / 2]) {
-        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                out[i] = dev::f32x2(__uint_as_float(words[i] << 16),
-                                    __uint_as_float(words[i] & 0xFFFF0000u));
-            }
-        } else {
-            out[0] = dev::f32x2(__uint_as_float(words[0]), __uint_as_float(words[1]));
-            out[1] = dev::f32x2(__uint_as_float(words[2]), __uint_as_float(words[3]));
-        }
-    }
-};
+// Copies 16 bytes to shared memory asynchronously, or zeros.
+__device__ __forceinline__ void copy_async(uint4* to, const float* p, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dev::smem_u32(to)), "l"(p),
+                 "r"(live ? 16 : 0)
+                 : "memory");
+}
 
 __host__ __device__ constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 
@@ -110,13 +95,11 @@ __device__ __forceinline__ void merge_factors(float m, float other, float& top, 
     theirs = exp2f(other - base);
 }
 
-template <typename T, int Lanes, int Rows>
+template <int Lanes, int Rows>
 __global__ void __launch_bounds__(kThreads)
     attention_rows_kernel(const VarlenParams p, int queries_per_block, int head_chunks) {
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
-    constexpr int kElems = Lane<T>::kElems;
-    constexpr int kPairs = kElems / 2;
     constexpr int kUnroll = kUnrollOf<Rows>;
     using Halves = Halving<Lanes, Rows, kUnroll>;
     constexpr int kGroups = kThreads / Lanes; // key streams of the block
@@ -169,10 +152,10 @@ __global__ void __launch_bounds__(kThreads)
             q[r][j] = 0u;
         }
         if (r < rows && in_row) {
-            Lane<T>::unpack(Lane<T>::load(static_cast<const T*>(p.q) +
-                                          (s.q_first + query) * p.q_stride +
-                                          static_cast<long long>(head) * p.head_dim + element),
-                            q[r]);
+            const float* const from = static_cast<const float*>(p.q) +
+                                      (s.q_first + query) * p.q_stride +
+                                      static_cast<long long>(head) * p.head_dim + element;
+            unpack(__ldg(reinterpret_cast<const uint4*>(from)), q[r]);
             const uint64_t scale = dev::f32x2(p.scale_log2, p.scale_log2);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
@@ -198,10 +181,10 @@ __global__ void __launch_bounds__(kThreads)
         top[h] = -INFINITY;
         sum[h] = 0.0F;
     }
-    const T* const k0 = static_cast<const T*>(p.q); // never read: copies of no bytes name it
-    const T* const k = static_cast<const T*>(p.k) + s.kv_begin * p.k_stride +
+    const float* const k0 = static_cast<const float*>(p.q); // never read: copies of no bytes name it
+    const float* const k = static_cast<const float*>(p.k) + s.kv_begin * p.k_stride +
                        static_cast<long long>(kv_head) * p.head_dim + element;
-    const T* const v = static_cast<const T*>(p.v) + s.kv_begin * p.v_stride +
+    const float* const v = static_cast<const float*>(p.v) + s.kv_begin * p.v_stride +
                        static_cast<long long>(kv_head) * p.head_dim + element;
 
     uint64_t o[Rows][kPairs];
@@ -225,10 +208,10 @@ __global__ void __launch_bounds__(kThreads)
             const int key = base + u * kGroups + group;
             const bool live = key < end_key && in_row;
             const long long row = live ? key : 0;
-            Lane<T>::copy(&shared.ring[stage][u][0][threadIdx.x], live ? k + row * p.k_stride : k0,
-                          live);
-            Lane<T>::copy(&shared.ring[stage][u][1][threadIdx.x], live ? v + row * p.v_stride : k0,
-                          live);
+            copy_async(&shared.ring[stage][u][0][threadIdx.x], live ? k + row * p.k_stride : k0,
+                       live);
+            copy_async(&shared.ring[stage][u][1][threadIdx.x], live ? v + row * p.v_stride : k0,
+                       live);
         }
     };
 #pragma unroll
@@ -245,7 +228,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             uint64_t kf[kPairs];
-            Lane<T>::unpack(shared.ring[stage][u][0][threadIdx.x], kf);
+            unpack(shared.ring[stage][u][0][threadIdx.x], kf);
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
                 uint64_t dot = dev::mul_f32x2(q[r][0], kf[0]);
@@ -314,7 +297,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             uint64_t vf[kPairs];
-            Lane<T>::unpack(shared.ring[stage][u][1][threadIdx.x], vf);
+            unpack(shared.ring[stage][u][1][threadIdx.x], vf);
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
                 const float weight = from_lane(score[Halves::place_of(r * kUnroll + u)],
@@ -417,13 +400,8 @@ __global__ void __launch_bounds__(kThreads)
             }
         } else {
             value = total == 0.0F ? 0.0F : value / total;
-            T* const out = static_cast<T*>(p.out) + row * p.out_stride +
-                           static_cast<long long>(head) * p.head_dim + e;
-            if constexpr (sizeof(T) == 2) {
-                *out = __float2bfloat16_rn(value);
-            } else {
-                *out = value;
-            }
+            static_cast<float*>(p.out)[row * p.out_stride +
+                                       static_cast<long long>(head) * p.head_dim + e] = value;
         }
     }
 }
@@ -538,53 +516,32 @@ int head_chunks(const VarlenParams& p) {
     return (p.group + heads - 1) / heads;
 }
 
-template <typename T, int Lanes>
-int launch_lanes(const VarlenParams& p, cudaStream_t stream) {
-    const long long blocks = rows_kernel_items(p) * p.splits;
-    if (blocks > 0x7FFFFFFFLL) {
-        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
-    }
+template <int Lanes>
+int launch_lanes(const VarlenParams& p, unsigned blocks, cudaStream_t stream) {
     const auto start = [&](auto* kernel) {
-        host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p,
-                         queries_per_block(p), head_chunks(p));
+        host::pdl_launch(kernel, dim3(blocks), dim3(kThreads), 0, stream, p, queries_per_block(p),
+                         head_chunks(p));
         return host::after_launch("attention_rows_kernel");
     };
     switch (rows_kernel_rows(p)) {
     case 1:
-        return start(&attention_rows_kernel<T, Lanes, 1>);
+        return start(&attention_rows_kernel<Lanes, 1>);
     case 2:
-        return start(&attention_rows_kernel<T, Lanes, 2>);
+        return start(&attention_rows_kernel<Lanes, 2>);
     case 4:
-        return start(&attention_rows_kernel<T, Lanes, 4>);
+        return start(&attention_rows_kernel<Lanes, 4>);
     default:
-        return start(&attention_rows_kernel<T, Lanes, 8>);
+        return start(&attention_rows_kernel<Lanes, 8>);
     }
-}
-
-template <typename T>
-int launch_typed(const VarlenParams& p, cudaStream_t stream) {
-    const int chunks = p.head_dim / Lane<T>::kElems;
-    if (chunks <= 4) {
-        return launch_lanes<T, 4>(p, stream);
-    }
-    if (chunks <= 8) {
-        return launch_lanes<T, 8>(p, stream);
-    }
-    if (chunks <= 16) {
-        return launch_lanes<T, 16>(p, stream);
-    }
-    if constexpr (sizeof(T) == 4) {
-        return launch_lanes<T, 32>(p, stream);
-    }
-    return host::fail(CUVIT_RUNTIME_ERROR, "attention head_dim out of range");
 }
 
 } // namespace
 
-// Rows of one key head taken together: as many as an average sequence has, up to kMaxRows.
+// Rows of one key head taken together: for floats as many as an average sequence has, up to
+// kMaxRows; the bfloat16 kernel's products have place for eight.
 int rows_kernel_rows(const VarlenParams& p) {
     const long long queries = (p.q_tokens + static_cast<long long>(p.batch) - 1) / p.batch;
-    int rows = 1;
+    int rows = p.bf16 ? kMaxRows : 1;
     while (rows < kMaxRows && rows < queries * p.group) {
         rows *= 2;
     }
@@ -596,11 +553,13 @@ long long rows_kernel_items(const VarlenParams& p) {
            head_chunks(p);
 }
 
-// 16-byte rows of q, k and v heads, and on average no more rows than the kernel takes at once.
+// 16-byte rows of q, k and v heads, at distances whose 16-fold fits 31 bits, and on average no more
+// rows than the kernel takes at once.
 bool rows_kernel_takes(const VarlenParams& p) {
     const int size = p.bf16 ? 2 : 4;
     const auto fits = [size](const void* base, long long stride) {
-        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride * size % 16 == 0;
+        return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride * size % 16 == 0 &&
+               stride < (1LL << 26);
     };
     return static_cast<long long>(p.q_tokens) * p.group <=
                static_cast<long long>(kMaxRows) * p.batch &&
@@ -609,7 +568,22 @@ bool rows_kernel_takes(const VarlenParams& p) {
 }
 
 int launch_rows(const VarlenParams& p, cudaStream_t stream) {
-    return p.bf16 ? launch_typed<__nv_bfloat16>(p, stream) : launch_typed<float>(p, stream);
+    const long long blocks = rows_kernel_items(p) * p.splits;
+    if (blocks > 0x7FFFFFFFLL) {
+        return host::fail(CUVIT_LENGTH_ERROR, "attention launch exceeds the CUDA grid limit");
+    }
+    const unsigned count = static_cast<unsigned>(blocks);
+    if (p.bf16) {
+        return launch_few(p, queries_per_block(p), head_chunks(p), count, stream);
+    }
+    const int chunks = p.head_dim / kElems;
+    if (chunks <= 4) {
+        return launch_lanes<4>(p, count, stream);
+    }
+    if (chunks <= 8) {
+        return launch_lanes<8>(p, count, stream);
+    }
+    return chunks <= 16 ? launch_lanes<16>(p, count, stream) : launch_lanes<32>(p, count, stream);
 }
 
 int launch_join(const VarlenParams& p, cudaStream_t stream) {

@@ -42,13 +42,15 @@ struct VarlenParams {
     float2* part_stats;
 };
 
-// Few query rows per sequence (attention_rows.cu): one pass over the keys for up to kMaxRows
-// rows (queries times the heads that share a key head) at a time.
+// Few query rows per sequence (attention_few.cu for bfloat16, attention_rows.cu for float): one pass
+// over the keys for up to kMaxRows rows (queries times the heads that share a key head) at a time.
 constexpr int kMaxRows = 8;
 bool rows_kernel_takes(const VarlenParams& p);
 int rows_kernel_rows(const VarlenParams& p);
 long long rows_kernel_items(const VarlenParams& p); // blocks of a launch per split
 int launch_rows(const VarlenParams& p, cudaStream_t stream);
+int launch_few(const VarlenParams& p, int queries_per_block, int head_chunks, unsigned blocks,
+               cudaStream_t stream);
 
 // bfloat16 on the tensor cores (attention_tiles.cu).
 bool tiles_kernel_takes(const VarlenParams& p);

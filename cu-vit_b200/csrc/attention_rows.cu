@@ -424,25 +424,34 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const VarlenPa
     }
     const long long pitch = static_cast<long long>(p.q_tokens) * p.q_heads;
     const float2* const stats = p.part_stats + row * p.q_heads + head;
-    static_assert(kMaxSplits <= 64, "two splits' statistics per lane");
-    float2 stat[2];
+    constexpr int kEach = kMaxSplits / 32; // splits' statistics per lane
+    static_assert(kMaxSplits % 32 == 0, "whole statistics per lane");
+    __shared__ float factors[kWarps][kMaxSplits];
+    float2 stat[kEach];
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kEach; ++i) {
         const int at = lane + 32 * i;
         stat[i] = at < p.splits ? stats[at * pitch] : make_float2(-INFINITY, 0.0F);
+        top = fmaxf(top, stat[i].x);
     }
-    float top = fmaxf(stat[0].x, stat[1].x);
 #pragma unroll
     for (int offset = 16; offset > 0; offset /= 2) {
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, offset));
     }
     const float stand = top == -INFINITY ? 0.0F : top;
-    const float factor[2] = {exp2f(stat[0].x - stand), exp2f(stat[1].x - stand)};
-    float total = factor[0] * stat[0].y + factor[1] * stat[1].y;
+    float total = 0.0F;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const float factor = exp2f(stat[i].x - stand);
+        total = fmaf(factor, stat[i].y, total);
+        factors[warp][lane + 32 * i] = factor;
+    }
 #pragma unroll
     for (int offset = 16; offset > 0; offset /= 2) {
         total += __shfl_xor_sync(0xFFFFFFFFu, total, offset);
     }
+    __syncwarp();
     // Lane's elements: 4 lane .. + 3 as one vector, or lane, lane + 32, ... where rows are not whole
     // vectors. Eight splits' loads are in flight at a time.
     const float* const parts = p.part_out + (row * p.q_heads + head) * p.head_dim;
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const VarlenPa
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const int at = first + warp + kWarps * i;
-            weight[i] = __shfl_sync(0xFFFFFFFFu, at < 32 ? factor[0] : factor[1], at % 32);
+            weight[i] = at < p.splits ? factors[warp][at] : 0.0F;
             loaded[i] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
             if (at < p.splits) {
                 const float* const from = parts + at * pitch * p.head_dim;

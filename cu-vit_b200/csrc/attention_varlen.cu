@@ -347,7 +347,7 @@ int splits_of(Kernel kernel, const VarlenParams& p, int sm_count) {
     switch (kernel) {
     case Kernel::kRows:
         // About half of the launch's bound on blocks have rows (varlen.cuh).
-        return choose_splits(p, rows_kernel_items(p) / 2, 6, 128, sm_count);
+        return choose_splits(p, rows_kernel_items(p) / 2, 4, 128, sm_count);
     case Kernel::kTiles:
         return choose_splits(p, tiles_kernel_items(p), 1, 512, sm_count);
     case Kernel::kSplit:

@@ -251,6 +251,8 @@ _library: ctypes.CDLL | None = None
 def library() -> ctypes.CDLL:
     """Loads libcuvit_b200.so once and attaches every signature. Raises when missing."""
     global _library
+    if _library is not None:
+        return _library
     with _lock:
         if _library is None:
             if not LIBRARY_PATH.exists():

@@ -16,6 +16,7 @@
 
 #include <cuda_runtime_api.h>
 
+#include <cstddef>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -179,6 +180,53 @@ inline void launch_attention(const void* qkv, void* context, int dtype, int batc
                              int heads, int head_dim, float scale, cudaStream_t stream = nullptr) {
     detail::raise_on(cuvit_attention(qkv, context, dtype, batch, tokens, heads, head_dim, scale,
                                      detail::stream_of(stream)));
+}
+
+// Encoder blocks over packed images and videos of any size (cuvit_b200.h; no reference counterpart).
+
+/// Turns query and key pairs by their positions, int32 [axes, tokens] on the device.
+inline void launch_rotary(const void* q, const void* k, void* q_out, void* k_out,
+                          const std::int32_t* positions, const cuvit_rotary& rotary,
+                          const cuvit_qk_problem& problem, cudaStream_t stream = nullptr) {
+    detail::raise_on(cuvit_rotary_qk(q, k, q_out, k_out, positions, &rotary, &problem,
+                                     detail::stream_of(stream)));
+}
+
+/// Per-head norms of queries and keys, then (rotary not null) the rotation, in one pass.
+inline void launch_qk_norm_rotary(const void* q, const void* k, void* q_out, void* k_out,
+                                  const cuvit_qk_norm& norm, const std::int32_t* positions,
+                                  const cuvit_rotary* rotary, const cuvit_qk_problem& problem,
+                                  cudaStream_t stream = nullptr) {
+    detail::raise_on(cuvit_qk_norm_rotary(q, k, q_out, k_out, &norm, positions, rotary, &problem,
+                                          detail::stream_of(stream)));
+}
+
+/// Bytes of workspace with which launch_attention_varlen may split long key ranges.
+inline std::size_t attention_varlen_workspace(const cuvit_attention_problem& problem) {
+    std::size_t bytes = 0;
+    detail::raise_on(cuvit_attention_varlen_workspace(&problem, &bytes));
+    return bytes;
+}
+
+/// Attention over packed sequences given by int32 device offsets [batch + 1]; kv_offsets null:
+/// the queries' own.
+inline void launch_attention_varlen(const void* q, const void* k, const void* v, void* out,
+                                    const std::int32_t* q_offsets, const std::int32_t* kv_offsets,
+                                    const cuvit_attention_problem& problem,
+                                    void* workspace = nullptr, std::size_t workspace_bytes = 0,
+                                    cudaStream_t stream = nullptr) {
+    detail::raise_on(cuvit_attention_varlen(q, k, v, out, q_offsets, kv_offsets, &problem,
+                                            workspace, workspace_bytes,
+                                            detail::stream_of(stream)));
+}
+
+/// out = residual + scale * activation(x weight^T + bias), with a gate when problem.gated; bias,
+/// scale and residual may be null.
+inline void launch_linear(const void* x, const void* weight, const float* bias, const float* scale,
+                          const void* residual, void* out, const cuvit_linear_problem& problem,
+                          cudaStream_t stream = nullptr) {
+    detail::raise_on(cuvit_linear(x, weight, bias, scale, residual, out, &problem,
+                                  detail::stream_of(stream)));
 }
 
 // Device counterpart of cuvit::preprocess (include/cuvit/image.hpp of the reference, a host

@@ -375,11 +375,12 @@ typedef struct cuvit_attention_problem {
 
 /* out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j] per head, over the keys query i sees; a
  * query that sees none gets zeros. Softmax statistics and sums are FP32; BF16 rounds the
- * weights to bfloat16 for the product with v, F32 is FP32 throughout. Rows of out outside every
- * sequence are not written, and rows of q, k and v outside a sequence may hold anything, NaN
- * included, without reaching it. (Within a sequence a causal query's weight for a later key is
- * zero, but zero times a NaN or infinite value is NaN, as in the plain product.) kv_offsets null: q_offsets (self-attention). out must not
- * overlap q, k or v.
+ * weights to bfloat16 for the product with v, F32 has FP32-faithful products (each as three of
+ * TF32 halves, as CUVIT_MATH_FP32). Rows of out outside every sequence are not written, and rows
+ * of q, k and v outside a sequence may hold anything, NaN included, without reaching it. Within a
+ * sequence a NaN or infinite value reaches every query of its tile of keys: a causal query's
+ * weight for a later key is zero, but zero times such a value is NaN, as in the plain product.
+ * kv_offsets null: q_offsets (self-attention). out must not overlap q, k or v.
  * The workspace (device, 16-byte aligned, cuvit_attention_varlen_workspace() bytes, contents
  * irrelevant before and after) lets calls with few query rows split long key ranges over the
  * whole GPU; calls that may run at the same time need one each. Null: no split. */
@@ -418,7 +419,8 @@ typedef struct cuvit_linear_problem {
 /* y = x weight^T + bias (FP32 accumulation), then
  *   out = residual + scale * activation(y)                        plain
  *   out = residual + scale * activation(y[:, :n]) * y[:, n:]      gated
- * with one rounding at the store. bias float [n] (gated [2n]), scale float [n] and residual may
+ * with one rounding at the store. With CUVIT_MATH_FP32 an infinite element of x or the weight gives
+ * NaN where the plain product gives an infinity. bias float [n] (gated [2n]), scale float [n] and residual may
  * be null. out may be residual itself (same pointer and row distance); any other overlap of
  * out with an operand is refused. */
 int cuvit_linear(const void* x, const void* weight, const float* bias, const float* scale,

@@ -4,11 +4,13 @@ host and before any launch, and what they take as a no-op; and the rotary plan's
 from __future__ import annotations
 
 import math
+import pathlib
+import subprocess
 
 import numpy as np
 import pytest
 
-from cuvit import kernels
+from cuvit import _lib, kernels
 from cuvit.errors import InvalidArgument, LengthError
 from cuvit.kernels import AttentionProblem, LinearProblem, QkNorm, QkProblem
 
@@ -218,3 +220,52 @@ def test_positions_wrap_exactly():
             difference = np.remainder(fraction * 2 * math.pi - want + math.pi, 2 * math.pi) - math.pi
             # A double's angle: 2^-53 relative, twice (the power and the product).
             assert abs(difference) <= 4 * 2.0 ** -53 * max(abs(position), 8.0)
+
+
+CPP = r"""
+#include "cuvit/kernels.hpp"
+#include <cstdio>
+template <typename Call> static bool refused(Call call) {
+    try { call(); } catch (const std::invalid_argument&) { return true; }
+    return false;
+}
+int main() {
+    cuvit_rotary rotary;
+    const int sections[2] = {8, 8};
+    if (cuvit_rotary_init(&rotary, 2, sections, 10000.0, CUVIT_ROTARY_HALVES,
+                          CUVIT_ROTARY_LADDER_AXIS) != CUVIT_OK) return 1;
+    cuvit_qk_problem qk{};
+    qk.tokens = -1; qk.head_dim = 32;
+    cuvit_qk_norm norm{};
+    cuvit_attention_problem attention{};
+    attention.batch = -1;
+    cuvit_linear_problem linear{};
+    linear.m = -1;
+    if (!refused([&] { cuvit::launch_rotary(nullptr, nullptr, nullptr, nullptr, nullptr, rotary, qk); }))
+        return 2;
+    if (!refused([&] { cuvit::launch_qk_norm_rotary(nullptr, nullptr, nullptr, nullptr, norm, nullptr,
+                                                   &rotary, qk); })) return 3;
+    if (!refused([&] { cuvit::attention_varlen_workspace(attention); })) return 4;
+    if (!refused([&] { cuvit::launch_attention_varlen(nullptr, nullptr, nullptr, nullptr, nullptr,
+                                                     nullptr, attention); })) return 5;
+    if (!refused([&] { cuvit::launch_linear(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr,
+                                           linear); })) return 6;
+    linear.m = 0;
+    cuvit::launch_linear(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, linear);
+    return 0;
+}
+"""
+
+
+def test_cpp_wrappers_compile_and_refuse(tmp_path):
+    """The header-only wrappers of include/cuvit/kernels.hpp raise what the C entries report."""
+    root = pathlib.Path(__file__).resolve().parent.parent
+    source = tmp_path / "wrappers.cpp"
+    source.write_text(CPP)
+    program = tmp_path / "wrappers"
+    library = _lib.LIBRARY_PATH
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", f"-I{root / 'include'}",
+                    "-I/usr/local/cuda/include", str(source), "-o", str(program), str(library),
+                    f"-Wl,-rpath,{library.parent}", "-L/usr/local/cuda/lib64", "-lcudart"],
+                   check=True, timeout=120)
+    assert subprocess.run([str(program)], timeout=60).returncode == 0

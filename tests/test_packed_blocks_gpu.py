@@ -11,6 +11,7 @@ import math
 import pytest
 
 from cuvit import kernels
+from cuvit.errors import InvalidArgument
 from cuvit.kernels import AttentionProblem, LinearProblem, QkNorm, QkProblem
 
 pytestmark = pytest.mark.gpu
@@ -726,3 +727,165 @@ def test_linear_f32_long_rows(k, cuda):
     # to the whole: half of k / 64 2^-24, at most.
     bound = 4 * 2.0 ** -23 + 13 * 2.0 ** -23 + (k / 128 + 1) * 2.0 ** -24
     assert ((out.double() - exact).abs() <= bound * exact).all()
+
+
+# ---- calls around the edges ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("group", [1, 3, 5, 8, 16])
+def test_attention_many_ragged_causal_sequences(group, kind, cuda):
+    """More sequences than are ordered by length, some empty, some of one token."""
+    torch = cuda
+    lengths = [(17 * i * i) % 211 for i in range(45)] + [1, 0, 400]
+    dim, kv_heads = 64, 2
+    tokens = sum(lengths)
+    q = normal(torch, (tokens, kv_heads * group, dim), 1, kind)
+    k, v = (normal(torch, (tokens, kv_heads, dim), seed, kind) for seed in (2, 3))
+    problem = AttentionProblem(len(lengths), tokens, tokens, kv_heads * group, kv_heads, dim,
+                               dtype_of(kind), True, 0.2)
+    want, bound = attention_64(torch, q, k, v, lengths, lengths, 0.2, True, kind)
+    got = run_attention(torch, q, k, v, offsets(torch, lengths), None, problem)
+    check(got, want, bound)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("group,queries", [(1, 8), (2, 3), (3, 2), (5, 1), (7, 1), (8, 1), (3, 1)])
+@pytest.mark.parametrize("dim", [8, 40, 64, 88, 128])
+def test_attention_few_rows(group, queries, dim, kind, cuda):
+    """Every division of eight rows into queries and heads, lengths on both sides of the steps."""
+    torch = cuda
+    keys = [1, 15, 16, 17, 33, 64, 65, 700, 0, 5]
+    rows = [queries] * len(keys)
+    kv_heads = 2
+    q = normal(torch, (sum(rows), kv_heads * group, dim), 4, kind)
+    k, v = (normal(torch, (sum(keys), kv_heads, dim), seed, kind) for seed in (5, 6))
+    for causal in (False, True):
+        problem = AttentionProblem(len(keys), sum(rows), sum(keys), kv_heads * group, kv_heads, dim,
+                                   dtype_of(kind), causal, 0.3)
+        want, bound = attention_64(torch, q, k, v, rows, keys, 0.3, causal, kind)
+        got = run_attention(torch, q, k, v, offsets(torch, rows), offsets(torch, keys), problem)
+        check(got, want, bound, f"causal {causal}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("queries", [1, 150])
+def test_attention_offsets_past_32_bits(queries, kind, cuda):
+    """Rows whose element offsets pass 2^32: the keys of the last sequence lie there."""
+    torch = cuda
+    stride, tokens, heads, dim = 2 ** 16, 70000, 1, 64
+    rows = torch.empty(tokens * stride, dtype=torch_type(torch, kind), device="cuda").view(tokens,
+                                                                                          stride)
+    keys = [tokens - 200, 200]
+    live = rows[tokens - 200:]
+    live[:, :dim] = normal(torch, (200, dim), 1, kind)
+    live[:, dim:2 * dim] = normal(torch, (200, dim), 2, kind)
+    k, v = rows[:, :dim].unsqueeze(1), rows[:, dim:2 * dim].unsqueeze(1)
+    q = normal(torch, (queries, heads, dim), 3, kind)
+    problem = AttentionProblem(2, queries, tokens, heads, heads, dim, dtype_of(kind), False, 0.125,
+                               0, stride, stride)
+    want, bound = attention_64(torch, q, k[tokens - 200:], v[tokens - 200:], [queries], [200], 0.125,
+                               False, kind)
+    got = run_attention(torch, q, k, v, offsets(torch, [0, queries]), offsets(torch, keys), problem)
+    check(got, want, bound)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("queries", [1, 100])
+def test_attention_split_calls_on_two_streams(queries, kind, cuda):
+    """Calls that split their keys, at the same time and captured, each with its own workspace."""
+    torch = cuda
+    dim, heads, keys = 64, 4, 6000
+    problem = AttentionProblem(1, queries, keys, heads, heads, dim, dtype_of(kind), False, 0.125)
+    size = kernels.attention_varlen_workspace(problem)
+    assert size > 0
+    q_offsets, kv_offsets = offsets(torch, [queries]), offsets(torch, [keys])
+    sides = []
+    for seed in (1, 2):
+        q = normal(torch, (queries, heads, dim), seed, kind)
+        k, v = (normal(torch, (keys, heads, dim), 10 * seed + i, kind) for i in range(2))
+        sides.append(dict(q=q, k=k, v=v, out=torch.empty_like(q),
+                          area=torch.empty(size, dtype=torch.uint8, device="cuda")))
+
+    def launch(side, stream):
+        kernels.launch_attention_varlen(side["q"], side["k"], side["v"], side["out"], q_offsets,
+                                        kv_offsets, problem, side["area"], size, stream)
+
+    want = []
+    for side in sides:
+        launch(side, None)
+        torch.cuda.synchronize()
+        want.append(side["out"].clone())
+    streams = [torch.cuda.Stream() for _ in sides]
+    for _ in range(20):
+        for side, stream in zip(sides, streams):
+            launch(side, stream)
+    torch.cuda.synchronize()
+    for side, expected in zip(sides, want):
+        assert torch.equal(side["out"], expected)
+    graphs = []
+    for side in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            launch(side, torch.cuda.current_stream())
+        side["out"].zero_()
+        side["area"].fill_(0xFF)
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for side, expected in zip(sides, want):
+        assert torch.equal(side["out"], expected)
+
+
+def test_attention_workspace_refusals(cuda):
+    torch = cuda
+    problem = AttentionProblem(1, 1, 9000, 2, 2, 64, kernels.DTYPE_BF16, False, 0.125)
+    size = kernels.attention_varlen_workspace(problem)
+    q = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(9000, 2, 64, dtype=torch.bfloat16, device="cuda")
+    area = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    one, many = offsets(torch, [1]), offsets(torch, [9000])
+    out = torch.zeros_like(q)
+    for workspace, given in ((area, 16), (area[1:], size), (k, size), (area.cpu(), size)):
+        with pytest.raises(InvalidArgument):
+            kernels.launch_attention_varlen(q, k, k, out, one, many, problem, workspace, given)
+    torch.cuda.synchronize()
+    assert (out == 0).all()
+
+
+def test_operands_of_another_device_are_refused(cuda):
+    torch = cuda
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    x = torch.zeros(4, 1, 8, device="cuda:1")
+    out = torch.zeros(4, 1, 8, device="cuda:0")
+    with torch.cuda.device(0), pytest.raises(InvalidArgument, match="another device"):
+        kernels.launch_rotary(x, None, out, None, torch.zeros(4, dtype=torch.int32, device="cuda:0"),
+                              kernels.rotary_axes([4]), QkProblem(4, 1, 0, 8, kernels.DTYPE_F32))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("m,n,k", [(9, 48, 64), (12, 16, 4), (15, 145, 96), (128, 289, 32),
+                                   (130, 1000, 260), (2000, 100, 64)])
+def test_linear_around_the_tiles(m, n, k, gated, kind, cuda):
+    """Tile widths from one step of columns to the widest, all with every optional operand."""
+    torch = cuda
+    x = normal(torch, (m, k), 1, kind)
+    w = normal(torch, ((2 if gated else 1) * n, k), 2, kind, k ** -0.5)
+    bias = normal(torch, (w.shape[0],), 3)
+    scale = normal(torch, (n,), 4)
+    residual = normal(torch, (m, n), 5, kind)
+    out = torch.empty_like(residual)
+    math_mode = kernels.MATH_BF16 if kind == "bf16" else kernels.MATH_FP32
+    kernels.launch_linear(x, w, bias, scale, residual, out,
+                          LinearProblem(m, n, k, math_mode, dtype_of(kind), kernels.ACTIVATION_GELU,
+                                        gated))
+    torch.cuda.synchronize()
+    want, bound = linear_64(torch, x, w, bias, scale, residual, kernels.ACTIVATION_GELU, gated, kind,
+                            kind, n)
+    check(out, want, bound)

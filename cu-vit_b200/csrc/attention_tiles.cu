@@ -27,11 +27,16 @@
 //   scores giving both them and their maximum; only where a maximum turns out too high (and in the
 //   first step) are O and the sums rescaled and the scores read again.
 // * Scores are read 32 at a time, the next 32 in flight meanwhile. Two threads per row (64 scores
-//   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes %CLIP%
-//   (16384 tokens, 16 heads of 128): their exchanges cost more than the shorter rows saved.
+//   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes 1.81 ms
+//   (16384 tokens, 16 heads of 128: 1214 TFLOP/s, of 1672 measured for one large product; heads of
+//   64: 1.27 ms, 867 TFLOP/s, bound by exponentials: 3.4 of the special-function units' 4.5 10^12
+//   a second, a quarter of them on the FMA pipe). Their exchanges cost more than the shorter rows
+//   saved.
 // * head_dim <= 64: P has tensor memory of its own, so the next S is issued as soon as the rows
 //   have read the current one. Up to 128: P overlays S (S 2 x 128, O 2 x 128 columns fill the 512),
-//   and the next S follows P V.
+//   and the next S follows P V. (Steps of 96 keys, which leave P a place of its own for heads up to
+//   112: 336 us against 292 for images of 64 to 4096 tokens, 16 heads of 72. A step's waits take
+//   about 1.4 us whatever its keys.)
 // * A sequence may end inside a tile. K rows past the end only make scores that are replaced by
 //   -inf. V rows past the end would be multiplied by P = 0, which leaves NaN where they hold NaN
 //   or infinity (they belong to other sequences, or to nobody): the at most 15 of them that the

@@ -197,19 +197,32 @@ __global__ void __launch_bounds__(kThreads) qk_scalar_kernel(const __grid_consta
 // vectors of V elements that turn together (V elements apart by the pairing, or next to each
 // other), so the rotation needs no exchange between lanes and a norm one sum over the `chunks`
 // lanes of a head, as many heads side by side in a warp as fit (6 of 5 lanes for head_dim 80; with
-// heads padded to 8 lanes 3 in 8 would idle). A block takes a few tokens with all their query and
-// key heads and first fills a table of their turns in shared memory: one sine and cosine per
-// (token, pair), however many heads share it. The next head's vectors are loaded before the
-// current one's are used: at HBM's latency a block's threads have to keep 64 bytes each in flight.
-constexpr int kWarps = kThreads / 32;
+// heads padded to 8 lanes 3 in 8 would idle). A block takes a few tokens and first fills a table of
+// their turns in shared memory: one sine and cosine per (token, pair), however many heads share it.
+// Its lane groups are the heads of `slots` tokens, each going from token to token with its own head,
+// so that a step is its loads, arithmetic and stores; finding a head and its gains for each of the
+// heads in turn took more instructions than they. The next token's vectors are loaded before the
+// current one's are used.
+//
+// 12544 tokens, 16 + 16 heads of 80: 26 us, 5.0 TB/s; with RMS norms, 50432 tokens, 12 + 12 heads of
+// 64: 67 us, 4.6 TB/s, of 6.5 for a copy. What keeps norms from the copy's rate is the chain of sum,
+// root, gains and turns in every step, which 36 warps an SM do not quite hide.
+template <int Norm>
+constexpr int kMaxWarps = Norm == kNormNone ? 12 : 9;
+// Norms spill a little at 56 registers, but four blocks of nine warps beat three (69 and 74 us for
+// 50432 tokens, 12 + 12 heads of 64); two tokens ahead instead of one, for fewer warps: 96 us.
+template <int Norm>
+constexpr int kMinBlocks = Norm == kNormNone ? 3 : 4;
 constexpr int kTableVectors = 512; // float4 of two turns each: 8 KB
-constexpr int kMaxHeads = 8192;    // of both sides: item numbers and their reciprocal stay exact
+constexpr int kMaxHeads = 1 << 18; // of both sides: the second grid dimension stays in 16 bits
 
 struct VectorShape {
     int chunks;       // lanes per head
     int warp_groups;  // heads side by side in a warp: 32 / chunks
-    int block_tokens; // tokens per block
-    unsigned magic;   // ceil(2^32 / heads of both sides)
+    int heads;        // of a block (a second grid dimension goes through the others)
+    int slots;        // tokens side by side in a block
+    int block_tokens; // tokens of a block
+    int warps;
 };
 
 template <typename T, int V>
@@ -217,26 +230,17 @@ struct alignas(sizeof(T) * V) Vec {
     T value[V];
 };
 
-// Sum over the `count` lanes from lane `first` on, of which this is number `position`: windows of
-// 1, 2, 4, ... lanes (around the group's end) and from them the sum of `count`.
+// Sum over the `count` lanes from lane `first` on, of which this is number `position`, the same in
+// all of them: halves added onto halves, then handed out.
 __device__ __forceinline__ float group_sum(float value, int first, int position, int count) {
-    const auto from = [&](float v, int distance) {
-        int at = position + distance;
-        at -= at >= count ? count : 0;
-        return __shfl_sync(0xFFFFFFFFu, v, first + at);
-    };
-    float total = 0.0F;
-    int covered = 0;
-    for (int width = 1; width <= count; width *= 2) {
-        if (count & width) {
-            total = covered == 0 ? value : total + from(value, covered);
-            covered += width;
-        }
-        if (2 * width <= count) {
-            value += from(value, width);
+#pragma unroll
+    for (int offset = 16; offset > 0; offset /= 2) {
+        if (offset < count) { // the same for the launch
+            const float other = __shfl_down_sync(0xFFFFFFFFu, value, offset);
+            value += position + offset < count && position < offset ? other : 0.0F;
         }
     }
-    return total;
+    return __shfl_sync(0xFFFFFFFFu, value, first);
 }
 
 // A lane's V elements as V / 2 packed pairs.
@@ -287,7 +291,7 @@ __device__ __forceinline__ void shared_pairs(const float* p, uint64_t (&out)[V /
 }
 
 template <typename T, int V, int Norm, bool Adjacent>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kMaxWarps<Norm>, kMinBlocks<Norm>)
     qk_vector_kernel(const __grid_constant__ Params p, const VectorShape s) {
     __shared__ float4 table[kTableVectors];
     __shared__ __align__(16) float gains[Norm == kNormNone ? 1 : 4][kMaxHeadDim];
@@ -298,14 +302,17 @@ __global__ void __launch_bounds__(kThreads)
     const int tokens = min(s.block_tokens, p.tokens - token0);
     const int half = p.head_dim / 2;
 
-    const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     const int group_of_warp = lane / s.chunks;
     const int chunk = lane - group_of_warp * s.chunks;
-    const bool in_group = group_of_warp < s.warp_groups;
     const int first_lane = group_of_warp * s.chunks;
-    const int group = warp * s.warp_groups + group_of_warp;
-    const int groups = kWarps * s.warp_groups;
+    const int group = static_cast<int>(threadIdx.x) / 32 * s.warp_groups + group_of_warp;
+    const int slot = group / s.heads;
+    int head = static_cast<int>(blockIdx.y) * s.heads + group - slot * s.heads; // queries first
+    const bool key = head >= p.side[0].heads;
+    const Side& side = p.side[key ? 1 : 0];
+    head -= key ? p.side[0].heads : 0;
+    const bool in_group = group_of_warp < s.warp_groups && slot < s.slots && head < side.heads;
     int first, second; // this lane's elements
     if constexpr (Adjacent) {
         first = 2 * V * chunk;
@@ -313,36 +320,28 @@ __global__ void __launch_bounds__(kThreads)
     } else {
         pair_elements(V * chunk, p.pairs, half, 0, first, second);
     }
-    const int q_heads = p.side[0].heads;
-    const int heads = q_heads + p.side[1].heads;
-    const int items = tokens * heads; // heads of a token, queries first
-    const auto token_of = [&](int item) {
-        return heads == 1 ? item : static_cast<int>(__umulhi(static_cast<unsigned>(item), s.magic));
-    };
-    const T* const in[2] = {
-        static_cast<const T*>(p.side[0].in) + token0 * p.side[0].in_stride,
-        static_cast<const T*>(p.side[1].in) + token0 * p.side[1].in_stride -
-            static_cast<long long>(q_heads) * p.head_dim};
-    const auto load_item = [&](int item, Vec<T, V>& x, Vec<T, V>& y) {
-        if (item < items && in_group) {
-            const int t = token_of(item);
-            const int head = item - t * heads;
-            const bool key = head >= q_heads;
-            const T* const at = (key ? in[1] : in[0]) +
-                                t * (key ? p.side[1].in_stride : p.side[0].in_stride) +
-                                head * p.head_dim;
-            x = *reinterpret_cast<const Vec<T, V>*>(at + first);
-            y = *reinterpret_cast<const Vec<T, V>*>(at + second);
-        }
-    };
+    const long long in_step = s.slots * side.in_stride;
+    const long long out_step = s.slots * side.out_stride;
+    const T* in = static_cast<const T*>(side.in) + (token0 + slot) * side.in_stride +
+                  static_cast<long long>(head) * p.head_dim;
+    T* out = static_cast<T*>(side.out) + (token0 + slot) * side.out_stride +
+             static_cast<long long>(head) * p.head_dim;
     Vec<T, V> x_next{}, y_next{};
-    load_item(group, x_next, y_next);
+    const auto load_token = [&](int t) {
+        if (t < tokens && in_group) {
+            x_next = *reinterpret_cast<const Vec<T, V>*>(in + first);
+            y_next = *reinterpret_cast<const Vec<T, V>*>(in + second);
+        }
+        in += in_step;
+    };
+    load_token(slot);
 
     // Two neighbouring pairs of a token per float4, placed so that the lanes of a head read
     // consecutive vectors: chunk c's pairs 2q, 2q + 1 at q * chunks + c, as cos, cos, sin, sin for
     // pairs in two halves (whose elements are packed with their neighbours) and cos, sin, cos, sin
     // for adjacent ones.
-    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+    const int threads = 32 * s.warps;
+    for (int i = threadIdx.x; i < tokens * half; i += threads) {
         const int t = i / half;
         const int pair = i - t * half;
         const int c = pair / V;
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(kThreads)
         at[Adjacent ? 2 * (within & 1) + 1 : 2 + (within & 1)] = turn.y;
     }
     if constexpr (Norm != kNormNone) {
-        for (int i = threadIdx.x; i < 2 * p.head_dim; i += kThreads) {
+        for (int i = threadIdx.x; i < 2 * p.head_dim; i += threads) {
             const int k = i >= p.head_dim ? 1 : 0;
             const int e = i - k * p.head_dim;
             gains[2 * k][e] = p.side[k].gamma != nullptr ? p.side[k].gamma[e] : 1.0F;
@@ -365,17 +364,13 @@ __global__ void __launch_bounds__(kThreads)
 
     const bool offsets = p.side[0].beta != nullptr || p.side[1].beta != nullptr;
     const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
-    // Whole warps go round together: the sums need every lane of a group.
-    for (int base = 0; base < items; base += groups) {
-        const int item = base + group;
-        const bool live = item < items && in_group;
+    const float4* turns = table + slot * (half / 2) + chunk;
+    // All groups go round together: the sums need every lane of a warp.
+    for (int t = slot; t - slot < tokens; t += s.slots) {
         uint64_t x[kPairs], y[kPairs];
         unpack2(x_next, x);
         unpack2(y_next, y);
-        load_item(item + groups, x_next, y_next);
-        const int t = live ? token_of(item) : 0;
-        const int head = live ? item - t * heads : 0;
-        const bool key = head >= q_heads;
+        load_token(t + s.slots);
         if constexpr (Norm != kNormNone) {
             if constexpr (Norm == CUVIT_NORM_LAYER) {
                 uint64_t sums = dev::add_f32x2(x[0], y[0]);
@@ -430,8 +425,7 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        if (live) {
-            const float4* const turns = table + t * (half / 2) + chunk;
+        if (t < tokens && in_group) {
             if constexpr (Adjacent) {
                 // Pair j of the chunk is element pair j of x followed by y: with the turn (c, s),
                 // (a, b) becomes (a c - b s, b c + a s).
@@ -464,12 +458,11 @@ __global__ void __launch_bounds__(kThreads)
                     x[j] = turned;
                 }
             }
-            const Side& side = p.side[key ? 1 : 0];
-            T* const out = static_cast<T*>(side.out) + (token0 + t) * side.out_stride +
-                           (head - (key ? q_heads : 0)) * p.head_dim;
             store2<T, V>(out + first, x);
             store2<T, V>(out + second, y);
         }
+        out += out_step;
+        turns += s.slots * (half / 2);
     }
 }
 
@@ -480,8 +473,8 @@ int vector_width(const Params& p) {
     const int half = p.head_dim / 2;
     for (int v = 16 / static_cast<int>(sizeof(T)); v >= 2; v /= 2) {
         const int bytes = v * static_cast<int>(sizeof(T));
-        bool ok = half % v == 0 && half / v <= 32 &&
-                  p.side[0].heads <= kMaxHeads / 2 && p.side[1].heads <= kMaxHeads / 2;
+        bool ok = half % v == 0 && half / v <= 32 && p.side[0].heads <= kMaxHeads / 2 &&
+                  p.side[1].heads <= kMaxHeads / 2;
         ok = ok && (p.adjacent || (p.pairs % v == 0 && (half - p.pairs) % v == 0));
         for (const Side& side : p.side) {
             if (side.heads == 0) {
@@ -506,18 +499,37 @@ int launch_vector(const Params& p, int sm_count, cudaStream_t stream) {
     const int half = p.head_dim / 2;
     s.chunks = half / V;
     s.warp_groups = 32 / s.chunks;
-    const unsigned heads = static_cast<unsigned>(p.side[0].heads + p.side[1].heads);
-    s.magic = heads > 1 ? static_cast<unsigned>((0x100000000ull + heads - 1) / heads) : 0u;
-    // As many tokens as the table holds, up to 8 (more leave too few blocks to balance), but no
-    // more than give every SM 12 blocks.
-    int tokens = kTableVectors * 2 / half;
-    tokens = tokens > 8 ? 8 : tokens;
-    const int spread = p.tokens / (12 * sm_count);
-    s.block_tokens = tokens < spread ? tokens : (spread > 0 ? spread : 1);
-    const int blocks = (p.tokens + s.block_tokens - 1) / s.block_tokens;
+    const int heads = p.side[0].heads + p.side[1].heads;
+    // Warps of a block: the number from 4 on that leaves fewest lane groups without a head, next to
+    // 8 of equals.
+    double best = 0.0;
+    for (const int warps : {8, 9, 7, 10, 6, 11, 5, 12, 4}) {
+        if (warps > kMaxWarps<Norm>) {
+            continue;
+        }
+        const int groups = warps * s.warp_groups;
+        const int parts = (heads + groups - 1) / groups;
+        const int taken = parts > 1 ? heads : groups / heads * heads;
+        const double used = static_cast<double>(taken) / (static_cast<double>(parts) * groups);
+        if (used > best + 0.02) {
+            best = used;
+            s.warps = warps;
+        }
+    }
+    const int table_tokens = kTableVectors * 2 / half;
+    const int groups = s.warps * s.warp_groups;
+    s.heads = heads < groups ? heads : groups;
+    s.slots = groups / s.heads < table_tokens ? groups / s.heads : table_tokens;
+    // Tokens of a block: as many steps as the table holds, but no more than give every SM 12 blocks.
+    const int steps = p.tokens / (12 * sm_count * s.slots);
+    const int most = table_tokens / s.slots;
+    s.block_tokens = s.slots * (steps < 1 ? 1 : (steps < most ? steps : most));
+    const int blocks = (p.tokens - 1) / s.block_tokens + 1;
+    const int parts = (heads + s.heads - 1) / s.heads;
     host::pdl_launch(p.adjacent ? qk_vector_kernel<T, V, Norm, true>
                                 : qk_vector_kernel<T, V, Norm, false>,
-                     dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p, s);
+                     dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)),
+                     dim3(static_cast<unsigned>(32 * s.warps)), 0, stream, p, s);
     return host::after_launch("qk_vector_kernel");
 }
 

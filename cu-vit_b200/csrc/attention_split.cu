@@ -6,16 +6,17 @@
 // into one of two buffers there, weights go back as halves, and a tile's weighted values are added
 // to registers, so no accumulator sums more than 64 products or a head's width.
 //
-// 4096 tokens, 8 heads of 64: 320 us, 107 TFLOP/s (products in the FP32 pipe: 954 us); heads of 128
-// 760 us; 8 x 197 tokens, 12 heads 41 us (78). The tensor core would allow three times that (its
-// products take 1540 cycles of the 4700 a tile of 64 keys and 64 elements takes): what bounds it is
+// 4096 tokens, 8 heads of 64: 311 us, 111 TFLOP/s (products in the FP32 pipe: 954 us); heads of 128
+// 659 us; 8 x 197 tokens, 12 heads 39 us (78). The tensor core would allow three times that (its
+// products take 1540 cycles of the 4600 a tile of 64 keys and 64 elements takes): what bounds it is
 // the softmax warps' chain of waits (scores, maximum, exponentials, previous sum, weights), and a
-// quarter is the loading warps' share of the issue slots. Two softmax warps a scheduler do not hide
-// the chain; a second set on alternate tiles would need more registers than an SM has.
+// quarter is the loading warps' share of the issue slots. A second set of softmax warps on alternate
+// tiles would need more registers than an SM has.
 //
-//   warps 0-7    softmax: two threads per row, one for each half of a tile's keys; they exchange
-//                the row's maximum through shared memory, and each keeps half of the output row
-//   warps 8-15   (wide heads: 8-11) bring keys and values in (each thread its own pieces, several tiles ahead, without
+//   first 8 (wide heads: 16) warps   softmax: two (four) threads per row, each with its part of a
+//                tile's keys; they exchange the row's maximum through shared memory, and each keeps
+//                its part of the output row
+//   next 8       bring keys and values in (each thread its own pieces, several tiles ahead, without
 //                any wait for one another), split them, and lay them out for the tensor core:
 //                keys as they are, values transposed
 //   last warp    issues the products: S(0), S(1), PV(0), S(2), PV(1), ...
@@ -30,7 +31,7 @@ namespace cuvit::attn {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kSoftmaxWarps = 8;
+constexpr int kMaxParts = 4;
 // A tile is 1024 16-byte pieces (64 keys of 64 or 32 of 128), four to a place.
 constexpr int kPieces = 4;
 constexpr int kPlaces = 256;
@@ -42,8 +43,8 @@ constexpr int kTiles = 4; // split tiles: the tensor core works on one, up to th
 constexpr int kRaw = 4;   // tiles being fetched
 constexpr int kRawBytes = kPlaces * kPieces * 16;
 constexpr int kRawOffset = kTiles * kTileBytes;
-constexpr int kTopOffset = kRawOffset + kRaw * kRawBytes; // [2][2][kRows] floats
-constexpr int kBarrierOffset = kTopOffset + 4 * kRows * 4;
+constexpr int kTopOffset = kRawOffset + kRaw * kRawBytes; // [2][parts][kRows] floats
+constexpr int kBarrierOffset = kTopOffset + 2 * kMaxParts * kRows * 4;
 constexpr int kBarriers = 2 * kTiles + 1 + 4 + 2 + 4 + 1;
 constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 8;
 static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
@@ -52,18 +53,19 @@ constexpr int kTmemColumns = 512;
 template <bool Wide> // heads of 65 to 128
 struct Shape {
     static constexpr int kKeys = Wide ? 32 : 64;
-    static constexpr int kOwn = kKeys / 2;         // keys of a softmax thread
-    static constexpr int kGroups = Wide ? 4 : 2;   // 16-column groups of its output half
+    // Threads of a row. Narrow heads' fit 96 registers with two (four, with 72: 369 us against 320 for
+    // 4096 tokens, 8 heads of 64), wide ones spill with two (760 us against 659 for heads of 128).
+    static constexpr int kParts = Wide ? 4 : 2;
+    static constexpr int kSoftmaxWarps = 4 * kParts;
+    static constexpr int kOwn = kKeys / kParts; // keys of a softmax thread
+    static constexpr int kGroups = 2;           // 16-column groups of its part of the output
     static constexpr int kQ = 0;                   // hi, then lo
     static constexpr int kWidth = Wide ? 128 : 64; // of Q's halves and of the output
     static constexpr int kS = 2 * kWidth;          // two buffers
     static constexpr int kP = kS + 2 * kKeys;      // hi, then lo
     static constexpr int kO = kP + 2 * kKeys;
     static_assert(kO + kWidth <= kTmemColumns, "tensor memory");
-    // Loading warps. Wide heads' outputs take 32 more registers in the softmax warps: more than
-    // 16 warps a block would leave too few (4 loading warps 760 us, 8 870 us for 4096 tokens, 8
-    // heads of 128); narrow heads fit, and loading twice as wide pays (384 and 325 us for 64).
-    static constexpr int kLoadWarps = Wide ? 4 : 8;
+    static constexpr int kLoadWarps = 8;
     static constexpr int kMmaWarp = kSoftmaxWarps + kLoadWarps;
     static constexpr int kThreads = 32 * (kMmaWarp + 1);
     static constexpr int kLoaders = 32 * kLoadWarps;
@@ -113,10 +115,14 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
     constexpr int kLoaders = S::kLoaders;
     constexpr int kSets = S::kSets;
     constexpr int kMmaWarp = S::kMmaWarp;
+    constexpr int kParts = S::kParts;
+    constexpr int kSoftmaxWarps = S::kSoftmaxWarps;
     dev::grid_dependency_wait();
     dev::grid_launch_dependents();
-    const int item = static_cast<int>(blockIdx.x) / p.splits;
-    const int split = static_cast<int>(blockIdx.x) - item * p.splits;
+    // Causal: a sequence's last rows, which see most keys, first.
+    const int index = static_cast<int>(p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    const int item = index / p.splits;
+    const int split = index - item * p.splits;
     const int block = item / p.q_heads;
     const int head = item - block * p.q_heads;
     const Sequence s = find_block_warp(p.q_offsets, p.kv_offsets, p.batch, p.q_tokens, p.kv_tokens,
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
     const auto s_empty = [&](int i) -> uint32_t { return bars + 8u * (2 * kTiles + 3 + i); };
     const uint32_t p_full = bars + 8u * (2 * kTiles + 5);
     const uint32_t o_full = bars + 8u * (2 * kTiles + 6);
-    const auto pair_bar = [&](int i) -> uint32_t { return bars + 8u * (2 * kTiles + 7 + i); };
+    const auto row_bar = [&](int i) -> uint32_t { return bars + 8u * (2 * kTiles + 7 + i); };
     const uint32_t drain_bar = bars + 8u * (2 * kTiles + 11);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarrierOffset + 8 * kBarriers);
     const int warp = threadIdx.x / 32;
@@ -169,7 +175,7 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
         dev::mbar_init(p_full, kSoftmaxWarps);
         dev::mbar_init(o_full, 1);
         for (int i = 0; i < 4; ++i) {
-            dev::mbar_init(pair_bar(i), 2); // the two warps of a quarter of the rows
+            dev::mbar_init(row_bar(i), kParts); // the warps of a quarter of the rows
         }
         dev::mbar_init(drain_bar, 1);
         dev::fence_barrier_init();
@@ -186,13 +192,12 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
     if (warp < kSoftmaxWarps) {
         // ---------------- softmax ----------------
         const int quarter = warp & 3;
-        const int half = warp >> 2;
+        const int part = warp >> 2;
         const int row = quarter * 32 + lane;
         const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-        // This half's 16-column groups of Q and of the output.
-        const int groups = padded / kGroup;
-        const int group0 = half == 0 ? 0 : (groups + 1) / 2;
-        const int count = half == 0 ? (groups + 1) / 2 : groups / 2;
+        // This thread's 16-column groups of Q and of the output.
+        const int group0 = part * S::kGroups;
+        const int count = min(S::kGroups, max(0, padded / kGroup - group0));
         float* const tops = reinterpret_cast<float*>(smem + kTopOffset);
 
         const float* const q = static_cast<const float*>(p.q) + (s.q_first + row) * p.q_stride +
@@ -250,17 +255,22 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
         float maximum = -INFINITY; // of the row, times scale and log2 e
         float sum = 0.0F;          // of this thread's weights
         float pending = 1.0F;      // what o is to be multiplied by
-        uint32_t pair_phase = 0, o_phase = 0;
-        // The other half's value of this row.
-        const auto exchange = [&](int buffer, float value, bool& ok) -> float {
-            tops[(2 * buffer + half) * kRows + row] = value;
+        uint32_t row_phase = 0, o_phase = 0;
+        // Hands this thread's value of the row to the others; `all` are in their order.
+        const auto exchange = [&](int buffer, float value, float (&all)[kParts]) -> bool {
+            float* const at = tops + buffer * kParts * kRows + row;
+            at[part * kRows] = value;
             __syncwarp();
             if (lane == 0) {
-                dev::mbar_arrive(pair_bar(quarter));
+                dev::mbar_arrive(row_bar(quarter));
             }
-            ok = dev::mbar_wait_warp(pair_bar(quarter), pair_phase, status);
-            pair_phase ^= 1u;
-            return tops[(2 * buffer + 1 - half) * kRows + row];
+            const bool done = dev::mbar_wait_warp(row_bar(quarter), row_phase, status);
+            row_phase ^= 1u;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                all[i] = at[i * kRows];
+            }
+            return done;
         };
         const auto drain = [&]() -> bool {
             if (!dev::mbar_wait_warp(o_full, o_phase, status)) {
@@ -283,11 +293,11 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
             dev::tc_fence_before();
             return true;
         };
-        // The end of the keys that the row sees, less this half's place in a tile.
+        // The end of the keys that the row sees, less this thread's place in a tile.
         const int seen =
             (p.causal ? static_cast<int>(min(static_cast<long long>(last_key), max(0LL, reach + row + 1)))
                       : last_key) -
-            half * S::kOwn;
+            part * S::kOwn;
         bool ok = true;
 #pragma unroll 1
         for (int tile = 0; tile < tiles; ++tile) {
@@ -298,14 +308,20 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
             }
             dev::tc_fence_after();
             float w[S::kOwn / 4][4];
+            const uint32_t scores = mine + S::kS + buffer * kKeys + part * S::kOwn;
+            constexpr int kRead = S::kOwn < kGroup ? S::kOwn : kGroup;
 #pragma unroll
-            for (int g = 0; g < S::kOwn / kGroup; ++g) {
-                uint32_t raw[kGroup];
-                dev::tmem_load_16(mine + S::kS + buffer * kKeys + half * S::kOwn + g * kGroup, raw);
+            for (int g = 0; g < S::kOwn / kRead; ++g) {
+                uint32_t raw[kRead];
+                if constexpr (kRead == 16) {
+                    dev::tmem_load_16(scores + g * kRead, raw);
+                } else {
+                    dev::tmem_load_8(scores, raw);
+                }
                 dev::tmem_wait_load();
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) {
-                    w[4 * g + j / 4][j % 4] = __uint_as_float(raw[j]);
+                for (int j = 0; j < kRead; ++j) {
+                    w[(g * kRead + j) / 4][j % 4] = __uint_as_float(raw[j]);
                 }
             }
             dev::tc_fence_before();
@@ -327,11 +343,16 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
                 top = dev::max3(top, w[i / 4][i % 4], w[(i + 1) / 4][(i + 1) % 4]);
             }
             top = fmaxf(top, w[S::kOwn / 4 - 1][3]);
-            const float other = exchange(buffer, top, ok);
+            float all[kParts];
+            ok = exchange(buffer, top, all);
             if (!ok) {
                 break;
             }
-            const float raised = fmaxf(maximum, fmaxf(top, other));
+            float raised = maximum;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                raised = fmaxf(raised, all[i]);
+            }
             // A row without a key so far: any finite stand-in keeps 2^(-inf - m) at zero.
             const float stand = raised == -INFINITY ? 0.0F : raised;
             const float factor = dev::ex2_approx(maximum - stand);
@@ -349,14 +370,13 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
                 break;
             }
             pending = factor;
-            // Eight at a time: registers are short.
             uint64_t check = 0u; // weights are at most 1, or NaN, which lo keeps
 #pragma unroll
             for (int c = 0; c < S::kOwn / 4; c += 2) {
                 float hi[2][4];
                 dev::split4(w[c], hi[0], check);
                 dev::split4(w[c + 1], hi[1], check);
-                const uint32_t to = mine + S::kP + half * S::kOwn + 4 * c;
+                const uint32_t to = mine + S::kP + part * S::kOwn + 4 * c;
                 dev::tmem_store_8(to, hi[0], hi[1]);
                 dev::tmem_store_8(to + kKeys, w[c], w[c + 1]);
             }
@@ -371,7 +391,13 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
             ok = drain();
         }
         if (ok) {
-            sum += exchange(tiles & 1, sum, ok);
+            float all[kParts];
+            ok = exchange(tiles & 1, sum, all);
+            sum = 0.0F;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                sum += all[i];
+            }
         }
         if (ok && row < rows) {
             float* to;
@@ -381,7 +407,7 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
                     (static_cast<long long>(split) * p.q_tokens + s.q_first + row) * p.q_heads +
                     head;
                 to = p.part_out + at * d;
-                if (half == 0) {
+                if (part == 0) {
                     p.part_stats[at] = make_float2(maximum, sum);
                 }
             } else {

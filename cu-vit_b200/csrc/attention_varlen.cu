@@ -427,9 +427,13 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
     const int64_t q_width = static_cast<int64_t>(p.q_heads) * p.head_dim * element;
     const int64_t kv_width = static_cast<int64_t>(p.kv_heads) * p.head_dim * element;
     const host::RowSpan out_span{out, p.q_tokens, q_width, p.out_stride * element};
+    const int64_t offset_bytes = (static_cast<int64_t>(p.batch) + 1) * 4;
+    const host::RowSpan q_offset_span{q_offsets, 1, offset_bytes, offset_bytes};
+    const host::RowSpan kv_offset_span{kv_offsets, 1, offset_bytes, offset_bytes};
     if (host::rows_overlap(out_span, {q, p.q_tokens, q_width, p.q_stride * element}) ||
         host::rows_overlap(out_span, {k, p.kv_tokens, kv_width, p.k_stride * element}) ||
-        host::rows_overlap(out_span, {v, p.kv_tokens, kv_width, p.v_stride * element})) {
+        host::rows_overlap(out_span, {v, p.kv_tokens, kv_width, p.v_stride * element}) ||
+        host::rows_overlap(out_span, q_offset_span) || host::rows_overlap(out_span, kv_offset_span)) {
         return host::fail(CUVIT_INVALID_ARGUMENT, "the attention output overlaps an operand");
     }
     p.q = q;
@@ -454,6 +458,7 @@ int run(const void* q, const void* k, const void* v, void* out, const int32_t* q
         if (host::rows_overlap(span, {q, p.q_tokens, q_width, p.q_stride * element}) ||
             host::rows_overlap(span, {k, p.kv_tokens, kv_width, p.k_stride * element}) ||
             host::rows_overlap(span, {v, p.kv_tokens, kv_width, p.v_stride * element}) ||
+            host::rows_overlap(span, q_offset_span) || host::rows_overlap(span, kv_offset_span) ||
             host::rows_overlap(span, out_span)) {
             return host::fail(CUVIT_INVALID_ARGUMENT, "the attention workspace overlaps an operand");
         }

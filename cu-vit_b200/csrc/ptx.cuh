@@ -567,6 +567,14 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
         : "memory");
 }
 
+// Loads 8 consecutive 32-bit TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_load_8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                   "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+
 // Eight values into 8 consecutive columns.
 __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const float (&a)[4],
                                              const float (&b)[4]) {

@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps<Norm>, kMinBlocks<Norm>)
     }
     const long long in_step = s.slots * side.in_stride;
     const long long out_step = s.slots * side.out_stride;
-    const T* in = static_cast<const T*>(side.in) + (token0 + slot) * side.in_stride +
+    const T* in = static_cast<const T*>(side.in) + (token0 + static_cast<long long>(slot)) * side.in_stride +
                   static_cast<long long>(head) * p.head_dim;
-    T* out = static_cast<T*>(side.out) + (token0 + slot) * side.out_stride +
+    T* out = static_cast<T*>(side.out) + (token0 + static_cast<long long>(slot)) * side.out_stride +
              static_cast<long long>(head) * p.head_dim;
     Vec<T, V> x_next{}, y_next{};
     const auto load_token = [&](int t) {
@@ -693,6 +693,23 @@ int run(const void* q, const void* k, void* q_out, void* k_out, const cuvit_qk_n
         }
         if (reinterpret_cast<uintptr_t>(positions) % 4 != 0) {
             return host::fail(CUVIT_INVALID_ARGUMENT, "positions must be aligned to their type");
+        }
+    }
+    // What every block reads must not change under it.
+    const int64_t gain_bytes = static_cast<int64_t>(c.head_dim) * 4;
+    for (const host::RowSpan& out : out_spans) {
+        bool shared = p.positions != nullptr &&
+                      host::rows_overlap(out, {p.positions, rotary->axes, c.tokens * int64_t{4},
+                                               p.position_stride * 4});
+        for (const Side& side : p.side) {
+            for (const float* gains : {side.gamma, side.beta}) {
+                shared = shared || (gains != nullptr &&
+                                    host::rows_overlap(out, {gains, 1, gain_bytes, gain_bytes}));
+            }
+        }
+        if (shared) {
+            return host::fail(CUVIT_INVALID_ARGUMENT,
+                              "an output overlaps the positions or the norm's gains or offsets");
         }
     }
     const host::DeviceContext* context = nullptr;

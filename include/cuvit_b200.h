@@ -323,7 +323,7 @@ typedef struct cuvit_qk_problem {
 /* Turns pair (x, y) of every head of token t by the angle positions[a][t] * rate:
  * (x cos - y sin, x sin + y cos), in FP32 with one rounding at the store; elements past the
  * rotated pairs are copied. An output may be its own input (same pointer and stride); any other
- * overlap is refused. */
+ * overlap with an input, the positions or the norm's gains is refused. */
 int cuvit_rotary_qk(const void* q, const void* k, void* q_out, void* k_out,
                     const int32_t* positions, const cuvit_rotary* rotary,
                     const cuvit_qk_problem* problem, cuvit_stream_t stream);
@@ -380,7 +380,7 @@ typedef struct cuvit_attention_problem {
  * of q, k and v outside a sequence may hold anything, NaN included, without reaching it. Within a
  * sequence a NaN or infinite value reaches every query of its tile of keys: a causal query's
  * weight for a later key is zero, but zero times such a value is NaN, as in the plain product.
- * kv_offsets null: q_offsets (self-attention). out must not overlap q, k or v.
+ * kv_offsets null: q_offsets (self-attention). out must not overlap q, k, v or the offsets.
  * The workspace (device, 16-byte aligned, cuvit_attention_varlen_workspace() bytes, contents
  * irrelevant before and after) lets calls with few query rows split long key ranges over the
  * whole GPU; calls that may run at the same time need one each. Null: no split. */

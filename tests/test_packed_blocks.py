@@ -222,6 +222,22 @@ def test_positions_wrap_exactly():
             assert abs(difference) <= 4 * 2.0 ** -53 * max(abs(position), 8.0)
 
 
+def test_outputs_over_what_every_block_reads_are_refused():
+    rotary = kernels.rotary_axes([4])
+    with pytest.raises(InvalidArgument, match="overlaps the positions"):
+        kernels.launch_rotary(FAKE, None, FAR, None, FAR + 8, rotary, qk(k_heads=0))
+    for gains in ((FAR + 4, None), (None, FAR + 4)):
+        with pytest.raises(InvalidArgument, match="overlaps the positions"):
+            kernels.launch_qk_norm_rotary(FAKE, None, FAR, None,
+                                          QkNorm(kernels.NORM_RMS, 1e-6, *gains, None, None), None,
+                                          None, qk(k_heads=0))
+    for at in (0, 1):
+        offsets = [2 * FAR, 3 * FAR]
+        offsets[at] = FAR + 4
+        with pytest.raises(InvalidArgument, match="overlaps"):
+            kernels.launch_attention_varlen(FAKE, 2 * FAKE, 3 * FAKE, FAR, *offsets, attention())
+
+
 CPP = r"""
 #include "cuvit/kernels.hpp"
 #include <cstdio>

@@ -24,8 +24,8 @@
 // * m follows the true maximum only when that has risen by more than 2^8: P stays below 2^8, sums
 //   below 2^8 per key, well inside FP32's and bfloat16's range, and results do not change, since m
 //   cancels in the quotient. So a step takes its exponentials with the m it has, one read of the
-//   scores giving both them and their maximum; only where a maximum turns out too high (and in the
-//   first step) are O and the sums rescaled and the scores read again.
+//   scores giving both them and their maximum; only where a maximum turns out too high (in the first
+//   step, where m is 0, also too low) are O and the sums rescaled and the scores read again.
 // * Scores are read 32 at a time, the next 32 in flight meanwhile. Two threads per row (64 scores
 //   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes 1.81 ms
 //   (16384 tokens, 16 heads of 128: 1214 TFLOP/s, of 1672 measured for one large product; heads of
@@ -695,57 +695,47 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t packed[4][16];
                     float added = 0.0F;
                     float top = -INFINITY;
-                    bool raise = true;
-                    if (j > 0) {
-                        // Without branches inside, so that one chunk's maxima run under another's
-                        // exponentials: a warp has its scheduler almost to itself here.
-                        const auto weigh = [&](auto exact) {
-                            uint32_t s[2][32];
-                            dev::tmem_load_32(s_tmem, s[0]);
+                    // Without branches inside, so that one chunk's maxima run under another's
+                    // exponentials: a warp has its scheduler almost to itself here.
+                    const auto weigh = [&](auto exact) {
+                        uint32_t s[2][32];
+                        dev::tmem_load_32(s_tmem, s[0]);
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                dev::tmem_wait_load_of(s[c & 1]);
-                                if (c < 3) {
-                                    dev::tmem_load_32(s_tmem + 32 * (c + 1), s[(c + 1) & 1]);
-                                }
-                                if constexpr (exact.value) {
-                                    mask(s[c & 1], limit - 32 * c);
-                                }
-                                top = fmaxf(top, maximum(s[c & 1]));
-                                added += exponentials<exact.value>(s[c & 1], p.scale_log2, m,
-                                                                   packed[c]);
-                            }
-                        };
-                        if (masked || __any_sync(0xFFFFFFFFu,
-                                                 fabsf(m * p.scale_log2) > kLargeMaximum)) {
-                            weigh(std::true_type{});
-                        } else {
-                            weigh(std::false_type{});
-                        }
-                        raise = __any_sync(0xFFFFFFFFu, (top - m) * p.scale_log2 > kRescaleAbove);
-                        if (!S::kOverlay && !raise) {
-                            arrive(s_free + 8 * t);
-                        }
-                        if (!S::kOverlay) {
-                            // P V of the previous step has read P and written O.
-                            ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
-                            o_phase ^= 1u;
-                            if (!ok) {
-                                break;
-                            }
-                            dev::tc_fence_after();
-                        }
-                    } else {
-#pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
-                            uint32_t s[32];
-                            dev::tmem_load_32(s_tmem + 32 * c, s);
-                            dev::tmem_wait_load_of(s);
-                            if (masked) {
-                                mask(s, limit - 32 * c);
+                            dev::tmem_wait_load_of(s[c & 1]);
+                            if (c < 3) {
+                                dev::tmem_load_32(s_tmem + 32 * (c + 1), s[(c + 1) & 1]);
                             }
-                            top = fmaxf(top, maximum(s));
+                            if constexpr (exact.value) {
+                                mask(s[c & 1], limit - 32 * c);
+                            }
+                            top = fmaxf(top, maximum(s[c & 1]));
+                            added += exponentials<exact.value>(s[c & 1], p.scale_log2, m,
+                                                               packed[c]);
                         }
+                    };
+                    if (masked ||
+                        __any_sync(0xFFFFFFFFu, fabsf(m * p.scale_log2) > kLargeMaximum)) {
+                        weigh(std::true_type{});
+                    } else {
+                        weigh(std::false_type{});
+                    }
+                    // The first step has m = 0, which stays where the maximum is within 2^+-8 of it.
+                    const float above = (top - m) * p.scale_log2;
+                    const bool raise = __any_sync(
+                        0xFFFFFFFFu, above > kRescaleAbove ||
+                                         (j == 0 && above < -kRescaleAbove && top != -INFINITY));
+                    if (!S::kOverlay && !raise) {
+                        arrive(s_free + 8 * t);
+                    }
+                    if (!S::kOverlay && j > 0) {
+                        // P V of the previous step has read P and written O.
+                        ok = dev::mbar_wait_warp(o_done + 8 * t, o_phase, status);
+                        o_phase ^= 1u;
+                        if (!ok) {
+                            break;
+                        }
+                        dev::tc_fence_after();
                     }
                     if (raise) {
                         if (j == 0) {

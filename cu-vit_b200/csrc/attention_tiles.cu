@@ -249,7 +249,7 @@ __device__ __forceinline__ void issue_outputs(uint32_t d_tmem, uint32_t p_tmem, 
     }
 }
 
-template <int Atoms>
+template <int Atoms, bool Short>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap map_q,
                            const __grid_constant__ CUtensorMap map_k,
@@ -714,8 +714,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                                packed[c]);
                         }
                     };
-                    if (masked ||
-                        __any_sync(0xFFFFFFFFu, fabsf(m * p.scale_log2) > kLargeMaximum)) {
+                    const bool exact =
+                        masked || __any_sync(0xFFFFFFFFu, fabsf(m * p.scale_log2) > kLargeMaximum);
+                    if (Short && exact) {
+                        // Chunks that no row of the warp sees are zeros.
+                        const int seen = __reduce_max_sync(0xFFFFFFFFu, limit);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            if (32 * c < seen) { // the whole warp
+                                uint32_t s[32];
+                                dev::tmem_load_32(s_tmem + 32 * c, s);
+                                dev::tmem_wait_load_of(s);
+                                mask(s, limit - 32 * c);
+                                top = fmaxf(top, maximum(s));
+                                added += exponentials<true>(s, p.scale_log2, m, packed[c]);
+                            } else {
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) {
+                                    packed[c][x] = 0u;
+                                }
+                            }
+                        }
+                    } else if (exact) {
                         weigh(std::true_type{});
                     } else {
                         weigh(std::false_type{});
@@ -879,10 +899,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-template <int Atoms>
+template <int Atoms, bool Short>
 int launch_atoms(const VarlenParams& p, const host::DeviceContext& context,
                  const CUtensorMap (&maps)[3], cudaStream_t stream) {
-    auto* kernel = &attention_tiles_kernel<Atoms>;
+    auto* kernel = &attention_tiles_kernel<Atoms, Short>;
     constexpr int kBytes = Shape<Atoms>::kSmemBytes;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kBytes));
     const long long items = tiles_kernel_items(p) * p.splits;
@@ -940,8 +960,17 @@ int launch_tiles(const VarlenParams& p, cudaStream_t stream) {
         !describe(p.v, p.head_dim, p.kv_heads, p.kv_tokens, p.v_stride, &maps[2])) {
         return host::fail(CUVIT_CUDA_ERROR, "the attention operands' TMA descriptors failed");
     }
-    return p.head_dim <= 64 ? launch_atoms<1>(p, *context, maps, stream)
-                            : launch_atoms<2>(p, *context, maps, stream);
+    // Sequences of less than two tiles on average: most tiles end inside, and the warps skip the
+    // chunks behind (64 tokens, 16 heads of 64: 256 images 80 us against 95; of 197 tokens, 12 heads:
+    // 148 against 154). The branches cost whole tiles 6 % (one of 16384 tokens: 1327 us against
+    // 1252), so longer ones go without.
+    const bool short_keys = p.kv_tokens <= 224LL * p.batch;
+    if (p.head_dim <= 64) {
+        return short_keys ? launch_atoms<1, true>(p, *context, maps, stream)
+                          : launch_atoms<1, false>(p, *context, maps, stream);
+    }
+    return short_keys ? launch_atoms<2, true>(p, *context, maps, stream)
+                      : launch_atoms<2, false>(p, *context, maps, stream);
 }
 
 } // namespace cuvit::attn

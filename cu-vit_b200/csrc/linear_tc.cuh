@@ -7,6 +7,11 @@
 // Rows that TMA cannot describe (a row distance that is no multiple of 16 bytes: 3420 bfloat16
 // columns) move between global memory and the slab with the widest vectors their alignment allows,
 // consecutive lanes on consecutive bytes of a row.
+//
+// 50432 x 768 x 768 bfloat16: 51.1 us without any of it (a library product: 50.1), bias 52.5, bias and
+// scale 55.0, with the residual 62.7; 16411 x 3420 x 1280 gated SiLU 205 us, 1400 TFLOP/s. (A second
+// slab per warp, with the next chunk of the residual on its way while one is added, in place of one
+// of six operand stages: 64.2 us.)
 #pragma once
 
 #include "activation.cuh"

@@ -292,6 +292,9 @@ int run(const void* x, const void* weight, const float* bias, const float* scale
     if (c.math == CUVIT_MATH_FP32 && launch_split(p, *context, stream, &result)) {
         return result;
     }
+    if (bf16 && p.k > 0 && launch_slices(p, *context, stream, &result)) {
+        return result;
+    }
     TcPlan plan;
     if (c.math != CUVIT_MATH_FP32 && prepare(p, c.math, *context, &plan)) {
         return bf16 ? launch_tc_bf16(plan, stream) : launch_tc_tf32(plan, stream);

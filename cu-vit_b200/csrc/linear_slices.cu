@@ -1,0 +1,343 @@
+// bfloat16 linear layers with too few output tiles to fill the GPU (a few hundred rows and fewer):
+// a cluster of 2, 4 or 8 CTAs shares a tile, each going through its slice of k, and adds up the
+// slices over distributed shared memory.
+//
+// Bound by latency: with one CTA per tile, 64 columns of a weight of 4096 x 4096 come through one
+// SM's copies, 64 steps of about 0.25 us. Divided, every SM streams its part of the weight. Each
+// CTA's sums leave tensor memory for the CTA that owns their columns, which adds the slices in the
+// order of k, in FP32, and finishes its columns (bias, activation, gate, scale, residual, rounding).
+// %PERF%
+//
+//   warp 0      copies (TMA) into a ring of stages
+//   warp 1      issues the products
+//   warp 2      tensor memory
+//   warps 4-7   hand the sums out (a row per thread); then all warps finish the owned columns
+#include "activation.cuh"
+#include "linear.hpp"
+#include "ptx.cuh"
+
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+namespace cuvit::linear {
+namespace {
+
+constexpr int kBlockM = 128;
+constexpr int kBlockN = 64; // accumulator columns: of a gated layer 32 gate and 32 up
+constexpr int kBlockK = 64; // 128 bytes of a row
+constexpr int kRowBytes = 128;
+constexpr int kThreads = 256;
+constexpr int kHandOut = 4; // the first of four warps that read tensor memory
+constexpr int kMaxStages = 16;
+constexpr int kMaxSlices = 8;
+constexpr int kMinSteps = 4; // of k in a slice
+
+// A stage holds the rows of x that there are, then 64 of the weight. The products read 128 rows of x
+// all the same: what follows in shared memory makes rows of the sums that nobody reads.
+constexpr int kWBytes = kBlockN * kRowBytes;
+constexpr int kRingBytes = 6 * (kBlockM * kRowBytes + kWBytes);
+constexpr int kPartOffset = kRingBytes;
+// The owned columns' sums of every slice: rows of kBlockN / slices floats and one vector between
+// rows, so that neighbouring rows fall in different banks.
+constexpr int kPartBytes = 4 * kBlockM * (kBlockN + 4 * kMaxSlices);
+constexpr int kBarrierOffset = kPartOffset + kPartBytes;
+constexpr int kBarriers = 2 * kMaxStages + 2;
+constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 8;
+static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
+static_assert(kPartBytes >= kBlockM * kRowBytes, "the last stage's reads of x stay inside");
+
+struct SliceParams : OutRows {
+    int out_columns; // of a tile: kBlockN, or half of it for a gated layer
+    int n_tiles, k_blocks;
+    int slices;
+    int x_rows; // rows of x a stage holds
+    int stages;
+    unsigned* status;
+};
+
+__device__ __forceinline__ void store_remote(uint32_t at, const float (&v)[4]) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]),
+                 "f"(v[2]), "f"(v[3])
+                 : "memory");
+}
+
+__device__ __forceinline__ void add_columns(float (&v)[4], const float* vector, int col, int n) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] += col + j < n ? __ldg(vector + col + j) : 0.0F;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_slices_kernel(const __grid_constant__ CUtensorMap map_x,
+                         const __grid_constant__ CUtensorMap map_w,
+                         const __grid_constant__ SliceParams s) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = dev::smem_u32(smem_raw);
+    const uint32_t base = (raw_base + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - raw_base);
+    const uint32_t bars = base + kBarrierOffset;
+    const auto full = [&](int i) -> uint32_t { return bars + 8u * i; };
+    const auto empty = [&](int i) -> uint32_t { return bars + 8u * (kMaxStages + i); };
+    const uint32_t sums_full = bars + 8u * 2 * kMaxStages;
+    const uint32_t drain_bar = sums_full + 8u;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarrierOffset + 8 * kBarriers);
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < s.stages; ++i) {
+            dev::mbar_init(full(i), 1);
+            dev::mbar_init(empty(i), 1);
+        }
+        dev::mbar_init(sums_full, 1);
+        dev::mbar_init(drain_bar, 1);
+        dev::fence_barrier_init();
+    }
+    if (warp == 2) {
+        dev::tmem_alloc(dev::smem_u32(tmem_slot), kBlockN);
+        dev::tmem_relinquish();
+    }
+    dev::tc_fence_before();
+    __syncthreads();
+    dev::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    dev::cluster_sync(); // every CTA of the cluster runs before any writes to another's memory
+    dev::grid_dependency_wait();
+    dev::grid_launch_dependents();
+
+    const Params& p = s.p;
+    const int rank = static_cast<int>(dev::cluster_ctarank());
+    const int tile = static_cast<int>(blockIdx.x) / s.slices;
+    const int m_block = tile / s.n_tiles;
+    const int col0 = (tile - m_block * s.n_tiles) * s.out_columns;
+    const int first = static_cast<int>(static_cast<long long>(s.k_blocks) * rank / s.slices);
+    const int end = static_cast<int>(static_cast<long long>(s.k_blocks) * (rank + 1) / s.slices);
+    const int owned = s.out_columns / s.slices; // columns of the output that a CTA finishes
+    const int pitch = kBlockN / s.slices + 4;   // floats
+    const int x_bytes = s.x_rows * kRowBytes;
+    const int stage_bytes = x_bytes + kWBytes;
+
+    if (warp == 0 && lane == 0) {
+        // ---------------- copies ----------------
+        dev::tma_prefetch_descriptor(&map_x);
+        dev::tma_prefetch_descriptor(&map_w);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = first; kb < end; ++kb) {
+            ok = dev::mbar_wait(empty(stage), phase ^ 1u, s.status);
+            if (!ok) {
+                break;
+            }
+            dev::mbar_arrive_expect_tx(full(stage), stage_bytes);
+            const uint32_t at = base + stage * stage_bytes;
+            const int cw[2] = {kb * kBlockK, col0};
+            dev::tma_load(at + x_bytes, &map_w, full(stage), 2, cw);
+            if (p.gated) {
+                const int cu[2] = {kb * kBlockK, p.n + col0};
+                dev::tma_load(at + x_bytes + kWBytes / 2, &map_w, full(stage), 2, cu);
+            }
+            const int cx[2] = {kb * kBlockK, m_block * kBlockM};
+            dev::tma_load(at, &map_x, full(stage), 2, cx);
+            if (++stage == s.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (!ok) {
+            // Every load issued lands before the CTA exits.
+            for (int i = 0; i < s.stages; ++i) {
+                dev::mbar_drain_wait(full(i), phase ^ (i < stage ? 0u : 1u));
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- products: the warp stays together, one lane issues ----------------
+        const uint32_t idesc = dev::make_idesc(1u, kBlockM, kBlockN, false, false);
+        const uint32_t base0 = __shfl_sync(0xFFFFFFFFu, base, 0);
+        const uint32_t tmem0 = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = first; kb < end; ++kb) {
+            ok = dev::mbar_wait_warp(full(stage), phase, s.status);
+            if (!ok) {
+                break;
+            }
+            dev::tc_fence_after();
+            const uint64_t x = dev::smem_desc_sw128(base0 + stage * stage_bytes, 16, 1024);
+            const uint64_t w =
+                dev::smem_desc_sw128(base0 + stage * stage_bytes + x_bytes, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < kBlockK / 16; ++kk) { // 32 bytes on: 2 in a descriptor
+                dev::mma_ss_f16_warp(tmem0, x + 2 * kk, w + 2 * kk, idesc,
+                                     kb > first || kk > 0 ? 1u : 0u);
+            }
+            dev::tc_commit_warp(empty(stage));
+            if (++stage == s.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (ok) {
+            dev::tc_commit_warp(sums_full);
+        } else {
+            // No product still reads or writes when the CTA ends.
+            dev::tc_commit_warp(drain_bar);
+            dev::mbar_drain_wait(drain_bar, 0);
+        }
+    } else if (warp >= kHandOut) {
+        // ---------------- sums to their columns' owners ----------------
+        const int quarter = warp & 3;
+        const int row = quarter * 32 + lane;
+        if (dev::mbar_wait_warp(sums_full, 0, s.status)) {
+            dev::tc_fence_after();
+            const uint32_t from = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+            // This slice's rows in an owner's memory.
+            const uint32_t part = base + kPartOffset + 4u * ((rank * kBlockM + row) * pitch);
+#pragma unroll 1
+            for (int c = 0; c < kBlockN; c += 16) {
+                uint32_t raw[16];
+                dev::tmem_load_16(from + c, raw);
+                dev::tmem_wait_load();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int column = c + 4 * q; // gate and up columns of one output go together
+                    const bool up = p.gated && column >= kBlockN / 2;
+                    const int output = up ? column - kBlockN / 2 : column;
+                    const int owner = output / owned;
+                    const int at = output - owner * owned + (up ? owned : 0);
+                    const float four[4] = {
+                        __uint_as_float(raw[4 * q]), __uint_as_float(raw[4 * q + 1]),
+                        __uint_as_float(raw[4 * q + 2]), __uint_as_float(raw[4 * q + 3])};
+                    store_remote(dev::map_to_rank(part + 4u * at, owner), four);
+                }
+            }
+            dev::tc_fence_before();
+        }
+    }
+    __syncwarp();
+    dev::cluster_sync(); // all slices are here
+
+    // ---------------- the owned columns ----------------
+    const float* const parts = reinterpret_cast<const float*>(smem + kPartOffset);
+    const int vectors = owned / 4;
+    const auto sum_of = [&](int row, int at, float (&v)[4]) {
+        v[0] = v[1] = v[2] = v[3] = 0.0F;
+        for (int r = 0; r < s.slices; ++r) { // in the order of k
+            const float4 slice = *reinterpret_cast<const float4*>(
+                parts + (r * kBlockM + row) * pitch + at);
+            v[0] += slice.x;
+            v[1] += slice.y;
+            v[2] += slice.z;
+            v[3] += slice.w;
+        }
+    };
+    const int rows = min(kBlockM, p.m - m_block * kBlockM);
+    for (int i = threadIdx.x; i < rows * vectors; i += kThreads) {
+        const int row = i / vectors;
+        const int at = 4 * (i - row * vectors);
+        const int col = col0 + rank * owned + at;
+        const int valid = min(4, p.n - col);
+        if (valid <= 0) {
+            continue;
+        }
+        float v[4];
+        sum_of(row, at, v);
+        if (p.bias != nullptr) {
+            add_columns(v, p.bias, col, p.n);
+        }
+        if (p.out_kind == CUVIT_DTYPE_BF16) {
+            dev::activate<true>(p.activation, v);
+        } else {
+            dev::activate<false>(p.activation, v);
+        }
+        if (p.gated) {
+            float up[4];
+            sum_of(row, owned + at, up);
+            if (p.bias != nullptr) {
+                add_columns(up, p.bias + p.n, col, p.n);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] *= up[j];
+            }
+        }
+        if (p.scale != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] *= j < valid ? __ldg(p.scale + col + j) : 0.0F;
+            }
+        }
+        write_four(s, static_cast<long long>(m_block) * kBlockM + row, col, v, valid);
+    }
+
+    dev::tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        dev::tc_fence_after();
+        dev::tmem_dealloc(tmem, kBlockN);
+    }
+}
+
+} // namespace
+
+bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStream_t stream,
+                   int* result) {
+    if (!host::is_blackwell(context)) {
+        return false;
+    }
+    SliceParams s{};
+    s.p = p;
+    s.out_columns = p.gated ? kBlockN / 2 : kBlockN;
+    const long long row_blocks = (p.m + kBlockM - 1LL) / kBlockM;
+    const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
+    const long long tiles = row_blocks * n_tiles;
+    s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
+    // Slices while the GPU has SMs for them and each has steps enough to be worth its start.
+    s.slices = 1;
+    while (s.slices < kMaxSlices && tiles * s.slices * 2 <= context.sm_count &&
+           s.k_blocks >= kMinSteps * s.slices * 2) {
+        s.slices *= 2;
+    }
+    if (s.slices == 1) {
+        return false;
+    }
+    s.n_tiles = static_cast<int>(n_tiles);
+    s.x_rows = p.m < kBlockM ? (p.m + 7) / 8 * 8 : kBlockM;
+    const int stages = kRingBytes / (s.x_rows * kRowBytes + kWBytes);
+    s.stages = stages < kMaxStages ? stages : kMaxStages;
+    CUtensorMap map_x, map_w;
+    if (!describe(p.x, true, p.k, p.m, p.ldx, s.x_rows, &map_x) ||
+        !describe(p.w, true, p.k, p.n * (p.gated ? 2LL : 1LL), p.ldw, s.out_columns, &map_w)) {
+        return false;
+    }
+    const int out_bytes = p.out_kind == CUVIT_DTYPE_BF16 ? 2 : 4;
+    s.out_vector = access_bytes(p.out, p.ldo * out_bytes);
+    s.residual_vector = p.residual != nullptr ? access_bytes(p.residual, p.ldr * out_bytes) : 16;
+    s.status = context.status;
+    const auto start = [&]() -> int {
+        CUVIT_TRY_CUDA(host::allow_dynamic_smem(
+            reinterpret_cast<const void*>(&linear_slices_kernel), kSmemBytes));
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(static_cast<unsigned>(tiles * s.slices));
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = kSmemBytes;
+        config.stream = stream;
+        cudaLaunchAttribute attributes[2]{};
+        attributes[0].id = cudaLaunchAttributeClusterDimension;
+        attributes[0].val.clusterDim.x = static_cast<unsigned>(s.slices);
+        attributes[0].val.clusterDim.y = 1;
+        attributes[0].val.clusterDim.z = 1;
+        attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[1].val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = attributes;
+        config.numAttrs = host::pdl_enabled() ? 2 : 1;
+        cudaLaunchKernelEx(&config, &linear_slices_kernel, map_x, map_w, s);
+        return host::after_launch("linear_slices_kernel");
+    };
+    *result = start();
+    return true;
+}
+
+} // namespace cuvit::linear

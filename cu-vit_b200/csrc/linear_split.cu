@@ -76,13 +76,10 @@ constexpr int kTmemX = 2 * kSumPitch;
 constexpr int kTmemColumns = 512;
 static_assert(kMaxN <= kSumPitch && kTmemX + kSplit * 2 * kBlockK <= kTmemColumns, "tensor memory");
 
-struct SplitParams {
-    Params p;
+struct SplitParams : OutRows {
     int block_n;     // columns of the accumulator
     int out_columns; // block_n, or half of it for a gated layer
     int n_tiles, k_blocks, total_tiles;
-    int out_vector;      // bytes per access of out's rows
-    int residual_vector; // of the residual's
     int columns_ok;      // bias and scale are 16-byte aligned
     unsigned* status;
 };
@@ -133,82 +130,6 @@ __device__ __forceinline__ void activate_group(int activation, float (&v)[kGroup
         break;
     default:
         break;
-    }
-}
-
-// Four neighbouring outputs of a row, `valid` of them inside it: adds the residual, rounds and
-// stores.
-__device__ __forceinline__ void write_four(const SplitParams& s, long long row, int col,
-                                           const float4& sums, int valid) {
-    const Params& p = s.p;
-    float v[4] = {sums.x, sums.y, sums.z, sums.w};
-    if (p.out_kind == CUVIT_DTYPE_BF16) {
-        const __nv_bfloat16* const res = static_cast<const __nv_bfloat16*>(p.residual);
-        __nv_bfloat16* const out = static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col;
-        if (res != nullptr) {
-            const __nv_bfloat16* const from = res + row * p.ldr + col;
-            if (valid == 4 && s.residual_vector >= 8) {
-                const uint2 old = *reinterpret_cast<const uint2*>(from);
-                v[0] += __uint_as_float(old.x << 16);
-                v[1] += __uint_as_float(old.x & 0xFFFF0000u);
-                v[2] += __uint_as_float(old.y << 16);
-                v[3] += __uint_as_float(old.y & 0xFFFF0000u);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j < valid) {
-                        v[j] += __bfloat162float(from[j]);
-                    }
-                }
-            }
-        }
-        if (valid == 4 && s.out_vector >= 8) {
-            *reinterpret_cast<uint2*>(out) =
-                make_uint2(dev::pack_bf16x2(v[0], v[1]), dev::pack_bf16x2(v[2], v[3]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < valid) {
-                    out[j] = __float2bfloat16_rn(v[j]);
-                }
-            }
-        }
-    } else {
-        const float* const res = static_cast<const float*>(p.residual);
-        float* const out = static_cast<float*>(p.out) + row * p.ldo + col;
-        if (res != nullptr) {
-            const float* const from = res + row * p.ldr + col;
-            if (valid == 4 && s.residual_vector >= 16) {
-                const float4 old = *reinterpret_cast<const float4*>(from);
-                v[0] += old.x;
-                v[1] += old.y;
-                v[2] += old.z;
-                v[3] += old.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j < valid) {
-                        v[j] += from[j];
-                    }
-                }
-            }
-        }
-        if (p.out_kind == CUVIT_DTYPE_TF32) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = dev::round_to_tf32(v[j]);
-            }
-        }
-        if (valid == 4 && s.out_vector >= 16) {
-            *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j < valid) {
-                    out[j] = v[j];
-                }
-            }
-        }
     }
 }
 
@@ -475,8 +396,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < kSlabRows / 8; ++i) {
                         const int r = 8 * i + lane / 4;
                         const int c = 4 * (lane % 4);
-                        const float4 four =
+                        const float4 sums =
                             *reinterpret_cast<const float4*>(slab + r * kSlabPitch + c);
+                        const float four[4] = {sums.x, sums.y, sums.z, sums.w};
                         const int row = row0 + half * kSlabRows + r;
                         const int valid = min(4, p.n - col0 - c);
                         if (row < p.m && valid > 0) {

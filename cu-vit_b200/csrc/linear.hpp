@@ -6,7 +6,11 @@
 #include "linear_tc.cuh"
 #include "runtime.hpp"
 
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <cstdint>
+#include <utility>
 
 namespace cuvit::linear {
 
@@ -131,6 +135,101 @@ __device__ __forceinline__ void write_four(const OutRows& s, long long row, int 
             }
         }
     }
+}
+
+// ---- slices of k: a cluster's CTAs share a tile and add up their sums ------------------------
+
+__device__ __forceinline__ void store_remote(uint32_t at, const float (&v)[4]) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]),
+                 "f"(v[2]), "f"(v[3])
+                 : "memory");
+}
+
+// Four columns' sums of every slice, `distance` floats apart, in the order of k.
+__device__ __forceinline__ void sum_slices(const float* from, int slices, int distance,
+                                           float (&v)[4]) {
+    v[0] = v[1] = v[2] = v[3] = 0.0F;
+    for (int r = 0; r < slices; ++r) {
+        const float4 slice = *reinterpret_cast<const float4*>(from + r * distance);
+        v[0] += slice.x;
+        v[1] += slice.y;
+        v[2] += slice.z;
+        v[3] += slice.w;
+    }
+}
+
+// Four neighbouring outputs from their sums: sum(at, v) gives the four of (gate) column `at` of the
+// tile, `up_at` the ones that multiply them.
+template <class Sum>
+__device__ __forceinline__ void finish_four(const OutRows& s, long long row, int col, int at,
+                                            int up_at, Sum&& sum) {
+    const Params& p = s.p;
+    const int valid = min(4, p.n - col);
+    if (valid <= 0) {
+        return;
+    }
+    const auto add_columns = [&](float(&v)[4], const float* vector) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] += j < valid ? __ldg(vector + col + j) : 0.0F;
+        }
+    };
+    float v[4];
+    sum(at, v);
+    if (p.bias != nullptr) {
+        add_columns(v, p.bias);
+    }
+    if (p.out_kind == CUVIT_DTYPE_BF16) {
+        dev::activate<true>(p.activation, v);
+    } else {
+        dev::activate<false>(p.activation, v);
+    }
+    if (p.gated) {
+        float up[4];
+        sum(up_at, up);
+        if (p.bias != nullptr) {
+            add_columns(up, p.bias + p.n);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] *= up[j];
+        }
+    }
+    if (p.scale != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] *= j < valid ? __ldg(p.scale + col + j) : 0.0F;
+        }
+    }
+    write_four(s, row, col, v, valid);
+}
+
+// A launch in clusters of `size` CTAs (1: without).
+template <class... KernelArgs, class... Args>
+void launch_cluster(void (*kernel)(KernelArgs...), int size, unsigned blocks, int threads,
+                    size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks);
+    config.blockDim = dim3(static_cast<unsigned>(threads));
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2]{};
+    int count = 0;
+    if (size > 1) {
+        attributes[count].id = cudaLaunchAttributeClusterDimension;
+        attributes[count].val.clusterDim.x = static_cast<unsigned>(size);
+        attributes[count].val.clusterDim.y = 1;
+        attributes[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    if (host::pdl_enabled()) {
+        attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[count].val.programmaticStreamSerializationAllowed = 1;
+        ++count;
+    }
+    config.attrs = attributes;
+    config.numAttrs = static_cast<unsigned>(count);
+    cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...);
 }
 
 // A few rows (linear_rows.cu).

@@ -6,7 +6,10 @@
 // SM's copies, 64 steps of about 0.25 us. Divided, every SM streams its part of the weight. Each
 // CTA's sums leave tensor memory for the CTA that owns their columns, which adds the slices in the
 // order of k, in FP32, and finishes its columns (bias, activation, gate, scale, residual, rounding).
-// %PERF%
+//
+// 16 x 4096 x 4096: 18.5 us (28.7 with one CTA per tile, 20.5 with six stages of fixed size: what is in
+// flight bounds it, so a stage holds only the rows of x that there are); 64 x 1280 x 1280 12.2 us
+// (16.4), of which about 8 are launch, exchange and end.
 //
 //   warp 0      copies (TMA) into a ring of stages
 //   warp 1      issues the products
@@ -55,19 +58,6 @@ struct SliceParams : OutRows {
     int stages;
     unsigned* status;
 };
-
-__device__ __forceinline__ void store_remote(uint32_t at, const float (&v)[4]) {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[0]), "f"(v[1]),
-                 "f"(v[2]), "f"(v[3])
-                 : "memory");
-}
-
-__device__ __forceinline__ void add_columns(float (&v)[4], const float* vector, int col, int n) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[j] += col + j < n ? __ldg(vector + col + j) : 0.0F;
-    }
-}
 
 __global__ void __launch_bounds__(kThreads, 1)
     linear_slices_kernel(const __grid_constant__ CUtensorMap map_x,
@@ -222,54 +212,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- the owned columns ----------------
     const float* const parts = reinterpret_cast<const float*>(smem + kPartOffset);
     const int vectors = owned / 4;
-    const auto sum_of = [&](int row, int at, float (&v)[4]) {
-        v[0] = v[1] = v[2] = v[3] = 0.0F;
-        for (int r = 0; r < s.slices; ++r) { // in the order of k
-            const float4 slice = *reinterpret_cast<const float4*>(
-                parts + (r * kBlockM + row) * pitch + at);
-            v[0] += slice.x;
-            v[1] += slice.y;
-            v[2] += slice.z;
-            v[3] += slice.w;
-        }
-    };
     const int rows = min(kBlockM, p.m - m_block * kBlockM);
     for (int i = threadIdx.x; i < rows * vectors; i += kThreads) {
         const int row = i / vectors;
         const int at = 4 * (i - row * vectors);
-        const int col = col0 + rank * owned + at;
-        const int valid = min(4, p.n - col);
-        if (valid <= 0) {
-            continue;
-        }
-        float v[4];
-        sum_of(row, at, v);
-        if (p.bias != nullptr) {
-            add_columns(v, p.bias, col, p.n);
-        }
-        if (p.out_kind == CUVIT_DTYPE_BF16) {
-            dev::activate<true>(p.activation, v);
-        } else {
-            dev::activate<false>(p.activation, v);
-        }
-        if (p.gated) {
-            float up[4];
-            sum_of(row, owned + at, up);
-            if (p.bias != nullptr) {
-                add_columns(up, p.bias + p.n, col, p.n);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] *= up[j];
-            }
-        }
-        if (p.scale != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] *= j < valid ? __ldg(p.scale + col + j) : 0.0F;
-            }
-        }
-        write_four(s, static_cast<long long>(m_block) * kBlockM + row, col, v, valid);
+        finish_four(s, static_cast<long long>(m_block) * kBlockM + row, col0 + rank * owned + at, at,
+                    owned + at, [&](int from, float(&v)[4]) {
+                        sum_slices(parts + row * pitch + from, s.slices, kBlockM * pitch, v);
+                    });
     }
 
     dev::tc_fence_before();
@@ -319,21 +269,8 @@ bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStre
     const auto start = [&]() -> int {
         CUVIT_TRY_CUDA(host::allow_dynamic_smem(
             reinterpret_cast<const void*>(&linear_slices_kernel), kSmemBytes));
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(static_cast<unsigned>(tiles * s.slices));
-        config.blockDim = dim3(kThreads);
-        config.dynamicSmemBytes = kSmemBytes;
-        config.stream = stream;
-        cudaLaunchAttribute attributes[2]{};
-        attributes[0].id = cudaLaunchAttributeClusterDimension;
-        attributes[0].val.clusterDim.x = static_cast<unsigned>(s.slices);
-        attributes[0].val.clusterDim.y = 1;
-        attributes[0].val.clusterDim.z = 1;
-        attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attributes[1].val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = attributes;
-        config.numAttrs = host::pdl_enabled() ? 2 : 1;
-        cudaLaunchKernelEx(&config, &linear_slices_kernel, map_x, map_w, s);
+        launch_cluster(&linear_slices_kernel, s.slices, static_cast<unsigned>(tiles * s.slices),
+                       kThreads, kSmemBytes, stream, map_x, map_w, s);
         return host::after_launch("linear_slices_kernel");
     };
     *result = start();

@@ -17,6 +17,9 @@
 // bound is the splitting warps' latency (without the weight's splitting a quarter less); more of
 // them (8 for the weight) leave the draining warps too few registers and take 15 % longer.
 //
+// Where the tiles do not fill the GPU, a cluster's CTAs share one, each with a slice of k; their sums
+// meet in the memory of the CTA that owns the row, in the order of k.
+//
 //   warp 0        copies (TMA) into rings of kX and kW stages
 //   warp 1        issues the products
 //   warp 2        tensor memory
@@ -65,6 +68,12 @@ constexpr int kSlabOffset = kLowOffset + kSplit * kWBytes;
 constexpr int kSlabRows = 16;          // of a warp's 32 at a time
 constexpr int kSlabPitch = kGroup + 4; // floats; rows' 16-byte accesses fall in different banks
 constexpr int kSlabBytes = kSlabRows * kSlabPitch * 4;
+// Slices' sums, in the stages' place: rows of the tile's columns and a vector, so that neighbouring
+// rows fall in different banks.
+constexpr int kPartPad = 4;
+static_assert(4 * kBlockM * (kMaxN + kPartPad) <= kSlabOffset, "the slices' sums fit the stages");
+constexpr int kMaxSlices = 8;
+constexpr int kMinSteps = 4; // of k in a slice
 constexpr int kBarrierOffset = kSlabOffset + kDrainWarps * kSlabBytes;
 constexpr int kBarriers = 2 * kX + 2 * kW + 2 * kSplit + 4 + 1;
 constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 8;
@@ -77,6 +86,7 @@ constexpr int kTmemColumns = 512;
 static_assert(kMaxN <= kSumPitch && kTmemX + kSplit * 2 * kBlockK <= kTmemColumns, "tensor memory");
 
 struct SplitParams : OutRows {
+    int slices;      // CTAs of a cluster that share a tile, each with its part of k
     int block_n;     // columns of the accumulator
     int out_columns; // block_n, or half of it for a gated layer
     int n_tiles, k_blocks, total_tiles;
@@ -192,10 +202,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev::grid_launch_dependents();
 
     const Params& p = s.p;
-    const int my_tiles = (s.total_tiles - static_cast<int>(blockIdx.x) +
-                          static_cast<int>(gridDim.x) - 1) /
-                         static_cast<int>(gridDim.x);
-    const int steps = my_tiles * s.k_blocks; // k blocks of all this CTA's tiles (host: in 31 bits)
+    const int slice = s.slices > 1 ? static_cast<int>(dev::cluster_ctarank()) : 0;
+    const int tile0 = static_cast<int>(blockIdx.x) / s.slices;
+    const int tile_step = static_cast<int>(gridDim.x) / s.slices;
+    const int k_first = static_cast<int>(static_cast<long long>(s.k_blocks) * slice / s.slices);
+    const int k_end = static_cast<int>(static_cast<long long>(s.k_blocks) * (slice + 1) / s.slices);
+    const int k_blocks = k_end - k_first; // of this CTA
+    const int my_tiles = (s.total_tiles - tile0 + tile_step - 1) / tile_step;
+    const int steps = my_tiles * k_blocks; // k blocks of all this CTA's tiles (host: in 31 bits)
 
     if (warp == 0 && lane == 0) {
         // ---------------- copies ----------------
@@ -204,11 +218,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         int xs = 0, ws = 0;
         uint32_t x_phase = 0, w_phase = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < s.total_tiles && ok; tile += gridDim.x) {
+        for (int tile = tile0; tile < s.total_tiles && ok; tile += tile_step) {
             const int m_block = tile / s.n_tiles;
             const int n_block = tile - m_block * s.n_tiles;
             const int col = n_block * s.out_columns;
-            for (int kb = 0; kb < s.k_blocks; ++kb) {
+            for (int kb = k_first; kb < k_end; ++kb) {
                 if (!dev::mbar_wait(w_empty(ws), w_phase ^ 1u, s.status)) {
                     ok = false;
                     break;
@@ -256,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t split_phase = 0, acc_phase = 0;
         bool ok = true;
         for (int tile = 0; tile < my_tiles && ok; ++tile) {
-            for (int kb = 0; kb < s.k_blocks; ++kb) {
+            for (int kb = 0; kb < k_blocks; ++kb) {
                 const uint32_t sums = tmem0 + acc * kSumPitch;
                 const bool first = kb % kChunk == 0;
                 if ((first && !dev::mbar_wait_warp(acc_empty(acc), acc_phase ^ 1u, s.status)) ||
@@ -279,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 dev::tc_commit_warp(w_empty(ws));
                 dev::tc_commit_warp(split_empty(split));
-                if (kb % kChunk == kChunk - 1 || kb == s.k_blocks - 1) {
+                if (kb % kChunk == kChunk - 1 || kb == k_blocks - 1) {
                     dev::tc_commit_warp(acc_full(acc));
                     acc ^= 1;
                     acc_phase ^= acc == 0 ? 1u : 0u;
@@ -313,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < s.total_tiles && ok; tile += gridDim.x) {
+        for (int tile = tile0; tile < s.total_tiles && ok; tile += tile_step) {
             float v[kGroups][kGroup];
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
@@ -322,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     v[g][j] = 0.0F;
                 }
             }
-            for (int kb = 0; kb < s.k_blocks; kb += kChunk) {
+            for (int kb = 0; kb < k_blocks; kb += kChunk) {
                 if (!dev::mbar_wait_warp(acc_full(acc), acc_phase, s.status)) {
                     ok = false;
                     break;
@@ -348,6 +362,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 acc ^= 1;
                 acc_phase ^= acc == 0 ? 1u : 0u;
+            }
+            if (s.slices > 1) {
+                // The only tile: its sums go to the CTA that owns the row, into the stages' place.
+                dev::cluster_sync(); // no CTA's stages are in use any more
+                const int row = quarter * 32 + lane;
+                const int owned = kBlockM / s.slices;
+                const int owner = row / owned;
+                const uint32_t part =
+                    dev::map_to_rank(base, owner) +
+                    4u * ((slice * owned + row - owner * owned) * (s.block_n + kPartPad));
+                const bool live = ok && tile / s.n_tiles * kBlockM + row < p.m;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+#pragma unroll
+                    for (int q = 0; q < kGroup / 4; ++q) {
+                        if (g < count && live) {
+                            const float four[4] = {v[g][4 * q], v[g][4 * q + 1], v[g][4 * q + 2],
+                                                   v[g][4 * q + 3]};
+                            store_remote(part + 4u * (from0 + g * from_step + 4 * q), four);
+                        }
+                    }
+                }
+                break;
             }
             if (!ok) {
                 break;
@@ -543,6 +580,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     __syncwarp(); // lanes of the copying and issuing warps come together
+    if (s.slices > 1) {
+        if (warp < kDrainWarp || warp >= kSplitXWarp) {
+            dev::cluster_sync(); // the draining warps' first
+        }
+        __syncwarp();
+        dev::cluster_sync(); // all slices are here
+        const float* const parts = reinterpret_cast<const float*>(smem);
+        const int owned = kBlockM / s.slices;
+        const int pitch = s.block_n + kPartPad;
+        const int vectors = s.out_columns / 4;
+        const int m_block = tile0 / s.n_tiles;
+        const int col0 = (tile0 - m_block * s.n_tiles) * s.out_columns;
+        const int row0 = m_block * kBlockM + slice * owned;
+        const int rows = min(owned, p.m - row0);
+        for (int i = threadIdx.x; i < rows * vectors; i += kThreads) {
+            const int row = i / vectors;
+            const int at = 4 * (i - row * vectors);
+            finish_four(s, row0 + static_cast<long long>(row), col0 + at, at, s.out_columns + at,
+                        [&](int from, float(&v)[4]) {
+                            sum_slices(parts + row * pitch + from, s.slices, owned * pitch, v);
+                        });
+        }
+    }
     dev::tc_fence_before();
     __syncthreads();
     if (warp == 2) {
@@ -551,22 +611,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Columns of a tile: the width whose waves cost least, a tile's 32 of k taking the shared-memory
-// cycles counted above (256 for x, 7 per column). 1576 x 1536 outputs: 143 tiles of 144 columns,
-// one wave, where 128 columns leave 156 tiles and a second wave of eight.
-int choose_columns(long long row_blocks, int n, bool gated, int sm_count) {
-    int best = 0;
+// Columns of a tile and slices of k: what takes least time, a tile's 32 of k taking the shared-memory
+// cycles counted above (256 for x, 7 per column), but 1200 at least, the length of the chain from
+// copies to products. 1576 x 1536 outputs: 143 tiles of 144 columns, one wave, where 128 columns
+// leave 156 tiles and a second wave of eight. 16 x 4096 with k = 4096: 32 tiles of 128 columns, 4
+// CTAs to each, 41 us (one to each of 128 tiles of 32 columns: 93).
+void choose_shape(long long row_blocks, int n, bool gated, int k_blocks, int sm_count, int* block_n,
+                  int* slices) {
     long long best_cost = 0;
+    *block_n = 0;
     for (int bn = gated ? kMaxGatedN : kMaxN; bn > 0; bn -= gated ? 32 : 16) {
         const int columns = gated ? bn / 2 : bn;
         const long long tiles = row_blocks * ((n + columns - 1LL) / columns);
-        const long long cost = (tiles + sm_count - 1) / sm_count * (256 + 7 * bn);
-        if (best == 0 || cost < best_cost) {
-            best = bn;
+        int parts = 1;
+        while (parts < kMaxSlices && tiles * parts * 2 <= sm_count &&
+               k_blocks >= kMinSteps * parts * 2) {
+            parts *= 2;
+        }
+        const long long step = 256 + 7 * bn > 1200 ? 256 + 7 * bn : 1200;
+        const long long waves = (tiles * parts + sm_count - 1) / sm_count;
+        // The exchange costs about as much as two steps.
+        const long long cost =
+            waves * ((k_blocks + parts - 1) / parts + (parts > 1 ? 2 : 0)) * step;
+        if (*block_n == 0 || cost < best_cost) {
+            *block_n = bn;
+            *slices = parts;
             best_cost = cost;
         }
     }
-    return best;
 }
 
 } // namespace
@@ -579,12 +651,12 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     const long long row_blocks = (p.m + kBlockM - 1LL) / kBlockM;
     SplitParams s{};
     s.p = p;
-    s.block_n = choose_columns(row_blocks, p.n, p.gated != 0, context.sm_count);
+    s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
+    choose_shape(row_blocks, p.n, p.gated != 0, s.k_blocks, context.sm_count, &s.block_n, &s.slices);
     s.out_columns = p.gated ? s.block_n / 2 : s.block_n;
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
     const long long total = row_blocks * n_tiles;
     s.n_tiles = static_cast<int>(n_tiles);
-    s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
     s.total_tiles = static_cast<int>(total);
     const long long tiles_each = (total + context.sm_count - 1) / context.sm_count;
     CUtensorMap map_x, map_w;
@@ -602,10 +674,10 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     const auto start = [&]() -> int {
         CUVIT_TRY_CUDA(host::allow_dynamic_smem(
             reinterpret_cast<const void*>(&linear_split_kernel), kSmemBytes));
-        host::pdl_launch(&linear_split_kernel,
-                         dim3(static_cast<unsigned>(total < context.sm_count ? total
-                                                                             : context.sm_count)),
-                         dim3(kThreads), kSmemBytes, stream, map_x, map_w, s);
+        const long long blocks =
+            s.slices > 1 ? total * s.slices : (total < context.sm_count ? total : context.sm_count);
+        launch_cluster(&linear_split_kernel, s.slices, static_cast<unsigned>(blocks), kThreads,
+                       kSmemBytes, stream, map_x, map_w, s);
         return host::after_launch("linear_split_kernel");
     };
     *result = start();

@@ -889,3 +889,30 @@ def test_linear_around_the_tiles(m, n, k, gated, kind, cuda):
     want, bound = linear_64(torch, x, w, bias, scale, residual, kernels.ACTIVATION_GELU, gated, kind,
                             kind, n)
     check(out, want, bound)
+
+
+@pytest.mark.parametrize("kind,out_kind", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32"),
+                                           ("f32", "bf16")])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("m,n,k", [(9, 1000, 4104), (16, 64, 512), (33, 200, 2048), (128, 31, 1024),
+                                   (130, 70, 1160), (197, 768, 3848), (300, 130, 520), (12, 9, 8192)])
+def test_linear_with_divided_k(m, n, k, gated, kind, out_kind, cuda):
+    """Few tiles and a long k: the CTAs of a cluster share a tile. Twice, bitwise the same."""
+    torch = cuda
+    x = normal(torch, (m, k), 1, kind)
+    w = normal(torch, ((2 if gated else 1) * n, k), 2, kind, k ** -0.5)
+    bias = normal(torch, (w.shape[0],), 3)
+    scale = normal(torch, (n,), 4)
+    residual = normal(torch, (m, n), 5, out_kind)
+    outs = [torch.full((m, n), float("nan"), dtype=torch_type(torch, out_kind), device="cuda")
+            for _ in range(2)]
+    math_mode = kernels.MATH_BF16 if kind == "bf16" else kernels.MATH_FP32
+    for out in outs:
+        kernels.launch_linear(x, w, bias, scale, residual, out,
+                              LinearProblem(m, n, k, math_mode, dtype_of(out_kind),
+                                            kernels.ACTIVATION_SILU, gated))
+    torch.cuda.synchronize()
+    want, bound = linear_64(torch, x, w, bias, scale, residual, kernels.ACTIVATION_SILU, gated, kind,
+                            out_kind, n)
+    check(outs[0], want, bound)
+    assert torch.equal(*outs)

@@ -204,6 +204,45 @@ __device__ __forceinline__ void finish_four(const OutRows& s, long long row, int
     write_four(s, row, col, v, valid);
 }
 
+// How many clusters of 1, 2, 4 and 8 CTAs of a kernel the current device holds at once (clusters do
+// not span its processor clusters, so less than the SMs would: 15 of 8, 33 of 4 on B200). Zeros where
+// that cannot be told.
+struct ClusterLimits {
+    int of[4] = {};
+};
+
+template <auto Kernel>
+ClusterLimits cluster_limits(int threads, size_t smem) {
+    constexpr auto* kernel = Kernel;
+    constexpr int kMaxDevices = 64;
+    static ClusterLimits limits[kMaxDevices];
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) {
+        return {};
+    }
+    const cudaError_t error = host::once_per_device(
+        reinterpret_cast<const void*>(kernel), [&](int current) {
+            cudaError_t status = cudaFuncSetAttribute(
+                kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            for (int i = 0; i < 4 && status == cudaSuccess; ++i) {
+                cudaLaunchAttribute attribute{};
+                attribute.id = cudaLaunchAttributeClusterDimension;
+                attribute.val.clusterDim.x = 1u << i;
+                attribute.val.clusterDim.y = 1;
+                attribute.val.clusterDim.z = 1;
+                cudaLaunchConfig_t probe{};
+                probe.gridDim = dim3(1u << i);
+                probe.blockDim = dim3(static_cast<unsigned>(threads));
+                probe.dynamicSmemBytes = smem;
+                probe.attrs = &attribute;
+                probe.numAttrs = 1;
+                status = cudaOccupancyMaxActiveClusters(&limits[current].of[i], kernel, &probe);
+            }
+            return status;
+        });
+    return error == cudaSuccess ? limits[device] : ClusterLimits{};
+}
+
 // A launch in clusters of `size` CTAs (1: without).
 template <class... KernelArgs, class... Args>
 void launch_cluster(void (*kernel)(KernelArgs...), int size, unsigned blocks, int threads,

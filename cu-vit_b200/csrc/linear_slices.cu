@@ -244,11 +244,15 @@ bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStre
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
     const long long tiles = row_blocks * n_tiles;
     s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
-    // Slices while the GPU has SMs for them and each has steps enough to be worth its start.
+    if (tiles * 2 > context.sm_count || s.k_blocks < kMinSteps * 2) {
+        return false;
+    }
+    // Slices while the GPU holds all clusters at once and each slice has steps enough to be worth its
+    // start.
+    const ClusterLimits limits = cluster_limits<&linear_slices_kernel>(kThreads, kSmemBytes);
     s.slices = 1;
-    while (s.slices < kMaxSlices && tiles * s.slices * 2 <= context.sm_count &&
-           s.k_blocks >= kMinSteps * s.slices * 2) {
-        s.slices *= 2;
+    for (int i = 1; i < 4 && tiles <= limits.of[i] && s.k_blocks >= kMinSteps << i; ++i) {
+        s.slices = 1 << i;
     }
     if (s.slices == 1) {
         return false;
@@ -267,8 +271,6 @@ bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStre
     s.residual_vector = p.residual != nullptr ? access_bytes(p.residual, p.ldr * out_bytes) : 16;
     s.status = context.status;
     const auto start = [&]() -> int {
-        CUVIT_TRY_CUDA(host::allow_dynamic_smem(
-            reinterpret_cast<const void*>(&linear_slices_kernel), kSmemBytes));
         launch_cluster(&linear_slices_kernel, s.slices, static_cast<unsigned>(tiles * s.slices),
                        kThreads, kSmemBytes, stream, map_x, map_w, s);
         return host::after_launch("linear_slices_kernel");

@@ -72,7 +72,6 @@ constexpr int kSlabBytes = kSlabRows * kSlabPitch * 4;
 // rows fall in different banks.
 constexpr int kPartPad = 4;
 static_assert(4 * kBlockM * (kMaxN + kPartPad) <= kSlabOffset, "the slices' sums fit the stages");
-constexpr int kMaxSlices = 8;
 constexpr int kMinSteps = 4; // of k in a slice
 constexpr int kBarrierOffset = kSlabOffset + kDrainWarps * kSlabBytes;
 constexpr int kBarriers = 2 * kX + 2 * kW + 2 * kSplit + 4 + 1;
@@ -616,17 +615,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 // copies to products. 1576 x 1536 outputs: 143 tiles of 144 columns, one wave, where 128 columns
 // leave 156 tiles and a second wave of eight. 16 x 4096 with k = 4096: 32 tiles of 128 columns, 4
 // CTAs to each, 41 us (one to each of 128 tiles of 32 columns: 93).
-void choose_shape(long long row_blocks, int n, bool gated, int k_blocks, int sm_count, int* block_n,
-                  int* slices) {
+void choose_shape(long long row_blocks, int n, bool gated, int k_blocks, int sm_count,
+                  const ClusterLimits& limits, int* block_n, int* slices) {
     long long best_cost = 0;
     *block_n = 0;
     for (int bn = gated ? kMaxGatedN : kMaxN; bn > 0; bn -= gated ? 32 : 16) {
         const int columns = gated ? bn / 2 : bn;
         const long long tiles = row_blocks * ((n + columns - 1LL) / columns);
         int parts = 1;
-        while (parts < kMaxSlices && tiles * parts * 2 <= sm_count &&
-               k_blocks >= kMinSteps * parts * 2) {
-            parts *= 2;
+        for (int i = 1; i < 4 && tiles <= limits.of[i] && k_blocks >= kMinSteps << i; ++i) {
+            parts = 1 << i;
         }
         const long long step = 256 + 7 * bn > 1200 ? 256 + 7 * bn : 1200;
         const long long waves = (tiles * parts + sm_count - 1) / sm_count;
@@ -652,7 +650,8 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     SplitParams s{};
     s.p = p;
     s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
-    choose_shape(row_blocks, p.n, p.gated != 0, s.k_blocks, context.sm_count, &s.block_n, &s.slices);
+    choose_shape(row_blocks, p.n, p.gated != 0, s.k_blocks, context.sm_count,
+                 cluster_limits<&linear_split_kernel>(kThreads, kSmemBytes), &s.block_n, &s.slices);
     s.out_columns = p.gated ? s.block_n / 2 : s.block_n;
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
     const long long total = row_blocks * n_tiles;
@@ -672,8 +671,6 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
                    reinterpret_cast<uintptr_t>(p.scale) % 16 == 0;
     s.status = context.status;
     const auto start = [&]() -> int {
-        CUVIT_TRY_CUDA(host::allow_dynamic_smem(
-            reinterpret_cast<const void*>(&linear_split_kernel), kSmemBytes));
         const long long blocks =
             s.slices > 1 ? total * s.slices : (total < context.sm_count ? total : context.sm_count);
         launch_cluster(&linear_split_kernel, s.slices, static_cast<unsigned>(blocks), kThreads,

@@ -142,6 +142,9 @@ __device__ __forceinline__ void activate_group(int activation, float (&v)[kGroup
     }
 }
 
+// Sliced: a cluster of s.slices CTAs to each tile. (One kernel for both spills more in the ordinary
+// case.)
+template <bool Sliced>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_split_kernel(const __grid_constant__ CUtensorMap map_x,
                         const __grid_constant__ CUtensorMap map_w,
@@ -201,11 +204,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev::grid_launch_dependents();
 
     const Params& p = s.p;
-    const int slice = s.slices > 1 ? static_cast<int>(dev::cluster_ctarank()) : 0;
-    const int tile0 = static_cast<int>(blockIdx.x) / s.slices;
-    const int tile_step = static_cast<int>(gridDim.x) / s.slices;
-    const int k_first = static_cast<int>(static_cast<long long>(s.k_blocks) * slice / s.slices);
-    const int k_end = static_cast<int>(static_cast<long long>(s.k_blocks) * (slice + 1) / s.slices);
+    const int slices = Sliced ? s.slices : 1;
+    const int slice = Sliced ? static_cast<int>(dev::cluster_ctarank()) : 0;
+    const int tile0 = static_cast<int>(blockIdx.x) / slices;
+    const int tile_step = static_cast<int>(gridDim.x) / slices;
+    const int k_first =
+        Sliced ? static_cast<int>(static_cast<long long>(s.k_blocks) * slice / slices) : 0;
+    const int k_end =
+        Sliced ? static_cast<int>(static_cast<long long>(s.k_blocks) * (slice + 1) / slices)
+               : s.k_blocks;
     const int k_blocks = k_end - k_first; // of this CTA
     const int my_tiles = (s.total_tiles - tile0 + tile_step - 1) / tile_step;
     const int steps = my_tiles * k_blocks; // k blocks of all this CTA's tiles (host: in 31 bits)
@@ -362,11 +369,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 acc ^= 1;
                 acc_phase ^= acc == 0 ? 1u : 0u;
             }
-            if (s.slices > 1) {
+            if constexpr (Sliced) {
                 // The only tile: its sums go to the CTA that owns the row, into the stages' place.
                 dev::cluster_sync(); // no CTA's stages are in use any more
                 const int row = quarter * 32 + lane;
-                const int owned = kBlockM / s.slices;
+                const int owned = kBlockM / slices;
                 const int owner = row / owned;
                 const uint32_t part =
                     dev::map_to_rank(base, owner) +
@@ -579,14 +586,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     __syncwarp(); // lanes of the copying and issuing warps come together
-    if (s.slices > 1) {
+    if constexpr (Sliced) {
         if (warp < kDrainWarp || warp >= kSplitXWarp) {
             dev::cluster_sync(); // the draining warps' first
         }
         __syncwarp();
         dev::cluster_sync(); // all slices are here
         const float* const parts = reinterpret_cast<const float*>(smem);
-        const int owned = kBlockM / s.slices;
+        const int owned = kBlockM / slices;
         const int pitch = s.block_n + kPartPad;
         const int vectors = s.out_columns / 4;
         const int m_block = tile0 / s.n_tiles;
@@ -598,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int at = 4 * (i - row * vectors);
             finish_four(s, row0 + static_cast<long long>(row), col0 + at, at, s.out_columns + at,
                         [&](int from, float(&v)[4]) {
-                            sum_slices(parts + row * pitch + from, s.slices, owned * pitch, v);
+                            sum_slices(parts + row * pitch + from, slices, owned * pitch, v);
                         });
         }
     }
@@ -651,7 +658,7 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     s.p = p;
     s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
     choose_shape(row_blocks, p.n, p.gated != 0, s.k_blocks, context.sm_count,
-                 cluster_limits<&linear_split_kernel>(kThreads, kSmemBytes), &s.block_n, &s.slices);
+                 cluster_limits<&linear_split_kernel<true>>(kThreads, kSmemBytes), &s.block_n, &s.slices);
     s.out_columns = p.gated ? s.block_n / 2 : s.block_n;
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
     const long long total = row_blocks * n_tiles;
@@ -673,8 +680,13 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     const auto start = [&]() -> int {
         const long long blocks =
             s.slices > 1 ? total * s.slices : (total < context.sm_count ? total : context.sm_count);
-        launch_cluster(&linear_split_kernel, s.slices, static_cast<unsigned>(blocks), kThreads,
-                       kSmemBytes, stream, map_x, map_w, s);
+        if (s.slices == 1) {
+            CUVIT_TRY_CUDA(host::allow_dynamic_smem(
+                reinterpret_cast<const void*>(&linear_split_kernel<false>), kSmemBytes));
+        }
+        launch_cluster(s.slices > 1 ? &linear_split_kernel<true> : &linear_split_kernel<false>,
+                       s.slices, static_cast<unsigned>(blocks), kThreads, kSmemBytes, stream, map_x,
+                       map_w, s);
         return host::after_launch("linear_split_kernel");
     };
     *result = start();

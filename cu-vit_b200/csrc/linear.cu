@@ -122,16 +122,19 @@ int launch_simt(const Params& p, cudaStream_t stream) {
     return host::after_launch("linear_simt_kernel");
 }
 
-// Plans a tensor-core launch; false where TMA cannot describe x or the weight, or k is 0.
-bool prepare(const Params& p, int math, const host::DeviceContext& context, TcPlan* plan) {
+// Plans a tensor-core launch, bfloat16 math in tiles of block_n accumulator columns; false where TMA
+// cannot describe x or the weight, or k is 0.
+bool prepare(const Params& p, int math, int block_n, const host::DeviceContext& context,
+             TcPlan* plan) {
     if (!host::is_blackwell(context) || p.k == 0) {
         return false;
     }
     const bool bf16 = math == CUVIT_MATH_BF16;
     const long long row_blocks = (p.m + gemm::kBlockM - 1LL) / gemm::kBlockM;
     const long long weight_rows = static_cast<long long>(p.n) * (p.gated ? 2 : 1);
-    int bn = gemm::choose_block_n(row_blocks, static_cast<int>(weight_rows), false, bf16,
-                                  context.sm_count);
+    int bn = bf16 ? block_n
+                  : gemm::choose_block_n(row_blocks, static_cast<int>(weight_rows), false, false,
+                                         context.sm_count);
     if (p.gated && bn < 128) {
         bn = 128; // a half tile's columns of one operand stay a whole 32-column step
     }
@@ -292,11 +295,13 @@ int run(const void* x, const void* weight, const float* bias, const float* scale
     if (c.math == CUVIT_MATH_FP32 && launch_split(p, *context, stream, &result)) {
         return result;
     }
-    if (bf16 && p.k > 0 && launch_slices(p, *context, stream, &result)) {
+    const TileChoice choice =
+        bf16 && p.k > 0 ? choose_tiles(p, *context) : TileChoice{256, 1, 0};
+    if (choice.slices > 1 && launch_slices(p, choice, *context, stream, &result)) {
         return result;
     }
     TcPlan plan;
-    if (c.math != CUVIT_MATH_FP32 && prepare(p, c.math, *context, &plan)) {
+    if (c.math != CUVIT_MATH_FP32 && prepare(p, c.math, choice.block_n, *context, &plan)) {
         return bf16 ? launch_tc_bf16(plan, stream) : launch_tc_tf32(plan, stream);
     }
     return bf16 ? launch_simt<__nv_bfloat16>(p, stream) : launch_simt<float>(p, stream);

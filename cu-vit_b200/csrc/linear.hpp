@@ -288,10 +288,19 @@ bool describe(const void* base, bool bf16, long long columns, long long rows, lo
 bool launch_split(const Params& p, const host::DeviceContext& context, cudaStream_t stream,
                   int* result);
 
-// BF16 math for too few output tiles to fill the GPU: k is divided among the CTAs of a cluster
-// (linear_slices.cu). False where that does not apply; else *result is the launch's status.
-bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStream_t stream,
-                   int* result);
+// BF16 math: the accumulator columns of a tile with one CTA to each, and where a cluster of CTAs to
+// each, k divided among them, takes less time, theirs (slices 1: it does not).
+struct TileChoice {
+    int block_n;
+    int slices;
+    int slice_n;
+};
+TileChoice choose_tiles(const Params& p, const host::DeviceContext& context);
+
+// k divided among the CTAs of a cluster (linear_slices.cu). False where TMA cannot describe x or the
+// weight; else *result is the launch's status.
+bool launch_slices(const Params& p, const TileChoice& choice, const host::DeviceContext& context,
+                   cudaStream_t stream, int* result);
 
 // A prepared launch on the tensor-core kernels of one product.
 struct TcPlan {

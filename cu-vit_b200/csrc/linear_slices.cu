@@ -27,7 +27,6 @@ namespace cuvit::linear {
 namespace {
 
 constexpr int kBlockM = 128;
-constexpr int kBlockN = 64; // accumulator columns: of a gated layer 32 gate and 32 up
 constexpr int kBlockK = 64; // 128 bytes of a row
 constexpr int kRowBytes = 128;
 constexpr int kThreads = 256;
@@ -36,22 +35,26 @@ constexpr int kMaxStages = 16;
 constexpr int kMaxSlices = 8;
 constexpr int kMinSteps = 4; // of k in a slice
 
-// A stage holds the rows of x that there are, then 64 of the weight. The products read 128 rows of x
-// all the same: what follows in shared memory makes rows of the sums that nobody reads.
-constexpr int kWBytes = kBlockN * kRowBytes;
-constexpr int kRingBytes = 6 * (kBlockM * kRowBytes + kWBytes);
-constexpr int kPartOffset = kRingBytes;
-// The owned columns' sums of every slice: rows of kBlockN / slices floats and one vector between
-// rows, so that neighbouring rows fall in different banks.
-constexpr int kPartBytes = 4 * kBlockM * (kBlockN + 4 * kMaxSlices);
-constexpr int kBarrierOffset = kPartOffset + kPartBytes;
-constexpr int kBarriers = 2 * kMaxStages + 2;
-constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 8;
-static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
-static_assert(kPartBytes >= kBlockM * kRowBytes, "the last stage's reads of x stay inside");
+// N: accumulator columns; of a gated layer half gate and half up. A stage holds the rows of x that
+// there are, then N of the weight. The products read 128 rows of x all the same: what follows in
+// shared memory makes rows of the sums that nobody reads.
+template <int N>
+struct Shape {
+    static constexpr int kWBytes = N * kRowBytes;
+    static constexpr int kRingBytes = (N == 64 ? 6 : 4) * (kBlockM * kRowBytes + kWBytes);
+    static constexpr int kPartOffset = kRingBytes;
+    // The owned columns' sums of every slice: rows of N / slices floats and one vector between rows,
+    // so that neighbouring rows fall in different banks.
+    static constexpr int kPartBytes = 4 * kBlockM * (N + 4 * kMaxSlices);
+    static constexpr int kBarrierOffset = kPartOffset + kPartBytes;
+    static constexpr int kBarriers = 2 * kMaxStages + 2;
+    static constexpr int kSmemBytes = 1024 + kBarrierOffset + 8 * kBarriers + 8;
+    static_assert(kSmemBytes <= 232448, "shared memory over the per-block limit");
+    static_assert(kPartBytes >= kBlockM * kRowBytes, "the last stage's reads of x stay inside");
+};
 
 struct SliceParams : OutRows {
-    int out_columns; // of a tile: kBlockN, or half of it for a gated layer
+    int out_columns; // of a tile: N, or half of it for a gated layer
     int n_tiles, k_blocks;
     int slices;
     int x_rows; // rows of x a stage holds
@@ -59,20 +62,24 @@ struct SliceParams : OutRows {
     unsigned* status;
 };
 
+template <int N>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_slices_kernel(const __grid_constant__ CUtensorMap map_x,
                          const __grid_constant__ CUtensorMap map_w,
                          const __grid_constant__ SliceParams s) {
+    using S = Shape<N>;
+    constexpr int kWBytes = S::kWBytes;
+    constexpr int kPartOffset = S::kPartOffset;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = dev::smem_u32(smem_raw);
     const uint32_t base = (raw_base + 1023u) & ~1023u;
     uint8_t* const smem = smem_raw + (base - raw_base);
-    const uint32_t bars = base + kBarrierOffset;
+    const uint32_t bars = base + S::kBarrierOffset;
     const auto full = [&](int i) -> uint32_t { return bars + 8u * i; };
     const auto empty = [&](int i) -> uint32_t { return bars + 8u * (kMaxStages + i); };
     const uint32_t sums_full = bars + 8u * 2 * kMaxStages;
     const uint32_t drain_bar = sums_full + 8u;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + kBarrierOffset + 8 * kBarriers);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kBarrierOffset + 8 * S::kBarriers);
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
@@ -85,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         dev::fence_barrier_init();
     }
     if (warp == 2) {
-        dev::tmem_alloc(dev::smem_u32(tmem_slot), kBlockN);
+        dev::tmem_alloc(dev::smem_u32(tmem_slot), N);
         dev::tmem_relinquish();
     }
     dev::tc_fence_before();
@@ -104,7 +111,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int first = static_cast<int>(static_cast<long long>(s.k_blocks) * rank / s.slices);
     const int end = static_cast<int>(static_cast<long long>(s.k_blocks) * (rank + 1) / s.slices);
     const int owned = s.out_columns / s.slices; // columns of the output that a CTA finishes
-    const int pitch = kBlockN / s.slices + 4;   // floats
+    const int pitch = N / s.slices + 4;   // floats
+    const int rows = min(kBlockM, p.m - m_block * kBlockM);
     const int x_bytes = s.x_rows * kRowBytes;
     const int stage_bytes = x_bytes + kWBytes;
 
@@ -143,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         // ---------------- products: the warp stays together, one lane issues ----------------
-        const uint32_t idesc = dev::make_idesc(1u, kBlockM, kBlockN, false, false);
+        const uint32_t idesc = dev::make_idesc(1u, kBlockM, N, false, false);
         const uint32_t base0 = __shfl_sync(0xFFFFFFFFu, base, 0);
         const uint32_t tmem0 = __shfl_sync(0xFFFFFFFFu, tmem, 0);
         int stage = 0;
@@ -186,21 +194,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             // This slice's rows in an owner's memory.
             const uint32_t part = base + kPartOffset + 4u * ((rank * kBlockM + row) * pitch);
 #pragma unroll 1
-            for (int c = 0; c < kBlockN; c += 16) {
+            for (int c = 0; c < N; c += 16) {
                 uint32_t raw[16];
+                __syncwarp(); // the read is warp-wide: lanes with and without a row meet first
                 dev::tmem_load_16(from + c, raw);
                 dev::tmem_wait_load();
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int column = c + 4 * q; // gate and up columns of one output go together
-                    const bool up = p.gated && column >= kBlockN / 2;
-                    const int output = up ? column - kBlockN / 2 : column;
+                    const bool up = p.gated && column >= N / 2;
+                    const int output = up ? column - N / 2 : column;
                     const int owner = output / owned;
                     const int at = output - owner * owned + (up ? owned : 0);
                     const float four[4] = {
                         __uint_as_float(raw[4 * q]), __uint_as_float(raw[4 * q + 1]),
                         __uint_as_float(raw[4 * q + 2]), __uint_as_float(raw[4 * q + 3])};
-                    store_remote(dev::map_to_rank(part + 4u * at, owner), four);
+                    if (row < rows) {
+                        store_remote(dev::map_to_rank(part + 4u * at, owner), four);
+                    }
                 }
             }
             dev::tc_fence_before();
@@ -212,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------- the owned columns ----------------
     const float* const parts = reinterpret_cast<const float*>(smem + kPartOffset);
     const int vectors = owned / 4;
-    const int rows = min(kBlockM, p.m - m_block * kBlockM);
     for (int i = threadIdx.x; i < rows * vectors; i += kThreads) {
         const int row = i / vectors;
         const int at = 4 * (i - row * vectors);
@@ -226,41 +236,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (warp == 2) {
         dev::tc_fence_after();
-        dev::tmem_dealloc(tmem, kBlockN);
+        dev::tmem_dealloc(tmem, N);
     }
 }
 
 } // namespace
 
-bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStream_t stream,
-                   int* result) {
-    if (!host::is_blackwell(context)) {
-        return false;
+// A step of 64 of k takes 0.32, 0.34 or 0.45 us with 64, 128 or 256 columns (a tile per SM, 128 rows:
+// 1024 x 4096 x 4096 takes 89, 51 and 37 us in 4, 2 and 1 waves), and an exchange of slices as much as
+// three steps and one for every 1000 sums of a tile. 700 x 1280 x 5120: 60 tiles of 128 columns and two slices, 27 us (33 with one
+// CTA to each of 120 tiles of 64).
+TileChoice choose_tiles(const Params& p, const host::DeviceContext& context) {
+    const long long row_blocks = (p.m + kBlockM - 1LL) / kBlockM;
+    const int k_blocks = (p.k + kBlockK - 1) / kBlockK;
+    const auto tiles_of = [&](int bn) {
+        const int columns = p.gated ? bn / 2 : bn;
+        return row_blocks * ((p.n + columns - 1LL) / columns);
+    };
+    const auto step = [](int bn) { return bn == 64 ? 0.32 : (bn == 128 ? 0.34 : 0.45); };
+    TileChoice choice{256, 1, 0};
+    double best = 0.0;
+    for (const int bn : {256, 128, 64}) {
+        if (p.gated && bn == 64) {
+            continue; // half a tile's columns of one operand stay a whole 32-column step
+        }
+        const long long waves = (tiles_of(bn) + context.sm_count - 1) / context.sm_count;
+        const double cost = static_cast<double>(waves) * k_blocks * step(bn);
+        if (best == 0.0 || cost < best) {
+            best = cost;
+            choice.block_n = bn;
+        }
     }
+    for (const int bn : {128, 64}) {
+        const long long tiles = tiles_of(bn);
+        if (tiles * 2 > context.sm_count) {
+            continue;
+        }
+        const ClusterLimits limits =
+            bn == 64 ? cluster_limits<&linear_slices_kernel<64>>(kThreads, Shape<64>::kSmemBytes)
+                     : cluster_limits<&linear_slices_kernel<128>>(kThreads, Shape<128>::kSmemBytes);
+        for (int i = 1; i < 4 && tiles <= limits.of[i] && k_blocks >= kMinSteps << i; ++i) {
+            const double exchange = 3.0 + 1.0e-3 * bn * (p.m < kBlockM ? p.m : kBlockM);
+            const double cost = (((k_blocks - 1) >> i) + 1 + exchange) * step(bn);
+            if (cost < best) {
+                best = cost;
+                choice.slices = 1 << i;
+                choice.slice_n = bn;
+            }
+        }
+    }
+    return choice;
+}
+
+bool launch_slices(const Params& p, const TileChoice& choice, const host::DeviceContext& context,
+                   cudaStream_t stream, int* result) {
     SliceParams s{};
     s.p = p;
-    s.out_columns = p.gated ? kBlockN / 2 : kBlockN;
+    s.slices = choice.slices;
+    s.out_columns = p.gated ? choice.slice_n / 2 : choice.slice_n;
     const long long row_blocks = (p.m + kBlockM - 1LL) / kBlockM;
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
-    const long long tiles = row_blocks * n_tiles;
+    const long long tiles = row_blocks * n_tiles; // no more than clusters fit the GPU
     s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
-    if (tiles * 2 > context.sm_count || s.k_blocks < kMinSteps * 2) {
-        return false;
-    }
-    // Slices while the GPU holds all clusters at once and each slice has steps enough to be worth its
-    // start.
-    const ClusterLimits limits = cluster_limits<&linear_slices_kernel>(kThreads, kSmemBytes);
-    s.slices = 1;
-    for (int i = 1; i < 4 && tiles <= limits.of[i] && s.k_blocks >= kMinSteps << i; ++i) {
-        s.slices = 1 << i;
-    }
-    if (s.slices == 1) {
-        return false;
-    }
     s.n_tiles = static_cast<int>(n_tiles);
     s.x_rows = p.m < kBlockM ? (p.m + 7) / 8 * 8 : kBlockM;
-    const int stages = kRingBytes / (s.x_rows * kRowBytes + kWBytes);
-    s.stages = stages < kMaxStages ? stages : kMaxStages;
     CUtensorMap map_x, map_w;
     if (!describe(p.x, true, p.k, p.m, p.ldx, s.x_rows, &map_x) ||
         !describe(p.w, true, p.k, p.n * (p.gated ? 2LL : 1LL), p.ldw, s.out_columns, &map_w)) {
@@ -270,12 +309,18 @@ bool launch_slices(const Params& p, const host::DeviceContext& context, cudaStre
     s.out_vector = access_bytes(p.out, p.ldo * out_bytes);
     s.residual_vector = p.residual != nullptr ? access_bytes(p.residual, p.ldr * out_bytes) : 16;
     s.status = context.status;
-    const auto start = [&]() -> int {
-        launch_cluster(&linear_slices_kernel, s.slices, static_cast<unsigned>(tiles * s.slices),
-                       kThreads, kSmemBytes, stream, map_x, map_w, s);
+    const auto start = [&](auto* kernel, int ring_bytes, int w_bytes, int smem_bytes) {
+        const int stages = ring_bytes / (s.x_rows * kRowBytes + w_bytes);
+        s.stages = stages < kMaxStages ? stages : kMaxStages;
+        launch_cluster(kernel, s.slices, static_cast<unsigned>(tiles * s.slices), kThreads,
+                       smem_bytes, stream, map_x, map_w, s);
         return host::after_launch("linear_slices_kernel");
     };
-    *result = start();
+    *result = choice.slice_n == 64
+                  ? start(&linear_slices_kernel<64>, Shape<64>::kRingBytes, Shape<64>::kWBytes,
+                          Shape<64>::kSmemBytes)
+                  : start(&linear_slices_kernel<128>, Shape<128>::kRingBytes, Shape<128>::kWBytes,
+                          Shape<128>::kSmemBytes);
     return true;
 }
 

@@ -43,11 +43,15 @@ int init_context(int device, DeviceContext* context) {
     context->major = properties.major;
     context->minor = properties.minor;
     context->max_smem_optin = properties.sharedMemPerBlockOptin;
+    // The status word is zero when the module is loaded. Nothing here touches a stream, and loading is
+    // allowed for the time of the query, so that a process's first call may be one that is captured.
     void* address = nullptr;
-    CUVIT_TRY_CUDA(cudaGetSymbolAddress(&address, g_device_status));
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    CUVIT_TRY_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t error = cudaGetSymbolAddress(&address, g_device_status);
+    CUVIT_TRY_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    CUVIT_TRY_CUDA(error);
     context->status = static_cast<unsigned*>(address);
-    CUVIT_TRY_CUDA(cudaMemset(context->status, 0, sizeof(unsigned)));
-    CUVIT_TRY_CUDA(cudaDeviceSynchronize());
     return CUVIT_OK;
 }
 

@@ -916,3 +916,31 @@ def test_linear_with_divided_k(m, n, k, gated, kind, out_kind, cuda):
                             out_kind, n)
     check(outs[0], want, bound)
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_linear_with_divided_k_captured_beside_others(kind, cuda):
+    """Clusters on two streams at once, captured and replayed on new inputs."""
+    torch = cuda
+    m, n, k = 40, 300, 4096
+    math_mode = kernels.MATH_BF16 if kind == "bf16" else kernels.MATH_FP32
+    problem = LinearProblem(m, n, k, math_mode, dtype_of(kind))
+    sides = [dict(x=normal(torch, (m, k), seed, kind), w=normal(torch, (n, k), seed + 1, kind, 0.02),
+                  out=torch.zeros(m, n, dtype=torch_type(torch, kind), device="cuda"),
+                  stream=torch.cuda.Stream(), graph=torch.cuda.CUDAGraph()) for seed in (1, 3)]
+    torch.cuda.synchronize()
+    for side in sides:
+        with torch.cuda.graph(side["graph"]):
+            kernels.launch_linear(side["x"], side["w"], None, None, None, side["out"], problem,
+                                  torch.cuda.current_stream())
+    for side in sides:
+        side["x"].copy_(normal(torch, (m, k), 9, kind))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for side in sides:
+            with torch.cuda.stream(side["stream"]):
+                side["graph"].replay()
+    torch.cuda.synchronize()
+    for side in sides:
+        want, bound = linear_64(torch, side["x"], side["w"], None, None, None, 0, False, kind, kind, n)
+        check(side["out"], want, bound)

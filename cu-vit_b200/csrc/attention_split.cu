@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
         };
         // The end of the keys that the row sees, less this thread's place in a tile.
         const int seen =
-            (p.causal ? static_cast<int>(min(static_cast<long long>(last_key), max(0LL, reach + row + 1)))
+            (p.causal ? static_cast<int>(
+                            min(static_cast<long long>(last_key), max(0LL, reach + row + 1)))
                       : last_key) -
             part * S::kOwn;
         bool ok = true;
@@ -670,8 +671,9 @@ int launch_split(const VarlenParams& p, unsigned* status, cudaStream_t stream) {
     const bool wide = p.head_dim > 64;
     auto* kernel = wide ? &attention_split_kernel<true> : &attention_split_kernel<false>;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kSmemBytes));
-    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)), dim3(wide ? Shape<true>::kThreads : Shape<false>::kThreads), kSmemBytes,
-                     stream, p, flags, status);
+    const int threads = wide ? Shape<true>::kThreads : Shape<false>::kThreads;
+    host::pdl_launch(kernel, dim3(static_cast<unsigned>(blocks)),
+                     dim3(static_cast<unsigned>(threads)), kSmemBytes, stream, p, flags, status);
     return host::after_launch("attention_split_kernel");
 }
 

@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 item = find_item(p, order, index, gridDim.x);
             }
             if (!more_items || item.rows > 0) {
-                ok = dev::mbar_wait_warp(item_empty + 8 * item_at, item_phase ^ 1u, status, kItemWaitNs);
+                ok = dev::mbar_wait_warp(item_empty + 8 * item_at, item_phase ^ 1u, status,
+                                         kItemWaitNs);
                 if (!ok) {
                     break;
                 }

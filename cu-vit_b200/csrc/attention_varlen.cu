@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4 * kGroups; ++j) {
-                score[j / 4][r][j % 4] = tx + kX * j < limit ? score[j / 4][r][j % 4] * p.scale_log2 : -INFINITY;
-                top = fmaxf(top, score[j / 4][r][j % 4]);
+                float& value = score[j / 4][r][j % 4];
+                value = tx + kX * j < limit ? value * p.scale_log2 : -INFINITY;
+                top = fmaxf(top, value);
             }
 #pragma unroll
             for (int offset = kX / 2; offset > 0; offset /= 2) {
@@ -196,8 +197,10 @@ __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
         for (int j = 0; j < 4 * kGroups; ++j) {
             float4* const at =
                 reinterpret_cast<float4*>(ps + (tx + kX * j) * kRowPitch + 8 * ty);
-            at[0] = make_float4(score[j / 4][0][j % 4], score[j / 4][1][j % 4], score[j / 4][2][j % 4], score[j / 4][3][j % 4]);
-            at[1] = make_float4(score[j / 4][4][j % 4], score[j / 4][5][j % 4], score[j / 4][6][j % 4], score[j / 4][7][j % 4]);
+            const float(&s8)[8][4] = score[j / 4];
+            const int c = j % 4;
+            at[0] = make_float4(s8[0][c], s8[1][c], s8[2][c], s8[3][c]);
+            at[1] = make_float4(s8[4][c], s8[5][c], s8[6][c], s8[7][c]);
         }
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {

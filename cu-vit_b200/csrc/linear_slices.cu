@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto empty = [&](int i) -> uint32_t { return bars + 8u * (kMaxStages + i); };
     const uint32_t sums_full = bars + 8u * 2 * kMaxStages;
     const uint32_t drain_bar = sums_full + 8u;
-    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kBarrierOffset + 8 * S::kBarriers);
+    uint32_t* const tmem_slot =
+        reinterpret_cast<uint32_t*>(smem + S::kBarrierOffset + 8 * S::kBarriers);
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
@@ -243,9 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 } // namespace
 
 // A step of 64 of k takes 0.32, 0.34 or 0.45 us with 64, 128 or 256 columns (a tile per SM, 128 rows:
-// 1024 x 4096 x 4096 takes 89, 51 and 37 us in 4, 2 and 1 waves), and an exchange of slices as much as
-// three steps and one for every 1000 sums of a tile. 700 x 1280 x 5120: 60 tiles of 128 columns and two slices, 27 us (33 with one
-// CTA to each of 120 tiles of 64).
+// 1024 x 4096 x 4096 takes 89, 51 and 37 us in 4, 2 and 1 waves), and an exchange of slices as
+// much as three steps and one for every 1000 sums of a tile. 700 x 1280 x 5120: 60 tiles of 128
+// columns and two slices, 27 us (33 with one CTA to each of 120 tiles of 64).
 TileChoice choose_tiles(const Params& p, const host::DeviceContext& context) {
     const long long row_blocks = (p.m + kBlockM - 1LL) / kBlockM;
     const int k_blocks = (p.k + kBlockK - 1) / kBlockK;

@@ -658,7 +658,8 @@ bool launch_split(const Params& p, const host::DeviceContext& context, cudaStrea
     s.p = p;
     s.k_blocks = (p.k + kBlockK - 1) / kBlockK;
     choose_shape(row_blocks, p.n, p.gated != 0, s.k_blocks, context.sm_count,
-                 cluster_limits<&linear_split_kernel<true>>(kThreads, kSmemBytes), &s.block_n, &s.slices);
+                 cluster_limits<&linear_split_kernel<true>>(kThreads, kSmemBytes), &s.block_n,
+                 &s.slices);
     s.out_columns = p.gated ? s.block_n / 2 : s.block_n;
     const long long n_tiles = (p.n + s.out_columns - 1LL) / s.out_columns;
     const long long total = row_blocks * n_tiles;

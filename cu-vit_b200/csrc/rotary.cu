@@ -322,9 +322,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps<Norm>, kMinBlocks<Norm>)
     }
     const long long in_step = s.slots * side.in_stride;
     const long long out_step = s.slots * side.out_stride;
-    const T* in = static_cast<const T*>(side.in) + (token0 + static_cast<long long>(slot)) * side.in_stride +
+    const long long token = token0 + static_cast<long long>(slot);
+    const T* in = static_cast<const T*>(side.in) + token * side.in_stride +
                   static_cast<long long>(head) * p.head_dim;
-    T* out = static_cast<T*>(side.out) + (token0 + static_cast<long long>(slot)) * side.out_stride +
+    T* out = static_cast<T*>(side.out) + token * side.out_stride +
              static_cast<long long>(head) * p.head_dim;
     Vec<T, V> x_next{}, y_next{};
     const auto load_token = [&](int t) {

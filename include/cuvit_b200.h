@@ -419,9 +419,9 @@ typedef struct cuvit_linear_problem {
 /* y = x weight^T + bias (FP32 accumulation), then
  *   out = residual + scale * activation(y)                        plain
  *   out = residual + scale * activation(y[:, :n]) * y[:, n:]      gated
- * with one rounding at the store. With CUVIT_MATH_FP32 an infinite element of x or the weight gives
- * NaN where the plain product gives an infinity. bias float [n] (gated [2n]), scale float [n] and residual may
- * be null. out may be residual itself (same pointer and row distance); any other overlap of
+ * with one rounding at the store. With CUVIT_MATH_FP32 an infinite element of x or the weight
+ * gives NaN where the plain product gives an infinity. bias float [n] (gated [2n]), scale float
+ * [n] and residual may be null. out may be residual itself (same pointer and row distance); any other overlap of
  * out with an operand is refused. */
 int cuvit_linear(const void* x, const void* weight, const float* bias, const float* scale,
                  const void* residual, void* out, const cuvit_linear_problem* problem,

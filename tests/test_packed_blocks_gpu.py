@@ -944,3 +944,42 @@ def test_linear_with_divided_k_captured_beside_others(kind, cuda):
     for side in sides:
         want, bound = linear_64(torch, side["x"], side["w"], None, None, None, 0, False, kind, kind, n)
         check(side["out"], want, bound)
+
+
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 64), (130, 200, 72), (700, 300, 500), (40, 33, 30)])
+def test_linear_tf32(m, n, k, gated, cuda):
+    """One product of TF32 values: each operand keeps 11 bits, cut off at most: 2^-10 of it, twice.
+    Few rows and rows that are not whole 16-byte vectors have FP32 products, which is within that."""
+    torch = cuda
+    x, residual = normal(torch, (m, k), 1, "f32"), normal(torch, (m, n), 2, "f32")
+    w = normal(torch, ((2 if gated else 1) * n, k), 3, "f32")
+    out = torch.empty_like(residual)
+    kernels.launch_linear(x, w, None, None, residual, out,
+                          LinearProblem(m, n, k, kernels.MATH_TF32, kernels.DTYPE_F32,
+                                        kernels.ACTIVATION_NONE, gated))
+    torch.cuda.synchronize()
+    y = x.double() @ w.double().t()
+    # The sum's k additions cut off less than 2^-23 of the partial sums each.
+    error = (2.0 ** -9 + 2.0 ** -20 + (k + 4) * 2.0 ** -23) * (x.double().abs() @ w.double().abs().t())
+    value, off = y[:, :n], error[:, :n]
+    if gated:
+        off = off * (y[:, n:].abs() + error[:, n:]) + value.abs() * error[:, n:]
+        value = value * y[:, n:]
+    want = value + residual.double()
+    check(out, want, off + 4 * U32 * (value.abs() + residual.double().abs()))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dim", [3, 9, 17, 24, 33, 48, 56, 65, 81, 88, 104, 112, 113, 120, 127])
+def test_attention_head_widths(dim, kind, cuda):
+    """Widths on both sides of the kernels' groups of columns, with and without whole vectors."""
+    torch = cuda
+    lengths, heads = [130, 40, 67, 1], 2
+    q, k, v = (normal(torch, (sum(lengths), heads, dim), seed, kind) for seed in (1, 2, 3))
+    for causal in (False, True):
+        problem = AttentionProblem(len(lengths), sum(lengths), sum(lengths), heads, heads, dim,
+                                   dtype_of(kind), causal, dim ** -0.5)
+        want, bound = attention_64(torch, q, k, v, lengths, lengths, dim ** -0.5, causal, kind)
+        got = run_attention(torch, q, k, v, offsets(torch, lengths), None, problem)
+        check(got, want, bound, f"causal {causal}")

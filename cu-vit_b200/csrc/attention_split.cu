@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
                 if (g < count) { // warp-uniform
                     uint32_t part[kGroup];
                     dev::tmem_load_16(mine + S::kO + (group0 + g) * kGroup, part);
-                    dev::tmem_wait_load();
+                    dev::tmem_wait_load_of(part);
 #pragma unroll
                     for (int j = 0; j < kGroup; ++j) {
                         o[g][j] = fmaf(o[g][j], pending, __uint_as_float(part[j]));
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(Shape<Wide>::kThreads, 1)
                 } else {
                     dev::tmem_load_8(scores, raw);
                 }
-                dev::tmem_wait_load();
+                dev::tmem_wait_load_of(raw);
 #pragma unroll
                 for (int j = 0; j < kRead; ++j) {
                     w[(g * kRead + j) / 4][j % 4] = __uint_as_float(raw[j]);

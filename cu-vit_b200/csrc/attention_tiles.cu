@@ -771,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             for (int c = 0; c < o_columns; c += 16) {
                                 uint32_t o[16];
                                 dev::tmem_load_16(o_tmem + c, o);
-                                dev::tmem_wait_load();
+                                dev::tmem_wait_load_of(o);
 #pragma unroll
                                 for (int x = 0; x < 16; ++x) {
                                     o[x] = __float_as_uint(__uint_as_float(o[x]) * factor);

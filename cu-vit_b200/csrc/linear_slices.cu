@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t raw[16];
                 __syncwarp(); // the read is warp-wide: lanes with and without a row meet first
                 dev::tmem_load_16(from + c, raw);
-                dev::tmem_wait_load();
+                dev::tmem_wait_load_of(raw);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int column = c + 4 * q; // gate and up columns of one output go together

@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint32_t part_sums[kGroup];
                         dev::tmem_load_16(sums + acc * kSumPitch + from0 + g * from_step,
                                           part_sums);
-                        dev::tmem_wait_load();
+                        dev::tmem_wait_load_of(part_sums);
 #pragma unroll
                         for (int j = 0; j < kGroup; ++j) {
                             v[g][j] += __uint_as_float(part_sums[j]);

@@ -26,6 +26,8 @@
 //   cancels in the quotient. So a step takes its exponentials with the m it has, one read of the
 //   scores giving both them and their maximum; only where a maximum turns out too high (in the first
 //   step, where m is 0, also too low) are O and the sums rescaled and the scores read again.
+// * NaN and minus infinity take that second reading too, in its exact form: the exponentials on the
+//   FMA pipe would make 2^-125 of both. The maximum keeps NaN, so it shows them at no cost.
 // * Scores are read 32 at a time, the next 32 in flight meanwhile. Two threads per row (64 scores
 //   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes 1.81 ms
 //   (16384 tokens, 16 heads of 128: 1214 TFLOP/s, of 1672 measured for one large product; heads of
@@ -162,6 +164,7 @@ __device__ __forceinline__ void mask(uint32_t (&s)[32], int limit) {
     }
 }
 
+// NaN where a score is.
 __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
     float m[2];
 #pragma unroll
@@ -169,12 +172,12 @@ __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
         m[c] = __uint_as_float(s[16 * c]);
 #pragma unroll
         for (int j = 1; j < 15; j += 2) {
-            m[c] = dev::max3(m[c], __uint_as_float(s[16 * c + j]),
-                             __uint_as_float(s[16 * c + j + 1]));
+            m[c] = dev::max3_or_nan(m[c], __uint_as_float(s[16 * c + j]),
+                                    __uint_as_float(s[16 * c + j + 1]));
         }
-        m[c] = fmaxf(m[c], __uint_as_float(s[16 * c + 15]));
+        m[c] = dev::max_or_nan(m[c], __uint_as_float(s[16 * c + 15]));
     }
-    return fmaxf(m[0], m[1]);
+    return dev::max_or_nan(m[0], m[1]);
 }
 
 // P = 2^(scale (s - m)) of 32 scores, packed, and their sum. The plain form
@@ -710,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if constexpr (exact.value) {
                                 mask(s[c & 1], limit - 32 * c);
                             }
-                            top = fmaxf(top, maximum(s[c & 1]));
+                            top = dev::max_or_nan(top, maximum(s[c & 1]));
                             added += exponentials<exact.value>(s[c & 1], p.scale_log2, m,
                                                                packed[c]);
                         }
@@ -727,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 dev::tmem_load_32(s_tmem + 32 * c, s);
                                 dev::tmem_wait_load_of(s);
                                 mask(s, limit - 32 * c);
-                                top = fmaxf(top, maximum(s));
+                                top = dev::max_or_nan(top, maximum(s));
                                 added += exponentials<true>(s, p.scale_log2, m, packed[c]);
                             } else {
 #pragma unroll
@@ -741,11 +744,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else {
                         weigh(std::false_type{});
                     }
-                    // The first step has m = 0, which stays where the maximum is within 2^+-8 of it.
+                    // A row without a weight so far has m = 0, which stays where the maximum is
+                    // within 2^+-8 of it. A NaN maximum is not within anything.
+                    const bool fresh = sum == 0.0F;
+                    const bool some = top != -INFINITY;
                     const float above = (top - m) * p.scale_log2;
                     const bool raise = __any_sync(
-                        0xFFFFFFFFu, above > kRescaleAbove ||
-                                         (j == 0 && above < -kRescaleAbove && top != -INFINITY));
+                        0xFFFFFFFFu, !(above <= kRescaleAbove) ||
+                                         (some ? fresh && above < -kRescaleAbove : !exact));
                     if (!S::kOverlay && !raise) {
                         arrive(s_free + 8 * t);
                     }
@@ -760,11 +766,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (raise) {
                         if (j == 0) {
-                            m = top == -INFINITY ? 0.0F : top;
+                            m = some ? top : 0.0F;
                         } else {
                             const float raised =
-                                (top - m) * p.scale_log2 > kRescaleAbove ? top : m;
-                            const float factor = dev::ex2_approx((m - raised) * p.scale_log2);
+                                some && (fresh || above > kRescaleAbove) ? top : m;
+                            const float factor =
+                                fresh ? 0.0F : dev::ex2_approx((m - raised) * p.scale_log2);
                             m = raised;
                             sum *= factor;
 #pragma unroll 1

@@ -378,8 +378,10 @@ typedef struct cuvit_attention_problem {
  * weights to bfloat16 for the product with v, F32 has FP32-faithful products (each as three of
  * TF32 halves, as CUVIT_MATH_FP32). Rows of out outside every sequence are not written, and rows
  * of q, k and v outside a sequence may hold anything, NaN included, without reaching it. Within a
- * sequence a NaN or infinite value reaches every query of its tile of keys: a causal query's
- * weight for a later key is zero, but zero times such a value is NaN, as in the plain product.
+ * sequence a NaN score makes its query's outputs NaN, one of minus infinity leaves its key out (a
+ * query with no other counts as one that sees none), and a NaN or infinite element of v reaches
+ * every query of its tile of keys: a causal query's weight for a later key is zero, but zero times
+ * such a value is NaN, as in the plain product. F32 may have NaN where a score is infinite.
  * kv_offsets null: q_offsets (self-attention). out must not overlap q, k, v or the offsets.
  * The workspace (device, 16-byte aligned, cuvit_attention_varlen_workspace() bytes, contents
  * irrelevant before and after) lets calls with few query rows split long key ranges over the

@@ -1,0 +1,98 @@
+"""The operators over packed images and videos on NaN, infinities and the ends of their ranges: what
+each formula gives there, through every kernel a call may take."""
+
+from __future__ import annotations
+
+import pytest
+
+from cuvit import kernels
+from cuvit.kernels import AttentionProblem
+from test_packed_blocks_gpu import (TYPES, attention_64, check, dtype_of, normal, offsets,
+                                    run_attention)
+
+pytestmark = pytest.mark.gpu
+
+# Places of a key: every one of a group of eight, ends of 32, 64 and 128 keys, a sequence's last.
+PLACES = [*range(8), 14, 15, 30, 31, 62, 63, 94, 95, 110, 126, 127, 128, 134, 143, 200, 255, 256, 299]
+
+
+def attention_case(torch, kind, queries, keys, dim, causal, seed=0):
+    heads = 2
+    q = normal(torch, (queries, heads, dim), seed + 1, kind)
+    k, v = (normal(torch, (keys, heads, dim), seed + i, kind) for i in (2, 3))
+    problem = AttentionProblem(1, queries, keys, heads, heads, dim, dtype_of(kind), causal, 0.125)
+    return q, k, v, problem
+
+
+# ---- attention: NaN and infinite keys ------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("queries", [2, 300])
+@pytest.mark.parametrize("dim", [32, 64, 80, 128, 13])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_nan_key_reaches_every_query_that_sees_it(causal, dim, queries, kind, cuda):
+    """Wherever the key stands in its tile. The other head keeps its results, and so do, but for
+    roundings, the queries that do not see the key: rows that share a warp with one that reads its
+    scores again do so too, and take all their exponentials in the exact form, where a quarter of
+    them may have come from the polynomial that attention_64's bound counts."""
+    torch = cuda
+    keys = 300
+    q, k, v, problem = attention_case(torch, kind, queries, keys, dim, causal)
+    places = offsets(torch, [queries]), offsets(torch, [keys])
+    clean = run_attention(torch, q, k, v, *places, problem)
+    assert clean.isfinite().all()
+    want, bound = attention_64(torch, q, k, v, [queries], [keys], 0.125, causal, kind)
+    for at in PLACES:
+        poisoned = k.clone()
+        poisoned[at, 0, dim // 2] = float("nan")
+        got = run_attention(torch, q, poisoned, v, *places, problem)
+        sees = torch.ones(queries, dtype=torch.bool, device="cuda")
+        if causal:
+            sees = torch.arange(queries, device="cuda") + keys - queries >= at
+        assert got[sees, 0].isnan().all(), f"key {at}"
+        check(got[~sees], want[~sees], bound[~sees], f"key {at}")
+        assert torch.equal(got[:, 1], clean[:, 1])
+
+
+@pytest.mark.parametrize("queries", [2, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_infinite_keys(queries, dim, cuda):
+    """A score of plus infinity leaves no weight to divide by, one of minus infinity leaves its key
+    out; a query whose scores are all minus infinity counts as one that sees no key, also where
+    only its first tile's are."""
+    torch = cuda
+    keys = 300
+    q, k, v, problem = attention_case(torch, "bf16", queries, keys, dim, False)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    q[queries // 2, :, 0] = -1.0
+    places = offsets(torch, [queries]), offsets(torch, [keys])
+    for out_of, left in ((range(7, 8), None), (range(0, 130), None), (range(0, keys), 0)):
+        poisoned = k.clone()
+        poisoned[out_of.start:out_of.stop, 0, 0] = -float("inf")
+        got = run_attention(torch, q, poisoned, v, *places, problem)
+        assert got[queries // 2, 0].isnan().all()
+        rest = [i for i in range(queries) if i != queries // 2]
+        if left == 0:
+            assert (got[rest, 0] == 0.0).all()
+            continue
+        kept = [j for j in range(keys) if j not in out_of]
+        want, bound = attention_64(torch, q, k[kept], v[kept], [queries], [len(kept)], 0.125, False,
+                                   "bf16")
+        check(got[rest, 0], want[rest, 0], bound[rest, 0], f"without {out_of}")
+
+
+@pytest.mark.parametrize("queries", [2, 300])
+def test_attention_first_tile_minus_infinity_then_low_scores(queries, cuda):
+    """The first tile's keys are left out and the next ones' scores lie thousands below zero: the
+    maximum has to come down to them."""
+    torch = cuda
+    keys, dim = 300, 64
+    q, k, v, _ = attention_case(torch, "bf16", queries, keys, dim, False)
+    q[:, :, 0] = 64.0
+    k[:, :, 0] = -64.0
+    k[:130, :, 0] = -float("inf")
+    problem = AttentionProblem(1, queries, keys, 2, 2, dim, dtype_of("bf16"), False, 1.0)
+    got = run_attention(torch, q, k, v, offsets(torch, [queries]), offsets(torch, [keys]), problem)
+    want, bound = attention_64(torch, q, k[130:], v[130:], [queries], [keys - 130], 1.0, False, "bf16")
+    check(got, want, bound)

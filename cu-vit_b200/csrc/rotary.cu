@@ -366,6 +366,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps<Norm>, kMinBlocks<Norm>)
     const bool offsets = p.side[0].beta != nullptr || p.side[1].beta != nullptr;
     const float inverse_dim = 1.0F / static_cast<float>(p.head_dim);
     const float4* turns = table + slot * (half / 2) + chunk;
+    // Of this lane's pairs the first ones turn. The others stay what they are: turned by (1, 0), a
+    // NaN or an infinity would reach its partner.
+    const int turned_pairs = p.pairs - V * chunk;
     // All groups go round together: the sums need every lane of a warp.
     for (int t = slot; t - slot < tokens; t += s.slots) {
         uint64_t x[kPairs], y[kPairs];
@@ -439,16 +442,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps<Norm>, kMinBlocks<Norm>)
 #pragma unroll
                 for (int q = 0; q < kPairs; ++q) {
                     const float4 two = turns[q * s.chunks];
-                    if constexpr (kQuarter > 0) {
-                        uint64_t* const at = q < kQuarter ? &x[2 * q] : &y[2 * (q - kQuarter)];
-                        at[0] = turn(at[0], two.x, two.y);
-                        at[1] = turn(at[1], two.z, two.w);
-                    } else {
-                        x[0] = turn(x[0], two.x, two.y);
-                        y[0] = turn(y[0], two.z, two.w);
-                    }
+                    uint64_t& even = kQuarter == 0 ? x[0] : (q < kQuarter ? x[2 * q]
+                                                                          : y[2 * (q - kQuarter)]);
+                    uint64_t& odd = kQuarter == 0 ? y[0] : (q < kQuarter ? x[2 * q + 1]
+                                                                         : y[2 * (q - kQuarter) + 1]);
+                    even = 2 * q < turned_pairs ? turn(even, two.x, two.y) : even;
+                    odd = 2 * q + 1 < turned_pairs ? turn(odd, two.z, two.w) : odd;
                 }
-            } else {
+            } else if (turned_pairs > 0) { // all of them or none (vector_width)
 #pragma unroll
                 for (int j = 0; j < kPairs; ++j) {
                     const ulonglong2 two =

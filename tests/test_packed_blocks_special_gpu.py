@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 
 from cuvit import kernels
-from cuvit.kernels import AttentionProblem
+from cuvit.kernels import AttentionProblem, QkNorm, QkProblem
 from test_packed_blocks_gpu import (TYPES, attention_64, check, dtype_of, normal, offsets,
                                     run_attention)
 
@@ -96,3 +96,63 @@ def test_attention_first_tile_minus_infinity_then_low_scores(queries, cuda):
     got = run_attention(torch, q, k, v, offsets(torch, [queries]), offsets(torch, [keys]), problem)
     want, bound = attention_64(torch, q, k[130:], v[130:], [queries], [keys - 130], 1.0, False, "bf16")
     check(got, want, bound)
+
+
+# ---- rotary: elements past the rotated pairs -----------------------------------------------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("pairing", [kernels.ROTARY_HALVES, kernels.ROTARY_ADJACENT],
+                         ids=["halves", "adjacent"])
+@pytest.mark.parametrize("dim,pairs", [(64, 16), (64, 8), (72, 32), (80, 12), (24, 5), (96, 44), (12, 2),
+                                       (64, 31), (10, 3)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_rotary_copies_what_it_does_not_turn(shift, dim, pairs, pairing, kind, cuda):
+    """Bit for bit, whatever their neighbours hold: NaN, infinities and negative zeros beside the
+    elements that turn and beside each other. At any alignment."""
+    torch = cuda
+    tokens, heads = 5, 3
+    buffer = normal(torch, (tokens * heads * dim + shift,), dim + pairs, kind)
+    x = buffer[shift:].view(tokens, heads, dim)
+    rest = x[..., 2 * pairs:]
+    for i, value in enumerate((float("nan"), float("inf"), -float("inf"), -0.0)):
+        rest[:, :, i::7] = value
+    x[2, 1, 0] = float("nan")
+    out = torch.zeros_like(x)
+    positions = torch.arange(1, tokens + 1, dtype=torch.int32, device="cuda")
+    problem = QkProblem(tokens, heads, 0, dim, dtype_of(kind))
+    kernels.launch_rotary(x, None, out, None, positions, kernels.rotary_axes([pairs], 10.0, pairing),
+                          problem)
+    torch.cuda.synchronize()
+    bits = torch.int16 if kind == "bf16" else torch.int32
+    got, want = (t[..., 2 * pairs:] for t in (out, x))
+    alike = (got.contiguous().view(bits) == want.contiguous().view(bits)) | (got.isnan() & want.isnan())
+    assert alike.all()
+    clean = torch.ones_like(out[..., :2 * pairs], dtype=torch.bool)
+    clean[2, 1] = False
+    assert out[..., :2 * pairs][clean].isfinite().all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("norm", [kernels.NORM_RMS, kernels.NORM_LAYER], ids=["rms", "layer"])
+@pytest.mark.parametrize("pairs", [0, 8])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_norm_of_gains_that_are_not_finite(shift, pairs, norm, kind, cuda):
+    """An infinite or NaN gain of an element that does not turn reaches that element alone, with
+    and without a rotation."""
+    torch = cuda
+    tokens, heads, dim = 4, 2, 64
+    buffer = normal(torch, (tokens * heads * dim + shift,), 3, kind)
+    x = buffer[shift:].view(tokens, heads, dim)
+    gamma = normal(torch, (dim,), 4)
+    gamma[20], gamma[43] = float("nan"), float("inf")
+    out = torch.zeros_like(x)
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    kernels.launch_qk_norm_rotary(x, None, out, None, QkNorm(norm, 1e-6, gamma), positions,
+                                  kernels.rotary_axes([pairs]) if pairs else None,
+                                  QkProblem(tokens, heads, 0, dim, dtype_of(kind)))
+    torch.cuda.synchronize()
+    clean = torch.ones(dim, dtype=torch.bool, device="cuda")
+    clean[20] = clean[43] = False
+    assert out[..., clean].isfinite().all()
+    assert out[..., 20].isnan().all() and out[..., 43].isinf().all()

@@ -41,8 +41,8 @@ __device__ __forceinline__ float gelu_exact(float x) {
     const float square = x * x;
     const float tail =
         exp2_product(square, kHalfLog2e, fmaf(x, x, -square) * kHalfLog2e);
-    // An infinite x: its square's low part is NaN, and Q is zero there.
-    return z > 14.0F ? fmaxf(x, 0.0F) : fmaf(-z * t * p, tail, fmaxf(x, 0.0F));
+    // Beyond: x, or a zero of its sign and, for minus infinity, NaN, as in the formula.
+    return z > 14.0F ? (x > 0.0F ? x : x * 0.0F) : fmaf(-z * t * p, tail, fmaxf(x, 0.0F));
 }
 
 // x / (1 + exp(-x)).
@@ -53,13 +53,13 @@ __device__ __forceinline__ float logistic_times(float x, float t, float low) {
 
 __device__ __forceinline__ float silu_exact(float x) {
     const float t = fmaxf(-1.4426950409F * x, -126.0F); // below, exp(-x) does not change 1 + it
-    return t > 126.0F ? 0.0F : logistic_times(x, t, t == -126.0F ? 0.0F : fmaf(-1.4426950409F, x, -t));
+    return t > 126.0F ? x * 0.0F : logistic_times(x, t, t == -126.0F ? 0.0F : fmaf(-1.4426950409F, x, -t));
 }
 
 // x (1 + tanh u) / 2 = x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3).
 __device__ __forceinline__ float gelu_tanh_exact(float x) {
     const float t = fmaxf(-2.3022081985F * fmaf(0.044715F * x * x, x, x), -126.0F);
-    return t > 126.0F ? 0.0F : logistic_times(x, t, 0.0F);
+    return t > 126.0F ? x * 0.0F : logistic_times(x, t, 0.0F);
 }
 
 __device__ __forceinline__ float activate_exact(int activation, float x) {
@@ -96,8 +96,10 @@ __device__ __forceinline__ float gelu_tanh_fast(float x) {
 // t = 1 / (1 + 0.375 z) and P of degree 4, fitted here for minimax relative error on [0, 13.5]
 // (2.9e-5 in FP32; beyond, Q is below the smallest float). Two values, the multiply-adds packed.
 __device__ __forceinline__ float2 gelu_fast2(float x0, float x1) {
-    const float m0 = fabsf(x0);
-    const float m1 = fabsf(x1);
+    // Bounded above: for a positive infinity |x| times t = 0 would be NaN. A negative one has NaN, as
+    // in the formula.
+    const float m0 = fabsf(fminf(x0, 1.0e18F));
+    const float m1 = fabsf(fminf(x1, 1.0e18F));
     const uint64_t m = f32x2(m0, m1);
     const float2 den = f32x2_split(fma_f32x2(f32x2(0.375F, 0.375F), m, f32x2(1.0F, 1.0F)));
     const uint64_t t = f32x2(rcp_approx(den.x), rcp_approx(den.y));

@@ -3,12 +3,14 @@ each formula gives there, through every kernel a call may take."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 
 from cuvit import kernels
-from cuvit.kernels import AttentionProblem, QkNorm, QkProblem
+from cuvit.kernels import AttentionProblem, LinearProblem, QkNorm, QkProblem
 from test_packed_blocks_gpu import (TYPES, attention_64, check, dtype_of, normal, offsets,
-                                    run_attention)
+                                    run_attention, torch_type)
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +158,81 @@ def test_norm_of_gains_that_are_not_finite(shift, pairs, norm, kind, cuda):
     clean[20] = clean[43] = False
     assert out[..., clean].isfinite().all()
     assert out[..., 20].isnan().all() and out[..., 43].isinf().all()
+
+
+# ---- linear layers: activations at infinities and in their tails ---------------------------
+
+ACTIVATIONS = pytest.mark.parametrize("activation", range(4), ids=["none", "gelu", "gelu_tanh", "silu"])
+# A few rows; a cluster's slices of k; whole tiles; operands that TMA cannot describe.
+PATHS = pytest.mark.parametrize("m,k,shift", [(3, 64, 0), (24, 2048, 0), (300, 64, 0), (20, 64, 1)],
+                                ids=["rows", "slices", "tiles", "simt"])
+MODES = pytest.mark.parametrize("kind,out_kind", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32"),
+                                                  ("f32", "bf16")])
+
+
+def activated(torch, activation, y):
+    """The formulas in 64 bits, none of which cancels for negative y."""
+    if activation == kernels.ACTIVATION_GELU:
+        return y * torch.special.erfc(y * -math.sqrt(0.5)) / 2
+    if activation == kernels.ACTIVATION_GELU_TANH:
+        return y / (1 + (-2 * math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)).exp())
+    return y / (1 + (-y).exp()) if activation == kernels.ACTIVATION_SILU else y
+
+
+def run_layer(torch, m, k, shift, w0, kind, out_kind, activation, gated, bias=None):
+    """x has a one at the first place and zeros after: every sum is the one product w0[column]."""
+    n = w0.numel() // (2 if gated else 1)
+    x = torch.zeros(m * (k + shift), dtype=torch_type(torch, kind), device="cuda").view(m, k + shift)
+    w = torch.zeros(w0.numel(), k + shift, dtype=x.dtype, device="cuda")
+    x[:, 0] = 1.0
+    w[:, 0] = w0
+    out = torch.full((m, n), 3.0, dtype=torch_type(torch, out_kind), device="cuda")
+    kernels.launch_linear(x, w, bias, None, None, out,
+                          LinearProblem(m, n, k, kernels.MATH_BF16 if kind == "bf16"
+                                        else kernels.MATH_FP32, dtype_of(out_kind), activation, gated,
+                                        k + shift, k + shift))
+    torch.cuda.synchronize()
+    return out
+
+
+@ACTIVATIONS
+@MODES
+@PATHS
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+def test_linear_infinite_sums(gated, m, k, shift, kind, out_kind, activation, cuda):
+    """What the formula gives for a sum of plus infinity (itself), minus infinity (NaN, but for no
+    activation) and NaN, whichever kernel a call takes; its neighbours keep their values."""
+    torch = cuda
+    n = 96
+    w0 = torch.linspace(-4, 4, 2 * n if gated else n, device="cuda")
+    bias = torch.zeros(w0.numel(), device="cuda")
+    clean = run_layer(torch, m, k, shift, w0, kind, out_kind, activation, gated, bias)
+    bias[5], bias[42], bias[77] = float("inf"), -float("inf"), float("nan")
+    if gated:
+        w0[n + 5] = w0[n + 42] = 1.0
+    got = run_layer(torch, m, k, shift, w0, kind, out_kind, activation, gated, bias)
+    assert (got[:, 5] == float("inf")).all()
+    if activation == kernels.ACTIVATION_NONE:
+        assert (got[:, 42] == -float("inf")).all()
+    else:
+        assert got[:, 42].isnan().all()
+    assert got[:, 77].isnan().all()
+    same = [c for c in range(n) if c not in (5, 42, 77)]
+    assert clean.isfinite().all() and torch.equal(got[:, same], clean[:, same])
+
+
+@ACTIVATIONS
+@MODES
+@PATHS
+def test_linear_large_finite_sums(m, k, shift, kind, out_kind, activation, cuda):
+    """Sums up to the largest bfloat16, where squares and cubes are infinite: themselves, or zero."""
+    torch = cuda
+    sizes = torch.tensor([1e2, 1e6, 1e12, 9e17, 2e18, 1e19, 1e20, 1e30, 1e37, 3.3e38], device="cuda")
+    w0 = torch.cat([sizes, -sizes])
+    got = run_layer(torch, m, k, shift, w0, kind, out_kind, activation, False).double()
+    y = w0.to(torch_type(torch, kind)).double()
+    want = activated(torch, activation, y) if activation == kernels.ACTIVATION_NONE else y.clamp_min(0.0)
+    want = want.to(torch_type(torch, out_kind)).double()
+    # The value itself, times a factor that is 1 to within a few steps.
+    step = 2.0 ** -7 if out_kind == "bf16" else 32 * 2.0 ** -24
+    check(got, want.expand_as(got), (step * want.abs() + 1e-30).expand_as(got))

@@ -1,6 +1,7 @@
-// The activations of cuvit_linear in FP32: forms for float outputs (about 1e-6 relative, from the
-// hardware's exponential and reciprocal with their roundings corrected), and cheaper ones for
-// bfloat16 outputs.
+// The activations of cuvit_linear in FP32: forms for float outputs (within 6e-7 relative, from the
+// hardware's exponential and reciprocal with their roundings corrected), and cheaper ones for bfloat16
+// outputs. Where the exponential leaves the normal floats (the erf form at -13, tanh GELU at -10, SiLU
+// at -87, values below 1e-36) they give zero.
 #pragma once
 
 #include "cuvit_b200.h"
@@ -8,24 +9,22 @@
 
 namespace cuvit::dev {
 
-// 2^(a b) with the product's rounding error carried along: an exponent of -100 rounded to FP32
-// alone would cost 2^-18 of the result. The hardware exponential is within 2^-22.
-__device__ __forceinline__ float exp2_product(float a, float b, float rest) {
-    const float t = a * b;
-    const float low = fmaf(a, b, -t) + rest;
+// 2^(t + low) where low carries what rounding the exponent t cost it: for -100 that alone would be
+// 2^-18 of the result. The hardware exponential is within 2^-22.
+__device__ __forceinline__ float exp2_sum(float t, float low) {
     const float e = ex2_approx(t);
     return fmaf(e * 0.6931471806F, low, e);
 }
 
-// 1 / d for d >= 1: the hardware's reciprocal and one Newton step. (An infinite d gives 0.)
+// 1 / d for d >= 1: the hardware's reciprocal and one Newton step. (NaN for an infinite d.)
 __device__ __forceinline__ float reciprocal(float d) {
     const float r = rcp_approx(d);
-    return d < 1.0e38F ? fmaf(r, fmaf(-d, r, 1.0F), r) : r;
+    return fmaf(r, fmaf(-d, r, 1.0F), r);
 }
 
 // x Phi(x) = max(x, 0) - |x| Q(|x|), Q(z) = erfc(z / sqrt 2) / 2 = exp(-z^2 / 2) t P(t) with
 // t = 1 / (1 + 0.3 z) and P of degree 7, fitted here for minimax relative error on [0, 13.5]
-// (1.3e-7; 4.7e-7 as evaluated in FP32; beyond, Q is below the smallest float). It keeps its
+// (1.3e-7; 5.1e-7 as evaluated in FP32; beyond, Q is below the smallest float). It keeps its
 // relative accuracy in the negative tail, where 1 + erf cancels.
 __device__ __forceinline__ float gelu_exact(float x) {
     const float z = fabsf(x);
@@ -37,29 +36,50 @@ __device__ __forceinline__ float gelu_exact(float x) {
     p = fmaf(t, p, 0.09963749349117279F);
     p = fmaf(t, p, 0.12079835683107376F);
     p = fmaf(t, p, 0.11962638795375824F);
-    constexpr float kHalfLog2e = -0.7213475204F;
-    const float square = x * x;
-    const float tail =
-        exp2_product(square, kHalfLog2e, fmaf(x, x, -square) * kHalfLog2e);
+    constexpr float kHalf = -0.7213475204F;  // -log2(e) / 2
+    constexpr float kHalfLow = -9.629815e-9F; // what the float leaves of it
+    const float square = __fmul_rn(x, x);
+    const float exponent = __fmul_rn(square, kHalf);
+    const float low = fmaf(square, kHalfLow,
+                           fmaf(fmaf(x, x, -square), kHalf, fmaf(square, kHalf, -exponent)));
+    const float tail = exp2_sum(exponent, low);
     // Beyond: x, or a zero of its sign and, for minus infinity, NaN, as in the formula.
     return z > 14.0F ? (x > 0.0F ? x : x * 0.0F) : fmaf(-z * t * p, tail, fmaxf(x, 0.0F));
 }
 
-// x / (1 + exp(-x)).
+// x / (1 + 2^(t + low)), within 3e-7: with s = 2^-|t + low|, x / (1 + s) or x s / (1 + s). Far from
+// zero (where low may be infinite or NaN) x itself, or a zero of its sign and, for minus infinity, NaN.
 __device__ __forceinline__ float logistic_times(float x, float t, float low) {
-    const float e = ex2_approx(t);
-    return x * reciprocal(1.0F + fmaf(e * 0.6931471806F, low, e));
+    const bool negative = t > 0.0F; // x is
+    const float s = exp2_sum(-fabsf(t), negative ? -low : low);
+    const float factor = (negative ? s : 1.0F) * reciprocal(1.0F + s);
+    return x * (fabsf(t) < 190.0F ? factor : (negative ? 0.0F : 1.0F));
 }
 
 __device__ __forceinline__ float silu_exact(float x) {
-    const float t = fmaxf(-1.4426950409F * x, -126.0F); // below, exp(-x) does not change 1 + it
-    return t > 126.0F ? x * 0.0F : logistic_times(x, t, t == -126.0F ? 0.0F : fmaf(-1.4426950409F, x, -t));
+    constexpr float kRate = -1.4426950409F;   // -log2(e)
+    constexpr float kRateLow = -1.925963e-8F; // what the float leaves of it
+    const float t = kRate * x;
+    return logistic_times(x, t, fmaf(kRateLow, x, fmaf(kRate, x, -t)));
 }
 
-// x (1 + tanh u) / 2 = x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3).
+// x (1 + tanh u) / 2 = x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3). The exponent
+// t = x (a + b x^2) is formed with the roundings of its square, products and sum carried along (without
+// them the result was off by 2e-6 at -5 and 1e-5 at -9).
 __device__ __forceinline__ float gelu_tanh_exact(float x) {
-    const float t = fmaxf(-2.3022081985F * fmaf(0.044715F * x * x, x, x), -126.0F);
-    return t > 126.0F ? x * 0.0F : logistic_times(x, t, 0.0F);
+    constexpr float kA = -2.3022081985F;                        // -2 sqrt(2/pi) log2(e)
+    constexpr float kB = -0.1029432397F, kBLow = 2.0161983e-9F; // 0.044715 times that
+    const float square = __fmul_rn(x, x);
+    const float product = __fmul_rn(kB, square);
+    const float sum = __fadd_rn(kA, product);
+    // What the sum lost: of two numbers of one sign, the smaller less what it added to the larger.
+    const float lost =
+        __fadd_rn(fmaxf(kA, product), -__fadd_rn(sum, -fminf(kA, product)));
+    float rest = fmaf(kB, square, -product);
+    rest = fmaf(kB, fmaf(x, x, -square), rest);
+    rest = fmaf(kBLow, square, rest);
+    const float t = __fmul_rn(x, sum);
+    return logistic_times(x, t, fmaf(x, lost + rest, fmaf(x, sum, -t)));
 }
 
 __device__ __forceinline__ float activate_exact(int activation, float x) {
@@ -75,7 +95,7 @@ __device__ __forceinline__ float activate_exact(int activation, float x) {
     }
 }
 
-// ---- for bfloat16 outputs: errors far below the store's 2^-9 -------------------------------
+// ---- for bfloat16 outputs: errors far below the store's 2^-8 -------------------------------
 
 // 1 / (1 + 2^t) with the hardware's exponential and reciprocal (2^-21 relative).
 __device__ __forceinline__ float logistic_of_exp2(float t) {

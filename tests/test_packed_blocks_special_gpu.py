@@ -236,3 +236,37 @@ def test_linear_large_finite_sums(m, k, shift, kind, out_kind, activation, cuda)
     # The value itself, times a factor that is 1 to within a few steps.
     step = 2.0 ** -7 if out_kind == "bf16" else 32 * 2.0 ** -24
     check(got, want.expand_as(got), (step * want.abs() + 1e-30).expand_as(got))
+
+
+@pytest.mark.parametrize("activation", range(1, 4), ids=["gelu", "gelu_tanh", "silu"])
+@MODES
+@PATHS
+@pytest.mark.parametrize("short", [False, True], ids=["full", "short"])
+def test_linear_activation_tails(short, m, k, shift, kind, out_kind, activation, cuda):
+    """Relative accuracy alone, into the negative tail: every sum is one product by 1, so the
+    activation sees just that value. Float outputs: 12 u32 (six of them the polynomial of the erf
+    form, the others a power, a reciprocal and products), bfloat16 ones 2^-12 and the store's half
+    step, within a factor of 1 + 2^-8. Powers of two below 2^-126 may be flushed, with them values
+    below |y| times that.
+    The products of TF32 halves keep all but 2^-23 of a float, which the activation's slope passes on
+    (in the tail of GELU y^2 times as much of the value); short values, of eight bits, are kept
+    whole."""
+    torch = cuda
+    y = torch.cat([torch.linspace(-95.0, 12.0, 700), torch.linspace(-14.5, -0.01, 500),
+                   torch.logspace(-30, 0, 60), -torch.logspace(-30, 0, 60)]).cuda()
+    if short:
+        y = y.bfloat16().float()
+    got = run_layer(torch, m, k, shift, y, kind, out_kind, activation, False)
+    y = y.to(torch_type(torch, kind)).double().requires_grad_()
+    want = activated(torch, activation, y)
+    slope, = torch.autograd.grad(want.sum(), y)
+    slope = slope.nan_to_num(0.0)  # infinite over infinite where a double's power is: below 1e-150
+    y, want = y.detach(), want.detach()
+    if out_kind == "bf16":
+        bound = (2.0 ** -12 * (1 + 2.0 ** -8) + 2.0 ** -8) * want.abs()
+    else:
+        bound = 12 * 2.0 ** -24 * want.abs()
+    bound = bound + 128 * 2.0 ** -126
+    if kind == "f32" and not short:
+        bound = bound + 1.01 * 2.0 ** -23 * (slope * y).abs()
+    check(got, want.expand(m, -1), bound.expand(m, -1))

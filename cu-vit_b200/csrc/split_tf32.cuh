@@ -38,8 +38,11 @@ __device__ __forceinline__ void split4_checked(const float (&x)[4], float (&hi)[
                                                float (&lo)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        hi[j] = round_to_tf32(x[j]);
-        lo[j] = (__float_as_uint(x[j]) & 0x7F800000u) == 0x7F800000u ? 0.0F : x[j] - hi[j];
+        const bool special = (__float_as_uint(x[j]) & 0x7F800000u) == 0x7F800000u;
+        // The tensor core takes the upper 19 bits: a NaN whose payload lies below them would be an
+        // infinity there. A sum gives the NaN whose bits are all set.
+        hi[j] = special ? x[j] + x[j] : round_to_tf32(x[j]);
+        lo[j] = special ? 0.0F : x[j] - hi[j];
     }
 }
 

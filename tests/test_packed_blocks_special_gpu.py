@@ -270,3 +270,40 @@ def test_linear_activation_tails(short, m, k, shift, kind, out_kind, activation,
     if kind == "f32" and not short:
         bound = bound + 1.01 * 2.0 ** -23 * (slope * y).abs()
     check(got, want.expand(m, -1), bound.expand(m, -1))
+
+
+# ---- float products of TF32 halves: every NaN ----------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [0x7F800001, 0x7F801FFF, 0x7FC00000, 0x7FFFFFFF, -0x7FFFFF, -1],
+                         ids=lambda b: f"{b & 0xFFFFFFFF:08x}")
+def test_float_nan_of_any_payload(bits, cuda):
+    """A NaN with its payload in the last bits only is one all the same."""
+    torch = cuda
+    for m, n, k in ((40, 64, 96), (300, 200, 64), (12, 64, 4096)):
+        for side in range(2):
+            x, w = normal(torch, (m, k), 1), normal(torch, (n, k), 2)
+            (x, w)[side].view(torch.int32)[5, 33] = bits
+            out = torch.zeros(m, n, device="cuda")
+            kernels.launch_linear(x, w, None, None, None, out,
+                                  LinearProblem(m, n, k, kernels.MATH_FP32, kernels.DTYPE_F32))
+            torch.cuda.synchronize()
+            bad = torch.zeros_like(out, dtype=torch.bool)
+            (bad if side == 0 else bad.t())[5] = True
+            assert out[bad].isnan().all() and out[~bad].isfinite().all()
+    for dim in (64, 128):
+        for queries in (2, 200):
+            q, k, v, problem = attention_case(torch, "f32", queries, 300, dim, False)
+            places = offsets(torch, [queries]), offsets(torch, [300])
+            for side in range(3):
+                operands = [t.clone() for t in (q, k, v)]
+                operands[side].view(torch.int32)[1, 0, 7] = bits
+                got = run_attention(torch, *operands, *places, problem)
+                bad = torch.zeros_like(got, dtype=torch.bool)
+                if side == 0:
+                    bad[1, 0] = True
+                elif side == 1:
+                    bad[:, 0] = True
+                else:
+                    bad[:, 0, 7] = True
+                assert got[bad].isnan().all() and got[~bad].isfinite().all()

@@ -229,7 +229,9 @@ int run(const void* x, const void* weight, const float* bias, const float* scale
     if (out == nullptr || (c.k > 0 && (x == nullptr || weight == nullptr))) {
         return host::fail(CUVIT_INVALID_ARGUMENT, "linear operands cannot be null");
     }
-    constexpr int kMaxExtent = 0x7FFFFFFF - 4096; // tile ends past the last row stay in int
+    // Tile ends past the last row stay in int, and the steps past the end of k that the kernels
+    // count (at most 8192 further: linear_rows.cu).
+    constexpr int kMaxExtent = 0x7FFFFFFF - 65536;
     if (c.m > kMaxExtent || c.n > kMaxExtent / 2 || c.k > kMaxExtent) {
         return host::fail(CUVIT_LENGTH_ERROR, "linear dimensions are too large");
     }

@@ -198,6 +198,25 @@ def test_linear_pointer_refusals():
         call(FAKE, 2 * FAKE, None, None, None, FAR, linear(m=2 ** 31 - 1))
 
 
+@pytest.mark.parametrize("extent", ["m", "n", "k"])
+def test_linear_extents_whose_steps_pass_32_bits(extent):
+    """The kernels count up to 8192 elements past an extent's end; what that takes past 2^31 - 1 is
+    refused."""
+    largest = 2 ** 31 - 1 - 65536
+    sizes = dict(m=1, n=1, k=8)
+    if extent == "n":
+        largest //= 2
+    for size in (largest + 1, 2 ** 31 - 1 - 4096 if extent != "n" else (2 ** 31 - 1 - 4096) // 2):
+        with pytest.raises(LengthError):
+            kernels.launch_linear(FAKE, 2 * FAKE, None, None, None, 2 ** 48,
+                                  linear(**{**sizes, extent: size}))
+    # The next smaller one passes this check (and fails only later, for the fake addresses).
+    with pytest.raises(Exception) as caught:
+        kernels.launch_linear(FAKE, 2 ** 40, None, None, None, 2 ** 48,
+                              linear(**{**sizes, extent: largest}))
+    assert "too large" not in str(caught.value)
+
+
 def test_interleaved_columns_do_not_overlap():
     """Outputs in other columns of their inputs' rows pass the overlap check (and fail only
     later, on a machine without a device or for the fake addresses)."""

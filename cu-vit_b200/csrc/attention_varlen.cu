@@ -288,8 +288,11 @@ int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* emp
     if (c.dtype != CUVIT_DTYPE_F32 && c.dtype != CUVIT_DTYPE_BF16) {
         return host::fail(CUVIT_INVALID_ARGUMENT, "packed attention operands must be F32 or BF16");
     }
-    if (!std::isfinite(c.scale) || c.scale <= 0.0F) {
-        return host::fail(CUVIT_INVALID_ARGUMENT, "the attention scale must be finite and positive");
+    // The kernels work with scale * log2(e), which has to be a float too.
+    constexpr float kLog2e = 1.4426950408889634F;
+    if (!(c.scale > 0.0F) || !std::isfinite(c.scale * kLog2e)) {
+        return host::fail(CUVIT_INVALID_ARGUMENT,
+                          "the attention scale must be positive and finite, also times log2(e)");
     }
     constexpr int kMaxTokens = 0x7FFFFFFF - 4096; // tile ends past the last row stay in int
     if (c.q_tokens > kMaxTokens || c.kv_tokens > kMaxTokens) {
@@ -313,7 +316,7 @@ int resolve(const cuvit_attention_problem* problem, VarlenParams* out, bool* emp
     p.causal = c.causal ? 1 : 0;
     p.bf16 = c.dtype == CUVIT_DTYPE_BF16 ? 1 : 0;
     p.splits = 1;
-    p.scale_log2 = c.scale * 1.4426950408889634F;
+    p.scale_log2 = c.scale * kLog2e;
     const int64_t q_width = static_cast<int64_t>(c.q_heads) * c.head_dim;
     const int64_t kv_width = static_cast<int64_t>(c.kv_heads) * c.head_dim;
     p.q_stride = c.q_stride != 0 ? c.q_stride : q_width;

@@ -366,7 +366,7 @@ typedef struct cuvit_attention_problem {
     int head_dim; /* 1..128 */
     int dtype;    /* CUVIT_DTYPE_F32 or CUVIT_DTYPE_BF16 */
     int causal;   /* query i of n sees keys j <= i + (keys - n): aligned at the ends */
-    float scale;  /* finite and > 0 */
+    float scale;  /* > 0 and finite, also times log2(e) */
     int64_t q_stride;
     int64_t k_stride;
     int64_t v_stride;

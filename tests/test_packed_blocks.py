@@ -164,6 +164,18 @@ def test_attention_pointer_refusals():
         call(FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, FAR, FAR, attention(k_stride=2 ** 60))
 
 
+def test_attention_scale_times_log2e_is_finite():
+    """The kernels scale scores for powers of two; 3e38 log2(e) is no float."""
+    for scale in (3.0e38, 2.4e38):
+        with pytest.raises(InvalidArgument, match="scale"):
+            kernels.launch_attention_varlen(FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, FAR, FAR,
+                                            attention(scale=scale))
+    with pytest.raises(Exception) as caught:
+        kernels.launch_attention_varlen(FAKE, 2 * FAKE, 3 * FAKE, 4 * FAKE, FAR, FAR,
+                                        attention(scale=2.3e38))
+    assert "scale" not in str(caught.value)
+
+
 def test_linear_no_ops():
     for changes in (dict(m=0), dict(n=0)):
         kernels.launch_linear(None, None, None, None, None, None, linear(**changes))

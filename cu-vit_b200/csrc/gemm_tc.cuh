@@ -123,13 +123,14 @@ __device__ __forceinline__ void load_accumulator(uint32_t taddr, float (&v)[Cols
         if constexpr (Split) {
             uint32_t small[32];
             dev::tmem_load_32(taddr + g * 32 + BN, small);
-            dev::tmem_wait_load();
+            dev::tmem_wait_load_of(raw);
+            dev::tmem_wait_load_of(small); // the same wait, for these registers' uses
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 v[g * 32 + j] = __uint_as_float(raw[j]) + __uint_as_float(small[j]);
             }
         } else {
-            dev::tmem_wait_load();
+            dev::tmem_wait_load_of(raw);
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 v[g * 32 + j] = __uint_as_float(raw[j]);

@@ -64,7 +64,7 @@ struct TcParams {
 
 // The epilogue of linear layers (linear_tc.cuh).
 struct LinearParams;
-template <int BN, bool Split>
+template <int BN>
 __device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uint32_t tmem_cols,
                             int n_block, int row_base, int half, uint8_t* slab, uint32_t slab_addr,
                             uint32_t residual_bar, uint32_t& residual_phase, int lane);
@@ -582,9 +582,10 @@ __global__ void __launch_bounds__(TcShape<ElemBytes, BN, Split>::kThreads, 1)
             const int first = half * kHalf;
             const int col_base = n_block * BN;
             if constexpr (Params::kLinear) {
-                if (!linear_tile<BN, Split>(p, &tma_c, tmem_cols, n_block, row_base, half, slab,
-                                            slab_addr, base + Shape::kResidualOffset + 8u * e,
-                                            residual_phase, lane)) {
+                static_assert(!Split, "FP32 linear layers have a kernel of their own");
+                if (!linear_tile<BN>(p, &tma_c, tmem_cols, n_block, row_base, half, slab, slab_addr,
+                                     base + Shape::kResidualOffset + 8u * e, residual_phase,
+                                     lane)) {
                     break;
                 }
             } else

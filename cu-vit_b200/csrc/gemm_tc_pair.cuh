@@ -277,9 +277,9 @@ __global__ void __launch_bounds__(PairShape<BN>::kThreads, 1)
             const int first = half * kHalf;
             const int col_base = n_block * BN;
             if constexpr (Params::kLinear) {
-                if (!linear_tile<BN, false>(p, &tma_c, tmem_cols, n_block, row_base, half, slab,
-                                            slab_addr, base + Shape::kResidualOffset + 8u * e,
-                                            residual_phase, lane)) {
+                if (!linear_tile<BN>(p, &tma_c, tmem_cols, n_block, row_base, half, slab, slab_addr,
+                                     base + Shape::kResidualOffset + 8u * e, residual_phase,
+                                     lane)) {
                     break;
                 }
             } else if (p.c_tma && (p.c_kind != 1 || kHalf >= 64)) {

@@ -136,7 +136,7 @@ __device__ __forceinline__ void apply_columns(float (&v)[32], const float* vecto
 
 // The epilogue of one warp's part of a tile: rows row_base .. + 31, one half of the tile's output
 // columns. False when a bounded wait gave up (no load is then in flight).
-template <int BN, bool Split>
+template <int BN>
 __device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uint32_t tmem_cols,
                             int n_block, int row_base, int half, uint8_t* slab, uint32_t slab_addr,
                             uint32_t residual_bar, uint32_t& residual_phase, int lane) {
@@ -184,7 +184,7 @@ __device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uin
         for (int s = 0; s < chunk; s += 32) {
             float v[32];
             __syncwarp(); // the accumulator's reads are warp-wide
-            load_accumulator<32, BN, Split>(tmem_cols + c + s, v);
+            load_accumulator<32, BN, false>(tmem_cols + c + s, v);
             if (p.bias != nullptr) {
                 apply_columns<false>(v, p.bias, col0 + s, p.n, p.bias_vector_ok);
             }
@@ -195,7 +195,7 @@ __device__ bool linear_tile(const LinearParams& p, const CUtensorMap* tma_c, uin
             }
             if (p.gated) {
                 float up[32];
-                load_accumulator<32, BN, Split>(tmem_cols + BN / 2 + c + s, up);
+                load_accumulator<32, BN, false>(tmem_cols + BN / 2 + c + s, up);
                 if (p.bias != nullptr) {
                     apply_columns<false>(up, p.bias + p.n, col0 + s, p.n, p.up_vector_ok);
                 }

@@ -73,11 +73,11 @@ int launch_tc_bf16(const TcPlan& plan, cudaStream_t stream) {
     }
     switch (plan.block_n) {
     case 64:
-        return launch_instance<2, 64, false>(plan, stream);
+        return launch_instance<2, 64>(plan, stream);
     case 128:
-        return launch_instance<2, 128, false>(plan, stream);
+        return launch_instance<2, 128>(plan, stream);
     default:
-        return launch_instance<2, 256, false>(plan, stream);
+        return launch_instance<2, 256>(plan, stream);
     }
 }
 

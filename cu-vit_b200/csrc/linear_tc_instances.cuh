@@ -6,10 +6,10 @@
 
 namespace cuvit::linear {
 
-template <int ElemBytes, int BN, bool Split>
+template <int ElemBytes, int BN>
 int launch_instance(const TcPlan& plan, cudaStream_t stream) {
-    using Shape = gemm::TcShape<ElemBytes, BN, Split>;
-    auto* kernel = &gemm::tc_gemm_kernel<ElemBytes, BN, false, Split, gemm::LinearParams>;
+    using Shape = gemm::TcShape<ElemBytes, BN, false>;
+    auto* kernel = &gemm::tc_gemm_kernel<ElemBytes, BN, false, false, gemm::LinearParams>;
     CUVIT_TRY_CUDA(host::allow_dynamic_smem(reinterpret_cast<const void*>(kernel),
                                             Shape::kSmemBytes));
     host::pdl_launch(kernel, dim3(static_cast<unsigned>(plan.grid)), dim3(Shape::kThreads),

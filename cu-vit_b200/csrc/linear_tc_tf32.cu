@@ -6,11 +6,11 @@ namespace cuvit::linear {
 int launch_tc_tf32(const TcPlan& plan, cudaStream_t stream) {
     switch (plan.block_n) {
     case 64:
-        return launch_instance<4, 64, false>(plan, stream);
+        return launch_instance<4, 64>(plan, stream);
     case 128:
-        return launch_instance<4, 128, false>(plan, stream);
+        return launch_instance<4, 128>(plan, stream);
     default:
-        return launch_instance<4, 256, false>(plan, stream);
+        return launch_instance<4, 256>(plan, stream);
     }
 }
 

@@ -307,3 +307,48 @@ def test_float_nan_of_any_payload(bits, cuda):
                 else:
                     bad[:, 0, 7] = True
                 assert got[bad].isnan().all() and got[~bad].isfinite().all()
+
+
+# ---- attention: more query heads to a key head than the few-row kernels take at once -------
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("group", [9, 12, 16, 17, 40])
+@pytest.mark.parametrize("empty", [0, 1, 5], ids=lambda n: f"{n}empty")
+def test_attention_wide_groups_of_single_queries(empty, group, kind, cuda):
+    """One query a sequence, with and without sequences that have none: on the average over the
+    batch the former have more rows than the few-row kernels take, the latter few enough, so that
+    their blocks divide a key head's query heads into chunks of eight."""
+    torch = cuda
+    kv_heads, dim = 2, 64
+    queries = ([1] + [0] * empty) * 3
+    keys = ([300, *[0] * empty, 17, *[4] * empty, 2000, *[64] * empty])
+    q = normal(torch, (sum(queries), kv_heads * group, dim), 1, kind)
+    k, v = (normal(torch, (sum(keys), kv_heads, dim), seed, kind) for seed in (2, 3))
+    for causal in (False, True):
+        problem = AttentionProblem(len(queries), sum(queries), sum(keys), kv_heads * group, kv_heads,
+                                   dim, dtype_of(kind), causal, 0.2)
+        want, bound = attention_64(torch, q, k, v, queries, keys, 0.2, causal, kind)
+        for workspace in (True, False):
+            got = run_attention(torch, q, k, v, offsets(torch, queries), offsets(torch, keys), problem,
+                                workspace)
+            check(got, want, bound, f"causal {causal} workspace {workspace}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("long", [40, 700])
+def test_attention_one_long_sequence_among_single_queries(long, kind, cuda):
+    """A prompt beside new tokens of other sequences: the average sends it to the few-row kernels in
+    one batch and the new tokens to the tile kernels in the other."""
+    torch = cuda
+    queries = [1] * 20 + [long] + [1] * 20
+    keys = [37 * i % 400 + 1 for i in range(20)] + [long + 5] + [91 * i % 700 + 1 for i in range(20)]
+    heads, kv_heads, dim = 4, 2, 64
+    q = normal(torch, (sum(queries), heads, dim), 1, kind)
+    k, v = (normal(torch, (sum(keys), kv_heads, dim), seed, kind) for seed in (2, 3))
+    for causal in (False, True):
+        problem = AttentionProblem(len(queries), sum(queries), sum(keys), heads, kv_heads, dim,
+                                   dtype_of(kind), causal, 0.2)
+        want, bound = attention_64(torch, q, k, v, queries, keys, 0.2, causal, kind)
+        got = run_attention(torch, q, k, v, offsets(torch, queries), offsets(torch, keys), problem)
+        check(got, want, bound, f"causal {causal}")

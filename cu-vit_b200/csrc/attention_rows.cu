@@ -563,17 +563,22 @@ long long rows_kernel_items(const VarlenParams& p) {
 }
 
 // 16-byte rows of q, k and v heads, at distances whose 16-fold fits 31 bits, and on average no more
-// rows than the kernel takes at once.
+// rows than the kernels take at once, or one query a sequence, whose heads are then taken eight at a
+// time. The kernels for many rows read the keys once for each query head, these once for eight rows:
+// 16 sequences of 2000 keys, one query, heads of 128, bfloat16 (float): 16 heads over 2 key heads 16 us
+// (28) against 59 (325), over one 16 (28) against 60 (325); 256 of 197 keys, 12 heads of 64, 8 queries
+// 40 (119) against 101 (293). With 16 queries the former take 102.
 bool rows_kernel_takes(const VarlenParams& p) {
     const int size = p.bf16 ? 2 : 4;
     const auto fits = [size](const void* base, long long stride) {
         return reinterpret_cast<uintptr_t>(base) % 16 == 0 && stride * size % 16 == 0 &&
                stride < (1LL << 26);
     };
-    return static_cast<long long>(p.q_tokens) * p.group <=
-               static_cast<long long>(kMaxRows) * p.batch &&
-           p.head_dim * size % 16 == 0 && fits(p.q, p.q_stride) && fits(p.k, p.k_stride) &&
-           fits(p.v, p.v_stride);
+    const bool few = p.q_tokens <= p.batch ||
+                     static_cast<long long>(p.q_tokens) * p.group <=
+                         static_cast<long long>(kMaxRows) * p.batch;
+    return few && p.head_dim * size % 16 == 0 && fits(p.q, p.q_stride) &&
+           fits(p.k, p.k_stride) && fits(p.v, p.v_stride);
 }
 
 int launch_rows(const VarlenParams& p, cudaStream_t stream) {

@@ -352,3 +352,23 @@ def test_attention_one_long_sequence_among_single_queries(long, kind, cuda):
         want, bound = attention_64(torch, q, k, v, queries, keys, 0.2, causal, kind)
         got = run_attention(torch, q, k, v, offsets(torch, queries), offsets(torch, keys), problem)
         check(got, want, bound, f"causal {causal}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("group", [16, 24])
+def test_attention_single_queries_of_a_wide_group_share_their_keys(group, kind, cuda):
+    """The few-row kernels take a wide group's heads eight at a time: without a split of the keys that
+    is bit for bit the calls of eight heads each."""
+    torch = cuda
+    keys, dim = [300, 17, 1000], 128
+    q = normal(torch, (3, group, dim), 1, kind)
+    k, v = (normal(torch, (sum(keys), 1, dim), seed, kind) for seed in (2, 3))
+    places = offsets(torch, [1, 1, 1]), offsets(torch, keys)
+
+    def run(part):
+        problem = AttentionProblem(3, 3, sum(keys), part.shape[1], 1, dim, dtype_of(kind), True, 0.1)
+        return run_attention(torch, part, k, v, *places, problem, workspace=False)
+
+    whole = run(q)
+    for first in range(0, group, 8):
+        assert torch.equal(whole[:, first:first + 8], run(q[:, first:first + 8].contiguous()))

@@ -27,7 +27,7 @@
 //   scores giving both them and their maximum; only where a maximum turns out too high (in the first
 //   step, where m is 0, also too low) are O and the sums rescaled and the scores read again.
 // * NaN and minus infinity take that second reading too, in its exact form: the exponentials on the
-//   FMA pipe would make 2^-125 of both. The maximum keeps NaN, so it shows them at no cost.
+//   FMA pipe would make something finite of both.
 // * Scores are read 32 at a time, the next 32 in flight meanwhile. Two threads per row (64 scores
 //   each, maxima or a "too high" flag exchanged every step) took 1.94 ms where this takes 1.81 ms
 //   (16384 tokens, 16 heads of 128: 1214 TFLOP/s, of 1672 measured for one large product; heads of
@@ -68,6 +68,8 @@ constexpr int kThreads = 352;
 constexpr float kRescaleAbove = 8.0F; // log2
 // Above this |m scale| (log2) the plain and the exact form of P would differ by more than 2^-14.
 constexpr float kLargeMaximum = 1024.0F;
+// A step's weights add up to 2^15 at most where none is NaN (the FMA pipe's form makes 2^128 of it).
+constexpr float kLargeSum = 1.0e30F;
 // Exponentials of these pairs of a 32-key chunk run on the FMA pipe (see attention.cu).
 constexpr uint32_t kPolyPairs = 0x8888u;
 
@@ -164,7 +166,6 @@ __device__ __forceinline__ void mask(uint32_t (&s)[32], int limit) {
     }
 }
 
-// NaN where a score is.
 __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
     float m[2];
 #pragma unroll
@@ -172,12 +173,12 @@ __device__ __forceinline__ float maximum(const uint32_t (&s)[32]) {
         m[c] = __uint_as_float(s[16 * c]);
 #pragma unroll
         for (int j = 1; j < 15; j += 2) {
-            m[c] = dev::max3_or_nan(m[c], __uint_as_float(s[16 * c + j]),
-                                    __uint_as_float(s[16 * c + j + 1]));
+            m[c] = dev::max3(m[c], __uint_as_float(s[16 * c + j]),
+                             __uint_as_float(s[16 * c + j + 1]));
         }
-        m[c] = dev::max_or_nan(m[c], __uint_as_float(s[16 * c + 15]));
+        m[c] = fmaxf(m[c], __uint_as_float(s[16 * c + 15]));
     }
-    return dev::max_or_nan(m[0], m[1]);
+    return fmaxf(m[0], m[1]);
 }
 
 // P = 2^(scale (s - m)) of 32 scores, packed, and their sum. The plain form
@@ -201,7 +202,7 @@ __device__ __forceinline__ float exponentials(const uint32_t (&s)[32], float sca
         const float2 x = dev::f32x2_split(x2);
         float2 e;
         if (!Exact && ((kPolyPairs >> j) & 1u)) {
-            e = dev::exp2_poly2(x.x, x.y);
+            e = dev::exp2_poly2<true>(x.x, x.y);
         } else {
             e = make_float2(dev::ex2_approx(x.x), dev::ex2_approx(x.y));
         }
@@ -713,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if constexpr (exact.value) {
                                 mask(s[c & 1], limit - 32 * c);
                             }
-                            top = dev::max_or_nan(top, maximum(s[c & 1]));
+                            top = fmaxf(top, maximum(s[c & 1]));
                             added += exponentials<exact.value>(s[c & 1], p.scale_log2, m,
                                                                packed[c]);
                         }
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 dev::tmem_load_32(s_tmem + 32 * c, s);
                                 dev::tmem_wait_load_of(s);
                                 mask(s, limit - 32 * c);
-                                top = dev::max_or_nan(top, maximum(s));
+                                top = fmaxf(top, maximum(s));
                                 added += exponentials<true>(s, p.scale_log2, m, packed[c]);
                             } else {
 #pragma unroll
@@ -745,12 +746,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         weigh(std::false_type{});
                     }
                     // A row without a weight so far has m = 0, which stays where the maximum is
-                    // within 2^+-8 of it. A NaN maximum is not within anything.
+                    // within 2^+-8 of it. NaN shows in the weights' sum.
                     const bool fresh = sum == 0.0F;
                     const bool some = top != -INFINITY;
                     const float above = (top - m) * p.scale_log2;
                     const bool raise = __any_sync(
-                        0xFFFFFFFFu, !(above <= kRescaleAbove) ||
+                        0xFFFFFFFFu, above > kRescaleAbove || !(added < kLargeSum) ||
                                          (some ? fresh && above < -kRescaleAbove : !exact));
                     if (!S::kOverlay && !raise) {
                         arrive(s_free + 8 * t);
@@ -969,9 +970,11 @@ int launch_tiles(const VarlenParams& p, cudaStream_t stream) {
         return host::fail(CUVIT_CUDA_ERROR, "the attention operands' TMA descriptors failed");
     }
     // Sequences of less than two tiles on average: most tiles end inside, and the warps skip the
-    // chunks behind (64 tokens, 16 heads of 64: 256 images 80 us against 95; of 197 tokens, 12 heads:
-    // 148 against 154). The branches cost whole tiles 6 % (one of 16384 tokens: 1327 us against
-    // 1252), so longer ones go without.
+    // chunks behind (64 tokens, 16 heads of 64: 256 images 83 us against 95; 100 of 160 68 against 75;
+    // 256 of 197, 12 heads, 151 against 156; where little is skipped the branches cost up to 6 %: 160 of
+    // 100 68 against 65, 128 of 197 with heads of 80 120 against 114). Of longer ones a smaller part is
+    // skipped, and whole tiles pay (300 tokens 86 against 87, 384 68 against 65, 16 images of 64 to 4096
+    // with heads of 72 275 against 262, one of 16384 1327 against 1252), so they go without.
     const bool short_keys = p.kv_tokens <= 224LL * p.batch;
     if (p.head_dim <= 64) {
         return short_keys ? launch_atoms<1, true>(p, *context, maps, stream)

@@ -698,16 +698,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// The maximum, or NaN where an operand is NaN (max.f32 gives the other operands).
+// The maximum, or NaN where an operand is NaN (max.f32 gives the other operand).
 __device__ __forceinline__ float max_or_nan(float a, float b) {
     float d;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
-__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -734,9 +728,12 @@ __device__ __forceinline__ float exp2_poly(float x) {
 }
 
 // exp2_poly on two values, the additions and the polynomial two per instruction: the same
-// operations in the same order, so the same results.
+// operations in the same order, so the same results. KeepNan: a NaN gives the largest float (its bits
+// take part in the sum of the exponent), otherwise 2^-125.
+template <bool KeepNan = false>
 __device__ __forceinline__ float2 exp2_poly2(float x0, float x1) {
-    const uint64_t x = f32x2(fmaxf(x0, -125.0F), fmaxf(x1, -125.0F));
+    const uint64_t x = KeepNan ? f32x2(max_or_nan(x0, -125.0F), max_or_nan(x1, -125.0F))
+                               : f32x2(fmaxf(x0, -125.0F), fmaxf(x1, -125.0F));
     const uint64_t shifted = add_f32x2(x, f32x2(12582912.0F, 12582912.0F));
     const uint64_t n = add_f32x2(shifted, f32x2(-12582912.0F, -12582912.0F));
     const uint64_t f = sub_f32x2(x, n);

@@ -9,13 +9,13 @@
 // more than half of the time that the bytes take). tcgen05 has no shape for it: 128 rows are its
 // least.
 //
-// Each warp goes through every fourth group of 16 keys with a ring of its own (asynchronous copies,
-// no barrier in the loop) and its own maximum, sum and output; warps and splits are merged at the
-// end. Outputs are rescaled only when a maximum has risen by more than 2^8.
+// Each warp of a block of two goes through every second group of 16 keys with a ring of its own
+// (asynchronous copies, no barrier in the loop) and its own maximum, sum and output; warps and splits
+// are merged at the end. Outputs are rescaled only when a maximum has risen by more than 2^8.
 //
 // One query of 16 heads over 4 key heads of 128, 16001 + 9000 keys (51 MB): 15.7 us (dot products
 // 23.5), where the copy rate would allow 7.8; then the join. 256 queries over 197 keys each, 12 heads
-// of 64: 41 us of 24. Half of the rest is a block's start (offsets, then its first keys) and end.
+// of 64: 36 us of 24. Half of the rest is a block's start (offsets, then its first keys) and end.
 // Blocks of two warps: 4 take a tenth longer (fewer blocks start beside each other's ends), and so do
 // 4 or 6 stages.
 #include "attention_varlen.hpp"

@@ -62,12 +62,14 @@ __device__ __forceinline__ void outer(const float* rows, const float4& b, float 
 // 8 ty .. + 7 and, of the scores, the keys tx + kX m, of the output, elements 4 tx .. + 3 of every
 // 4 kX. Operands come from shared memory as whole vectors (Q and P with rows contiguous): for heads
 // up to 64, 64 multiply-adds share four loads, and two blocks fit an SM and load under each other's
-// arithmetic. 4096 tokens, 8 heads of 64: 954 us, 36 TFLOP/s of the FP32 pipe's 74. (8 x 4 products
-// a thread on twice the threads: 990 us, shared memory then takes as many cycles as the arithmetic;
-// packed multiply-adds on pairs of rows: 1050 us, since doubling the other operand takes moves on
-// the same pipe. Heads up to 128 use 8 x 4 for the scores: the outputs take the registers.) A tile's
-// keys lie in the order the threads read them, kX apart, which also lets a warp write its weights
-// without bank conflicts.
+// arithmetic. 4096 tokens, 8 heads whose base lies an element off a vector: heads of 64 1.20 ms,
+// 29 TFLOP/s of the FP32 pipe's 74, heads of 128 2.62 ms. What keeps it from more are the loads of
+// single elements, converted one by one: operands of floats, which attention_split.cu takes, took
+// 0.95 ms (and 8 x 4 products a thread on twice the threads 0.99, shared memory then taking as many
+// cycles as the arithmetic; packed multiply-adds on pairs of rows 1.05, since doubling the other
+// operand takes moves on the same pipe). Heads up to 128 use 8 x 4 for the scores: the outputs take the
+// registers. A tile's keys lie in the order the threads read them, kX apart, which also lets a warp
+// write its weights without bank conflicts.
 template <int DPad>
 __global__ void __launch_bounds__(SimtShape<DPad>::kThreads, DPad == 64 ? 2 : 1)
     attention_varlen_simt(const VarlenParams p) {

@@ -6,8 +6,8 @@
 // into one of two buffers there, weights go back as halves, and a tile's weighted values are added
 // to registers, so no accumulator sums more than 64 products or a head's width.
 //
-// 4096 tokens, 8 heads of 64: 311 us, 111 TFLOP/s (products in the FP32 pipe: 954 us); heads of 128
-// 659 us; 8 x 197 tokens, 12 heads 39 us (78). The tensor core would allow three times that (its
+// 4096 tokens, 8 heads of 64: 285 us, 121 TFLOP/s (products in the FP32 pipe: 954 us); heads of 128
+// 665 us; 8 x 197 tokens, 12 heads 35 us (78). The tensor core would allow three times that (its
 // products take 1540 cycles of the 4600 a tile of 64 keys and 64 elements takes): what bounds it is
 // the softmax warps' chain of waits (scores, maximum, exponentials, previous sum, weights), and a
 // quarter is the loading warps' share of the issue slots. A second set of softmax warps on alternate

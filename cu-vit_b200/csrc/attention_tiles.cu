@@ -685,6 +685,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue;
             }
             const bool live_warp = quarter * 32 < rows;
+            // Of the warp's rows the first ones exist. What stands behind them is another
+            // sequence's, or nobody's, and takes no part in the warp's choices.
+            const unsigned live_rows = 0xFFFFFFFFu >> (32 - min(32, max(1, rows - quarter * 32)));
             float m = 0.0F; // unscaled
             float sum = 0.0F;
             for (int j = 0; j < steps && ok; ++j) {
@@ -719,8 +722,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                                packed[c]);
                         }
                     };
-                    const bool exact =
-                        masked || __any_sync(0xFFFFFFFFu, fabsf(m * p.scale_log2) > kLargeMaximum);
+                    const unsigned large_rows =
+                        __ballot_sync(0xFFFFFFFFu, fabsf(m * p.scale_log2) > kLargeMaximum);
+                    const bool exact = masked || (large_rows & live_rows) != 0u;
                     if (Short && exact) {
                         // Chunks that no row of the warp sees are zeros.
                         const int seen = __reduce_max_sync(0xFFFFFFFFu, limit);
@@ -750,9 +754,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool fresh = sum == 0.0F;
                     const bool some = top != -INFINITY;
                     const float above = (top - m) * p.scale_log2;
-                    const bool raise = __any_sync(
+                    const unsigned raised_rows = __ballot_sync(
                         0xFFFFFFFFu, above > kRescaleAbove || !(added < kLargeSum) ||
                                          (some ? fresh && above < -kRescaleAbove : !exact));
+                    const bool raise = (raised_rows & live_rows) != 0u;
                     if (!S::kOverlay && !raise) {
                         arrive(s_free + 8 * t);
                     }

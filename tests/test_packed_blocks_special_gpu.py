@@ -372,3 +372,22 @@ def test_attention_single_queries_of_a_wide_group_share_their_keys(group, kind, 
     whole = run(q)
     for first in range(0, group, 8):
         assert torch.equal(whole[:, first:first + 8], run(q[:, first:first + 8].contiguous()))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("queries", [20, 150, 300])
+def test_attention_rows_behind_a_sequence_change_no_bit_of_it(queries, dim, kind, cuda):
+    """The next sequence's queries stand in the same tile: what they are, or that they are large,
+    infinite or NaN, leaves this one's results as they are, also in their roundings."""
+    torch = cuda
+    keys = 700
+    q, k, v, _ = attention_case(torch, kind, queries + 100, keys, dim, False)
+    problem = AttentionProblem(2, queries + 100, keys, 2, 2, dim, dtype_of(kind), False, 0.125)
+    places = offsets(torch, [queries, 100]), offsets(torch, [600, 100])
+    want = run_attention(torch, q, k, v, *places, problem)[:queries]
+    for tail in (1000.0 * q[queries:], torch.full_like(q[queries:], 1e30),
+                 torch.full_like(q[queries:], float("inf")),
+                 torch.full_like(q[queries:], float("nan"))):
+        other = torch.cat([q[:queries], tail])
+        assert torch.equal(run_attention(torch, other, k, v, *places, problem)[:queries], want)

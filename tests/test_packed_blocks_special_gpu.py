@@ -4,6 +4,9 @@ each formula gives there, through every kernel a call may take."""
 from __future__ import annotations
 
 import math
+import pathlib
+import subprocess
+import sys
 
 import pytest
 
@@ -391,3 +394,66 @@ def test_attention_rows_behind_a_sequence_change_no_bit_of_it(queries, dim, kind
                  torch.full_like(q[queries:], float("nan"))):
         other = torch.cat([q[:queries], tail])
         assert torch.equal(run_attention(torch, other, k, v, *places, problem)[:queries], want)
+
+
+# ---- a process whose first call is a captured one ------------------------------------------
+
+FIRST_CALL = r"""
+import sys
+sys.path[:0] = {paths!r}
+import torch
+from cuvit import kernels as K
+from test_packed_blocks_gpu import dtype_of, normal, offsets
+kind, name = {kind!r}, {name!r}
+torch.zeros(1, device="cuda")  # the caller's context, nothing of the library's
+math = K.MATH_BF16 if kind == "bf16" else K.MATH_FP32
+if name.startswith("linear"):
+    m, k, n = dict(rows=(3, 64, 96), slices=(24, 4096, 96), tiles=(300, 64, 96), pairs=(9000, 64, 2048),
+                   simt=(20, 65, 96))[name[7:]]
+    x, w = normal(torch, (m, k), 1, kind), normal(torch, (n, k), 2, kind)
+    out = torch.zeros(m, n, dtype=x.dtype, device="cuda")
+    problem = K.LinearProblem(m, n, k, math, dtype_of(kind))
+    call = lambda stream: K.launch_linear(x, w, None, None, None, out, problem, stream)
+elif name.startswith("attention"):
+    queries, keys, dim = dict(few=(1, 9000, 64), many=(300, 5000, 64), wide=(300, 300, 128),
+                              odd=(70, 90, 13))[name[10:]]
+    q = normal(torch, (queries, 2, dim), 1, kind)
+    k, v = (normal(torch, (keys, 2, dim), i, kind) for i in (2, 3))
+    out, places = torch.zeros_like(q), (offsets(torch, [queries]), offsets(torch, [keys]))
+    area = torch.zeros(32 << 20, dtype=torch.uint8, device="cuda")
+    problem = K.AttentionProblem(1, queries, keys, 2, 2, dim, dtype_of(kind), False, 0.1)
+    call = lambda stream: K.launch_attention_varlen(q, k, v, out, *places, problem, area,
+                                                    area.numel(), stream)
+else:
+    x = normal(torch, (40, 3, 64), 1, kind)
+    out, positions = torch.zeros_like(x), torch.arange(40, dtype=torch.int32, device="cuda")
+    rotary, problem = K.rotary_axes([16]), K.QkProblem(40, 3, 0, 64, dtype_of(kind))
+    call = lambda stream: K.launch_qk_norm_rotary(x, None, out, None, K.QkNorm(), positions, rotary,
+                                                  problem, stream)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    call(torch.cuda.current_stream())
+graph.replay()
+torch.cuda.synchronize()
+got = out.clone()
+out.zero_()
+torch.cuda.synchronize()
+call(None)
+torch.cuda.synchronize()
+assert got.abs().sum() > 0 and torch.equal(got, out) and K.device_status() == 0
+print("same")
+"""
+
+
+@pytest.mark.parametrize("name,kind", [("rotary", "bf16"), ("linear_slices", "bf16"),
+                                       ("linear_pairs", "bf16"), ("linear_tiles", "f32"),
+                                       ("attention_few", "bf16"), ("attention_wide", "bf16"),
+                                       ("attention_many", "f32")])
+def test_first_call_of_a_process_is_captured(name, kind, cuda):
+    """Nothing that a call sets up once (context, function attributes, cluster sizes, tensor maps) is
+    forbidden under capture."""
+    here = pathlib.Path(__file__).resolve().parent
+    program = FIRST_CALL.format(paths=[str(here), str(here.parent / "cu-vit_b200")], kind=kind, name=name)
+    run = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
